@@ -182,6 +182,30 @@ class PrologueDesc(ctypes.Structure):
     ]
 
 
+class QkNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("norm_mode", ctypes.c_int32),
+        ("rope_halves", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("q_out_stride", ctypes.c_int64 * 3),
+        ("k_out_stride", ctypes.c_int64 * 3),
+        ("dq_stride", ctypes.c_int64 * 3),
+        ("dk_stride", ctypes.c_int64 * 3),
+        ("rope_batch_stride", ctypes.c_int64),
+    ]
+
+
 # Every symbol include/dgxm_sp.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -247,6 +271,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                               _I32, ctypes.c_float, _P, _P, _P]),
     "dgxm_full_context_attn_fwd": (ctypes.c_int, [_P, ctypes.POINTER(AttnDesc), _P, _P, _P, _P, _P,
                                                   _P]),
+    "dgxm_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormDesc), _P, _P, _P, _P, _P, _P, _P, _P]),
+    "dgxm_qk_norm_rope_backward_workspace": (ctypes.c_int64, [ctypes.POINTER(QkNormDesc)]),
+    "dgxm_qk_norm_rope_backward": (ctypes.c_int, [ctypes.POINTER(QkNormDesc), _P, _P, _P, _P, _P, _P, _P, _P,
+                                                  _P, _P, _P, _P, ctypes.c_int64, _P]),
 }
 
 _lock = threading.Lock()

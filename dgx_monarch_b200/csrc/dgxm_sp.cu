@@ -16,3 +16,4 @@
 #include "cfg.cu"
 #include "qkv_gemm.cu"
 #include "prologue.cu"
+#include "qk_norm.cu"

@@ -620,6 +620,56 @@ int dgxm_qkv_gemm_prologue_scatter_streams(const dgxm_qkv_gemm_desc* desc, int32
 int dgxm_cfg_combine(const void* cond, const void* uncond, int64_t n, int32_t dtype,
                      double cfg_scale, void* out, void* stream);
 
+/* ------------------------------------------------------------ local Q/K norm + RoPE */
+/*
+ * RMSNorm of every query and key head (DGXM_NORM_HEAD; DGXM_NORM_NONE rotates
+ * alone) and the rotary position embedding in the same pass, on tensors of
+ * this rank: q (batch, seq, q_heads, head_dim), k (batch, seq, k_heads,
+ * head_dim), any strides (elements: batch, row, head) with a contiguous
+ * head_dim, a multiple of 8 up to 256.  A tensor of zero heads may be NULL.
+ *   y = R (x / sqrt(mean(x^2) + eps) * w)
+ * R turns the first rot_dim values of a head (even; 0 or a NULL rope: none)
+ * by the row's angles: rope holds fp32 (seq, rot_dim / 2, 2) cosines and
+ * sines, rope_batch_stride floats apart by batch item (0: one table).  Pair i
+ * is values 2i and 2i + 1, or i and rot_dim / 2 + i with rope_halves.  Weights
+ * are head_dim values of weight_dtype (dtype, or F32), or NULL.  fp32 inside,
+ * rounded once.  The outputs may be the inputs themselves (same strides).
+ *
+ * Serves the reference's Q/K norm and RoPE (adapters/wan_family.py:70-73)
+ * where no scatter follows.
+ */
+typedef struct dgxm_qk_norm_desc {
+  int32_t batch, seq, q_heads, k_heads, head_dim, rot_dim;
+  int32_t dtype;                 /* of the tensors: BF16, F16 or F32 */
+  int32_t weight_dtype;          /* of the norm weights: dtype or F32 */
+  int32_t norm_mode;             /* DGXM_NORM_NONE or DGXM_NORM_HEAD */
+  int32_t rope_halves;
+  float eps;
+  int32_t reserved;              /* 0 */
+  int64_t q_stride[3], k_stride[3];
+  int64_t q_out_stride[3], k_out_stride[3];  /* of y; backward: of the inputs' gradients */
+  int64_t dq_stride[3], dk_stride[3];        /* backward: of the upstream gradients */
+  int64_t rope_batch_stride;     /* floats */
+} dgxm_qk_norm_desc;
+
+int dgxm_qk_norm_rope(const dgxm_qk_norm_desc* desc, const void* q, const void* k,
+                      const void* norm_q_w, const void* norm_k_w, const float* rope, void* q_out,
+                      void* k_out, void* stream);
+
+/*
+ * Its gradient: gq, gk from the upstream gradients dq, dk and the forward's
+ * inputs, and the weights' gradients (weight_dtype, summed over batch, rows
+ * and heads in a fixed order; either may be NULL, neither is written under
+ * DGXM_NORM_NONE).  With a weight gradient, `workspace` holds
+ * dgxm_qk_norm_rope_backward_workspace(desc) bytes (-1: a bad descriptor).
+ */
+int64_t dgxm_qk_norm_rope_backward_workspace(const dgxm_qk_norm_desc* desc);
+int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* desc, const void* dq, const void* dk,
+                               const void* q, const void* k, const void* norm_q_w,
+                               const void* norm_k_w, const float* rope, void* gq, void* gk,
+                               void* g_norm_q_w, void* g_norm_k_w, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
