@@ -206,6 +206,21 @@ class QkNormDesc(ctypes.Structure):
     ]
 
 
+FP4_NVFP4, FP4_MXFP4 = 0, 1
+
+
+class Fp4Desc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("format", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale_dtype", ctypes.c_int32),
+        ("scale_value", ctypes.c_float),
+    ]
+
+
 # Every symbol include/dgxm_sp.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -275,6 +290,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dgxm_qk_norm_rope_backward_workspace": (ctypes.c_int64, [ctypes.POINTER(QkNormDesc)]),
     "dgxm_qk_norm_rope_backward": (ctypes.c_int, [ctypes.POINTER(QkNormDesc), _P, _P, _P, _P, _P, _P, _P, _P,
                                                   _P, _P, _P, _P, ctypes.c_int64, _P]),
+    "dgxm_fp4_values_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
+    "dgxm_fp4_scales_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, _I32]),
+    "dgxm_quantize_fp4_workspace": (ctypes.c_int64, []),
+    "dgxm_quantize_fp4": (ctypes.c_int, [ctypes.POINTER(Fp4Desc), _P, _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
+    "dgxm_dequantize_fp4": (ctypes.c_int, [ctypes.POINTER(Fp4Desc), _P, _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

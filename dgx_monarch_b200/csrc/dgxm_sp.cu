@@ -17,3 +17,4 @@
 #include "qkv_gemm.cu"
 #include "prologue.cu"
 #include "qk_norm.cu"
+#include "fp4_quant.cu"

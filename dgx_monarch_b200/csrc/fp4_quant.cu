@@ -1,0 +1,421 @@
+// Microscaled 4-bit floating point: a matrix to e2m1 codes with block scales
+// (nvfp4, mxfp4) and back.
+//
+//   nvfp4  g = the tensor's scale (given, or amax / 2688), per block of 16
+//          s = e4m3(amax / (6 g)),  code = e2m1(x / (s g))
+//   mxfp4  per block of 32  s = 2^(floor(log2 amax) - 2),  code = e2m1(x / s)
+// each to the nearest value, ties to the even code, saturating.  A block with
+// a NaN or an infinity gets a NaN scale; an empty scale gives zero codes.
+//
+// The roundings are those of the real quotients, not of a rounded division:
+// an fp32 product with a reciprocal bounds the quotient within 2^-21, and
+// where both bounds round to the same code that code is right.  Where they
+// differ, one border b lies between them, and the sign of fma(b s, g, -|x|)
+// decides: b s has 7 bits, so the one rounding of the fma cannot change the
+// sign.  Bounds and decision are cheap enough to stay hidden behind DRAM,
+// which carries 2 bytes in and 0.56 out for each bf16 value: the kernel's
+// bound.  g is brought near 1 by a power of two first (with x, exactly), so
+// that no product leaves fp32's range.
+#include "common.h"
+#include "fp4.cuh"
+
+namespace dgxm {
+
+constexpr int kFp4Threads = 256;
+constexpr int kFp4Partials = 148 * 4;  // blocks of the amax pass, one partial maximum each
+
+struct Fp4Params {
+  const char* x;       // (rows, cols), row stride in elements; dequantise: the output
+  int64_t row_stride;
+  uint8_t* values;
+  uint8_t* scales;
+  const void* scale;   // the given scale, or NULL
+  float* scale_out;    // the fp32 scale of the tensor
+  uint32_t* partials;  // bit patterns of the blocks' amax
+  int64_t pitch, groups;
+  uint32_t items, per_row;  // an item is one block of one row, padded to whole groups of 4
+  int cols, n_partials, scale_dtype;
+  float scale_value;   // the given scale where `scale` is NULL
+};
+
+// One block's values as they lie in memory.
+template <typename T, int N>
+struct __align__(16) Fp4Raw {
+  T v[N];
+};
+
+// The n <= N values at p (the rest zero).  VEC: p is 16-byte aligned.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ Fp4Raw<T, N> fp4_load(const T* p, int n) {
+  Fp4Raw<T, N> r;
+  if (VEC && n >= N) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i)
+      reinterpret_cast<uint4*>(&r)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4)
+        reinterpret_cast<uint32_t*>(&r)[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
+      else
+        reinterpret_cast<uint16_t*>(&r)[i] = i < n ? __ldg(reinterpret_cast<const uint16_t*>(p) + i) : uint16_t(0);
+    }
+  }
+  return r;
+}
+
+// Bits of the largest magnitude.  As integers magnitudes order like their
+// values, infinity above all numbers and NaN above infinity.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t fp4_amax_bits(const Fp4Raw<T, N>& r) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    return max(m & 0xFFFFu, m >> 16);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float fp4_widen_bits(uint32_t bits);
+template <>
+__device__ __forceinline__ float fp4_widen_bits<float>(uint32_t bits) { return __uint_as_float(bits); }
+template <>
+__device__ __forceinline__ float fp4_widen_bits<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+template <>
+__device__ __forceinline__ float fp4_widen_bits<__half>(uint32_t bits) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
+template <typename T>
+__device__ __forceinline__ float fp4_widen(T v);
+template <>
+__device__ __forceinline__ float fp4_widen(float v) { return v; }
+template <>
+__device__ __forceinline__ float fp4_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float fp4_widen(__half v) { return __half2float(v); }
+
+// Largest magnitude of the matrix, as float bits, one partial a block.
+template <typename T, int BLOCK, bool VEC>
+__global__ void __launch_bounds__(kFp4Threads) fp4_amax_kernel(const __grid_constant__ Fp4Params p) {
+  constexpr int kUnroll = 2;
+  __shared__ uint32_t red[kFp4Threads / 32];
+  uint32_t m = 0;
+  const uint32_t step = gridDim.x * kFp4Threads;
+  for (uint64_t i0 = blockIdx.x * kFp4Threads + threadIdx.x; i0 < p.items; i0 += uint64_t(step) * kUnroll) {
+    Fp4Raw<T, BLOCK> raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const uint64_t item = i0 + uint64_t(u) * step;
+      const uint32_t row = static_cast<uint32_t>(item) / p.per_row, b = static_cast<uint32_t>(item) - row * p.per_row;
+      const int n = item < p.items ? p.cols - static_cast<int>(b) * BLOCK : 0;
+      raw[u] = fp4_load<T, BLOCK, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * BLOCK : 0), n);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) m = max(m, fp4_amax_bits<T, BLOCK>(raw[u]));
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < kFp4Threads / 32; ++i) m = max(m, red[i]);
+    p.partials[blockIdx.x] = __float_as_uint(fp4_widen_bits<T>(m));
+  }
+}
+
+// The nearest e4m3 code of amax / (6 g), and the decision at a border.
+__device__ __forceinline__ uint32_t fp4_e4m3_scale(float amax, float g, float inv6g) {
+  constexpr float kBelow = 1.f - 0x1p-21f, kAbove = 1.f + 0x1p-21f;
+  const float t = amax * inv6g;
+  const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(t * kBelow, t * kAbove), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = two & 0xFFu, hi = (two >> 8) & 0xFFu;
+  if (lo == hi) return lo;
+  const float mid = 0.5f * (fp4_scale_value<DGXM_FP4_NVFP4>(lo) + fp4_scale_value<DGXM_FP4_NVFP4>(hi));
+  const float d = fmaf(6.f * mid, g, -amax);
+  return d > 0.f ? lo : d < 0.f ? hi : (lo & 1u) ? hi : lo;
+}
+
+template <typename T, int FORMAT, bool VEC>
+__global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_constant__ Fp4Params p) {
+  constexpr int B = fp4_block(FORMAT);
+  constexpr float kBelow = 1.f - 0x1p-21f, kAbove = 1.f + 0x1p-21f;
+  float g = 1.f, up = 1.f, inv6g = 1.f;
+  bool bad = false;
+  if constexpr (FORMAT == DGXM_FP4_NVFP4) {
+    if (p.partials != nullptr) {
+      __shared__ uint32_t red[kFp4Threads / 32];
+      uint32_t m = 0;
+      for (int i = threadIdx.x; i < p.n_partials; i += kFp4Threads) m = max(m, p.partials[i]);
+      m = __reduce_max_sync(0xffffffffu, m);
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kFp4Threads / 32; ++i) m = max(m, red[i]);
+      g = __fdiv_rn(__uint_as_float(m), 2688.f);
+    } else {
+      g = p.scale != nullptr ? fp4_read_scale(p.scale, p.scale_dtype) : p.scale_value;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale_out = g;
+    bad = !(g >= 0.f) || __float_as_uint(g) >= 0x7F800000u;  // NaN, negative or infinite
+    up = g < 0x1p-64f ? 0x1p64f : g > 0x1p64f ? 0x1p-64f : 1.f;
+    g *= up;
+    inv6g = g > 0.f ? __frcp_rn(6.f * g) : 0.f;
+  }
+  const uint32_t step = gridDim.x * kFp4Threads;
+  for (uint64_t i0 = blockIdx.x * kFp4Threads + (threadIdx.x & ~31u); i0 < p.items; i0 += step) {
+    const uint32_t item = static_cast<uint32_t>(i0) + (threadIdx.x & 31u);
+    const bool live = item < p.items;  // the items come in fours: so do the live lanes
+    const uint32_t row = item / p.per_row, b = item - row * p.per_row;
+    const int n = live ? p.cols - static_cast<int>(b) * B : 0;  // <= 0: padding
+    const Fp4Raw<T, B> raw =
+        fp4_load<T, B, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * B : 0), n);
+    const uint32_t abits = fp4_amax_bits<T, B>(raw);
+    const float amax = fp4_widen_bits<T>(abits);
+    uint32_t byte;
+    uint32_t codes[B / 8];
+    if constexpr (FORMAT == DGXM_FP4_NVFP4) {
+      byte = bad || __float_as_uint(amax) >= 0x7F800000u ? 0x7Fu : inv6g == 0.f ? 0u : fp4_e4m3_scale(amax * up, g, inv6g);
+      const float s = fp4_scale_value<FORMAT>(byte);
+      const bool on = s > 0.f;  // false for zero and NaN
+      const float r = on ? __frcp_rn(s * g) : 0.f;
+      const float r0 = r * kBelow, r1 = r * kAbove;
+#pragma unroll
+      for (int j = 0; j < B / 8; ++j) {
+        float v[8], lo[8], hi[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = fp4_widen<T>(raw.v[8 * j + i]) * up;
+          lo[i] = v[i] * r0;
+          hi[i] = v[i] * r1;
+        }
+        uint32_t c = fp4_encode8(lo);
+        const uint32_t d = c ^ fp4_encode8(hi);
+        if (d != 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (((d >> (4 * i)) & 15u) == 0) continue;
+            const int k = (c >> (4 * i)) & 7;  // the border lies between codes k and k + 1
+            const float border = k < 4 ? 0.5f * k + 0.25f : k == 6 ? 5.f : k - 1.5f;
+            const float e = fmaf(border * s, g, -fabsf(v[i]));
+            if (e < 0.f || (e == 0.f && (k & 1))) c += 1u << (4 * i);
+          }
+        }
+        codes[j] = on ? c : 0u;
+      }
+    } else {
+      const uint32_t ab = __float_as_uint(amax);
+      const int e = static_cast<int>(ab >> 23) - 2;  // floor(log2 amax) - 2 + 127; the scale is exact, and so is x / s
+      byte = ab >= 0x7F800000u ? 0xFFu : static_cast<uint32_t>(e < 0 ? 0 : e);
+      const bool on = byte != 0xFFu;
+      const float r = on ? __uint_as_float((254u - byte) << 23) : 0.f;
+#pragma unroll
+      for (int j = 0; j < B / 8; ++j) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fp4_widen<T>(raw.v[8 * j + i]) * r;
+        const uint32_t c = fp4_encode8(v);
+        codes[j] = on ? c : 0u;
+      }
+    }
+    if (n <= 0) byte = 0u;
+    // Four blocks' scale bytes are one word of the tile.
+    const uint32_t at = threadIdx.x & 3u;
+    uint32_t word = byte << (8 * at);
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    if (live && at == 0) *reinterpret_cast<uint32_t*>(p.scales + fp4_scale_at(row, b, p.groups)) = word;
+    const int64_t off = int64_t(b) * (B / 2);
+    if (live && off < p.pitch) {
+      uint8_t* dst = p.values + row * p.pitch + off;
+      if constexpr (B == 16)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
+      else
+        *reinterpret_cast<uint4*>(dst) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    }
+  }
+}
+
+// The values that a packed tensor stands for: (code s) is exact in fp32, the
+// product with the tensor's scale is rounded once, and once more to a 16-bit
+// type.  One thread a run of 16 values.
+template <typename T, int FORMAT, bool VEC>
+__global__ void __launch_bounds__(kFp4Threads) fp4_dequantize_kernel(const __grid_constant__ Fp4Params p) {
+  constexpr int B = fp4_block(FORMAT);
+  const float g = p.scale != nullptr ? *static_cast<const float*>(p.scale) : 1.f;
+  const uint32_t step = gridDim.x * kFp4Threads;
+  for (uint64_t i0 = blockIdx.x * kFp4Threads + threadIdx.x; i0 < p.items; i0 += step) {
+    const uint32_t item = static_cast<uint32_t>(i0);
+    const uint32_t row = item / p.per_row, c16 = item - row * p.per_row;
+    const uint2 code = __ldg(reinterpret_cast<const uint2*>(p.values + row * p.pitch) + c16);
+    const float s = fp4_scale_value<FORMAT>(__ldg(p.scales + fp4_scale_at(row, c16 * 16 / B, p.groups)));
+    __half2 h[8];
+    fp4_decode8(code.x, *reinterpret_cast<__half2(*)[4]>(h));
+    fp4_decode8(code.y, *reinterpret_cast<__half2(*)[4]>(h + 4));
+    Fp4Raw<T, 16> out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __half22float2(h[i]);
+      out.v[2 * i] = static_cast<T>(f.x * s * g);
+      out.v[2 * i + 1] = static_cast<T>(f.y * s * g);
+    }
+    const int n = p.cols - static_cast<int>(c16) * 16;
+    T* dst = reinterpret_cast<T*>(const_cast<char*>(p.x)) + row * p.row_stride + int64_t(c16) * 16;
+    if (VEC && n >= 16) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(out) / 16); ++i)
+        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(&out)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i < n) dst[i] = out.v[i];
+    }
+  }
+}
+
+static int fp4_check(const dgxm_fp4_desc* d) {
+  if (d == nullptr) return fail(DGXM_ERR_INVALID, "NULL 4-bit descriptor");
+  if (d->format != DGXM_FP4_NVFP4 && d->format != DGXM_FP4_MXFP4)
+    return fail(DGXM_ERR_UNSUPPORTED, "4-bit format %d (nvfp4 or mxfp4)", d->format);
+  if (d->rows < 0 || d->cols <= 0 || d->cols > (1 << 30))
+    return fail(DGXM_ERR_INVALID, "%lld x %lld matrix", (long long)d->rows, (long long)d->cols);
+  if (d->dtype != DGXM_DTYPE_BF16 && d->dtype != DGXM_DTYPE_F16 && d->dtype != DGXM_DTYPE_F32)
+    return fail(DGXM_ERR_UNSUPPORTED, "dtype %d (bf16, f16 or f32)", d->dtype);
+  if (d->rows > 1 && d->row_stride < d->cols)
+    return fail(DGXM_ERR_INVALID, "row stride %lld below %lld columns", (long long)d->row_stride, (long long)d->cols);
+  if (d->scale_dtype != DGXM_DTYPE_BF16 && d->scale_dtype != DGXM_DTYPE_F16 && d->scale_dtype != DGXM_DTYPE_F32)
+    return fail(DGXM_ERR_UNSUPPORTED, "scale dtype %d (bf16, f16 or f32)", d->scale_dtype);
+  return DGXM_OK;
+}
+
+static int fp4_params(const dgxm_fp4_desc* d, const void* x, const void* values, const void* scales, int64_t per_row,
+                      Fp4Params* p, bool* vec) {
+  memset(p, 0, sizeof(*p));
+  const int elt = d->dtype == DGXM_DTYPE_F32 ? 4 : 2;
+  if (d->rows > 0 && (x == nullptr || values == nullptr || scales == nullptr))
+    return fail(DGXM_ERR_INVALID, "NULL matrix, values or scales");
+  if ((reinterpret_cast<uintptr_t>(values) | reinterpret_cast<uintptr_t>(scales)) % 16)
+    return fail(DGXM_ERR_INVALID, "values and scales must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(x) % elt) return fail(DGXM_ERR_INVALID, "the matrix is not aligned to its elements");
+  const int64_t items = d->rows * per_row;
+  if (per_row > 0 && (d->rows > (int64_t(1) << 31) || items > (int64_t(1) << 31) - 1))
+    return fail(DGXM_ERR_UNSUPPORTED, "%lld x %lld is more than 2^31 - 1 blocks", (long long)d->rows, (long long)d->cols);
+  *vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (d->rows == 1 || d->row_stride * elt % 16 == 0);
+  p->x = static_cast<const char*>(x);
+  p->row_stride = d->row_stride;
+  p->values = static_cast<uint8_t*>(const_cast<void*>(values));
+  p->scales = static_cast<uint8_t*>(const_cast<void*>(scales));
+  p->pitch = fp4_pitch(d->cols);
+  p->groups = fp4_groups(d->cols, d->format);
+  p->items = static_cast<uint32_t>(items);
+  p->per_row = static_cast<uint32_t>(per_row);
+  p->cols = static_cast<int>(d->cols);
+  p->scale_dtype = d->scale_dtype;
+  p->scale_value = d->scale_value;
+  return DGXM_OK;
+}
+
+static unsigned fp4_grid(uint32_t items, int per_sm) {
+  const unsigned want = (items + kFp4Threads - 1) / kFp4Threads, most = 148u * per_sm;
+  return want < 1 ? 1u : want < most ? want : most;
+}
+
+template <typename T, int FORMAT, bool VEC>
+static void fp4_launch_quantize(Fp4Params& p, bool amax, cudaStream_t st) {
+  constexpr int B = fp4_block(FORMAT);
+  if (amax) {
+    const unsigned grid = std::min<unsigned>(fp4_grid(p.items, 8), kFp4Partials);
+    p.n_partials = static_cast<int>(grid);
+    fp4_amax_kernel<T, B, VEC><<<grid, kFp4Threads, 0, st>>>(p);
+  }
+  fp4_quantize_kernel<T, FORMAT, VEC><<<fp4_grid(p.items, 8), kFp4Threads, 0, st>>>(p);
+}
+
+template <typename T, bool VEC>
+static void fp4_launch_dequantize(const Fp4Params& p, int format, cudaStream_t st) {
+  const unsigned grid = fp4_grid(p.items, 8);
+  if (format == DGXM_FP4_NVFP4) fp4_dequantize_kernel<T, DGXM_FP4_NVFP4, VEC><<<grid, kFp4Threads, 0, st>>>(p);
+  else fp4_dequantize_kernel<T, DGXM_FP4_MXFP4, VEC><<<grid, kFp4Threads, 0, st>>>(p);
+}
+
+template <typename T>
+static void fp4_quantize_typed(Fp4Params& p, int format, bool vec, bool amax, cudaStream_t st) {
+  if (format == DGXM_FP4_NVFP4)
+    vec ? fp4_launch_quantize<T, DGXM_FP4_NVFP4, true>(p, amax, st) : fp4_launch_quantize<T, DGXM_FP4_NVFP4, false>(p, amax, st);
+  else
+    vec ? fp4_launch_quantize<T, DGXM_FP4_MXFP4, true>(p, false, st) : fp4_launch_quantize<T, DGXM_FP4_MXFP4, false>(p, false, st);
+}
+
+}  // namespace dgxm
+
+extern "C" int64_t dgxm_fp4_values_bytes(int64_t rows, int64_t cols) {
+  return rows < 0 || cols <= 0 ? -1 : rows * dgxm::fp4_pitch(cols);
+}
+
+extern "C" int64_t dgxm_fp4_scales_bytes(int64_t rows, int64_t cols, int32_t format) {
+  if (rows < 0 || cols <= 0 || (format != DGXM_FP4_NVFP4 && format != DGXM_FP4_MXFP4)) return -1;
+  return (rows + 127) / 128 * dgxm::fp4_groups(cols, format) * 512;
+}
+
+extern "C" int64_t dgxm_quantize_fp4_workspace(void) { return dgxm::kFp4Partials * 4; }
+
+extern "C" int dgxm_quantize_fp4(const dgxm_fp4_desc* d, const void* x, const void* scale, void* values, void* scales,
+                                 float* scale_out, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace dgxm;
+  if (int rc = fp4_check(d)) return rc;
+  const bool nv = d->format == DGXM_FP4_NVFP4;
+  const bool amax = nv && scale == nullptr && d->scale_value == 0.f;
+  if (nv && (scale_out == nullptr || reinterpret_cast<uintptr_t>(scale_out) % 4))
+    return fail(DGXM_ERR_INVALID, "nvfp4 needs scale_out for the tensor's fp32 scale");
+  if (!nv && (scale != nullptr || d->scale_value != 0.f))
+    return fail(DGXM_ERR_INVALID, "mxfp4 has no scale for the tensor");
+  if (reinterpret_cast<uintptr_t>(scale) % (d->scale_dtype == DGXM_DTYPE_F32 ? 4 : 2))
+    return fail(DGXM_ERR_INVALID, "the given scale is not aligned to its type");
+  if (!(d->scale_value >= 0.f) || d->scale_value > 3.4e38f)
+    return fail(DGXM_ERR_INVALID, "the given scale must be finite and not negative");
+  if (amax && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 4 ||
+               workspace_bytes < dgxm_quantize_fp4_workspace()))
+    return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes,
+                (long long)dgxm_quantize_fp4_workspace());
+  if (d->rows == 0 && !nv) return DGXM_OK;  // nvfp4: the launch below still writes the scale (0 where none is given)
+  Fp4Params p;
+  bool vec = false;
+  if (int rc = fp4_params(d, x, values, scales, fp4_groups(d->cols, d->format) * 4, &p, &vec)) return rc;
+  p.scale = scale;
+  p.scale_out = scale_out;
+  p.partials = amax ? static_cast<uint32_t*>(workspace) : nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d->dtype == DGXM_DTYPE_BF16) fp4_quantize_typed<__nv_bfloat16>(p, d->format, vec, amax, st);
+  else if (d->dtype == DGXM_DTYPE_F16) fp4_quantize_typed<__half>(p, d->format, vec, amax, st);
+  else fp4_quantize_typed<float>(p, d->format, vec, amax, st);
+  DGXM_CUDA_TRY(cudaGetLastError());
+  return DGXM_OK;
+}
+
+extern "C" int dgxm_dequantize_fp4(const dgxm_fp4_desc* d, const void* values, const void* scales, const float* scale,
+                                   void* out, void* stream) {
+  using namespace dgxm;
+  if (int rc = fp4_check(d)) return rc;
+  if ((d->format == DGXM_FP4_NVFP4) != (scale != nullptr) || reinterpret_cast<uintptr_t>(scale) % 4)
+    return fail(DGXM_ERR_INVALID, "nvfp4 takes the tensor's fp32 scale, mxfp4 none");
+  if (d->rows == 0) return DGXM_OK;
+  Fp4Params p;
+  bool vec = false;
+  if (int rc = fp4_params(d, out, values, scales, (d->cols + 15) / 16, &p, &vec)) return rc;
+  p.scale = scale;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d->dtype == DGXM_DTYPE_BF16)
+    vec ? fp4_launch_dequantize<__nv_bfloat16, true>(p, d->format, st) : fp4_launch_dequantize<__nv_bfloat16, false>(p, d->format, st);
+  else if (d->dtype == DGXM_DTYPE_F16)
+    vec ? fp4_launch_dequantize<__half, true>(p, d->format, st) : fp4_launch_dequantize<__half, false>(p, d->format, st);
+  else
+    vec ? fp4_launch_dequantize<float, true>(p, d->format, st) : fp4_launch_dequantize<float, false>(p, d->format, st);
+  DGXM_CUDA_TRY(cudaGetLastError());
+  return DGXM_OK;
+}

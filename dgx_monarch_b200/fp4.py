@@ -1,0 +1,184 @@
+"""Microscaled 4-bit floating point: packed tensors, quantisation, reading
+back, and the product of two packed tensors on the tensor cores.
+
+nvfp4 (e2m1 codes, an e4m3 scale for 16 of them, one fp32 scale for the
+tensor) is the format whose activation scale the reference shares among the
+ranks of a sequence-parallel call (adapters/quant_activation_scale.py:133-142;
+shard.SharedActivationScale gives it); mxfp4 has a power of two for 32 codes.
+There is no CPU path, and no call records an autograd graph.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .ops import _dtype_code, _require_cuda
+from .qk_norm import _plan, _ptr
+
+FORMATS = {"nvfp4": _lib.FP4_NVFP4, "mxfp4": _lib.FP4_MXFP4}
+BLOCK = {"nvfp4": 16, "mxfp4": 32}
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def values_shape(rows: int, cols: int) -> tuple[int, int]:
+    """Two codes a byte, the even column in the low bits, rows of whole 16 bytes."""
+    return rows, (cols + 31) // 32 * 16
+
+
+def scales_shape(rows: int, cols: int, format: str) -> tuple[int, int, int, int, int]:
+    """(row tile, block group, r % 32, r % 128 // 32, b % 4) of row r and block b."""
+    return (rows + 127) // 128, -(-cols // (4 * BLOCK[format])), 32, 4, 4
+
+
+def _no_grad_inputs(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the 4-bit kernels record no autograd graph: call them under torch.no_grad()")
+
+
+def _check_format(format: str) -> int:
+    if format not in FORMATS:
+        raise ValueError(f"format {format!r} is not one of {sorted(FORMATS)}")
+    return FORMATS[format]
+
+
+class Fp4Tensor:
+    """A (..., cols) tensor in 4 bits, its leading dimensions folded into rows.
+
+    values: uint8 of values_shape, zero past the last column; scales: uint8 of
+    scales_shape, zero past a row's last block (bytes of rows past the last are not
+    read); scale: the fp32 scale of an nvfp4 tensor (one element on the device),
+    None for mxfp4.  quantize_fp4 makes them; a weight kept in this layout is
+    wrapped as it is."""
+
+    __slots__ = ("values", "scales", "shape", "format", "scale", "rows", "cols")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape, format: str,
+                 scale: torch.Tensor | None = None) -> None:
+        _check_format(format)
+        shape = tuple(shape)
+        if not shape or shape[-1] < 1 or min(shape) < 0:
+            raise ValueError(f"shape {shape} has no columns")
+        rows, cols = math.prod(shape[:-1]), shape[-1]
+        if values.shape != values_shape(rows, cols) or values.dtype != torch.uint8 or not values.is_contiguous():
+            raise ValueError(f"values {tuple(values.shape)} {values.dtype} is not a contiguous uint8 "
+                             f"{values_shape(rows, cols)} tensor")
+        if (scales.shape != scales_shape(rows, cols, format) or scales.dtype != torch.uint8
+                or not scales.is_contiguous()):
+            raise ValueError(f"scales {tuple(scales.shape)} {scales.dtype} is not a contiguous uint8 "
+                             f"{scales_shape(rows, cols, format)} tensor")
+        if (scale is None) != (format == "mxfp4") or (scale is not None and (
+                scale.dtype != torch.float32 or scale.numel() != 1)):
+            raise ValueError("an nvfp4 tensor has one fp32 scale, an mxfp4 tensor none")
+        self.values, self.scales, self.shape, self.format, self.scale = values, scales, shape, format, scale
+        self.rows, self.cols = rows, cols
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+    def __repr__(self) -> str:
+        return f"Fp4Tensor({self.shape}, {self.format}, {self.device})"
+
+
+def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor | float | None = None,
+                 out: Fp4Tensor | None = None) -> Fp4Tensor:
+    """x (..., cols) bf16, fp16 or fp32 with contiguous columns, in 4 bits
+    (dgxm_quantize_fp4).  Leading dimensions that do not fold into one stride
+    are copied first.
+
+    scale (nvfp4 only): the tensor's scale g as one element of fp32, bf16 or
+    fp16 on x's device (what shard.SharedActivationScale returns) or as a
+    positive float; None takes amax / 2688 over x, in which a NaN or an
+    infinity makes every value NaN.  Block scales are e4m3(amax / (6 g)), codes
+    e2m1(x / (s g)); mxfp4: 2^(floor(log2 amax) - 2) and e2m1(x / s).  Every
+    rounding is of the real quotient to the nearest, ties to even, saturating;
+    a block with a NaN or an infinity reads back as NaN, and so does everything
+    under a given g that is NaN, infinite or negative.
+
+    out: an Fp4Tensor of x's shape and the format to write into, its scale
+    included."""
+    given = scale if isinstance(scale, torch.Tensor) else None
+    key = ("q", x.shape, x.stride(), x.dtype, x.device, format,
+           scale if given is None else (given.dtype, given.device, given.numel()),
+           None if out is None else (out.shape, out.format, out.device))
+
+    def make():
+        code = _check_format(format)
+        _require_cuda(x, given)
+        if x.dtype not in _FLOATS:
+            raise TypeError(f"x is {x.dtype}: 4-bit quantisation takes bf16, fp16 or fp32")
+        if x.ndim < 1 or x.shape[-1] < 1:
+            raise ValueError(f"x {tuple(x.shape)} has no columns")
+        if x.stride(-1) != 1 and x.shape[-1] > 1:
+            raise ValueError("x must have contiguous columns")
+        if scale is not None and format == "mxfp4":
+            raise ValueError("mxfp4 has no scale for the tensor")
+        if given is not None and (given.dtype not in _FLOATS or given.numel() != 1):
+            raise ValueError(f"scale {tuple(given.shape)} {given.dtype} is not one element of fp32, bf16 or fp16")
+        if scale is not None and given is None and not (0.0 < scale < 3.4e38):
+            raise ValueError(f"scale {scale} is not a positive finite number")
+        if out is not None:
+            if out.shape != tuple(x.shape) or out.format != format:
+                raise ValueError(f"out is {out}, x is {tuple(x.shape)} for {format}")
+            _require_cuda(x, out.values, out.scales, out.scale)
+        desc = _lib.Fp4Desc()
+        desc.rows, desc.cols, desc.format = math.prod(x.shape[:-1]), x.shape[-1], code
+        desc.dtype = _dtype_code(x.dtype)
+        desc.scale_dtype = _lib.DTYPE_F32 if given is None else _dtype_code(given.dtype)
+        desc.scale_value = 0.0 if given is not None or scale is None else scale
+        if scale is not None and given is None and desc.scale_value == 0.0:
+            raise ValueError(f"scale {scale} is zero in fp32")
+        flat = x.reshape(-1, x.shape[-1]) if x.numel() else x
+        folds = x.numel() == 0 or (flat.data_ptr() == x.data_ptr()
+                                   and (desc.rows == 1 or flat.stride(0) >= desc.cols))  # not overlapping or expanded
+        desc.row_stride = flat.stride(0) if folds and desc.rows > 1 else desc.cols
+        return (desc, folds, values_shape(desc.rows, desc.cols),
+                scales_shape(desc.rows, desc.cols, format),
+                _lib.load().dgxm_quantize_fp4_workspace() if format == "nvfp4" and scale is None else 0)
+
+    desc, folds, vshape, sshape, need = _plan(key, make)
+    _no_grad_inputs(x, given)
+    if not folds:
+        x = x.reshape(-1, x.shape[-1]).contiguous()
+    dev = x.device
+    if out is None:
+        shape = key[1]
+        out = Fp4Tensor(torch.empty(vshape, device=dev, dtype=torch.uint8),
+                        torch.empty(sshape, device=dev, dtype=torch.uint8), shape, format,
+                        torch.empty((), device=dev, dtype=torch.float32) if format == "nvfp4" else None)
+    work = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    with torch.cuda.device(dev):
+        rc = _lib.load().dgxm_quantize_fp4(desc, x.data_ptr(), _ptr(given), out.values.data_ptr(),
+                                           out.scales.data_ptr(), _ptr(out.scale), _ptr(work), need,
+                                           torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "dgxm_quantize_fp4")
+    return out
+
+
+def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values that t stands for, in t.shape and dtype (dgxm_dequantize_fp4):
+    code * block scale * scale in fp32, then rounded to dtype.  out: a
+    contiguous tensor to write into."""
+    dev = _require_cuda(t.values, t.scales, t.scale, out)
+    if dtype not in _FLOATS:
+        raise TypeError(f"dtype {dtype} is not bf16, fp16 or fp32")
+    if out is None:
+        out = torch.empty(t.shape, device=dev, dtype=dtype)
+    elif tuple(out.shape) != t.shape or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not a contiguous {t.shape} {dtype} tensor")
+
+    def make():
+        desc = _lib.Fp4Desc()
+        desc.rows, desc.cols, desc.row_stride, desc.format = t.rows, t.cols, t.cols, FORMATS[t.format]
+        desc.dtype, desc.scale_dtype = _dtype_code(dtype), _lib.DTYPE_F32
+        return desc
+
+    desc = _plan(("d", t.rows, t.cols, t.format, dtype), make)
+    with torch.cuda.device(dev):
+        rc = _lib.load().dgxm_dequantize_fp4(desc, t.values.data_ptr(), t.scales.data_ptr(), _ptr(t.scale),
+                                             out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "dgxm_dequantize_fp4")
+    return out

@@ -670,6 +670,56 @@ int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* desc, const void* dq, co
                                void* g_norm_q_w, void* g_norm_k_w, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------ microscaled 4-bit floats */
+/*
+ * (rows, cols) matrices of e2m1 codes with one scale for a block of columns:
+ *   DGXM_FP4_NVFP4  blocks of 16, e4m3 scales, one fp32 scale for the tensor;
+ *   DGXM_FP4_MXFP4  blocks of 32, e8m0 scales (2^(byte - 127)).
+ * values: rows of ceil(cols / 32) * 16 bytes, two codes a byte, the even
+ * column in the low bits, zero past the last column.  scales: one byte a
+ * block, in tiles of 128 rows x 4 blocks (512 bytes; a row of tiles holds
+ * ceil(cols / (4 block)) of them), row r and block b of a tile at
+ * (r % 32) * 16 + (r / 32) * 4 + b; bytes past the last block of a row are
+ * zero, those of rows past the last are not read.  Both 16-byte aligned.
+ */
+#define DGXM_FP4_NVFP4 0
+#define DGXM_FP4_MXFP4 1
+
+typedef struct dgxm_fp4_desc {
+  int64_t rows, cols;
+  int64_t row_stride;    /* of the unpacked matrix, elements; columns are contiguous */
+  int32_t format;
+  int32_t dtype;         /* of the unpacked matrix: BF16, F16 or F32 */
+  int32_t scale_dtype;   /* of a scale given in device memory: F32, BF16 or F16 */
+  float scale_value;     /* a scale given by value; 0: none */
+} dgxm_fp4_desc;
+
+int64_t dgxm_fp4_values_bytes(int64_t rows, int64_t cols);
+int64_t dgxm_fp4_scales_bytes(int64_t rows, int64_t cols, int32_t format);
+
+/*
+ * Quantise.  nvfp4: the tensor's scale g is read from `scale` (device memory,
+ * scale_dtype; what dgxm_shared_amax_scale writes), or is scale_value, or
+ * amax / 2688 over the matrix (`workspace` then holds
+ * dgxm_quantize_fp4_workspace() bytes); it is written to scale_out as fp32.
+ * Block scales are e4m3(amax / (6 g)), codes e2m1(x / (s g)); mxfp4:
+ * 2^(floor(log2 amax) - 2) and e2m1(x / s).  Every rounding is of the real
+ * quotient to the nearest, ties to even, saturating.  A block with a NaN or
+ * an infinity, and every block under a NaN, infinite or negative g, gets the
+ * NaN scale; g = 0 gives zeros.
+ *
+ * Serves the NVFP4 Linear inputs whose shared scale
+ * adapters/quant_activation_scale.py:133-142 reduces.
+ */
+int64_t dgxm_quantize_fp4_workspace(void);
+int dgxm_quantize_fp4(const dgxm_fp4_desc* desc, const void* x, const void* scale, void* values,
+                      void* scales, float* scale_out, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* The values that a packed matrix stands for, in dtype: code * s * g. */
+int dgxm_dequantize_fp4(const dgxm_fp4_desc* desc, const void* values, const void* scales,
+                        const float* scale, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
