@@ -221,6 +221,19 @@ class Fp4Desc(ctypes.Structure):
     ]
 
 
+class Fp4GemmDesc(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("format", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # Every symbol include/dgxm_sp.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -295,6 +308,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dgxm_quantize_fp4_workspace": (ctypes.c_int64, []),
     "dgxm_quantize_fp4": (ctypes.c_int, [ctypes.POINTER(Fp4Desc), _P, _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
     "dgxm_dequantize_fp4": (ctypes.c_int, [ctypes.POINTER(Fp4Desc), _P, _P, _P, _P, _P]),
+    "dgxm_fp4_matmul": (ctypes.c_int, [ctypes.POINTER(Fp4GemmDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -18,3 +18,4 @@
 #include "prologue.cu"
 #include "qk_norm.cu"
 #include "fp4_quant.cu"
+#include "fp4_gemm.cu"

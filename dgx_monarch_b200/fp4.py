@@ -182,3 +182,58 @@ def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
                                              out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, "dgxm_dequantize_fp4")
     return out
+
+
+def fp4_matmul(a: Fp4Tensor, b: Fp4Tensor, *, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """a (..., k) times the transpose of b (n, k), a Linear's forward
+    (dgxm_fp4_matmul): (..., n) in out_dtype (bf16, fp16 or fp32).
+
+    Both operands have one format and share k; bias: (n,) in any of the three
+    types.  fp32 accumulation on the block-scaled tensor cores, one rounding.
+    out: a tensor of the result's shape and out_dtype to write into, with
+    contiguous columns and rows that fold into one stride."""
+    key = ("m", a.rows, a.cols, a.shape, a.format, a.device, b.rows, b.cols, b.format, b.device, out_dtype,
+           None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.device),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+
+    def make():
+        _require_cuda(a.values, a.scales, a.scale, b.values, b.scales, b.scale, bias, out)
+        if a.format != b.format:
+            raise ValueError(f"a product of {a.format} and {b.format}: both operands have one format")
+        if a.cols != b.cols:
+            raise ValueError(f"a has {a.cols} columns, b {b.cols}")
+        if out_dtype not in _FLOATS:
+            raise TypeError(f"out_dtype {out_dtype} is not bf16, fp16 or fp32")
+        shape = (*a.shape[:-1], b.rows)
+        desc = _lib.Fp4GemmDesc()
+        desc.m, desc.n, desc.k, desc.out_stride, desc.format = a.rows, b.rows, a.cols, b.rows, FORMATS[a.format]
+        desc.out_dtype = desc.bias_dtype = _dtype_code(out_dtype)
+        if bias is not None:
+            if bias.dtype not in _FLOATS or tuple(bias.shape) != (b.rows,) or not bias.is_contiguous():
+                raise ValueError(f"bias {tuple(bias.shape)} {bias.dtype} is not a contiguous ({b.rows},) vector of "
+                                 "bf16, fp16 or fp32")
+            desc.bias_dtype = _dtype_code(bias.dtype)
+        if out is not None:
+            if tuple(out.shape) != shape or out.dtype != out_dtype:
+                raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not a {shape} {out_dtype} tensor")
+            if out.numel():
+                flat = out.reshape(-1, b.rows)
+                if (flat.data_ptr() != out.data_ptr() or (b.rows > 1 and flat.stride(1) != 1)
+                        or (a.rows > 1 and flat.stride(0) < b.rows)):
+                    raise ValueError("out must have contiguous columns and rows that fold into one stride")
+                if a.rows > 1:
+                    desc.out_stride = flat.stride(0)
+        return desc, shape
+
+    desc, shape = _plan(key, make)
+    _no_grad_inputs(bias)
+    dev = a.device
+    if out is None:
+        out = torch.empty(shape, device=dev, dtype=out_dtype)
+    with torch.cuda.device(dev):
+        rc = _lib.load().dgxm_fp4_matmul(desc, a.values.data_ptr(), a.scales.data_ptr(), _ptr(a.scale),
+                                         b.values.data_ptr(), b.scales.data_ptr(), _ptr(b.scale), _ptr(bias),
+                                         out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "dgxm_fp4_matmul")
+    return out

@@ -720,6 +720,29 @@ int dgxm_quantize_fp4(const dgxm_fp4_desc* desc, const void* x, const void* scal
 int dgxm_dequantize_fp4(const dgxm_fp4_desc* desc, const void* values, const void* scales,
                         const float* scale, void* out, void* stream);
 
+/*
+ * out[i, j] = g_a g_b sum_k a[i, k] b[j, k] + bias[j] over two packed
+ * matrices of one format, (m, k) and (n, k): block-scaled tcgen05 products,
+ * fp32 accumulation, one rounding to out_dtype.  a_scale / b_scale: the
+ * tensors' fp32 scales (nvfp4; NULL for mxfp4).  bias: n values of bias_dtype,
+ * or NULL.  The same call gives the same bits.
+ *
+ * Serves the NVFP4 Linear itself, whose activation scale the reference's
+ * shared_activation_scale feeds (adapters/quant_activation_scale.py:222-246).
+ */
+typedef struct dgxm_fp4_gemm_desc {
+  int64_t m, n, k;
+  int64_t out_stride;    /* elements between output rows; columns are contiguous */
+  int32_t format;
+  int32_t out_dtype;     /* BF16, F16 or F32 */
+  int32_t bias_dtype;
+  int32_t reserved;      /* 0 */
+} dgxm_fp4_gemm_desc;
+
+int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* desc, const void* a_values, const void* a_scales,
+                    const float* a_scale, const void* b_values, const void* b_scales,
+                    const float* b_scale, const void* bias, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
