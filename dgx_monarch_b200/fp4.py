@@ -14,8 +14,8 @@ import math
 import torch
 
 from . import _lib
-from .ops import _dtype_code, _require_cuda
-from .qk_norm import _plan, _ptr
+from ._call import launch, no_graph, plan
+from .ops import _dtype_code, _ptr, _require_cuda
 
 FORMATS = {"nvfp4": _lib.FP4_NVFP4, "mxfp4": _lib.FP4_MXFP4}
 BLOCK = {"nvfp4": 16, "mxfp4": 32}
@@ -30,11 +30,6 @@ def values_shape(rows: int, cols: int) -> tuple[int, int]:
 def scales_shape(rows: int, cols: int, format: str) -> tuple[int, int, int, int, int]:
     """(row tile, block group, r % 32, r % 128 // 32, b % 4) of row r and block b."""
     return (rows + 127) // 128, -(-cols // (4 * BLOCK[format])), 32, 4, 4
-
-
-def _no_grad_inputs(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the 4-bit kernels record no autograd graph: call them under torch.no_grad()")
 
 
 def _check_format(format: str) -> int:
@@ -74,9 +69,20 @@ class Fp4Tensor:
         self.values, self.scales, self.shape, self.format, self.scale = values, scales, shape, format, scale
         self.rows, self.cols = rows, cols
 
+    @classmethod
+    def _made(cls, values, scales, shape, format, scale, rows, cols) -> "Fp4Tensor":
+        """Of buffers that this module has just allocated."""
+        t = cls.__new__(cls)
+        t.values, t.scales, t.shape, t.format, t.scale, t.rows, t.cols = values, scales, shape, format, scale, rows, cols
+        return t
+
     @property
     def device(self) -> torch.device:
         return self.values.device
+
+    def _devices(self):
+        return (self.values.get_device(), self.scales.get_device(),
+                None if self.scale is None else self.scale.get_device())
 
     def __repr__(self) -> str:
         return f"Fp4Tensor({self.shape}, {self.format}, {self.device})"
@@ -100,9 +106,9 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
     out: an Fp4Tensor of x's shape and the format to write into, its scale
     included."""
     given = scale if isinstance(scale, torch.Tensor) else None
-    key = ("q", x.shape, x.stride(), x.dtype, x.device, format,
-           scale if given is None else (given.dtype, given.device, given.numel()),
-           None if out is None else (out.shape, out.format, out.device))
+    key = ("q", x.shape, x.stride(), x.dtype, x.get_device(), format,
+           scale if given is None else (given.dtype, given.get_device(), given.numel()),
+           None if out is None else (out.shape, out.format, out._devices()))
 
     def make():
         code = _check_format(format)
@@ -134,26 +140,21 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
         folds = x.numel() == 0 or (flat.data_ptr() == x.data_ptr()
                                    and (desc.rows == 1 or flat.stride(0) >= desc.cols))  # not overlapping or expanded
         desc.row_stride = flat.stride(0) if folds and desc.rows > 1 else desc.cols
-        return (desc, folds, values_shape(desc.rows, desc.cols),
-                scales_shape(desc.rows, desc.cols, format),
-                _lib.load().dgxm_quantize_fp4_workspace() if format == "nvfp4" and scale is None else 0)
+        shape = tuple(x.shape)
+        return (desc, folds, values_shape(desc.rows, desc.cols), scales_shape(desc.rows, desc.cols, format), shape,
+                _lib.load().dgxm_quantize_fp4_workspace() if format == "nvfp4" and scale is None else 0,
+                math.prod(shape[:-1]), shape[-1])
 
-    desc, folds, vshape, sshape, need = _plan(key, make)
-    _no_grad_inputs(x, given)
+    desc, folds, vshape, sshape, shape, need, rows, cols = plan(key, make)
+    no_graph("", x, given)
     if not folds:
-        x = x.reshape(-1, x.shape[-1]).contiguous()
-    dev = x.device
+        x = x.reshape(-1, cols).contiguous()
     if out is None:
-        shape = key[1]
-        out = Fp4Tensor(torch.empty(vshape, device=dev, dtype=torch.uint8),
-                        torch.empty(sshape, device=dev, dtype=torch.uint8), shape, format,
-                        torch.empty((), device=dev, dtype=torch.float32) if format == "nvfp4" else None)
-    work = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-    with torch.cuda.device(dev):
-        rc = _lib.load().dgxm_quantize_fp4(desc, x.data_ptr(), _ptr(given), out.values.data_ptr(),
-                                           out.scales.data_ptr(), _ptr(out.scale), _ptr(work), need,
-                                           torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "dgxm_quantize_fp4")
+        out = Fp4Tensor._made(x.new_empty(vshape, dtype=torch.uint8), x.new_empty(sshape, dtype=torch.uint8), shape,
+                              format, x.new_empty((), dtype=torch.float32) if format == "nvfp4" else None, rows, cols)
+    work = x.new_empty(need, dtype=torch.uint8) if need else None
+    launch("dgxm_quantize_fp4", x.get_device(), desc, x.data_ptr(), _ptr(given), out.values.data_ptr(),
+           out.scales.data_ptr(), _ptr(out.scale), _ptr(work), need)
     return out
 
 
@@ -162,25 +163,28 @@ def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
     """The values that t stands for, in t.shape and dtype (dgxm_dequantize_fp4):
     code * block scale * scale in fp32, then rounded to dtype.  out: a
     contiguous tensor to write into."""
-    dev = _require_cuda(t.values, t.scales, t.scale, out)
-    if dtype not in _FLOATS:
-        raise TypeError(f"dtype {dtype} is not bf16, fp16 or fp32")
-    if out is None:
-        out = torch.empty(t.shape, device=dev, dtype=dtype)
-    elif tuple(out.shape) != t.shape or out.dtype != dtype or not out.is_contiguous():
-        raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not a contiguous {t.shape} {dtype} tensor")
+    key = ("d", t.rows, t.cols, t.format, dtype, t._devices(),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
 
     def make():
+        _require_cuda(t.values, t.scales, t.scale, out)
+        if dtype not in _FLOATS:
+            raise TypeError(f"dtype {dtype} is not bf16, fp16 or fp32")
+        if out is not None and (math.prod(out.shape) != t.rows * t.cols or out.dtype != dtype
+                                or not out.is_contiguous()):
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not a contiguous {t.shape} {dtype} tensor")
         desc = _lib.Fp4Desc()
         desc.rows, desc.cols, desc.row_stride, desc.format = t.rows, t.cols, t.cols, FORMATS[t.format]
         desc.dtype, desc.scale_dtype = _dtype_code(dtype), _lib.DTYPE_F32
         return desc
 
-    desc = _plan(("d", t.rows, t.cols, t.format, dtype), make)
-    with torch.cuda.device(dev):
-        rc = _lib.load().dgxm_dequantize_fp4(desc, t.values.data_ptr(), t.scales.data_ptr(), _ptr(t.scale),
-                                             out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "dgxm_dequantize_fp4")
+    desc = plan(key, make)
+    if out is None:
+        out = t.values.new_empty(t.shape, dtype=dtype)
+    elif out.shape != t.shape:
+        raise ValueError(f"out {tuple(out.shape)} is not a {t.shape} tensor")
+    launch("dgxm_dequantize_fp4", t.values.get_device(), desc, t.values.data_ptr(), t.scales.data_ptr(),
+           _ptr(t.scale), out.data_ptr())
     return out
 
 
@@ -193,9 +197,9 @@ def fp4_matmul(a: Fp4Tensor, b: Fp4Tensor, *, bias: torch.Tensor | None = None,
     types.  fp32 accumulation on the block-scaled tensor cores, one rounding.
     out: a tensor of the result's shape and out_dtype to write into, with
     contiguous columns and rows that fold into one stride."""
-    key = ("m", a.rows, a.cols, a.shape, a.format, a.device, b.rows, b.cols, b.format, b.device, out_dtype,
-           None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.device),
-           None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+    key = ("m", a.shape, a.format, a._devices(), b.shape, b.format, b._devices(), out_dtype,
+           None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.get_device()),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
 
     def make():
         _require_cuda(a.values, a.scales, a.scale, b.values, b.scales, b.scale, bias, out)
@@ -226,14 +230,10 @@ def fp4_matmul(a: Fp4Tensor, b: Fp4Tensor, *, bias: torch.Tensor | None = None,
                     desc.out_stride = flat.stride(0)
         return desc, shape
 
-    desc, shape = _plan(key, make)
-    _no_grad_inputs(bias)
-    dev = a.device
+    desc, shape = plan(key, make)
+    no_graph("", bias)
     if out is None:
-        out = torch.empty(shape, device=dev, dtype=out_dtype)
-    with torch.cuda.device(dev):
-        rc = _lib.load().dgxm_fp4_matmul(desc, a.values.data_ptr(), a.scales.data_ptr(), _ptr(a.scale),
-                                         b.values.data_ptr(), b.scales.data_ptr(), _ptr(b.scale), _ptr(bias),
-                                         out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "dgxm_fp4_matmul")
+        out = a.values.new_empty(shape, dtype=out_dtype)
+    launch("dgxm_fp4_matmul", a.values.get_device(), desc, a.values.data_ptr(), a.scales.data_ptr(), _ptr(a.scale),
+           b.values.data_ptr(), b.scales.data_ptr(), _ptr(b.scale), _ptr(bias), out.data_ptr())
     return out

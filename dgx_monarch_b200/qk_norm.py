@@ -10,20 +10,14 @@ trained.  There is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .ops import _dtype_code, _require_cuda
+from ._call import launch, no_graph, plan
+from .ops import _dtype_code, _ptr, _require_cuda
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
-
-
-def _no_graph(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the B200 kernels record no autograd graph: call them under torch.no_grad() and take "
-                           "the gradients from qk_norm_rope_backward")
+_GRADS = " and take the gradients from qk_norm_rope_backward"
 
 
 def _check_rows(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
@@ -43,6 +37,11 @@ def _check_out(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
                          "contiguous head_dim")
     if t.numel() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{name} is an expanded tensor: its rows share memory")
+
+
+def _check_in_place(name: str, out: torch.Tensor, src: torch.Tensor) -> None:
+    if out.data_ptr() == src.data_ptr() and out.stride() != src.stride() and src.numel():
+        raise ValueError(f"{name} shares its input's memory with other strides")
 
 
 def _describe(q, k, norm_mode, wq, wk, eps, rope, rope_halves) -> _lib.QkNormDesc:
@@ -88,23 +87,7 @@ def _describe(q, k, norm_mode, wq, wk, eps, rope, rope_halves) -> _lib.QkNormDes
 
 def _meta(t: torch.Tensor | None):
     """What the checks and the descriptor of a call read of a tensor."""
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-
-
-_PLANS: dict = {}  # checked descriptors by the tensors' sizes, strides, types and devices: no data, no address
-
-
-def _plan(key, make):
-    found = _PLANS.get(key)
-    if found is None:
-        if len(_PLANS) > 256:
-            _PLANS.clear()
-        found = _PLANS[key] = make()
-    return found
-
-
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: int = _lib.NORM_HEAD,
@@ -142,22 +125,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
                 stride[:] = [src.shape[1] * h * d, h * d, d]
         return desc
 
-    desc = _plan(key, make)
-    _no_graph(q, k, norm_q_w, norm_k_w)
-    if q_out is not None and q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride() and q.numel():
-        raise ValueError("q_out shares q's memory with other strides")
-    if k_out is not None and k_out.data_ptr() == k.data_ptr() and k_out.stride() != k.stride() and k.numel():
-        raise ValueError("k_out shares k's memory with other strides")
-    dev = q.device
+    desc = plan(key, make)
+    no_graph(_GRADS, q, k, norm_q_w, norm_k_w)
     if q_out is None:
-        q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    if k_out is None and k is not None:
-        k_out = torch.empty(k.shape, device=dev, dtype=k.dtype)
-    with torch.cuda.device(dev):
-        rc = _lib.load().dgxm_qk_norm_rope(desc, q.data_ptr(), _ptr(k), _ptr(norm_q_w), _ptr(norm_k_w), _ptr(rope),
-                                           q_out.data_ptr(), _ptr(k_out),
-                                           torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "dgxm_qk_norm_rope")
+        q_out = q.new_empty(q.shape)
+    else:
+        _check_in_place("q_out", q_out, q)
+    if k is not None:
+        if k_out is None:
+            k_out = k.new_empty(k.shape)
+        else:
+            _check_in_place("k_out", k_out, k)
+    launch("dgxm_qk_norm_rope", q.get_device(), desc, q.data_ptr(), _ptr(k), _ptr(norm_q_w), _ptr(norm_k_w),
+           _ptr(rope), q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
@@ -197,18 +177,14 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
             _lib.check(_lib.DGXM_ERR_INVALID, "dgxm_qk_norm_rope_backward_workspace")
         return desc, need
 
-    desc, need = _plan(key, make)
-    _no_graph(dq, dk, q, k, norm_q_w, norm_k_w)
-    dev = q.device
-    gq = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    gk = None if k is None else torch.empty(k.shape, device=dev, dtype=k.dtype)
+    desc, need = plan(key, make)
+    no_graph(_GRADS, dq, dk, q, k, norm_q_w, norm_k_w)
+    gq = q.new_empty(q.shape)
+    gk = None if k is None else k.new_empty(k.shape)
     gwq = None if norm_q_w is None else torch.empty_like(norm_q_w)
     gwk = None if norm_k_w is None else torch.empty_like(norm_k_w)
-    work = None if gwq is None else torch.empty(need, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        rc = _lib.load().dgxm_qk_norm_rope_backward(
-            desc, dq.data_ptr(), _ptr(dk), q.data_ptr(), _ptr(k), _ptr(norm_q_w), _ptr(norm_k_w), _ptr(rope),
-            gq.data_ptr(), _ptr(gk), _ptr(gwq), _ptr(gwk), _ptr(work), need if work is not None else 0,
-            torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "dgxm_qk_norm_rope_backward")
+    work = None if gwq is None else q.new_empty(need, dtype=torch.uint8)
+    launch("dgxm_qk_norm_rope_backward", q.get_device(), desc, dq.data_ptr(), _ptr(dk), q.data_ptr(), _ptr(k),
+           _ptr(norm_q_w), _ptr(norm_k_w), _ptr(rope), gq.data_ptr(), _ptr(gk), _ptr(gwq), _ptr(gwk), _ptr(work),
+           need if work is not None else 0)
     return gq, gk, gwq, gwk

@@ -125,6 +125,6 @@ def test_output_and_gradient_checks():
         qk_norm._check_out("q_out", torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16).expand(1, 4, 2, 64), like)
     w = torch.zeros(3, requires_grad=True)
     with pytest.raises(RuntimeError, match="no_grad"):
-        qk_norm._no_graph(w)
+        qk_norm.no_graph("", None, w)
     with torch.no_grad():
-        qk_norm._no_graph(w)
+        qk_norm.no_graph("", None, w)
