@@ -7,13 +7,17 @@
 //   dx = r (g w - n mean(g w n)).
 //
 // Both directions move each value once and compute a handful of operations
-// on it, so DRAM bounds them.  A head row is held by a group of 8, 16 or 32
-// lanes, eight values a lane (16 bytes of a 16-bit type), so a warp reads and
-// writes whole 32-byte sectors whatever the strides, the sums of a row are
-// shuffles within the group, and a row stays in registers between its load
-// and its store.  One warp takes several heads of one token: the token's
-// cosines and sines and the head weight are loaded once for all of them, and
-// the loads of kFwdRows (kBwdRows) rows are in flight together.
+// on it, so DRAM bounds them as long as the instructions stay few and enough
+// loads are under way.  A head row is held by a group of 8, 16 or 32 lanes,
+// eight values a lane (16 bytes of a 16-bit type), so a warp reads and writes
+// whole 32-byte sectors whatever the strides, and the sums of a row are
+// shuffles within the group.  One warp takes a chunk of the heads of one
+// token and tensor.  It sends for all their rows at once, by cp.async into
+// shared memory, where each lane finds its own values (and the halves order
+// its partners) again: loads in flight cost no registers, and the token's
+// cosines and sines and the head weight, which serve every row of the chunk,
+// are fetched and multiplied with one another meanwhile.  The arithmetic runs
+// on pairs of fp32, two rows at a time.
 //
 // Everything between the load and the store is fp32 and is rounded once, to
 // the tensors' type.  (The fused scatter of prologue.cu rounds after the
@@ -23,10 +27,24 @@
 
 namespace dgxm {
 
-constexpr int kQkThreads = 256;
+// The rotation's order; kQkHalvesOff: halves that are no whole number of a
+// lane's eight values.
+constexpr int kQkNoTurn = 0, kQkAdjacent = 1, kQkHalves = 2, kQkHalvesOff = 3;
+
+constexpr int kQkThreads = 128;
 constexpr int kQkWarps = kQkThreads / 32;
-constexpr int kFwdRows = 4;  // rows of a lane group in flight, forward
-constexpr int kBwdRows = 2;  // backward: two tensors are read for each row
+constexpr int kQkRing = 4096;     // bytes of rows a warp has under way, of each tensor it reads
+constexpr int kQkFwdPerSm = 8;    // blocks of an SM: 64 registers a thread, 128 KB of rows under way
+constexpr int kQkBwdPerSm = 6;    // 80 registers a thread, 192 KB
+constexpr int kQkBwdBlocks = 148 * kQkBwdPerSm;  // as many as run at one time, each with one partial sum of dw
+
+// Rows a lane group has under way.
+template <typename T>
+constexpr int kQkRows = kQkRing / (32 * 8 * static_cast<int>(sizeof(T)));
+
+static_assert(kQkRows<float> % 2 == 0 && kQkRows<__half> % 2 == 0, "rows go in twos");
+static_assert(kQkWarps * 2 * kQkRing <= 48 * 1024, "dynamic shared memory without an opt-in");
+static_assert(2 * kQkRing >= 1024, "the warps' sums fit");
 
 struct QkNormParams {
   // [0] q, [1] k; strides in elements: batch, row, head
@@ -39,8 +57,9 @@ struct QkNormParams {
   int64_t rope_sb;    // floats between batch items (0: shared)
   float* partial;     // backward: (grid, 2, head_dim) sums of g n, or NULL
   int heads[2], chunks[2];  // chunks: warps for one token's heads of the tensor
-  uint32_t seq, items;      // items: batch * seq * (chunks of q + chunks of k)
-  int dim, rot, halves, norm, w_f32, rope_vec;
+  uint32_t seq, tokens;     // tokens: batch * seq
+  int rows;                 // rows of a chunk for each lane group of its warp
+  int dim, rot, halves, norm, w_f32, rope_vec, w_vec;
   float eps, inv_dim;
 };
 
@@ -62,34 +81,78 @@ __device__ __forceinline__ __half qk_narrow(float v) { return __float2half_rn(v)
 template <>
 __device__ __forceinline__ float qk_narrow(float v) { return v; }
 
-// Eight values as they lie in memory.  VEC: 16-byte accesses (base and every
-// stride a multiple of 16 bytes); otherwise one access a value.
+// Eight values as they lie in memory.
 template <typename T>
 struct __align__(16) Qk8 {
   T v[8];
 };
 
+// A warp's rows in shared memory: row u of every lane group, 16-byte pieces
+// of 32 lanes side by side (one piece a lane for a 16-bit type, two for fp32).
+template <typename T>
+__device__ __forceinline__ uint8_t* qk_slot(uint8_t* ring, int u, int lane, int piece) {
+  constexpr int kPieces = static_cast<int>(sizeof(T)) / 2;
+  return ring + ((u * kPieces + piece) * 32 + lane) * 16;
+}
+
+// Send for a lane's values of row u.  VEC: 16-byte accesses (base and every
+// stride a multiple of 16 bytes); otherwise one access a value.
 template <typename T, bool VEC>
-__device__ __forceinline__ Qk8<T> qk_load(const char* base, int64_t elem) {
-  Qk8<T> r;
+__device__ __forceinline__ void qk_fetch(uint8_t* ring, int u, int lane, const char* base, int64_t elem) {
   const T* p = reinterpret_cast<const T*>(base) + elem;
-  if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i)
-      reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    if constexpr (VEC) {
+      cp_async16(smem_u32(qk_slot<T>(ring, u, lane, i)), reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      constexpr int kEach = 16 / static_cast<int>(sizeof(T));
+      T* dst = reinterpret_cast<T*>(qk_slot<T>(ring, u, lane, i));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = p[i];
+      for (int k = 0; k < kEach; ++k) dst[k] = p[i * kEach + k];
+    }
   }
+}
+
+// All the chunk's rows of a lane; lanes past head_dim hold zeros (qk_blank).
+template <typename T, bool VEC>
+__device__ __forceinline__ void qk_fetch_rows(uint8_t* ring, int lane, const char* base, int64_t at, int64_t step,
+                                              int n) {
+#pragma unroll 4
+  for (int u = 0; u < n; ++u, at += step) qk_fetch<T, VEC>(ring, u, lane, base, at);
+}
+
+template <typename T>
+__device__ __forceinline__ void qk_blank_row(uint8_t* ring, int u, int lane) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    *reinterpret_cast<uint4*>(qk_slot<T>(ring, u, lane, i)) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+template <typename T>
+__device__ __forceinline__ void qk_blank(uint8_t* ring, int lane) {
+  for (int u = 0; u < kQkRows<T>; ++u) qk_blank_row<T>(ring, u, lane);
+}
+
+template <typename T>
+__device__ __forceinline__ Qk8<T> qk_take(uint8_t* ring, int u, int lane) {
+  Qk8<T> r;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    reinterpret_cast<uint4*>(&r)[i] = *reinterpret_cast<const uint4*>(qk_slot<T>(ring, u, lane, i));
   return r;
 }
 
+template <typename T>
+__device__ __forceinline__ T qk_take1(uint8_t* ring, int u, int lane, int i) {
+  constexpr int kEach = 16 / static_cast<int>(sizeof(T));
+  return reinterpret_cast<const T*>(qk_slot<T>(ring, u, lane, i / kEach))[i % kEach];
+}
+
 template <typename T, bool VEC>
-__device__ __forceinline__ void qk_store(char* base, int64_t elem, const float (&y)[8]) {
+__device__ __forceinline__ void qk_store(T* p, const float (&y)[8]) {
   Qk8<T> r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r.v[i] = qk_narrow<T>(y[i]);
-  T* p = reinterpret_cast<T*>(base) + elem;
   if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i)
@@ -107,20 +170,46 @@ __device__ __forceinline__ float qk_group_sum(float v) {
   return v;
 }
 
-// What one warp works on: `first` .. of the heads of tensor t at one token.
+// A lane's eight values as four pairs: (0, 2), (1, 3), (4, 6), (5, 7).  The
+// adjacent rotation's partners of pair j are then pair j ^ 1 as it stands.
+__device__ __forceinline__ void qk_pair(const float (&x)[8], uint64_t (&v)[4]) {
+  v[0] = pk2(x[0], x[2]);
+  v[1] = pk2(x[1], x[3]);
+  v[2] = pk2(x[4], x[6]);
+  v[3] = pk2(x[5], x[7]);
+}
+
+__device__ __forceinline__ void qk_unpair(const uint64_t (&v)[4], float (&x)[8]) {
+  upk2(v[0], x[0], x[2]);
+  upk2(v[1], x[1], x[3]);
+  upk2(v[2], x[4], x[6]);
+  upk2(v[3], x[5], x[7]);
+}
+
+template <typename T>
+__device__ __forceinline__ void qk_pairs_of(const Qk8<T>& r, uint64_t (&v)[4]) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = qk_widen<T>(r.v[i]);
+  qk_pair(x, v);
+}
+
+__device__ __forceinline__ float qk_total(uint64_t a) {
+  float lo, hi;
+  upk2(a, lo, hi);
+  return lo + hi;
+}
+
+// The token that a warp works on, and which heads of tensor t.
 struct QkItem {
-  int t, first;
+  int first;
   uint32_t b, l;
 };
 
-__device__ __forceinline__ QkItem qk_item(const QkNormParams& p, uint32_t item, int rows_per_item) {
+__device__ __forceinline__ QkItem qk_item(const QkNormParams& p, uint32_t item, uint32_t chunks, int rows) {
   QkItem r;
-  const uint32_t per = p.chunks[0] + p.chunks[1];
-  const uint32_t token = item / per;
-  int c = static_cast<int>(item - token * per);
-  r.t = c >= p.chunks[0];
-  if (r.t) c -= p.chunks[0];
-  r.first = c * rows_per_item;
+  const uint32_t token = item / chunks;
+  r.first = static_cast<int>(item - token * chunks) * rows;
   r.b = token / p.seq;
   r.l = token - r.b * p.seq;
   return r;
@@ -132,12 +221,12 @@ __device__ __forceinline__ QkItem qk_item(const QkNormParams& p, uint32_t item, 
 //   halves:   pair e mod rot / 2, partner e +- rot / 2, the first half's
 //             sine negative.
 // SIGN = -1 gives the transposed rotation.
-template <int SIGN>
+template <int ROT, int SIGN>
 __device__ __forceinline__ void qk_angles(const QkNormParams& p, const QkItem& it, int sub, float (&c)[8],
                                           float (&s)[8]) {
   const float* row = p.rope + it.b * p.rope_sb + static_cast<int64_t>(it.l) * p.rot;
   const int e0 = 8 * sub, half = p.rot / 2;
-  if (!p.halves) {
+  if constexpr (ROT == kQkAdjacent) {
     if (p.rope_vec && e0 + 8 <= p.rot) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -159,7 +248,7 @@ __device__ __forceinline__ void qk_angles(const QkNormParams& p, const QkItem& i
         s[i + 1] = SIGN * v;
       }
     }
-  } else if (p.rope_vec && half % 8 == 0 && e0 + 8 <= p.rot) {
+  } else if (ROT == kQkHalves && p.rope_vec && e0 + 8 <= p.rot) {
     const bool low = e0 < half;
     const float4* v4 = reinterpret_cast<const float4*>(row + 2 * (low ? e0 : e0 - half));
     const float sg = low ? -SIGN : SIGN;
@@ -184,47 +273,61 @@ __device__ __forceinline__ void qk_angles(const QkNormParams& p, const QkItem& i
   }
 }
 
-// Rotate a lane's eight values.  Values past `rot` stay as they are (a
-// product with a zero sine would turn an infinite neighbour into NaN).  The
-// halves order meets its partners in `buf`, the warp's 256 floats.
-__device__ __forceinline__ void qk_rotate(const QkNormParams& p, int sub, int lane, const float (&c)[8],
-                                          const float (&s)[8], float* buf, float (&y)[8]) {
-  const int e0 = 8 * sub;
-  float q[8];
-  if (!p.halves) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = y[i ^ 1];
+// The lane's partners in the halves order, from the rows in shared memory.
+// A value that is not rotated gets itself.
+template <typename T, int ROT>
+__device__ __forceinline__ void qk_halves(const QkNormParams& p, int sub, int lane, uint8_t* ring, int u,
+                                          uint64_t (&q)[4]) {
+  const int e0 = 8 * sub, half = p.rot / 2;
+  if constexpr (ROT == kQkHalves) {
+    const int d = e0 < half ? half / 8 : e0 < p.rot ? -(half / 8) : 0;
+    qk_pairs_of<T>(qk_take<T>(ring, u, lane + d), q);
   } else {
-    const int half = p.rot / 2;
-    float* mine = buf + lane * 8;
-    __syncwarp();
-    reinterpret_cast<float4*>(mine)[0] = make_float4(y[0], y[1], y[2], y[3]);
-    reinterpret_cast<float4*>(mine)[1] = make_float4(y[4], y[5], y[6], y[7]);
-    __syncwarp();
-    if (half % 4 == 0) {
+    float f[8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int e = e0 + 4 * i;
-        const int d = e < half ? half : e < p.rot ? -half : 0;
-        const float4 v = *reinterpret_cast<const float4*>(mine + 4 * i + d);
-        q[4 * i] = v.x;
-        q[4 * i + 1] = v.y;
-        q[4 * i + 2] = v.z;
-        q[4 * i + 3] = v.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = e0 + i;
-        q[i] = mine[i + (e < half ? half : e < p.rot ? -half : 0)];
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int e = e0 + i, to = e < half ? e + half : e < p.rot ? e - half : e;
+      f[i] = qk_widen<T>(qk_take1<T>(ring, u, lane - sub + to / 8, to % 8));
     }
+    qk_pair(f, q);
+  }
+}
+
+// y = x a + x_partner b; values past `rot` take x a alone (a product with a
+// zero sine would turn an infinite neighbour into NaN).
+template <typename T, int ROT>
+__device__ __forceinline__ void qk_rotate(const QkNormParams& p, int sub, int lane, const uint64_t (&a)[4],
+                                          const uint64_t (&b)[4], uint8_t* ring, int u, const uint64_t (&x)[4],
+                                          uint64_t (&y)[4]) {
+  uint64_t q[4];
+  if constexpr (ROT != kQkAdjacent) {
+    qk_halves<T, ROT>(p, sub, lane, ring, u, q);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = x[j ^ 1];
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float v = fmaf(q[i], s[i], y[i] * c[i]);
-    y[i] = e0 + i < p.rot ? v : y[i];
+  for (int j = 0; j < 4; ++j) y[j] = fmul2(x[j], a[j]);
+  if (p.rot == p.dim) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = ffma2(q[j], b[j], y[j]);
+  } else {
+    float yf[8], zf[8];
+    uint64_t z[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = ffma2(q[j], b[j], y[j]);
+    qk_unpair(y, yf);
+    qk_unpair(z, zf);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) yf[i] = 8 * sub + i < p.rot ? zf[i] : yf[i];
+    qk_pair(yf, y);
   }
+}
+
+// Values e of a head weight, 1 without one.
+template <typename T>
+__device__ __forceinline__ float qk_weight1(const QkNormParams& p, int t, int e) {
+  return p.w_f32 ? __ldg(static_cast<const float*>(p.w[t]) + e) : qk_widen<T>(static_cast<const T*>(p.w[t])[e]);
 }
 
 template <typename T>
@@ -232,145 +335,232 @@ __device__ __forceinline__ void qk_weight(const QkNormParams& p, int t, int sub,
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = 1.f;
   if (p.w[t] == nullptr || !in) return;
+  if (!p.w_f32 && p.w_vec) {
+    Qk8<T> r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    w[i] = p.w_f32 ? __ldg(static_cast<const float*>(p.w[t]) + 8 * sub + i)
-                   : qk_widen<T>(static_cast<const T*>(p.w[t])[8 * sub + i]);
-}
-
-// One warp per (token, tensor, chunk of kFwdRows rows a lane group).
-template <typename T, int G, bool VEC>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const __grid_constant__ QkNormParams p) {
-  constexpr int kGroups = 32 / G;
-  __shared__ float stage[kQkWarps][256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t item = blockIdx.x * kQkWarps + warp;
-  if (item >= p.items) return;
-  const QkItem it = qk_item(p, item, kFwdRows * kGroups);
-  const int sub = lane % G, group = lane / G, t = it.t;
-  const bool in = 8 * sub < p.dim;
-  const char* x = p.x[t];
-  const int64_t x0 = it.b * p.xs[t][0] + it.l * p.xs[t][1] + 8 * sub;
-  const int64_t o0 = it.b * p.os[t][0] + it.l * p.os[t][1] + 8 * sub;
-  Qk8<T> raw[kFwdRows];
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      reinterpret_cast<uint4*>(&r)[i] =
+          __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.w[t]) + 8 * sub) + i);
 #pragma unroll
-  for (int u = 0; u < kFwdRows; ++u) {
-    const int h = it.first + u * kGroups + group;
-    if (in && h < p.heads[t]) {
-      raw[u] = qk_load<T, VEC>(x, x0 + h * p.xs[t][2]);
-    } else {
+    for (int i = 0; i < 8; ++i) w[i] = qk_widen<T>(r.v[i]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) raw[u].v[i] = qk_narrow<T>(0.f);
-    }
-  }
-  float w[8], c[8], s[8];
-  if (p.norm) qk_weight<T>(p, t, sub, in, w);
-  if (p.rope != nullptr) qk_angles<1>(p, it, sub, c, s);
-#pragma unroll
-  for (int u = 0; u < kFwdRows; ++u) {
-    if (it.first + u * kGroups >= p.heads[t]) break;  // uniform over the warp
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = qk_widen<T>(raw[u].v[i]);
-    if (p.norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
-      const float r = rsqrtf(fmaf(qk_group_sum<G>(ss), p.inv_dim, p.eps));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
-    }
-    if (p.rope != nullptr) qk_rotate(p, sub, lane, c, s, stage[warp], y);
-    const int h = it.first + u * kGroups + group;
-    if (in && h < p.heads[t]) qk_store<T, VEC>(p.out[t], o0 + h * p.os[t][2], y);
+    for (int i = 0; i < 8; ++i) w[i] = qk_weight1<T>(p, t, 8 * sub + i);
   }
 }
 
-// Gradients.  The blocks stride over the items; each lane adds g n of its
-// eight columns over all the rows it meets, q's and k's apart, the block sums
-// its warps in a fixed order, and qk_weight_grad_kernel sums the blocks: no
-// atomics, so the same call gives the same bits.
-template <typename T, int G, bool VEC>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_bwd_kernel(const __grid_constant__ QkNormParams p) {
-  constexpr int kGroups = 32 / G;
-  __shared__ float stage[kQkWarps][256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane % G, group = lane / G;
-  const bool in = 8 * sub < p.dim;
-  float dw[2][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) dw[0][i] = dw[1][i] = 0.f;
-  const uint32_t step = gridDim.x * kQkWarps;
-  for (uint32_t item = blockIdx.x * kQkWarps + warp; item < p.items; item += step) {
-    const QkItem it = qk_item(p, item, kBwdRows * kGroups);
-    const int t = it.t;
-    const int64_t x0 = it.b * p.xs[t][0] + it.l * p.xs[t][1] + 8 * sub;
-    const int64_t d0 = it.b * p.ds[t][0] + it.l * p.ds[t][1] + 8 * sub;
-    const int64_t o0 = it.b * p.os[t][0] + it.l * p.os[t][1] + 8 * sub;
-    Qk8<T> xr[kBwdRows], dr[kBwdRows];
-#pragma unroll
-    for (int u = 0; u < kBwdRows; ++u) {
-      const int h = it.first + u * kGroups + group;
-      if (in && h < p.heads[t]) {
-        dr[u] = qk_load<T, VEC>(p.dy[t], d0 + h * p.ds[t][2]);
-        if (p.norm) xr[u] = qk_load<T, VEC>(p.x[t], x0 + h * p.xs[t][2]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) xr[u].v[i] = dr[u].v[i] = qk_narrow<T>(0.f);
-      }
-    }
-    float w[8], c[8], s[8];
-    if (p.norm) qk_weight<T>(p, t, sub, in, w);
-    if (p.rope != nullptr) qk_angles<-1>(p, it, sub, c, s);
-#pragma unroll
-    for (int u = 0; u < kBwdRows; ++u) {
-      if (it.first + u * kGroups >= p.heads[t]) break;  // uniform over the warp
-      const int h = it.first + u * kGroups + group;
-      const bool mine = in && h < p.heads[t];
-      float g[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = qk_widen<T>(dr[u].v[i]);
-      if (p.rope != nullptr) qk_rotate(p, sub, lane, c, s, stage[warp], g);
-      if (p.norm) {
-        float x[8], xx = 0.f, gx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = qk_widen<T>(xr[u].v[i]);
-          xx = fmaf(x[i], x[i], xx);
-          gx = fmaf(g[i] * w[i], x[i], gx);
-        }
-        xx = qk_group_sum<G>(xx);
-        gx = qk_group_sum<G>(gx);
-        const float r = rsqrtf(fmaf(xx, p.inv_dim, p.eps));
-        const float m = gx * r * p.inv_dim;  // mean(g w n)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float n = x[i] * r;
-          if (mine) dw[t][i] = fmaf(g[i], n, dw[t][i]);
-          g[i] = r * fmaf(-n, m, g[i] * w[i]);
-        }
-      }
-      if (mine) qk_store<T, VEC>(p.out[t], o0 + h * p.os[t][2], g);
-    }
-  }
-  if (p.partial == nullptr) return;  // uniform over the grid
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    __syncthreads();
+// The weights of the partners of a lane's values.
+template <typename T, int ROT>
+__device__ __forceinline__ void qk_partner_weight(const QkNormParams& p, int t, int sub, bool in, const float (&w)[8],
+                                                  float (&wp)[8]) {
+  const int half = p.rot / 2, e0 = 8 * sub;
+  if constexpr (ROT == kQkHalves) {
+    qk_weight<T>(p, t, sub + (e0 < half ? half / 8 : e0 < p.rot ? -(half / 8) : 0), in, wp);
+  } else if constexpr (ROT == kQkHalvesOff) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = dw[t][i];
+      const int e = e0 + i, to = e < half ? e + half : e < p.rot ? e - half : e;
+      wp[i] = p.w[t] != nullptr && in ? qk_weight1<T>(p, t, to) : 1.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) wp[i] = w[i ^ 1];
+  }
+}
+
+// One warp per (token, tensor, chunk of heads).
+template <typename T, int G, int ROT, bool VEC>
+__global__ void __launch_bounds__(kQkThreads, kQkFwdPerSm) qk_norm_rope_kernel(const __grid_constant__ QkNormParams p) {
+  constexpr int kGroups = 32 / G;
+  extern __shared__ __align__(16) uint8_t qk_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = qk_smem + warp * kQkRing;
+  uint32_t item = blockIdx.x * kQkWarps + warp;
+  const uint32_t q_items = p.tokens * p.chunks[0];
+  const int t = item >= q_items;
+  if (t) item -= q_items;
+  if (t && item >= p.tokens * p.chunks[1]) return;
+  const QkItem it = qk_item(p, item, p.chunks[t], kGroups * p.rows);
+  const int sub = lane % G, group = lane / G;
+  const bool in = 8 * sub < p.dim;
+  const int end = min(it.first + kGroups * p.rows, p.heads[t]);
+  const int mine = (end - it.first - group + kGroups - 1) / kGroups;  // this lane group's rows
+  {
+    const int64_t at = it.b * p.xs[t][0] + it.l * p.xs[t][1] + (it.first + group) * p.xs[t][2] + 8 * sub;
+    if (!in) qk_blank<T>(ring, lane);
+    else qk_fetch_rows<T, VEC>(ring, lane, p.x[t], at, p.xs[t][2] * kGroups, mine);
+  }
+  // y = r (x a + x_partner b):  a = w c,  b = w_partner s
+  uint64_t a[4], b[4];
+  {
+    float w[8];
+    qk_weight<T>(p, t, sub, in, w);
+    if constexpr (ROT != kQkNoTurn) {
+      float c[8], s[8], wp[8];
+      qk_angles<ROT, 1>(p, it, sub, c, s);
+      qk_partner_weight<T, ROT>(p, t, sub, in, w, wp);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] *= c[i];
+        s[i] *= wp[i];
+      }
+      qk_pair(s, b);
+    }
+    qk_pair(w, a);
+  }
+  cp_async_wait_all();
+  __syncwarp();
+  const int64_t step = p.os[t][2] * kGroups;
+  T* out = reinterpret_cast<T*>(p.out[t]) + it.b * p.os[t][0] + it.l * p.os[t][1] + (it.first + group) * p.os[t][2] + 8 * sub;
+  const int n = (end - it.first + kGroups - 1) / kGroups;
+  for (int u0 = 0; u0 < n; u0 += 2, out += 2 * step) {
+    uint64_t x[2][4];
+    float r[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      qk_pairs_of<T>(qk_take<T>(ring, u0 + u, lane), x[u]);
+      uint64_t ss = fmul2(x[u][0], x[u][0]);
+#pragma unroll
+      for (int j = 1; j < 4; ++j) ss = ffma2(x[u][j], x[u][j], ss);
+      r[u] = qk_total(ss);
+    }
+    if (p.norm) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) r[u] = rsqrtf(fmaf(qk_group_sum<G>(r[u]), p.inv_dim, p.eps));
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint64_t y[4];
+      if constexpr (ROT != kQkNoTurn) {
+        qk_rotate<T, ROT>(p, sub, lane, a, b, ring, u0 + u, x[u], y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = fmul2(x[u][j], a[j]);
+      }
+      if (p.norm) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = fmul2(y[j], pk2(r[u], r[u]));
+      }
+      float yf[8];
+      qk_unpair(y, yf);
+      if (in && u0 + u < mine) qk_store<T, VEC>(out + u * step, yf);
+    }
+  }
+}
+
+// Gradients.  The blocks stride over q's items, then over k's; each lane adds
+// g n of its eight columns over all the rows it meets, the block sums its
+// warps in a fixed order, and qk_weight_grad_kernel sums the blocks: no
+// atomics, so the same call gives the same bits.
+template <typename T, int G, int ROT, bool VEC>
+__global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kernel(const __grid_constant__ QkNormParams p) {
+  constexpr int kGroups = 32 / G;
+  extern __shared__ __align__(16) uint8_t qk_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = qk_smem + warp * (2 * kQkRing);
+  uint8_t* xring = ring + kQkRing;
+  const int sub = lane % G, group = lane / G;
+  const bool in = 8 * sub < p.dim;
+  const uint32_t warps = gridDim.x * kQkWarps;
+  uint32_t skip = 0;  // q's items taken: k's go on with the next warp
+  for (int t = 0; t < 2; ++t) {
+    if (!in) {
+      qk_blank<T>(ring, lane);
+      qk_blank<T>(xring, lane);
+    }
+    uint64_t dw[4] = {0, 0, 0, 0};
+    uint64_t wv[4];
+    {
+      float w[8];
+      qk_weight<T>(p, t, sub, in, w);
+      qk_pair(w, wv);
+    }
+    const uint32_t items = p.tokens * p.chunks[t];
+    const int64_t step = p.os[t][2] * kGroups;
+    for (uint32_t item = (blockIdx.x * kQkWarps + warp + warps - skip) % warps; item < items; item += warps) {
+      const QkItem it = qk_item(p, item, p.chunks[t], kGroups * p.rows);
+      const int end = min(it.first + kGroups * p.rows, p.heads[t]);
+      const int mine = (end - it.first - group + kGroups - 1) / kGroups;
+      if (in) {
+        const int h = it.first + group;
+        qk_fetch_rows<T, VEC>(ring, lane, p.dy[t], it.b * p.ds[t][0] + it.l * p.ds[t][1] + h * p.ds[t][2] + 8 * sub,
+                              p.ds[t][2] * kGroups, mine);
+        if (p.norm)
+          qk_fetch_rows<T, VEC>(xring, lane, p.x[t], it.b * p.xs[t][0] + it.l * p.xs[t][1] + h * p.xs[t][2] + 8 * sub,
+                                p.xs[t][2] * kGroups, mine);
+        // rows that the other groups of the warp have and this one has not: nothing for dw
+        for (int u = mine; u < p.rows; ++u) {
+          qk_blank_row<T>(ring, u, lane);
+          qk_blank_row<T>(xring, u, lane);
+        }
+      }
+      uint64_t a[4], b[4];
+      if constexpr (ROT != kQkNoTurn) {
+        float c[8], s[8];
+        qk_angles<ROT, -1>(p, it, sub, c, s);
+        qk_pair(c, a);
+        qk_pair(s, b);
+      }
+      cp_async_wait_all();
+      __syncwarp();
+      T* out = reinterpret_cast<T*>(p.out[t]) + it.b * p.os[t][0] + it.l * p.os[t][1] + (it.first + group) * p.os[t][2] + 8 * sub;
+      const int n = (end - it.first + kGroups - 1) / kGroups;
+      for (int u = 0; u < n; ++u, out += step) {
+        uint64_t g[4];
+        qk_pairs_of<T>(qk_take<T>(ring, u, lane), g);
+        if constexpr (ROT != kQkNoTurn) {
+          uint64_t y[4];
+          qk_rotate<T, ROT>(p, sub, lane, a, b, ring, u, g, y);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[j] = y[j];
+        }
+        if (p.norm) {
+          uint64_t x[4];
+          qk_pairs_of<T>(qk_take<T>(xring, u, lane), x);
+          uint64_t sx = fmul2(x[0], x[0]), sg = fmul2(fmul2(g[0], wv[0]), x[0]);
+#pragma unroll
+          for (int j = 1; j < 4; ++j) {
+            sx = ffma2(x[j], x[j], sx);
+            sg = ffma2(fmul2(g[j], wv[j]), x[j], sg);
+          }
+          const float xx = qk_group_sum<G>(qk_total(sx)), gx = qk_group_sum<G>(qk_total(sg));
+          const float r = rsqrtf(fmaf(xx, p.inv_dim, p.eps));
+          const float m = -gx * r * p.inv_dim;  // -mean(g w n); n and m stay in range however small x is
+          const uint64_t rr = pk2(r, r), mm = pk2(m, m);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint64_t nj = fmul2(x[j], rr);
+            dw[j] = ffma2(g[j], nj, dw[j]);
+            g[j] = fmul2(rr, ffma2(nj, mm, fmul2(g[j], wv[j])));
+          }
+        }
+        float gf[8];
+        qk_unpair(g, gf);
+        if (in && u < mine) qk_store<T, VEC>(out, gf);
+      }
+      __syncwarp();  // every lane has read its values and partners: the next item's may come
+    }
+    skip = items % warps;
+    if (p.partial == nullptr) continue;  // uniform over the grid
+    float df[8];
+    qk_unpair(dw, df);
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(qk_smem);  // (warps, 256)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = df[i];
 #pragma unroll
       for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (group == 0 && in) stage[warp][8 * sub + i] = v;
+      if (group == 0 && in) sums[warp * 256 + 8 * sub + i] = v;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < p.dim; e += kQkThreads) {
       float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < kQkWarps; ++k) v += stage[k][e];
+      for (int k = 0; k < kQkWarps; ++k) v += sums[k * 256 + e];
       p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + t) * p.dim + e] = v;
     }
+    __syncthreads();
   }
 }
 
@@ -380,22 +570,23 @@ struct QkWeightGradParams {
   int blocks, dim, dtype;
 };
 
-// Sum of the blocks' partial sums: 32 columns a block, eight warps over the
-// rows, then the warps in order.
-__global__ void __launch_bounds__(256) qk_weight_grad_kernel(const __grid_constant__ QkWeightGradParams p) {
-  __shared__ float part[8][33];
+// Sum of the blocks' partial sums: 32 columns a block, 32 warps over the rows, then the warps in order.
+__global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const __grid_constant__ QkWeightGradParams p) {
+  __shared__ float part[32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * 32 + lane;  // over q | k
   float v = 0.f;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (col < 2 * p.dim)
-    for (int b = warp; b < p.blocks; b += 8) v += p.partial[static_cast<int64_t>(b) * 2 * p.dim + col];
+  if (col < 2 * p.dim) {
+#pragma unroll 8
+    for (int b = warp; b < p.blocks; b += 32) v += p.partial[static_cast<int64_t>(b) * 2 * p.dim + col];
+  }
   part[warp][lane] = v;
   __syncthreads();
   if (warp != 0 || col >= 2 * p.dim) return;
   v = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v += part[k][lane];
+  for (int k = 0; k < 32; ++k) v += part[k][lane];
   const int t = col >= p.dim, e = col - t * p.dim;
   if (p.out[t] == nullptr) return;
   if (p.dtype == DGXM_DTYPE_F32) static_cast<float*>(p.out[t])[e] = v;
@@ -403,13 +594,34 @@ __global__ void __launch_bounds__(256) qk_weight_grad_kernel(const __grid_consta
   else static_cast<__nv_bfloat16*>(p.out[t])[e] = __float2bfloat16_rn(v);
 }
 
-static int qk_group(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+// How a call is cut into warps: chunks of as many rows as a warp has under
+// way, of equal length, unless that gives fewer than twelve warps for every
+// SM partition; then shorter ones.
+struct QkCut {
+  int group, rows, chunks[2], blocks;
+  int64_t warps;
+};
 
-// Blocks of the backward kernel: six of 256 threads fit an SM's registers.
-static int qk_bwd_blocks(const dgxm_qk_norm_desc* d, int rows_per_item, int sms, int64_t* items) {
-  const int64_t per = (d->q_heads + rows_per_item - 1) / rows_per_item + (d->k_heads + rows_per_item - 1) / rows_per_item;
-  *items = static_cast<int64_t>(d->batch) * d->seq * per;
-  return static_cast<int>(std::min<int64_t>((*items + kQkWarps - 1) / kQkWarps, int64_t(sms) * 6));
+// Lanes for one row.  Tensors off 16 bytes take 32 whatever their head_dim
+// (one kernel for a rare case).
+static int qk_group(int dim, bool vec) { return !vec || dim > 128 ? 32 : dim > 64 ? 16 : 8; }
+
+static QkCut qk_cut(const dgxm_qk_norm_desc* d, bool back, bool vec) {
+  QkCut c;
+  c.group = qk_group(d->head_dim, vec);
+  const int groups = 32 / c.group, most = d->dtype == DGXM_DTYPE_F32 ? kQkRows<float> : kQkRows<__half>;
+  const int64_t tokens = static_cast<int64_t>(d->batch) * d->seq;
+  const int longest = (std::max(d->q_heads, d->k_heads) + groups - 1) / groups;  // rows of the longer tensor
+  for (int parts = (longest + most - 1) / most;; ++parts) {
+    c.rows = (longest + parts - 1) / parts;
+    c.chunks[0] = (d->q_heads + groups * c.rows - 1) / (groups * c.rows);
+    c.chunks[1] = (d->k_heads + groups * c.rows - 1) / (groups * c.rows);
+    c.warps = tokens * (c.chunks[0] + c.chunks[1]);
+    if (c.rows <= 1 || c.warps >= 148 * 4 * 12) break;
+  }
+  const int64_t blocks = std::min<int64_t>((c.warps + kQkWarps - 1) / kQkWarps, int64_t(1) << 30);
+  c.blocks = static_cast<int>(back ? std::min<int64_t>(blocks, kQkBwdBlocks) : blocks);
+  return c;
 }
 
 static int qk_check(const dgxm_qk_norm_desc* d) {
@@ -434,8 +646,8 @@ static int qk_check(const dgxm_qk_norm_desc* d) {
 // Fill the kernel parameters that both directions share; *vec says whether
 // every access may be 16 bytes wide.
 static int qk_params(const dgxm_qk_norm_desc* d, const void* const (&x)[2], const void* const (&dy)[2],
-                     void* const (&out)[2], const void* const (&w)[2], const float* rope, int rows_per_item,
-                     QkNormParams* p, bool* vec) {
+                     void* const (&out)[2], const void* const (&w)[2], const float* rope, QkNormParams* p,
+                     QkCut* cut, bool* vec) {
   memset(p, 0, sizeof(*p));
   const int elt = d->dtype == DGXM_DTYPE_F32 ? 4 : 2;
   const bool back = dy[0] != nullptr || dy[1] != nullptr;
@@ -468,17 +680,20 @@ static int qk_params(const dgxm_qk_norm_desc* d, const void* const (&x)[2], cons
   p->rope = d->rot_dim > 0 ? rope : nullptr;
   p->rope_sb = d->rope_batch_stride;
   p->rope_vec = reinterpret_cast<uintptr_t>(rope) % 16 == 0 && d->rot_dim % 4 == 0 && d->rope_batch_stride % 4 == 0;
-  for (int t = 0; t < 2; ++t) p->chunks[t] = (p->heads[t] + rows_per_item - 1) / rows_per_item;
-  const int64_t items = static_cast<int64_t>(d->batch) * d->seq * (p->chunks[0] + p->chunks[1]);
-  if (items > (int64_t(1) << 31) - 1)
-    return fail(DGXM_ERR_UNSUPPORTED, "%lld head groups in one call (up to 2^31 - 1)", (long long)items);
+  *cut = qk_cut(d, back, *vec);
+  if (cut->warps > (int64_t(1) << 31) - 1)
+    return fail(DGXM_ERR_UNSUPPORTED, "%lld head groups in one call (up to 2^31 - 1)", (long long)cut->warps);
+  p->rows = cut->rows;
+  p->chunks[0] = cut->chunks[0];
+  p->chunks[1] = cut->chunks[1];
   p->seq = static_cast<uint32_t>(d->seq);
-  p->items = static_cast<uint32_t>(items);
+  p->tokens = static_cast<uint32_t>(static_cast<int64_t>(d->batch) * d->seq);
   p->dim = d->head_dim;
   p->rot = p->rope != nullptr ? d->rot_dim : 0;
   p->halves = d->rope_halves != 0;
   p->norm = d->norm_mode == DGXM_NORM_HEAD;
   p->w_f32 = d->weight_dtype == DGXM_DTYPE_F32;
+  p->w_vec = (reinterpret_cast<uintptr_t>(w[0]) | reinterpret_cast<uintptr_t>(w[1])) % 16 == 0;
   p->eps = d->eps;
   p->inv_dim = 1.f / d->head_dim;
   return DGXM_OK;
@@ -486,23 +701,34 @@ static int qk_params(const dgxm_qk_norm_desc* d, const void* const (&x)[2], cons
 
 using QkKernel = void (*)(QkNormParams);
 
-template <bool BACK, typename T, bool VEC>
-static QkKernel qk_pick_group(int group) {
+template <bool BACK, typename T, int G, bool VEC>
+static QkKernel qk_pick_turn(int rot) {
   if constexpr (BACK)
-    return group == 8 ? qk_norm_rope_bwd_kernel<T, 8, VEC> : group == 16 ? qk_norm_rope_bwd_kernel<T, 16, VEC>
-                                                                         : qk_norm_rope_bwd_kernel<T, 32, VEC>;
+    return rot == kQkNoTurn ? qk_norm_rope_bwd_kernel<T, G, kQkNoTurn, VEC>
+           : rot == kQkAdjacent ? qk_norm_rope_bwd_kernel<T, G, kQkAdjacent, VEC>
+           : rot == kQkHalves   ? qk_norm_rope_bwd_kernel<T, G, kQkHalves, VEC>
+                                : qk_norm_rope_bwd_kernel<T, G, kQkHalvesOff, VEC>;
   else
-    return group == 8 ? qk_norm_rope_kernel<T, 8, VEC> : group == 16 ? qk_norm_rope_kernel<T, 16, VEC>
-                                                                     : qk_norm_rope_kernel<T, 32, VEC>;
+    return rot == kQkNoTurn ? qk_norm_rope_kernel<T, G, kQkNoTurn, VEC>
+           : rot == kQkAdjacent ? qk_norm_rope_kernel<T, G, kQkAdjacent, VEC>
+           : rot == kQkHalves   ? qk_norm_rope_kernel<T, G, kQkHalves, VEC>
+                                : qk_norm_rope_kernel<T, G, kQkHalvesOff, VEC>;
+}
+
+template <bool BACK, typename T>
+static QkKernel qk_pick_group(int group, int rot, bool vec) {
+  if (!vec) return qk_pick_turn<BACK, T, 32, false>(rot);
+  return group == 8    ? qk_pick_turn<BACK, T, 8, true>(rot)
+         : group == 16 ? qk_pick_turn<BACK, T, 16, true>(rot)
+                       : qk_pick_turn<BACK, T, 32, true>(rot);
 }
 
 template <bool BACK>
-static QkKernel qk_pick(int dtype, int group, bool vec) {
-  if (dtype == DGXM_DTYPE_BF16)
-    return vec ? qk_pick_group<BACK, __nv_bfloat16, true>(group) : qk_pick_group<BACK, __nv_bfloat16, false>(group);
-  if (dtype == DGXM_DTYPE_F16)
-    return vec ? qk_pick_group<BACK, __half, true>(group) : qk_pick_group<BACK, __half, false>(group);
-  return vec ? qk_pick_group<BACK, float, true>(group) : qk_pick_group<BACK, float, false>(group);
+static QkKernel qk_pick(int dtype, int group, const QkNormParams& p, bool vec) {
+  const int rot = p.rope == nullptr ? kQkNoTurn : !p.halves ? kQkAdjacent : p.rot % 16 ? kQkHalvesOff : kQkHalves;
+  if (dtype == DGXM_DTYPE_BF16) return qk_pick_group<BACK, __nv_bfloat16>(group, rot, vec);
+  if (dtype == DGXM_DTYPE_F16) return qk_pick_group<BACK, __half>(group, rot, vec);
+  return qk_pick_group<BACK, float>(group, rot, vec);
 }
 
 }  // namespace dgxm
@@ -512,13 +738,12 @@ extern "C" int dgxm_qk_norm_rope(const dgxm_qk_norm_desc* d, const void* q, cons
   using namespace dgxm;
   if (int rc = qk_check(d)) return rc;
   if (d->batch == 0 || d->seq == 0 || d->q_heads + d->k_heads == 0) return DGXM_OK;
-  const int group = qk_group(d->head_dim), rows = kFwdRows * (32 / group);
   QkNormParams p;
+  QkCut cut;
   bool vec = false;
-  if (int rc = qk_params(d, {q, k}, {nullptr, nullptr}, {q_out, k_out}, {norm_q_w, norm_k_w}, rope, rows, &p, &vec))
+  if (int rc = qk_params(d, {q, k}, {nullptr, nullptr}, {q_out, k_out}, {norm_q_w, norm_k_w}, rope, &p, &cut, &vec))
     return rc;
-  const unsigned blocks = (p.items + kQkWarps - 1) / kQkWarps;
-  qk_pick<false>(d->dtype, group, vec)<<<blocks, kQkThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  qk_pick<false>(d->dtype, cut.group, p, vec)<<<cut.blocks, kQkThreads, kQkWarps * kQkRing, static_cast<cudaStream_t>(stream)>>>(p);
   DGXM_CUDA_TRY(cudaGetLastError());
   return DGXM_OK;
 }
@@ -526,9 +751,7 @@ extern "C" int dgxm_qk_norm_rope(const dgxm_qk_norm_desc* d, const void* q, cons
 extern "C" int64_t dgxm_qk_norm_rope_backward_workspace(const dgxm_qk_norm_desc* d) {
   using namespace dgxm;
   if (qk_check(d)) return -1;
-  int64_t items = 0;
-  const int blocks = qk_bwd_blocks(d, kBwdRows * (32 / qk_group(d->head_dim)), 148, &items);
-  return std::max<int64_t>(int64_t(blocks) * 2 * d->head_dim * 4, 4);
+  return int64_t(kQkBwdBlocks) * 2 * d->head_dim * 4;
 }
 
 extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void* dq, const void* dk, const void* q,
@@ -537,7 +760,6 @@ extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void
                                           void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace dgxm;
   if (int rc = qk_check(d)) return rc;
-  const int group = qk_group(d->head_dim), rows = kBwdRows * (32 / group);
   const bool weights = d->norm_mode == DGXM_NORM_HEAD && (g_norm_q_w != nullptr || g_norm_k_w != nullptr);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   QkNormParams p;
@@ -547,17 +769,17 @@ extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void
     bool vec = false;
     if ((d->q_heads > 0 && dq == nullptr) || (d->k_heads > 0 && dk == nullptr))
       return fail(DGXM_ERR_INVALID, "NULL upstream gradient");
-    if (int rc = qk_params(d, {q, k}, {dq, dk}, {gq, gk}, {norm_q_w, norm_k_w}, rope, rows, &p, &vec)) return rc;
-    int64_t items = 0;
-    blocks = qk_bwd_blocks(d, rows, 148, &items);
+    QkCut cut;
+    if (int rc = qk_params(d, {q, k}, {dq, dk}, {gq, gk}, {norm_q_w, norm_k_w}, rope, &p, &cut, &vec)) return rc;
+    blocks = cut.blocks;
     if (weights) {
       if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 4 ||
-          workspace_bytes < int64_t(blocks) * 2 * d->head_dim * 4)
+          workspace_bytes < dgxm_qk_norm_rope_backward_workspace(d))
         return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes,
-                    (long long)blocks * 2 * d->head_dim * 4);
+                    (long long)dgxm_qk_norm_rope_backward_workspace(d));
       p.partial = static_cast<float*>(workspace);
     }
-    qk_pick<true>(d->dtype, group, vec)<<<blocks, kQkThreads, 0, st>>>(p);
+    qk_pick<true>(d->dtype, cut.group, p, vec)<<<blocks, kQkThreads, kQkWarps * 2 * kQkRing, st>>>(p);
     DGXM_CUDA_TRY(cudaGetLastError());
   }
   if (!weights) return DGXM_OK;
@@ -574,7 +796,7 @@ extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((2 * d->head_dim + 31) / 32);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(1024);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
