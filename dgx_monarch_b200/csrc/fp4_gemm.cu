@@ -3,20 +3,16 @@
 // with the codes, block scales and tensor scales of fp4.cuh, fp32
 // accumulation and one rounding to the output's type.
 //
-// One operand gives the 128 rows of a tile (P), the other its TN columns (Q).
+// One operand gives the rows of a tile (P), the other its columns (Q).
 // tcgen05.mma reads codes from shared memory and block scales from tensor
-// memory; a stage of the ring holds 256 columns of K: 128 + TN rows of 128
-// bytes (one swizzle atom) and their scale tiles, 512 bytes for 128 rows and
-// four blocks, which tcgen05.cp spreads over tensor memory just before the
-// MMAs that read them.
+// memory; a stage of the ring holds 256 columns of K: rows of 128 bytes (one
+// swizzle atom) and their scale tiles, 512 bytes for 128 rows and four
+// blocks, which tcgen05.cp spreads over tensor memory just before the MMAs
+// that read them.
 //
 // Roles (10 warps): warp 0 loads (one thread), warp 1 copies scales and
 // issues MMAs (one thread), warps 2-9 run the epilogue, each a quarter of the
 // tile's rows and half of its columns.
-//
-// A tile whose K is split runs as a cluster of `split` CTAs; each leaves its
-// partial tile in its own shared memory and sums its share of the columns
-// over the cluster in rank order, so the result does not depend on timing.
 #include "common.h"
 #include "fp4.cuh"
 #include "ptx.cuh"
@@ -28,41 +24,48 @@ constexpr int kGemmRows = 128;
 constexpr int kGemmK = 256;               // columns of K a stage: 128 bytes of codes
 constexpr int kGemmSmemMax = 227 * 1024;
 constexpr int kGemmCtrlBytes = 512;
+constexpr int kGemmStageRows = 32 * 128;  // a warp's staging: 32 rows of 128 bytes of output
 
 struct __align__(64) Fp4GemmParams {
-  CUtensorMap tmap_p, tmap_q;  // codes: dims (pitch, 1, rows, 1), boxes (128, 1, 128 or TN, 1)
-  const uint8_t* sf_p;
-  const uint8_t* sf_q;
-  const float* scale_a;        // the tensors' scales, or NULL
+  CUtensorMap tmap_p, tmap_q;    // codes: dims (pitch, 1, rows, 1), boxes (128, 1, 128 or TN, 1)
+  CUtensorMap tmap_sp, tmap_sq;  // scale tiles of 128 words: dims (128, groups, row tiles)
+  const float* scale_a;          // the tensors' scales, or NULL
   const float* scale_b;
-  const void* bias;            // n values of bias_dtype, or NULL
+  const void* bias;              // n values of bias_dtype, or NULL
   void* out;
-  int64_t ld_out;              // elements
-  int64_t groups;              // scale tiles in a row of tiles
+  int64_t ld_out;                // elements
   int p_rows, q_rows, k, k_tiles;
   int p_tiles, q_tiles, split;
-  int q_is_tokens;             // P holds the weight's rows: the tile is the output transposed
+  int q_is_tokens;               // P holds the weight's rows: the tile is the output transposed
   int out_dtype, bias_dtype, vec;
 };
 
-template <int TN, int FORMAT>
+// A tile of kRows x TN outputs: one CTA's 128 rows, or (PAIR) a CTA pair's 256,
+// each CTA loading its own 128 rows of P and its half of Q's rows.
+template <int TN, int FORMAT, bool PAIR>
 struct Fp4Tile {
+  static constexpr int kRows = PAIR ? 2 * kGemmRows : kGemmRows;
+  static constexpr int kQLoad = PAIR ? TN / 2 : TN;                // Q rows this CTA loads
   static constexpr int kAtoms = kGemmK / (4 * fp4_block(FORMAT));  // scale tiles of a stage, for 128 rows
   static constexpr int kQTiles = (TN + 127) / 128;                 // 128-row tiles of scales on the Q side
   static constexpr int kPBytes = kGemmRows * 128;
-  static constexpr int kQBytes = TN * 128;
+  static constexpr int kQBytes = kQLoad * 128;
   static constexpr int kSfBytes = kAtoms * 512;
   static constexpr int kStageBytes = kPBytes + kQBytes + kSfBytes * (1 + kQTiles);
-  static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes) / kStageBytes;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kGemmCtrlBytes;
+  static constexpr int kStagingBytes = 8 * kGemmStageRows;
+  static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes - kStagingBytes) / kStageBytes;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kGemmCtrlBytes;
   // Tensor memory: accumulators, then two buffers of scales (P's 4 columns a
   // tile, Q's 4 columns a tile and 128 rows).
   static constexpr int kAccs = TN <= 128 ? 2 : 1;
   static constexpr int kSfP = 4 * kAtoms, kSfQ = 4 * kAtoms * kQTiles;
   static constexpr int kSfCol = kAccs * TN;
   static_assert(kSfCol + 2 * (kSfP + kSfQ) <= 512, "tensor memory");
-  static_assert(TN * kGemmRows * 4 <= kStages * kStageBytes, "a partial tile fits the ring");
   static_assert(kStageBytes % 1024 == 0, "swizzle atoms stay aligned");
+  // A split tile's partial sums, rows of kPartPitch floats (16 bytes off a
+  // multiple of 128 bytes, so that neighbouring rows lie in other banks).
+  static constexpr int kPartPitch = TN + 4;
+  static_assert(kGemmRows * kPartPitch * 4 <= kStages * kStageBytes, "a partial tile fits the ring");
   // Barriers
   static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + kAccs,
                        kDrain = kAccEmpty + kAccs, kBars = kDrain + 1;
@@ -84,42 +87,73 @@ __device__ __forceinline__ uint64_t fp4_sf_desc(uint32_t saddr) {
          (uint64_t(1) << 46);
 }
 
-// Scale tile -> four tensor-memory columns, the same in all four lane quarters.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
+// The MMA warp runs its loop as one, every lane with the same values, and
+// `lead` (non-zero in one lane) predicates the instructions themselves:
+// their operands then stay in uniform registers, where a branch on the lane
+// would move each of them there before each instruction.
+#define DGXM_LEAD "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
 
-template <int FORMAT>
-__device__ __forceinline__ void umma_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  if constexpr (FORMAT == DGXM_FP4_NVFP4)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+// Scale tile -> four tensor-memory columns, the same in all four lane
+// quarters (PAIR: each CTA's own tile into its own tensor memory).
+template <bool PAIR>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t lead, uint32_t taddr, uint64_t desc) {
+  if constexpr (PAIR)
+    asm volatile(DGXM_LEAD "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%1], %2;\n\t}\n" ::"r"(lead), "r"(taddr), "l"(desc)
+                 : "memory");
   else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+    asm volatile(DGXM_LEAD "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%1], %2;\n\t}\n" ::"r"(lead), "r"(taddr), "l"(desc)
+                 : "memory");
 }
 
-// `bytes` (a multiple of 16) global -> this CTA's shared memory, counted on `bar`.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
+#define DGXM_UMMA_FP4(group, kind)                                                                   \
+  asm volatile(DGXM_LEAD                                                                             \
+               "setp.ne.b32 p, %7, 0;\n\t"                                                           \
+               "@q tcgen05.mma." group "." kind " [%1], %2, %3, %4, [%5], [%6], p;\n\t}\n" ::"r"(lead), \
+               "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) \
+               : "memory")
+
+template <int FORMAT, bool PAIR>
+__device__ __forceinline__ void umma_fp4_ss(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  if constexpr (FORMAT == DGXM_FP4_NVFP4) {
+    if constexpr (PAIR) DGXM_UMMA_FP4("cta_group::2", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+    else DGXM_UMMA_FP4("cta_group::1", "kind::mxf4nvf4.block_scale.scale_vec::4X");
+  } else {
+    if constexpr (PAIR) DGXM_UMMA_FP4("cta_group::2", "kind::mxf4.block_scale.scale_vec::2X");
+    else DGXM_UMMA_FP4("cta_group::1", "kind::mxf4.block_scale.scale_vec::2X");
+  }
+}
+
+// Arrive on `bar` (PAIR: in both CTAs) when what this thread issued has completed.
+template <bool PAIR>
+__device__ __forceinline__ void fp4_commit(uint32_t lead, uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile(DGXM_LEAD
+                 "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], "
+                 "%2;\n\t}\n" ::"r"(lead),
+                 "r"(bar), "h"(static_cast<uint16_t>(0x3))
+                 : "memory");
+  else
+    asm volatile(DGXM_LEAD "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(
+                     lead),
+                 "r"(bar)
+                 : "memory");
+}
+
+// Load a tile and report its bytes on `bar`: this CTA's barrier, or (PAIR)
+// the shared::cluster address of the even CTA's.
+template <bool PAIR>
+__device__ __forceinline__ void fp4_tma(uint32_t dst, const void* map, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (PAIR) tma_load_4d_pair(dst, map, bar, c0, c1, c2, 0);
+  else tma_load_4d(dst, map, bar, c0, c1, c2, 0);
+}
+
+__device__ __forceinline__ float4 ld_shared_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
                : "memory");
-}
-
-__device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
 
@@ -135,44 +169,53 @@ __device__ __forceinline__ void fp4_gemm_store(const Fp4GemmParams& p, int64_t a
   else static_cast<float*>(p.out)[at] = v;
 }
 
-// N accumulators (N <= 8) of one P row, columns q .. q + N - 1 of Q, finished and stored.
-template <int N>
-__device__ __forceinline__ void fp4_gemm_emit(const Fp4GemmParams& p, int pr, int q, float (&v)[N], float ga, float gb) {
-  if (pr >= p.p_rows || q >= p.q_rows) return;
+// A warp's 32 rows x NC columns of finished values (a row a lane) from row
+// pr0 and column q0 of the output, through its staging rows of 128 bytes, so
+// that neighbouring lanes store neighbouring pieces: 16-byte piece c of row
+// r lies at piece c ^ (r & 7).  ELT: bytes of an output element.
+template <int NC, int ELT>
+__device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* stage, const float (&v)[NC], int pr0,
+                                               int q0, int lane) {
+  constexpr int kEach = 16 / ELT;                         // elements of a piece
+  constexpr int kCols = NC < 128 / ELT ? NC : 128 / ELT;  // columns staged at one time
+  constexpr int kPieces = kCols / kEach;
+  char* out = static_cast<char*>(p.out);
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = v[i] * ga * gb;
-  if (p.q_is_tokens) {  // neighbouring lanes hold neighbouring output columns
-    const float b = p.bias != nullptr ? fp4_gemm_bias(p, pr) : 0.f;
+  for (int c0 = 0; c0 < NC; c0 += kCols) {
+    if (q0 + c0 >= p.q_rows) return;  // uniform over the warp
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (q + i < p.q_rows) fp4_gemm_store(p, (q + i) * p.ld_out + pr, v[i] + b);
-    return;
-  }
-  if (p.bias != nullptr) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (q + i < p.q_rows) v[i] += fp4_gemm_bias(p, q + i);
-  }
-  const int64_t at = pr * p.ld_out + q;
-  if constexpr (N == 8) {
-    if (p.vec && q + 8 <= p.q_rows) {
-      if (p.out_dtype == DGXM_DTYPE_F32) {
-        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+    for (int i = 0; i < kPieces; ++i) {
+      const float* f = v + c0 + i * kEach;
+      uint4 piece;
+      if constexpr (ELT == 4) {
+        piece = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
       } else if (p.out_dtype == DGXM_DTYPE_BF16) {
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) =
-            make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        piece = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
       } else {
-        *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at) =
-            make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+        piece = make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
       }
-      return;
+      *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = piece;
     }
-  }
+    __syncwarp();
+    if (p.vec && q0 + c0 + kCols <= p.q_rows) {
+      const int i = lane % kPieces;
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (q + i < p.q_rows) fp4_gemm_store(p, at + i, v[i]);
+      for (int r = lane / kPieces; r < 32; r += 32 / kPieces)
+        if (pr0 + r < p.p_rows)
+          *reinterpret_cast<uint4*>(out + ((pr0 + r) * p.ld_out + q0 + c0 + i * kEach) * ELT) =
+              *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
+    } else {
+      const int cols = min(kCols, p.q_rows - q0 - c0);
+      for (int r = 0; r < 32 && pr0 + r < p.p_rows; ++r)
+        for (int e = lane; e < cols; e += 32) {
+          const uint8_t* from = stage + r * 128 + (((e / kEach) ^ (r & 7)) << 4) + (e % kEach) * ELT;
+          char* to = out + ((pr0 + r) * p.ld_out + q0 + c0 + e) * ELT;
+          if constexpr (ELT == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+          else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+        }
+    }
+    __syncwarp();
+  }
 }
 
 // Tiles run in groups of eight P tiles, Q outermost within a group, so that
@@ -185,22 +228,30 @@ __device__ __forceinline__ void fp4_tile_coords(const Fp4GemmParams& p, int tile
   qt = r / rows;
 }
 
-template <int TN, int FORMAT>
+// One CTA a tile, `split` CTAs of a cluster sharing a tile's K (each leaves
+// its partial tile in its own shared memory and sums its share of the rows
+// over the cluster in rank order, so the result does not depend on timing),
+// or PAIR: a CTA pair a tile, the even CTA issuing the M256 MMAs of both.
+template <int TN, int FORMAT, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_constant__ Fp4GemmParams p) {
-  using C = Fp4Tile<TN, FORMAT>;
+  using C = Fp4Tile<TN, FORMAT, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - raw);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
+  uint8_t* staging = smem + C::kStages * C::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int first_tile = blockIdx.x / p.split, tile_step = gridDim.x / p.split;
+  const int cta = PAIR ? rank : 0;
+  const int share = PAIR ? 2 : p.split;  // CTAs of a tile
+  const int first_tile = blockIdx.x / share, tile_step = gridDim.x / share;
   const int tiles = p.p_tiles * p.q_tiles;
-  const int kt0 = rank * p.k_tiles / p.split, kt1 = (rank + 1) * p.k_tiles / p.split;  // this CTA's share of K
+  const int kt0 = PAIR ? 0 : rank * p.k_tiles / p.split;  // this CTA's share of K
+  const int kt1 = PAIR ? p.k_tiles : (rank + 1) * p.k_tiles / p.split;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -209,7 +260,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     }
     for (int a = 0; a < C::kAccs; ++a) {
       mbar_init(bar(C::kAccFull + a), 1);
-      mbar_init(bar(C::kAccEmpty + a), 8);  // every epilogue warp
+      mbar_init(bar(C::kAccEmpty + a), PAIR ? 16 : 8);  // every epilogue warp
     }
     mbar_init(bar(C::kDrain), 1);
     *abort_flag = 0;
@@ -218,15 +269,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&p.tmap_p);
     tma_prefetch_desc(&p.tmap_q);
+    tma_prefetch_desc(&p.tmap_sp);
+    tma_prefetch_desc(&p.tmap_sq);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (PAIR) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();  // the operands are there
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -242,72 +303,83 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
             ok = false;
             break;
           }
-          const uint32_t dst = base + s * C::kStageBytes, full = bar(C::kFull + s);
-          const int64_t left = p.groups - int64_t(kt) * C::kAtoms;
-          const uint32_t sf_bytes = static_cast<uint32_t>(left < C::kAtoms ? left : C::kAtoms) * 512;
-          const int q_sf = qt * TN / 128;  // first 128-row tile of Q's scales
-          const bool second = C::kQTiles == 2 && (q_sf + 1) * 128 < p.q_rows;
-          mbar_expect_tx(full, C::kPBytes + C::kQBytes + sf_bytes * (second ? 3 : 2));
-          tma_load_4d(dst, &p.tmap_p, full, kt * 128, 0, pt * kGemmRows, 0);
-          tma_load_4d(dst + C::kPBytes, &p.tmap_q, full, kt * 128, 0, qt * TN, 0);
+          const uint32_t dst = base + s * C::kStageBytes;
+          const uint32_t full = PAIR ? mapa_shared(bar(C::kFull + s), 0) : bar(C::kFull + s);
+          if (cta == 0) mbar_expect_tx(bar(C::kFull + s), (PAIR ? 2 : 1) * C::kStageBytes);
+          fp4_tma<PAIR>(dst, &p.tmap_p, full, kt * 128, 0, pt * C::kRows + cta * kGemmRows);
+          fp4_tma<PAIR>(dst + C::kPBytes, &p.tmap_q, full, kt * 128, 0, qt * TN + cta * C::kQLoad);
           const uint32_t sf = dst + C::kPBytes + C::kQBytes;
-          bulk_load(sf, p.sf_p + (pt * p.groups + int64_t(kt) * C::kAtoms) * 512, sf_bytes, full);
-          bulk_load(sf + C::kSfBytes, p.sf_q + (q_sf * p.groups + int64_t(kt) * C::kAtoms) * 512, sf_bytes, full);
-          if (second)
-            bulk_load(sf + 2 * C::kSfBytes, p.sf_q + ((q_sf + 1) * p.groups + int64_t(kt) * C::kAtoms) * 512, sf_bytes,
-                      full);
+          fp4_tma<PAIR>(sf, &p.tmap_sp, full, 0, kt * C::kAtoms, pt * (C::kRows / 128) + cta);
+          fp4_tma<PAIR>(sf + C::kSfBytes, &p.tmap_sq, full, 0, kt * C::kAtoms, qt * TN / 128);
         }
       }
       if (!ok) {
         report_device_error(kErrProducerTimeout);
         *abort_flag = 1;
+        // Let the loads already issued land before the CTA can exit.
+        if (cta == 0) {
+          const int first = it > C::kStages ? it - C::kStages : 0;
+          for (int i = first; i < it; ++i) mbar_wait(bar(C::kFull + i % C::kStages), (i / C::kStages) & 1, nullptr);
+        } else {
+          for (int i = 0; i < 50; ++i) __nanosleep(1000);  // the odd CTA cannot test the even one's barriers
+        }
       }
-      // Every load issued lands before the CTA can exit.
-      const int first = it > C::kStages ? it - C::kStages : 0;
-      for (int i = first; i < it; ++i) mbar_wait(bar(C::kFull + i % C::kStages), (i / C::kStages) & 1, nullptr);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ scales and MMAs
-    if (lane == 0) {
-      int it = 0, u = 0;
+    if (cta == 0) {
+      const uint32_t lead = lane == 0;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      int s = 0, parity = 0, sf_buf = 0, u = 0;
       bool ok = true;
       for (int tile = first_tile; ok && tile < tiles; tile += tile_step, ++u) {
         const int a = u % C::kAccs;
-        if (!(ok = mbar_wait(bar(C::kAccEmpty + a), ((u / C::kAccs) & 1) ^ 1, abort_flag))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kAccEmpty + a), ((u / C::kAccs) & 1) ^ 1, abort_flag)))) break;
         tc_fence_after();
-        const uint32_t acc = tmem + a * TN;
-        for (int kt = kt0; kt < kt1; ++kt, ++it) {
-          const int s = it % C::kStages;
-          if (!(ok = mbar_wait(bar(C::kFull + s), (it / C::kStages) & 1, abort_flag))) break;
+        const uint32_t acc = tm + a * TN;
+        for (int kt = kt0; kt < kt1; ++kt) {
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kFull + s), parity, abort_flag)))) break;
           tc_fence_after();
           const uint32_t sp = base + s * C::kStageBytes, sq = sp + C::kPBytes, sf = sq + C::kQBytes;
-          const uint32_t tp = tmem + C::kSfCol + (it & 1) * (C::kSfP + C::kSfQ), tq = tp + C::kSfP;
-          const int steps = min(kGemmK, p.k - kt * kGemmK + 63) / 64;  // K = 64 each; the rest of the last tile is empty
+          const uint32_t tp = tm + C::kSfCol + sf_buf * (C::kSfP + C::kSfQ), tq = tp + C::kSfP;
+          const uint64_t dp = sdesc_sw128(sp, 16, 1024), dq = sdesc_sw128(sq, 16, 1024), df = fp4_sf_desc(sf);
+          // K = 64 an MMA; the rest of the last tile is empty.
+          const int steps = min(kGemmK, p.k - kt * kGemmK + 63) / 64;
 #pragma unroll
-          for (int i = 0; i < C::kAtoms; ++i) {
-            tmem_cp_scales(tp + 4 * i, fp4_sf_desc(sf + 512 * i));
+          for (int kk = 0; kk < kGemmK / 64; ++kk) {
+            constexpr int kPer = 4 / C::kAtoms;  // MMAs a scale tile serves
+            const int i = kk / kPer;
+            if (kk % kPer == 0) {
+              tmem_cp_scales<PAIR>(lead, tp + 4 * i, df + 32 * i);
 #pragma unroll
-            for (int j = 0; j < C::kQTiles; ++j)
-              tmem_cp_scales(tq + 4 * (C::kQTiles * i + j), fp4_sf_desc(sf + (1 + j) * C::kSfBytes + 512 * i));
+              for (int j = 0; j < C::kQTiles; ++j)
+                tmem_cp_scales<PAIR>(lead, tq + 4 * (C::kQTiles * i + j), df + ((1 + j) * C::kSfBytes + 512 * i) / 16);
+            }
+            if (kk < steps)
+              umma_fp4_ss<FORMAT, PAIR>(lead, acc, dp + 2 * kk, dq + 2 * kk,
+                                        fp4_idesc(C::kRows, TN, FORMAT, kPer == 1 ? 0 : 2 * (kk % kPer)), tp + 4 * i,
+                                        tq + 4 * C::kQTiles * i, (kt > kt0 || kk > 0) ? 1u : 0u);
           }
-          for (int kk = 0; kk < steps; ++kk) {
-            const int i = FORMAT == DGXM_FP4_NVFP4 ? kk : kk >> 1;
-            const uint32_t idesc = FORMAT == DGXM_FP4_NVFP4 || (kk & 1) == 0 ? fp4_idesc(kGemmRows, TN, FORMAT, 0)
-                                                                            : fp4_idesc(kGemmRows, TN, FORMAT, 2);
-            umma_fp4_ss<FORMAT>(acc, sdesc_sw128(sp + kk * 32, 16, 1024), sdesc_sw128(sq + kk * 32, 16, 1024), idesc,
-                                tp + 4 * i, tq + 4 * C::kQTiles * i, (kt > kt0 || kk > 0) ? 1u : 0u);
+          fp4_commit<PAIR>(lead, bar(C::kEmpty + s));
+          sf_buf ^= 1;
+          if (++s == C::kStages) {
+            s = 0;
+            parity ^= 1;
           }
-          umma_commit(bar(C::kEmpty + s));
         }
-        if (ok) umma_commit(bar(C::kAccFull + a));
+        if (ok) fp4_commit<PAIR>(lead, bar(C::kAccFull + a));
       }
       if (!ok) {
         report_device_error(kErrMmaTimeout);
         *abort_flag = 1;
       }
-      umma_commit(bar(C::kDrain));
-      mbar_wait(bar(C::kDrain), 0, nullptr);
+      // Every MMA issued has completed before tensor memory is released.
+      if (lane == 0) {
+        if constexpr (PAIR) umma_commit_pair_to(bar(C::kDrain), 0x1);
+        else umma_commit(bar(C::kDrain));
+        mbar_wait(bar(C::kDrain), 0, nullptr);
+      }
     }
     __syncwarp();
   } else {
@@ -317,11 +389,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     const int row = quarter * 32 + lane;
     constexpr int kCols = TN / 2;  // this warp's columns
     const float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
+    const uint32_t acc_empty = PAIR ? mapa_shared(bar(C::kAccEmpty), 0) : bar(C::kAccEmpty);
+    uint8_t* stage = staging + (warp - 2) * kGemmStageRows;
     int u = 0;
     for (int tile = first_tile; tile < tiles; tile += tile_step, ++u) {
       const int a = u % C::kAccs;
       int pt, qt;
       fp4_tile_coords(p, tile, pt, qt);
+      const int pr0 = pt * C::kRows + cta * kGemmRows + quarter * 32;  // this warp's first row
+      const int q0 = qt * TN + half * kCols;
+      float bias[(kCols + 31) / 32];  // column 32 i + lane, or (tokens) this lane's row
+#pragma unroll
+      for (int i = 0; i < (kCols + 31) / 32; ++i) {
+        const int n = p.q_is_tokens ? pr0 + lane : q0 + 32 * i + lane;
+        bias[i] = p.bias != nullptr && n < (p.q_is_tokens ? p.p_rows : p.q_rows) ? fp4_gemm_bias(p, n) : 0.f;
+      }
       const bool got = __all_sync(0xffffffffu, mbar_wait(bar(C::kAccFull + a), (u / C::kAccs) & 1, abort_flag));
       if (!got) {
         report_device_error(kErrEpilogueTimeout);
@@ -329,110 +411,169 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         break;
       }
       tc_fence_after();
-      uint32_t v[kCols / 8][8];
+      uint32_t r[kCols / 8][8];
       const uint32_t from = tmem + lane_off + a * TN + half * kCols;
 #pragma unroll
-      for (int c = 0; c < kCols / 8; ++c) tmem_ld8(from + 8 * c, v[c]);
+      for (int c = 0; c < kCols / 8; ++c) tmem_ld8(from + 8 * c, r[c]);
       tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < kCols / 8; ++c) reg_fence8(v[c]);
+      for (int c = 0; c < kCols / 8; ++c) reg_fence8(r[c]);
       // The accumulator is in registers: the next tile's MMAs may start.
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::kAccEmpty + a));
-      if (p.split == 1) {
-#pragma unroll
-        for (int c = 0; c < kCols / 8; ++c) {
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[c][i]);
-          fp4_gemm_emit<8>(p, pt * kGemmRows + row, qt * TN + half * kCols + 8 * c, f, ga, gb);
-        }
-      } else {
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(acc_empty + a * 8);
+        else mbar_arrive(acc_empty + a * 8);
+      }
+      if (!PAIR && p.split > 1) {
         // The ring is drained (its last MMAs have completed): it takes the
-        // partial tile, column by column.
-        float* part = reinterpret_cast<float*>(smem) + row;
+        // partial tile, row by row.
+        float4* part = reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + row * C::kPartPitch + half * kCols);
 #pragma unroll
         for (int c = 0; c < kCols / 8; ++c)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) part[(half * kCols + 8 * c + i) * kGemmRows] = __uint_as_float(v[c][i]);
+          for (int i = 0; i < 2; ++i)
+            part[2 * c + i] = make_float4(__uint_as_float(r[c][4 * i]), __uint_as_float(r[c][4 * i + 1]),
+                                          __uint_as_float(r[c][4 * i + 2]), __uint_as_float(r[c][4 * i + 3]));
+        continue;
+      }
+      float v[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) v[c] = __uint_as_float(r[c / 8][c % 8]) * ga * gb;
+      if (p.q_is_tokens) {  // neighbouring lanes hold neighbouring output columns
+        if (pr0 + lane < p.p_rows) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            if (q0 + c < p.q_rows) fp4_gemm_store(p, (q0 + c) * p.ld_out + pr0 + lane, v[c] + bias[0]);
+        }
+      } else {
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) v[c] += __shfl_sync(0xffffffffu, bias[c / 32], c % 32);
+        }
+        if (p.out_dtype == DGXM_DTYPE_F32) fp4_store_rows<kCols, 4>(p, stage, v, pr0, q0, lane);
+        else fp4_store_rows<kCols, 2>(p, stage, v, pr0, q0, lane);
       }
     }
   }
   tc_fence_before();
-  if (p.split > 1) {
+  if (PAIR || p.split == 1) {
+    if constexpr (PAIR) cluster_sync();  // the pair's MMAs drained and every tensor-memory read done in both CTAs
+    else __syncthreads();
+  } else {
     cluster_sync();  // every partial tile is in place
     if (warp >= 2 && *abort_flag == 0) {
-      const int t = threadIdx.x - 64, row = t & 127;
       const float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
       int pt, qt;
       fp4_tile_coords(p, first_tile, pt, qt);
-      const int per = TN / p.split;  // columns this CTA sums: 2 at the least
-      for (int c = (t >> 7) * 8; c < per; c += 16) {
-        float v[8];
+      const int rows = kGemmRows / p.split;  // rows this CTA sums
+      constexpr int kFours = TN / 4;
+      for (int i = threadIdx.x - 64; i < rows * kFours; i += 256) {
+        // neighbouring lanes take neighbouring output columns
+        const int row = rank * rows + (p.q_is_tokens ? i % rows : i / kFours);
+        const int c = 4 * (p.q_is_tokens ? i / rows : i % kFours);
+        float4 part[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        const int c0 = rank * per + c;
-        for (int r = 0; r < p.split; ++r) {
-          const uint32_t from = mapa_shared(base, r) + (c0 * kGemmRows + row) * 4;
+        for (int k = 0; k < 8; ++k)
+          if (k < p.split) part[k] = ld_shared_cluster4(mapa_shared(base, k) + (row * C::kPartPitch + c) * 4);
+        float4 sum = part[0];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + i < per) v[i] += ld_shared_cluster(from + i * kGemmRows * 4);
+        for (int k = 1; k < 8; ++k) {
+          if (k >= p.split) break;
+          sum.x += part[k].x;
+          sum.y += part[k].y;
+          sum.z += part[k].z;
+          sum.w += part[k].w;
         }
-        const int q = qt * TN + c0, pr = pt * kGemmRows + row;
-        if (per >= 8) {
-          fp4_gemm_emit<8>(p, pr, q, v, ga, gb);
-        } else {
+        const int pr = pt * kGemmRows + row;
+        const float v[4] = {sum.x * ga * gb, sum.y * ga * gb, sum.z * ga * gb, sum.w * ga * gb};
+        if (pr >= p.p_rows) continue;
+        const float one = p.q_is_tokens && p.bias != nullptr ? fp4_gemm_bias(p, pr) : 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float one[1] = {v[i]};
-            if (i < per) fp4_gemm_emit<1>(p, pr, q + i, one, ga, gb);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int q = qt * TN + c + e;
+          if (q >= p.q_rows) break;
+          if (p.q_is_tokens) fp4_gemm_store(p, q * p.ld_out + pr, v[e] + one);
+          else fp4_gemm_store(p, pr * p.ld_out + q, v[e] + (p.bias != nullptr ? fp4_gemm_bias(p, q) : 0.f));
         }
       }
     }
     __syncwarp();
     cluster_sync();  // no CTA leaves while a peer reads its partial tile
-  } else {
-    __syncthreads();
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
-template <int TN, int FORMAT>
-static int fp4_gemm_launch(Fp4GemmParams& p, cudaStream_t st) {
-  using C = Fp4Tile<TN, FORMAT>;
+// Tensor map of packed scales: tiles of 128 words, `groups` of them in a row
+// of tiles; a box is one stage's tiles of `tiles` row tiles, zero out of bounds.
+static int fp4_scale_map(CUtensorMap* map, const void* scales, int64_t groups, int64_t row_tiles, int atoms, int tiles) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(DGXM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[4] = {128, (cuuint64_t)groups, (cuuint64_t)row_tiles, 1};
+  cuuint64_t strides[3] = {512, (cuuint64_t)groups * 512, (cuuint64_t)(groups * row_tiles) * 512};
+  cuuint32_t box[4] = {128, (cuuint32_t)atoms, (cuuint32_t)tiles, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<void*>(scales), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DGXM_ERR_INVALID, "cuTensorMapEncodeTiled returned %d", (int)r);
+  return DGXM_OK;
+}
+
+struct Fp4Operand {
+  const void *values, *scales;
+  int64_t rows;
+};
+
+template <int TN, int FORMAT, bool PAIR>
+static int fp4_gemm_launch(Fp4GemmParams& p, const Fp4Operand& po, const Fp4Operand& qo, cudaStream_t st) {
+  using C = Fp4Tile<TN, FORMAT, PAIR>;
   static std::atomic<uint64_t> configured{0};
-  DGXM_CUDA_TRY(set_smem_limit_once(fp4_gemm_kernel<TN, FORMAT>, C::kSmemBytes, configured));
-  const int tiles = p.p_tiles * p.q_tiles;
+  DGXM_CUDA_TRY(set_smem_limit_once(fp4_gemm_kernel<TN, FORMAT, PAIR>, C::kSmemBytes, configured));
+  const int64_t pitch = fp4_pitch(p.k), groups = fp4_groups(p.k, FORMAT);
+  if (int rc = encode_map_4d(&p.tmap_p, po.values, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pitch, 1, po.rows, 1, pitch, pitch,
+                             pitch * po.rows, 128, kGemmRows))
+    return rc;
+  if (int rc = encode_map_4d(&p.tmap_q, qo.values, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pitch, 1, qo.rows, 1, pitch, pitch,
+                             pitch * qo.rows, 128, C::kQLoad))
+    return rc;
+  if (int rc = fp4_scale_map(&p.tmap_sp, po.scales, groups, (po.rows + 127) / 128, C::kAtoms, 1)) return rc;
+  if (int rc = fp4_scale_map(&p.tmap_sq, qo.scales, groups, (qo.rows + 127) / 128, C::kAtoms, C::kQTiles)) return rc;
+  p.p_tiles = (p.p_rows + C::kRows - 1) / C::kRows;
+  p.q_tiles = (p.q_rows + TN - 1) / TN;
+  const int tiles = p.p_tiles * p.q_tiles, share = PAIR ? 2 : p.split;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.split;
+  attr[0].val.clusterDim.x = share;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(p.split > 1 ? tiles * p.split : std::min(tiles, 148));
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  // One tile at a time; a split tile's cluster has one tile.
+  cfg.gridDim = dim3(PAIR ? 2 * std::min(tiles, 74) : p.split > 1 ? tiles * p.split : std::min(tiles, 148));
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<TN, FORMAT>, p));
+  cfg.numAttrs = 2;
+  DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<TN, FORMAT, PAIR>, p));
   return DGXM_OK;
 }
 
 template <int FORMAT>
-static int fp4_gemm_pick(Fp4GemmParams& p, int tn, cudaStream_t st) {
+static int fp4_gemm_pick(Fp4GemmParams& p, const Fp4Operand& po, const Fp4Operand& qo, int tn, cudaStream_t st) {
   switch (tn) {
-    case 16: return fp4_gemm_launch<16, FORMAT>(p, st);
-    case 32: return fp4_gemm_launch<32, FORMAT>(p, st);
-    case 64: return fp4_gemm_launch<64, FORMAT>(p, st);
-    case 128: return fp4_gemm_launch<128, FORMAT>(p, st);
-    default: return fp4_gemm_launch<256, FORMAT>(p, st);
+    case 16: return fp4_gemm_launch<16, FORMAT, false>(p, po, qo, st);
+    case 32: return fp4_gemm_launch<32, FORMAT, false>(p, po, qo, st);
+    case 64: return fp4_gemm_launch<64, FORMAT, false>(p, po, qo, st);
+    case 128: return fp4_gemm_launch<128, FORMAT, false>(p, po, qo, st);
+    default: return fp4_gemm_launch<256, FORMAT, true>(p, po, qo, st);
   }
 }
 
@@ -466,38 +607,28 @@ extern "C" int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* d, const void* a_values
   if (reinterpret_cast<uintptr_t>(out) % out_elt || reinterpret_cast<uintptr_t>(bias) % bias_elt ||
       (reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) % 4)
     return fail(DGXM_ERR_INVALID, "output, bias or scale is not aligned to its elements");
+  const int64_t m = d->m, n = d->n;
+  if ((m + 127) / 128 * ((n + 127) / 128) > (1 << 28)) return fail(DGXM_ERR_UNSUPPORTED, "too many output tiles");
   Fp4GemmParams p;
   memset(&p, 0, sizeof(p));
-  // The tile: the wider side gives the 128 rows, unless both fill 256 x 128.
-  const int64_t m = d->m, n = d->n;
   const int64_t narrow = m < n ? m : n;
-  const bool q_is_tokens = narrow <= 64 && m <= n;
-  int tn = narrow <= 16 ? 16 : narrow <= 32 ? 32 : narrow <= 64 ? 64 : 128;
-  if (tn == 128 && (m + 127) / 128 * ((n + 255) / 256) >= 148) tn = 256;
-  const int64_t p_rows = q_is_tokens ? n : m, q_rows = q_is_tokens ? m : n;
-  const int64_t p_tiles = (p_rows + 127) / 128, q_tiles = (q_rows + tn - 1) / tn;
-  if (p_tiles * q_tiles > (1 << 28)) return fail(DGXM_ERR_UNSUPPORTED, "too many output tiles");
-  p.p_rows = static_cast<int>(p_rows);
-  p.q_rows = static_cast<int>(q_rows);
+  p.q_is_tokens = narrow <= 64 && m <= n;
+  p.p_rows = static_cast<int>(p.q_is_tokens ? n : m);
+  p.q_rows = static_cast<int>(p.q_is_tokens ? m : n);
   p.k = static_cast<int>(d->k);
   p.k_tiles = static_cast<int>((d->k + kGemmK - 1) / kGemmK);
-  p.p_tiles = static_cast<int>(p_tiles);
-  p.q_tiles = static_cast<int>(q_tiles);
+  int tn = narrow <= 16 ? 16 : narrow <= 32 ? 32 : narrow <= 64 ? 64 : 128;
+  if (tn == 128 && (m + 255) / 256 * ((n + 255) / 256) >= 74) tn = 256;
   p.split = 1;
-  while (p.split < 8 && p.split * 2 <= p.k_tiles && p_tiles * q_tiles * p.split * 2 <= 148) p.split *= 2;
-  p.q_is_tokens = q_is_tokens;
-  p.groups = fp4_groups(d->k, d->format);
-  const int64_t pitch = fp4_pitch(d->k);
-  const void* pv = q_is_tokens ? b_values : a_values;
-  const void* qv = q_is_tokens ? a_values : b_values;
-  if (int rc = encode_map_4d(&p.tmap_p, pv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pitch, 1, p_rows, 1, pitch, pitch,
-                             pitch * p_rows, 128, kGemmRows))
-    return rc;
-  if (int rc = encode_map_4d(&p.tmap_q, qv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, pitch, 1, q_rows, 1, pitch, pitch,
-                             pitch * q_rows, 128, tn))
-    return rc;
-  p.sf_p = static_cast<const uint8_t*>(q_is_tokens ? b_scales : a_scales);
-  p.sf_q = static_cast<const uint8_t*>(q_is_tokens ? a_scales : b_scales);
+  const int64_t tiles = (int64_t(p.p_rows) + 127) / 128 * ((int64_t(p.q_rows) + tn - 1) / tn);
+  if (tn < 256)
+    while (p.split < 8 && p.split * 2 <= p.k_tiles && tiles * p.split * 2 <= 148) p.split *= 2;
+#ifdef FP4_TUNE
+  if (getenv("TN")) tn = atoi(getenv("TN"));
+  if (getenv("SPLIT")) p.split = atoi(getenv("SPLIT"));
+#endif
+  const Fp4Operand a{a_values, a_scales, m}, b{b_values, b_scales, n};
+  const Fp4Operand &po = p.q_is_tokens ? b : a, &qo = p.q_is_tokens ? a : b;
   p.scale_a = a_scale;
   p.scale_b = b_scale;
   p.bias = bias;
@@ -507,5 +638,5 @@ extern "C" int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* d, const void* a_values
   p.bias_dtype = d->bias_dtype;
   p.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && d->out_stride * out_elt % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return nv ? fp4_gemm_pick<DGXM_FP4_NVFP4>(p, tn, st) : fp4_gemm_pick<DGXM_FP4_MXFP4>(p, tn, st);
+  return nv ? fp4_gemm_pick<DGXM_FP4_NVFP4>(p, po, qo, tn, st) : fp4_gemm_pick<DGXM_FP4_MXFP4>(p, po, qo, tn, st);
 }

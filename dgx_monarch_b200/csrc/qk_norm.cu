@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * 32 + lane;  // over q | k
   float v = 0.f;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  pdl_wait();
   if (col < 2 * p.dim) {
 #pragma unroll 8
     for (int b = warp; b < p.blocks; b += 32) v += p.partial[static_cast<int64_t>(b) * 2 * p.dim + col];
