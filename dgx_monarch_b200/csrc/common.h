@@ -40,6 +40,24 @@ cudaError_t set_smem_limit_once(Kernel kern, int bytes, std::atomic<uint64_t>& d
   return e;
 }
 
+// Launch a kernel whose prologue may overlap the end of the kernel before it
+// in the stream (it waits with pdl_wait before it touches global memory).
+template <typename Params>
+cudaError_t launch_overlapped(void (*kernel)(Params), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                              const Params& params) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
 // Encode a 4-D tiled tensor map over a (batch, row, head, col) tensor whose
 // innermost dimension `cols` is contiguous.  Strides are in elements.
 // box = {box_cols, 1, box_rows, 1}, 128-byte swizzle, zero fill out of bounds.

@@ -7,15 +7,30 @@
 // each to the nearest value, ties to the even code, saturating.  A block with
 // a NaN or an infinity gets a NaN scale; an empty scale gives zero codes.
 //
-// The roundings are those of the real quotients, not of a rounded division:
-// an fp32 product with a reciprocal bounds the quotient within 2^-21, and
-// where both bounds round to the same code that code is right.  Where they
-// differ, one border b lies between them, and the sign of fma(b s, g, -|x|)
-// decides: b s has 7 bits, so the one rounding of the fma cannot change the
-// sign.  Bounds and decision are cheap enough to stay hidden behind DRAM,
-// which carries 2 bytes in and 0.56 out for each bf16 value: the kernel's
-// bound.  g is brought near 1 by a power of two first (with x, exactly), so
-// that no product leaves fp32's range.
+// The roundings are those of the real quotients x / (s g), not of a rounded
+// division, and a kernel that DRAM is to bound has few instructions for it
+// (2 bytes in and 0.56 out for a bf16 value):
+//
+// - Away from the borders between codes a product with an fp32 reciprocal,
+//   good to 2^-21, rounds like the quotient.
+// - A 16-bit x can only come that near to a border b s g if b s g itself lies
+//   that near to a value of x's type.  The seven borders have four
+//   significands, so four products a block show whether it can happen; mostly
+//   it cannot (a chance of 1 in 1000 for bf16), and the block needs nothing more.
+// - Where it can, or x is fp32, two products bound the quotient from below
+//   and above.  Where they round alike that code is right; where not, one
+//   border lies between, and the sign of fma(b s, g, -|x|) decides: b s has 7
+//   bits, so the one rounding of the fma cannot change the sign.
+// - A g of at most 16 significant bits (a power of two, a scale that came as
+//   bf16 or fp16) makes b s g and ties with it exact numbers, so that many
+//   blocks would take the second way.  There the residual x - q s g, exact in
+//   an fma, corrects the product q: a tie becomes its border exactly, and
+//   nothing else can reach one, since b s g and x are at least 2^-23 apart.
+//
+// g is brought near 1 by a power of two first (with x, exactly), so that no
+// product leaves fp32's range.
+#include <type_traits>
+
 #include "common.h"
 #include "fp4.cuh"
 
@@ -34,21 +49,37 @@ struct Fp4Params {
   uint32_t* partials;  // bit patterns of the blocks' amax
   int64_t pitch, groups;
   uint32_t items, per_row;  // an item is one block of one row, padded to whole groups of 4
-  int cols, n_partials, scale_dtype;
+  int cols, n_partials, scale_dtype, wide;
   float scale_value;   // the given scale where `scale` is NULL
 };
 
 // One block's values as they lie in memory.
 template <typename T, int N>
-struct __align__(16) Fp4Raw {
+struct __align__(32) Fp4Raw {
   T v[N];
 };
 
-// The n <= N values at p (the rest zero).  VEC: p is 16-byte aligned.
+// 32 bytes at once (32-byte aligned): a whole sector a thread.
+__device__ __forceinline__ void ld_global_32(const void* p, uint32_t* r) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// The n <= N values at p (the rest zero).  VEC: p is 16-byte aligned, wide: 32-byte.
 template <typename T, int N, bool VEC>
-__device__ __forceinline__ Fp4Raw<T, N> fp4_load(const T* p, int n) {
+__device__ __forceinline__ Fp4Raw<T, N> fp4_load(const T* p, int n, bool wide) {
   Fp4Raw<T, N> r;
-  if (VEC && n >= N) {
+  if (VEC && n >= N && wide) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(r) / 32); ++i) ld_global_32(p + i * (32 / sizeof(T)), reinterpret_cast<uint32_t*>(&r) + 8 * i);
+  } else if (VEC && n >= N) {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i)
       reinterpret_cast<uint4*>(&r)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
@@ -105,6 +136,8 @@ __device__ __forceinline__ float fp4_widen(__half v) { return __half2float(v); }
 template <typename T, int BLOCK, bool VEC>
 __global__ void __launch_bounds__(kFp4Threads) fp4_amax_kernel(const __grid_constant__ Fp4Params p) {
   constexpr int kUnroll = 2;
+  pdl_launch_dependents();
+  pdl_wait();
   __shared__ uint32_t red[kFp4Threads / 32];
   uint32_t m = 0;
   const uint32_t step = gridDim.x * kFp4Threads;
@@ -115,7 +148,8 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_amax_kernel(const __grid_cons
       const uint64_t item = i0 + uint64_t(u) * step;
       const uint32_t row = static_cast<uint32_t>(item) / p.per_row, b = static_cast<uint32_t>(item) - row * p.per_row;
       const int n = item < p.items ? p.cols - static_cast<int>(b) * BLOCK : 0;
-      raw[u] = fp4_load<T, BLOCK, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * BLOCK : 0), n);
+      raw[u] = fp4_load<T, BLOCK, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * BLOCK : 0), n,
+                                    p.wide);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) m = max(m, fp4_amax_bits<T, BLOCK>(raw[u]));
@@ -142,12 +176,71 @@ __device__ __forceinline__ uint32_t fp4_e4m3_scale(float amax, float g, float in
   return d > 0.f ? lo : d < 0.f ? hi : (lo & 1u) ? hi : lo;
 }
 
+// Whether a value of T can lie within 2^-20 of v: v's bits past T's
+// significand are all zeros or ones but for the last few.
+template <typename T>
+__device__ __forceinline__ bool fp4_near(float v) {
+  constexpr uint32_t kPast = std::is_same<T, __nv_bfloat16>::value ? 0xFFFFu : 0x1FFFu;
+  return ((__float_as_uint(v) + 8u) & kPast) <= 16u;
+}
+
+// Eight codes of nvfp4 values under s g (g > 0 and near 1 after `up`), by the
+// ways that the head of this file gives.
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_codes_quick(const T* x, float r) {
+  const uint64_t rr = pk2(r, r);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) upk2(fmul2(pk2(fp4_widen<T>(x[i]), fp4_widen<T>(x[i + 1])), rr), q[i], q[i + 1]);
+  return fp4_encode8(q);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_codes_residual(const T* x, float up, float u, float r) {
+  const uint64_t nr = pk2(-r, -r), uu = pk2(u, u), nup = pk2(-up, -up);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t nv = fmul2(pk2(fp4_widen<T>(x[i]), fp4_widen<T>(x[i + 1])), nup);  // -x
+    const uint64_t a = fmul2(nv, nr);
+    upk2(ffma2(ffma2(a, uu, nv), nr, a), q[i], q[i + 1]);  // a - (a u - x) r; in these signs -0 stays -0
+  }
+  return fp4_encode8(q);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t fp4_codes_decided(const T* x, float up, float s, float g, float r) {
+  constexpr float kBelow = 1.f - 0x1p-21f, kAbove = 1.f + 0x1p-21f;
+  const float r0 = r * kBelow, r1 = r * kAbove;
+  float v[8], lo[8], hi[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = fp4_widen<T>(x[i]) * up;
+    lo[i] = v[i] * r0;
+    hi[i] = v[i] * r1;
+  }
+  uint32_t c = fp4_encode8(lo);
+  const uint32_t d = c ^ fp4_encode8(hi);
+  if (d != 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (((d >> (4 * i)) & 15u) == 0) continue;
+      const int k = (c >> (4 * i)) & 7;  // the border lies between codes k and k + 1
+      const float border = k < 4 ? 0.5f * k + 0.25f : k == 6 ? 5.f : k - 1.5f;
+      const float e = fmaf(border * s, g, -fabsf(v[i]));
+      if (e < 0.f || (e == 0.f && (k & 1))) c += 1u << (4 * i);
+    }
+  }
+  return c;
+}
+
 template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_constant__ Fp4Params p) {
   constexpr int B = fp4_block(FORMAT);
-  constexpr float kBelow = 1.f - 0x1p-21f, kAbove = 1.f + 0x1p-21f;
+  pdl_launch_dependents();
+  pdl_wait();
   float g = 1.f, up = 1.f, inv6g = 1.f;
-  bool bad = false;
+  bool bad = false, few_bits = false;
   if constexpr (FORMAT == DGXM_FP4_NVFP4) {
     if (p.partials != nullptr) {
       __shared__ uint32_t red[kFp4Threads / 32];
@@ -167,48 +260,42 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
     up = g < 0x1p-64f ? 0x1p64f : g > 0x1p64f ? 0x1p-64f : 1.f;
     g *= up;
     inv6g = g > 0.f ? __frcp_rn(6.f * g) : 0.f;
+    few_bits = (__float_as_uint(g) & 0xFFu) == 0;  // at most 16 significant bits
   }
-  const uint32_t step = gridDim.x * kFp4Threads;
-  for (uint64_t i0 = blockIdx.x * kFp4Threads + (threadIdx.x & ~31u); i0 < p.items; i0 += step) {
+  // From the last item to the first: behind an amax pass the end of the
+  // matrix is what L2 still holds.
+  const int64_t items = p.items, step = int64_t(gridDim.x) * kFp4Threads;
+  for (int64_t i0 = (items + step - 1) / step * step - step + blockIdx.x * kFp4Threads + (threadIdx.x & ~31u); i0 >= 0;
+       i0 -= step) {
+    if (i0 >= items) continue;  // only the first round is not full
     const uint32_t item = static_cast<uint32_t>(i0) + (threadIdx.x & 31u);
     const bool live = item < p.items;  // the items come in fours: so do the live lanes
     const uint32_t row = item / p.per_row, b = item - row * p.per_row;
     const int n = live ? p.cols - static_cast<int>(b) * B : 0;  // <= 0: padding
     const Fp4Raw<T, B> raw =
-        fp4_load<T, B, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * B : 0), n);
-    const uint32_t abits = fp4_amax_bits<T, B>(raw);
-    const float amax = fp4_widen_bits<T>(abits);
+        fp4_load<T, B, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * B : 0), n,
+                             p.wide);
+    const float amax = fp4_widen_bits<T>(fp4_amax_bits<T, B>(raw));
     uint32_t byte;
     uint32_t codes[B / 8];
     if constexpr (FORMAT == DGXM_FP4_NVFP4) {
       byte = bad || __float_as_uint(amax) >= 0x7F800000u ? 0x7Fu : inv6g == 0.f ? 0u : fp4_e4m3_scale(amax * up, g, inv6g);
       const float s = fp4_scale_value<FORMAT>(byte);
       const bool on = s > 0.f;  // false for zero and NaN
-      const float r = on ? __frcp_rn(s * g) : 0.f;
-      const float r0 = r * kBelow, r1 = r * kAbove;
+      const float u = s * g, r = on ? __frcp_rn(u) : 0.f;
+      if (few_bits) {
 #pragma unroll
-      for (int j = 0; j < B / 8; ++j) {
-        float v[8], lo[8], hi[8];
+        for (int j = 0; j < B / 8; ++j) codes[j] = fp4_codes_residual<T>(raw.v + 8 * j, up, u, r);
+      } else if (sizeof(T) == 4 || up != 1.f || fp4_near<T>(u) || fp4_near<T>(1.25f * u) || fp4_near<T>(1.5f * u) ||
+                 fp4_near<T>(1.75f * u)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = fp4_widen<T>(raw.v[8 * j + i]) * up;
-          lo[i] = v[i] * r0;
-          hi[i] = v[i] * r1;
-        }
-        uint32_t c = fp4_encode8(lo);
-        const uint32_t d = c ^ fp4_encode8(hi);
-        if (d != 0) {
+        for (int j = 0; j < B / 8; ++j) codes[j] = fp4_codes_decided<T>(raw.v + 8 * j, up, s, g, r);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (((d >> (4 * i)) & 15u) == 0) continue;
-            const int k = (c >> (4 * i)) & 7;  // the border lies between codes k and k + 1
-            const float border = k < 4 ? 0.5f * k + 0.25f : k == 6 ? 5.f : k - 1.5f;
-            const float e = fmaf(border * s, g, -fabsf(v[i]));
-            if (e < 0.f || (e == 0.f && (k & 1))) c += 1u << (4 * i);
-          }
-        }
-        codes[j] = on ? c : 0u;
+        for (int j = 0; j < B / 8; ++j) codes[j] = fp4_codes_quick<T>(raw.v + 8 * j, r);
       }
+#pragma unroll
+      for (int j = 0; j < B / 8; ++j) codes[j] = on ? codes[j] : 0u;
     } else {
       const uint32_t ab = __float_as_uint(amax);
       const int e = static_cast<int>(ab >> 23) - 2;  // floor(log2 amax) - 2 + 127; the scale is exact, and so is x / s
@@ -217,11 +304,8 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
       const float r = on ? __uint_as_float((254u - byte) << 23) : 0.f;
 #pragma unroll
       for (int j = 0; j < B / 8; ++j) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fp4_widen<T>(raw.v[8 * j + i]) * r;
-        const uint32_t c = fp4_encode8(v);
-        codes[j] = on ? c : 0u;
+        codes[j] = fp4_codes_quick<T>(raw.v + 8 * j, r);
+        codes[j] = on ? codes[j] : 0u;
       }
     }
     if (n <= 0) byte = 0u;
@@ -248,26 +332,42 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
 template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(kFp4Threads) fp4_dequantize_kernel(const __grid_constant__ Fp4Params p) {
   constexpr int B = fp4_block(FORMAT);
-  const float g = p.scale != nullptr ? *static_cast<const float*>(p.scale) : 1.f;
+  pdl_launch_dependents();
+  pdl_wait();
+  const float g = FORMAT == DGXM_FP4_NVFP4 ? *static_cast<const float*>(p.scale) : 1.f;
+  const uint64_t gg = pk2(g, g);
   const uint32_t step = gridDim.x * kFp4Threads;
   for (uint64_t i0 = blockIdx.x * kFp4Threads + threadIdx.x; i0 < p.items; i0 += step) {
     const uint32_t item = static_cast<uint32_t>(i0);
     const uint32_t row = item / p.per_row, c16 = item - row * p.per_row;
     const uint2 code = __ldg(reinterpret_cast<const uint2*>(p.values + row * p.pitch) + c16);
-    const float s = fp4_scale_value<FORMAT>(__ldg(p.scales + fp4_scale_at(row, c16 * 16 / B, p.groups)));
-    __half2 h[8];
-    fp4_decode8(code.x, *reinterpret_cast<__half2(*)[4]>(h));
-    fp4_decode8(code.y, *reinterpret_cast<__half2(*)[4]>(h + 4));
+    const uint32_t byte = __ldg(p.scales + fp4_scale_at(row, c16 * 16 / B, p.groups));
+    __half2 h[2][4];
+    fp4_decode8(code.x, h[0]);
+    fp4_decode8(code.y, h[1]);
     Fp4Raw<T, 16> out;
+    if constexpr (FORMAT == DGXM_FP4_NVFP4) {
+      // 6 significant bits between 2^-10 and 2688: exact in fp16 already.
+      const __half2 s = __half2half2(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(byte), __NV_E4M3)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i / 4][i % 4] = __hmul2(h[i / 4][i % 4], s);
+    }
+    const uint64_t ss = FORMAT == DGXM_FP4_NVFP4 ? gg : pk2(fp4_scale_value<FORMAT>(byte), fp4_scale_value<FORMAT>(byte));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 f = __half22float2(h[i]);
-      out.v[2 * i] = static_cast<T>(f.x * s * g);
-      out.v[2 * i + 1] = static_cast<T>(f.y * s * g);
+      const float2 f = __half22float2(h[i / 4][i % 4]);
+      float a, b;
+      upk2(fmul2(pk2(f.x, f.y), ss), a, b);
+      out.v[2 * i] = static_cast<T>(a);
+      out.v[2 * i + 1] = static_cast<T>(b);
     }
     const int n = p.cols - static_cast<int>(c16) * 16;
     T* dst = reinterpret_cast<T*>(const_cast<char*>(p.x)) + row * p.row_stride + int64_t(c16) * 16;
-    if (VEC && n >= 16) {
+    if (VEC && n >= 16 && p.wide) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(out) / 32); ++i)
+        st_global_32(dst + i * (32 / sizeof(T)), reinterpret_cast<const uint32_t*>(&out) + 8 * i);
+    } else if (VEC && n >= 16) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(out) / 16); ++i)
         reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(&out)[i];
@@ -306,7 +406,9 @@ static int fp4_params(const dgxm_fp4_desc* d, const void* x, const void* values,
   const int64_t items = d->rows * per_row;
   if (per_row > 0 && (d->rows > (int64_t(1) << 31) || items > (int64_t(1) << 31) - 1))
     return fail(DGXM_ERR_UNSUPPORTED, "%lld x %lld is more than 2^31 - 1 blocks", (long long)d->rows, (long long)d->cols);
-  *vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (d->rows == 1 || d->row_stride * elt % 16 == 0);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(d->rows == 1 ? 0 : d->row_stride * elt);
+  *vec = bits % 16 == 0;
+  p->wide = bits % 32 == 0;
   p->x = static_cast<const char*>(x);
   p->row_stride = d->row_stride;
   p->values = static_cast<uint8_t*>(const_cast<void*>(values));
@@ -327,29 +429,31 @@ static unsigned fp4_grid(uint32_t items, int per_sm) {
 }
 
 template <typename T, int FORMAT, bool VEC>
-static void fp4_launch_quantize(Fp4Params& p, bool amax, cudaStream_t st) {
-  constexpr int B = fp4_block(FORMAT);
+static cudaError_t fp4_launch_quantize(Fp4Params& p, bool amax, cudaStream_t st) {
   if (amax) {
     const unsigned grid = std::min<unsigned>(fp4_grid(p.items, 8), kFp4Partials);
     p.n_partials = static_cast<int>(grid);
-    fp4_amax_kernel<T, B, VEC><<<grid, kFp4Threads, 0, st>>>(p);
+    const cudaError_t e = launch_overlapped(fp4_amax_kernel<T, fp4_block(FORMAT), VEC>, grid, kFp4Threads, 0, st, p);
+    if (e != cudaSuccess) return e;
   }
-  fp4_quantize_kernel<T, FORMAT, VEC><<<fp4_grid(p.items, 8), kFp4Threads, 0, st>>>(p);
-}
-
-template <typename T, bool VEC>
-static void fp4_launch_dequantize(const Fp4Params& p, int format, cudaStream_t st) {
-  const unsigned grid = fp4_grid(p.items, 8);
-  if (format == DGXM_FP4_NVFP4) fp4_dequantize_kernel<T, DGXM_FP4_NVFP4, VEC><<<grid, kFp4Threads, 0, st>>>(p);
-  else fp4_dequantize_kernel<T, DGXM_FP4_MXFP4, VEC><<<grid, kFp4Threads, 0, st>>>(p);
+  return launch_overlapped(fp4_quantize_kernel<T, FORMAT, VEC>, fp4_grid(p.items, 8), kFp4Threads, 0, st, p);
 }
 
 template <typename T>
-static void fp4_quantize_typed(Fp4Params& p, int format, bool vec, bool amax, cudaStream_t st) {
+static cudaError_t fp4_quantize_typed(Fp4Params& p, int format, bool vec, bool amax, cudaStream_t st) {
   if (format == DGXM_FP4_NVFP4)
-    vec ? fp4_launch_quantize<T, DGXM_FP4_NVFP4, true>(p, amax, st) : fp4_launch_quantize<T, DGXM_FP4_NVFP4, false>(p, amax, st);
-  else
-    vec ? fp4_launch_quantize<T, DGXM_FP4_MXFP4, true>(p, false, st) : fp4_launch_quantize<T, DGXM_FP4_MXFP4, false>(p, false, st);
+    return vec ? fp4_launch_quantize<T, DGXM_FP4_NVFP4, true>(p, amax, st)
+               : fp4_launch_quantize<T, DGXM_FP4_NVFP4, false>(p, amax, st);
+  return vec ? fp4_launch_quantize<T, DGXM_FP4_MXFP4, true>(p, false, st)
+             : fp4_launch_quantize<T, DGXM_FP4_MXFP4, false>(p, false, st);
+}
+
+template <typename T>
+static cudaError_t fp4_dequantize_typed(const Fp4Params& p, int format, bool vec, cudaStream_t st) {
+  const auto kernel = format == DGXM_FP4_NVFP4
+                          ? (vec ? fp4_dequantize_kernel<T, DGXM_FP4_NVFP4, true> : fp4_dequantize_kernel<T, DGXM_FP4_NVFP4, false>)
+                          : (vec ? fp4_dequantize_kernel<T, DGXM_FP4_MXFP4, true> : fp4_dequantize_kernel<T, DGXM_FP4_MXFP4, false>);
+  return launch_overlapped(kernel, fp4_grid(p.items, 8), kFp4Threads, 0, st, p);
 }
 
 }  // namespace dgxm
@@ -391,10 +495,9 @@ extern "C" int dgxm_quantize_fp4(const dgxm_fp4_desc* d, const void* x, const vo
   p.scale_out = scale_out;
   p.partials = amax ? static_cast<uint32_t*>(workspace) : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (d->dtype == DGXM_DTYPE_BF16) fp4_quantize_typed<__nv_bfloat16>(p, d->format, vec, amax, st);
-  else if (d->dtype == DGXM_DTYPE_F16) fp4_quantize_typed<__half>(p, d->format, vec, amax, st);
-  else fp4_quantize_typed<float>(p, d->format, vec, amax, st);
-  DGXM_CUDA_TRY(cudaGetLastError());
+  DGXM_CUDA_TRY(d->dtype == DGXM_DTYPE_BF16  ? fp4_quantize_typed<__nv_bfloat16>(p, d->format, vec, amax, st)
+                : d->dtype == DGXM_DTYPE_F16 ? fp4_quantize_typed<__half>(p, d->format, vec, amax, st)
+                                             : fp4_quantize_typed<float>(p, d->format, vec, amax, st));
   return DGXM_OK;
 }
 
@@ -410,12 +513,8 @@ extern "C" int dgxm_dequantize_fp4(const dgxm_fp4_desc* d, const void* values, c
   if (int rc = fp4_params(d, out, values, scales, (d->cols + 15) / 16, &p, &vec)) return rc;
   p.scale = scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (d->dtype == DGXM_DTYPE_BF16)
-    vec ? fp4_launch_dequantize<__nv_bfloat16, true>(p, d->format, st) : fp4_launch_dequantize<__nv_bfloat16, false>(p, d->format, st);
-  else if (d->dtype == DGXM_DTYPE_F16)
-    vec ? fp4_launch_dequantize<__half, true>(p, d->format, st) : fp4_launch_dequantize<__half, false>(p, d->format, st);
-  else
-    vec ? fp4_launch_dequantize<float, true>(p, d->format, st) : fp4_launch_dequantize<float, false>(p, d->format, st);
-  DGXM_CUDA_TRY(cudaGetLastError());
+  DGXM_CUDA_TRY(d->dtype == DGXM_DTYPE_BF16  ? fp4_dequantize_typed<__nv_bfloat16>(p, d->format, vec, st)
+                : d->dtype == DGXM_DTYPE_F16 ? fp4_dequantize_typed<__half>(p, d->format, vec, st)
+                                             : fp4_dequantize_typed<float>(p, d->format, vec, st));
   return DGXM_OK;
 }
