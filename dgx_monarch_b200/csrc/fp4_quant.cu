@@ -13,19 +13,24 @@
 //
 // - Away from the borders between codes a product with an fp32 reciprocal,
 //   good to 2^-21, rounds like the quotient.
-// - A 16-bit x can only come that near to a border b s g if b s g itself lies
-//   that near to a value of x's type.  The seven borders have four
-//   significands, so four products a block show whether it can happen; mostly
-//   it cannot (a chance of 1 in 1000 for bf16), and the block needs nothing more.
-// - Where it can, or x is fp32, two products bound the quotient from below
-//   and above.  Where they round alike that code is right; where not, one
-//   border lies between, and the sign of fma(b s, g, -|x|) decides: b s has 7
-//   bits, so the one rounding of the fma cannot change the sign.
+// - A 16-bit x comes near a border b s g only if b s g itself lies near a
+//   value of x's type.  The seven borders have four significands and s has
+//   eight, so 32 products a warp show for which they do, within 2^-16.  Each such border
+//   has one value X beside it, and the sign of fma(b s, g, -X) says on which
+//   side (b s has 7 bits: the one rounding of the fma cannot change the sign).
+//   If all agree, a reciprocal moved by 2^-18 to that side decides them right,
+//   and no value near no border can notice.  With g = amax / 2688 a quarter
+//   of all blocks are of this kind: s = 1.75 meets the border 0.75 where
+//   21 divides out, and misses it by the rounding of g alone.
+// - Where they disagree or X lies on the border, or x is fp32, two products
+//   bound the quotient from below and above.  Where they round alike that
+//   code is right; where not, one border lies between, and the sign of
+//   fma(b s, g, -|x|) decides.
 // - A g of at most 16 significant bits (a power of two, a scale that came as
 //   bf16 or fp16) makes b s g and ties with it exact numbers, so that many
-//   blocks would take the second way.  There the residual x - q s g, exact in
-//   an fma, corrects the product q: a tie becomes its border exactly, and
-//   nothing else can reach one, since b s g and x are at least 2^-23 apart.
+//   blocks would take that way.  There the residual x - q s g, exact in an
+//   fma, corrects the product q: a tie becomes its border exactly, and nothing
+//   else can reach one, since b s g and x are at least 2^-23 apart.
 //
 // g is brought near 1 by a power of two first (with x, exactly), so that no
 // product leaves fp32's range.
@@ -37,6 +42,7 @@
 namespace dgxm {
 
 constexpr int kFp4Threads = 256;
+constexpr int kFp4Cols = 32;  // columns of an item: a block of mxfp4, two of nvfp4
 constexpr int kFp4Partials = 148 * 4;  // blocks of the amax pass, one partial maximum each
 
 struct Fp4Params {
@@ -48,7 +54,7 @@ struct Fp4Params {
   float* scale_out;    // the fp32 scale of the tensor
   uint32_t* partials;  // bit patterns of the blocks' amax
   int64_t pitch, groups;
-  uint32_t items, per_row;  // an item is one block of one row, padded to whole groups of 4
+  uint32_t items, per_row;  // an item is 32 columns of one row (16 where values are read back), padded to whole scale words
   int cols, n_partials, scale_dtype, wide;
   float scale_value;   // the given scale where `scale` is NULL
 };
@@ -98,8 +104,8 @@ __device__ __forceinline__ Fp4Raw<T, N> fp4_load(const T* p, int n, bool wide) {
 // Bits of the largest magnitude.  As integers magnitudes order like their
 // values, infinity above all numbers and NaN above infinity.
 template <typename T, int N>
-__device__ __forceinline__ uint32_t fp4_amax_bits(const Fp4Raw<T, N>& r) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t fp4_amax_bits(const T* v) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
   uint32_t m = 0;
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -133,7 +139,7 @@ template <>
 __device__ __forceinline__ float fp4_widen(__half v) { return __half2float(v); }
 
 // Largest magnitude of the matrix, as float bits, one partial a block.
-template <typename T, int BLOCK, bool VEC>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kFp4Threads) fp4_amax_kernel(const __grid_constant__ Fp4Params p) {
   constexpr int kUnroll = 2;
   pdl_launch_dependents();
@@ -142,17 +148,17 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_amax_kernel(const __grid_cons
   uint32_t m = 0;
   const uint32_t step = gridDim.x * kFp4Threads;
   for (uint64_t i0 = blockIdx.x * kFp4Threads + threadIdx.x; i0 < p.items; i0 += uint64_t(step) * kUnroll) {
-    Fp4Raw<T, BLOCK> raw[kUnroll];
+    Fp4Raw<T, kFp4Cols> raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const uint64_t item = i0 + uint64_t(u) * step;
       const uint32_t row = static_cast<uint32_t>(item) / p.per_row, b = static_cast<uint32_t>(item) - row * p.per_row;
-      const int n = item < p.items ? p.cols - static_cast<int>(b) * BLOCK : 0;
-      raw[u] = fp4_load<T, BLOCK, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * BLOCK : 0), n,
-                                    p.wide);
+      const int n = item < p.items ? p.cols - static_cast<int>(b) * kFp4Cols : 0;
+      raw[u] = fp4_load<T, kFp4Cols, VEC>(
+          reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * kFp4Cols : 0), n, p.wide);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) m = max(m, fp4_amax_bits<T, BLOCK>(raw[u]));
+    for (int u = 0; u < kUnroll; ++u) m = max(m, fp4_amax_bits<T, kFp4Cols>(raw[u].v));
   }
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
@@ -176,12 +182,36 @@ __device__ __forceinline__ uint32_t fp4_e4m3_scale(float amax, float g, float in
   return d > 0.f ? lo : d < 0.f ? hi : (lo & 1u) ? hi : lo;
 }
 
-// Whether a value of T can lie within 2^-20 of v: v's bits past T's
-// significand are all zeros or ones but for the last few.
+// What the borders' four significands times s g, u when rounded, have beside them: 0 no value
+// of T within 2^-16, 1 or -1 one or more, all above or all below their
+// borders, 2 both kinds, or one on its border.
 template <typename T>
-__device__ __forceinline__ bool fp4_near(float v) {
+__device__ __forceinline__ int fp4_beside(float s, float g, float u) {
+  // The bits of u past T's significand are all zeros or ones but for the last seven.
   constexpr uint32_t kPast = std::is_same<T, __nv_bfloat16>::value ? 0xFFFFu : 0x1FFFu;
-  return ((__float_as_uint(v) + 8u) & kPast) <= 16u;
+  const float w[4] = {u, 1.25f * u, 1.5f * u, 1.75f * u};
+  uint32_t past[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) past[i] = (__float_as_uint(w[i]) + 128u) & kPast;
+  if (min(min(past[0], past[1]), min(past[2], past[3])) > 256u) return 0;
+  bool above = false, below = false, on = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (past[i] > 256u) continue;
+    const float x = __uint_as_float((__float_as_uint(w[i]) + 128u) & ~kPast);  // the value of T
+    const float d = fmaf((1.f + 0.25f * i) * s, g, -x);
+    above |= d < 0.f;
+    below |= d > 0.f;
+    on |= d == 0.f;
+  }
+  return on || (above && below) ? 2 : above ? 1 : -1;
+}
+
+// 1 / v to 2^-23.
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 // Eight codes of nvfp4 values under s g (g > 0 and near 1 after `up`), by the
@@ -241,6 +271,7 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
   pdl_wait();
   float g = 1.f, up = 1.f, inv6g = 1.f;
   bool bad = false, few_bits = false;
+  uint32_t side_up = 0, side_down = 0, undecided = 0xFFu;  // fp4_beside by the significand of s
   if constexpr (FORMAT == DGXM_FP4_NVFP4) {
     if (p.partials != nullptr) {
       __shared__ uint32_t red[kFp4Threads / 32];
@@ -261,6 +292,13 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
     g *= up;
     inv6g = g > 0.f ? __frcp_rn(6.f * g) : 0.f;
     few_bits = (__float_as_uint(g) & 0xFFu) == 0;  // at most 16 significant bits
+    if constexpr (sizeof(T) == 2) {  // lane i: the block scales of significand 1 + i / 8
+      const float s = 1.f + 0.125f * (threadIdx.x & 7u);
+      const int side = up != 1.f ? 2 : fp4_beside<T>(s, g, s * g);
+      side_up = __ballot_sync(0xffffffffu, side == 1);
+      side_down = __ballot_sync(0xffffffffu, side == -1);
+      undecided = __ballot_sync(0xffffffffu, side == 2);
+    }
   }
   // From the last item to the first: behind an amax pass the end of the
   // matrix is what L2 still holds.
@@ -269,60 +307,63 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
        i0 -= step) {
     if (i0 >= items) continue;  // only the first round is not full
     const uint32_t item = static_cast<uint32_t>(i0) + (threadIdx.x & 31u);
-    const bool live = item < p.items;  // the items come in fours: so do the live lanes
-    const uint32_t row = item / p.per_row, b = item - row * p.per_row;
-    const int n = live ? p.cols - static_cast<int>(b) * B : 0;  // <= 0: padding
-    const Fp4Raw<T, B> raw =
-        fp4_load<T, B, VEC>(reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(b) * B : 0), n,
-                             p.wide);
-    const float amax = fp4_widen_bits<T>(fp4_amax_bits<T, B>(raw));
-    uint32_t byte;
-    uint32_t codes[B / 8];
-    if constexpr (FORMAT == DGXM_FP4_NVFP4) {
-      byte = bad || __float_as_uint(amax) >= 0x7F800000u ? 0x7Fu : inv6g == 0.f ? 0u : fp4_e4m3_scale(amax * up, g, inv6g);
-      const float s = fp4_scale_value<FORMAT>(byte);
-      const bool on = s > 0.f;  // false for zero and NaN
-      const float u = s * g, r = on ? __frcp_rn(u) : 0.f;
-      if (few_bits) {
+    const bool live = item < p.items;  // a scale word's items are live together
+    const uint32_t row = item / p.per_row, c32 = item - row * p.per_row;
+    const int n = live ? p.cols - static_cast<int>(c32) * kFp4Cols : 0;  // <= 0: padding
+    const Fp4Raw<T, kFp4Cols> raw = fp4_load<T, kFp4Cols, VEC>(
+        reinterpret_cast<const T*>(p.x) + (n > 0 ? row * p.row_stride + int64_t(c32) * kFp4Cols : 0), n, p.wide);
+    uint32_t codes[kFp4Cols / 8];
+    uint32_t word = 0;  // this item's scale bytes
 #pragma unroll
-        for (int j = 0; j < B / 8; ++j) codes[j] = fp4_codes_residual<T>(raw.v + 8 * j, up, u, r);
-      } else if (sizeof(T) == 4 || up != 1.f || fp4_near<T>(u) || fp4_near<T>(1.25f * u) || fp4_near<T>(1.5f * u) ||
-                 fp4_near<T>(1.75f * u)) {
+    for (int k = 0; k < kFp4Cols / B; ++k) {
+      const T* x = raw.v + k * B;
+      uint32_t* c = codes + k * (B / 8);
+      const float amax = fp4_widen_bits<T>(fp4_amax_bits<T, B>(x));
+      uint32_t byte;
+      if constexpr (FORMAT == DGXM_FP4_NVFP4) {
+        byte = bad || __float_as_uint(amax) >= 0x7F800000u ? 0x7Fu : inv6g == 0.f ? 0u : fp4_e4m3_scale(amax * up, g, inv6g);
+        const float s = fp4_scale_value<FORMAT>(byte);
+        const bool on = s > 0.f;  // false for zero and NaN
+        const float u = s * g, r = on ? rcp_approx(u) : 0.f;
+        if (few_bits) {
 #pragma unroll
-        for (int j = 0; j < B / 8; ++j) codes[j] = fp4_codes_decided<T>(raw.v + 8 * j, up, s, g, r);
+          for (int j = 0; j < B / 8; ++j) c[j] = fp4_codes_residual<T>(x + 8 * j, up, u, r);
+        } else {
+          const uint32_t bit = 1u << ((__float_as_uint(s) >> 20) & 7u);
+          if (undecided & bit) {
+#pragma unroll
+            for (int j = 0; j < B / 8; ++j) c[j] = fp4_codes_decided<T>(x + 8 * j, up, s, g, r);
+          } else {
+            const float moved = fmaf(r, (side_up & bit) ? 0x1p-18f : (side_down & bit) ? -0x1p-18f : 0.f, r);
+#pragma unroll
+            for (int j = 0; j < B / 8; ++j) c[j] = fp4_codes_quick<T>(x + 8 * j, moved);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < B / 8; ++j) c[j] = on ? c[j] : 0u;
       } else {
+        const uint32_t ab = __float_as_uint(amax);
+        const int e = static_cast<int>(ab >> 23) - 2;  // floor(log2 amax) - 2 + 127; the scale is exact, and so is x / s
+        byte = ab >= 0x7F800000u ? 0xFFu : static_cast<uint32_t>(e < 0 ? 0 : e);
+        const bool on = byte != 0xFFu;
+        const float r = on ? __uint_as_float((254u - byte) << 23) : 0.f;
 #pragma unroll
-        for (int j = 0; j < B / 8; ++j) codes[j] = fp4_codes_quick<T>(raw.v + 8 * j, r);
+        for (int j = 0; j < B / 8; ++j) {
+          c[j] = fp4_codes_quick<T>(x + 8 * j, r);
+          c[j] = on ? c[j] : 0u;
+        }
       }
-#pragma unroll
-      for (int j = 0; j < B / 8; ++j) codes[j] = on ? codes[j] : 0u;
-    } else {
-      const uint32_t ab = __float_as_uint(amax);
-      const int e = static_cast<int>(ab >> 23) - 2;  // floor(log2 amax) - 2 + 127; the scale is exact, and so is x / s
-      byte = ab >= 0x7F800000u ? 0xFFu : static_cast<uint32_t>(e < 0 ? 0 : e);
-      const bool on = byte != 0xFFu;
-      const float r = on ? __uint_as_float((254u - byte) << 23) : 0.f;
-#pragma unroll
-      for (int j = 0; j < B / 8; ++j) {
-        codes[j] = fp4_codes_quick<T>(raw.v + 8 * j, r);
-        codes[j] = on ? codes[j] : 0u;
-      }
+      if (n > k * B) word |= byte << (8 * k);  // zero past the last column
     }
-    if (n <= 0) byte = 0u;
-    // Four blocks' scale bytes are one word of the tile.
-    const uint32_t at = threadIdx.x & 3u;
-    uint32_t word = byte << (8 * at);
-    word |= __shfl_xor_sync(0xffffffffu, word, 1);
-    word |= __shfl_xor_sync(0xffffffffu, word, 2);
-    if (live && at == 0) *reinterpret_cast<uint32_t*>(p.scales + fp4_scale_at(row, b, p.groups)) = word;
-    const int64_t off = int64_t(b) * (B / 2);
-    if (live && off < p.pitch) {
-      uint8_t* dst = p.values + row * p.pitch + off;
-      if constexpr (B == 16)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
-      else
-        *reinterpret_cast<uint4*>(dst) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-    }
+    // The neighbouring items' bytes complete the word of the tile.
+    constexpr int kBytes = kFp4Cols / B, kItems = 4 / kBytes;
+    const uint32_t at = threadIdx.x % kItems;
+    word <<= 8 * kBytes * at;
+#pragma unroll
+    for (int o = 1; o < kItems; o *= 2) word |= __shfl_xor_sync(0xffffffffu, word, o);
+    if (live && at == 0) *reinterpret_cast<uint32_t*>(p.scales + fp4_scale_at(row, c32 * kBytes, p.groups)) = word;
+    if (live && int64_t(c32) * 16 < p.pitch)
+      *reinterpret_cast<uint4*>(p.values + row * p.pitch + int64_t(c32) * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
   }
 }
 
@@ -433,7 +474,7 @@ static cudaError_t fp4_launch_quantize(Fp4Params& p, bool amax, cudaStream_t st)
   if (amax) {
     const unsigned grid = std::min<unsigned>(fp4_grid(p.items, 8), kFp4Partials);
     p.n_partials = static_cast<int>(grid);
-    const cudaError_t e = launch_overlapped(fp4_amax_kernel<T, fp4_block(FORMAT), VEC>, grid, kFp4Threads, 0, st, p);
+    const cudaError_t e = launch_overlapped(fp4_amax_kernel<T, VEC>, grid, kFp4Threads, 0, st, p);
     if (e != cudaSuccess) return e;
   }
   return launch_overlapped(fp4_quantize_kernel<T, FORMAT, VEC>, fp4_grid(p.items, 8), kFp4Threads, 0, st, p);
@@ -490,7 +531,7 @@ extern "C" int dgxm_quantize_fp4(const dgxm_fp4_desc* d, const void* x, const vo
   if (d->rows == 0 && !nv) return DGXM_OK;  // nvfp4: the launch below still writes the scale (0 where none is given)
   Fp4Params p;
   bool vec = false;
-  if (int rc = fp4_params(d, x, values, scales, fp4_groups(d->cols, d->format) * 4, &p, &vec)) return rc;
+  if (int rc = fp4_params(d, x, values, scales, fp4_groups(d->cols, d->format) * 4 * fp4_block(d->format) / kFp4Cols, &p, &vec)) return rc;
   p.scale = scale;
   p.scale_out = scale_out;
   p.partials = amax ? static_cast<uint32_t*>(workspace) : nullptr;

@@ -107,6 +107,28 @@ def test_sizes(fmt, dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("amax", [2.0, 3.0, 5.25, 7.0, 2.625, 1.3125])
+def test_own_scale_with_borders_beside_values(dtype, amax):
+    """g = amax / 2688: where amax s b has the factor 21, a border misses a
+    value by the rounding of g alone.  Values around every border of every
+    block scale, and the values next to them in their type."""
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    x = torch.randn(64, 1024, device="cuda", generator=gen) * amax / 4
+    lead = amax * torch.arange(1, 65, device="cuda") / 64           # each block's largest, hence its scale
+    x = x.clamp(-amax, amax).view(64, 64, 16)
+    x = torch.minimum(torch.maximum(x, -lead[:, None]), lead[:, None])
+    x[..., 0] = lead
+    border = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device="cuda") / 6
+    x[..., 1:8] = (lead[:, None] * border).to(dtype).float()
+    x[..., 8:15] = -x[..., 1:8] * (1 + torch.randint(-2, 3, (64, 64, 7), device="cuda", generator=gen)
+                                  * float(torch.finfo(dtype).eps))
+    x = x.reshape(64, 1024).to(dtype)
+    x[0, 0] = amax
+    _check(x, "nvfp4")
+    _check(x, "nvfp4", float(x.abs().max()) / 2688)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("g", [1.0, 0.25, 0.3, 0.0078125, 1 / 2688])
 def test_given_scale_and_ties(dtype, g):
     """Values on a coarse grid: many quotients lie exactly on a border, and with g not a power of two next to one."""
