@@ -13,6 +13,8 @@
 // Roles (10 warps): warp 0 loads (one thread), warp 1 copies scales and
 // issues MMAs (one thread), warps 2-9 run the epilogue, each a quarter of the
 // tile's rows and half of its columns.
+#include <type_traits>
+
 #include "common.h"
 #include "fp4.cuh"
 #include "ptx.cuh"
@@ -47,25 +49,27 @@ struct Fp4Tile {
   static constexpr int kRows = PAIR ? 2 * kGemmRows : kGemmRows;
   static constexpr int kQLoad = PAIR ? TN / 2 : TN;                // Q rows this CTA loads
   static constexpr int kAtoms = kGemmK / (4 * fp4_block(FORMAT));  // scale tiles of a stage, for 128 rows
-  static constexpr int kQTiles = (TN + 127) / 128;                 // 128-row tiles of scales on the Q side
+  static constexpr int kQTiles = (TN + 127) / 128;                 // 128-row tiles of scales that Q's rows touch
   static constexpr int kPBytes = kGemmRows * 128;
   static constexpr int kQBytes = kQLoad * 128;
   static constexpr int kSfBytes = kAtoms * 512;
   static constexpr int kStageBytes = kPBytes + kQBytes + kSfBytes * (1 + kQTiles);
-  static constexpr int kStagingBytes = 8 * kGemmStageRows;
+  // A split tile's partial sums in the CTA that finishes their rows: (rank,
+  // row, column), rows 16 bytes off a multiple of 64, so that neighbouring
+  // ones lie in other banks.  They take the place of the staging rows.
+  static constexpr bool kSplits = !PAIR && TN <= 64;
+  static constexpr int kPartPitch = TN + 4;
+  static constexpr int kPartBytes = kSplits ? kGemmRows * kPartPitch * 4 : 0;
+  static constexpr int kStagingBytes = kPartBytes > 8 * kGemmStageRows ? kPartBytes : 8 * kGemmStageRows;
   static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes - kStagingBytes) / kStageBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kGemmCtrlBytes;
   // Tensor memory: accumulators, then two buffers of scales (P's 4 columns a
   // tile, Q's 4 columns a tile and 128 rows).
-  static constexpr int kAccs = TN <= 128 ? 2 : 1;
+  static constexpr int kAccs = TN <= 192 ? 2 : 1;
   static constexpr int kSfP = 4 * kAtoms, kSfQ = 4 * kAtoms * kQTiles;
   static constexpr int kSfCol = kAccs * TN;
   static_assert(kSfCol + 2 * (kSfP + kSfQ) <= 512, "tensor memory");
   static_assert(kStageBytes % 1024 == 0, "swizzle atoms stay aligned");
-  // A split tile's partial sums, rows of kPartPitch floats (16 bytes off a
-  // multiple of 128 bytes, so that neighbouring rows lie in other banks).
-  static constexpr int kPartPitch = TN + 4;
-  static_assert(kGemmRows * kPartPitch * 4 <= kStages * kStageBytes, "a partial tile fits the ring");
   // Barriers
   static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + kAccs,
                        kDrain = kAccEmpty + kAccs, kBars = kDrain + 1;
@@ -146,13 +150,10 @@ __device__ __forceinline__ void fp4_tma(uint32_t dst, const void* map, uint32_t 
   else tma_load_4d(dst, map, bar, c0, c1, c2, 0);
 }
 
-__device__ __forceinline__ float4 ld_shared_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
+// 16 bytes into the shared memory of a CTA of the cluster.
+__device__ __forceinline__ void st_shared_cluster(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
-  return v;
 }
 
 __device__ __forceinline__ float fp4_gemm_bias(const Fp4GemmParams& p, int n) {
@@ -175,7 +176,9 @@ template <int NC, int ELT>
 __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* stage, const float (&v)[NC], int pr0,
                                                int q0, int lane) {
   constexpr int kEach = 16 / ELT;                         // elements of a piece
-  constexpr int kCols = NC < 128 / ELT ? NC : 128 / ELT;  // columns staged at one time
+  constexpr int kMost = 128 / ELT;
+  constexpr int kCols = NC % kMost == 0 ? kMost : NC % (kMost / 2) == 0 ? kMost / 2 : NC;  // columns staged at one time
+  static_assert(kCols <= kMost && NC % kCols == 0, "whole chunks");
   constexpr int kPieces = kCols / kEach;
   char* out = static_cast<char*>(p.out);
 #pragma unroll
@@ -203,14 +206,18 @@ __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* 
           *reinterpret_cast<uint4*>(out + ((pr0 + r) * p.ld_out + q0 + c0 + i * kEach) * ELT) =
               *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
     } else {
-      const int cols = min(kCols, p.q_rows - q0 - c0);
-      for (int r = 0; r < 32 && pr0 + r < p.p_rows; ++r)
-        for (int e = lane; e < cols; e += 32) {
-          const uint8_t* from = stage + r * 128 + (((e / kEach) ^ (r & 7)) << 4) + (e % kEach) * ELT;
-          char* to = out + ((pr0 + r) * p.ld_out + q0 + c0 + e) * ELT;
-          if constexpr (ELT == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
-          else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
-        }
+      const int cols = min(kCols, p.q_rows - q0 - c0), rows = min(32, p.p_rows - pr0);
+      using Elt = typename std::conditional<ELT == 4, uint32_t, uint16_t>::type;
+      Elt* to = reinterpret_cast<Elt*>(p.out) + pr0 * p.ld_out + q0 + c0;
+#pragma unroll
+      for (int e = lane; e < kCols; e += 32) {
+        if (e >= cols) break;
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r)
+          if (r < rows)
+            to[r * p.ld_out + e] =
+                *reinterpret_cast<const Elt*>(stage + r * 128 + (((e / kEach) ^ (r & 7)) << 4) + (e % kEach) * ELT);
+      }
     }
     __syncwarp();
   }
@@ -226,10 +233,13 @@ __device__ __forceinline__ void fp4_tile_coords(const Fp4GemmParams& p, int tile
   qt = r / rows;
 }
 
-// One CTA a tile, `split` CTAs of a cluster sharing a tile's K (each leaves
-// its partial tile in its own shared memory and sums its share of the rows
-// over the cluster in rank order, so the result does not depend on timing),
-// or PAIR: a CTA pair a tile, the even CTA issuing the M256 MMAs of both.
+// One CTA a tile; or `split` CTAs of a cluster sharing a tile's K, each
+// finishing a share of its rows: every CTA stores its partial sums into the
+// shared memory of the row's owner (stores are not waited for, where loads
+// from a peer cost their latency over and over: 1003 x 777 x 1000 took 18 us
+// that way), and the owner sums them in rank order, so the result does not
+// depend on timing; or PAIR: a CTA pair a tile, the even CTA issuing the
+// M256 MMAs of both.
 template <int TN, int FORMAT, bool PAIR>
 __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_constant__ Fp4GemmParams p) {
   using C = Fp4Tile<TN, FORMAT, PAIR>;
@@ -280,7 +290,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     }
   }
   tc_fence_before();
-  if constexpr (PAIR) cluster_sync();
+  if (PAIR || (C::kSplits && p.split > 1)) cluster_sync();  // the peers' barriers, and their shared memory, are there
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -335,6 +345,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kAccEmpty + a), ((u / C::kAccs) & 1) ^ 1, abort_flag)))) break;
         tc_fence_after();
         const uint32_t acc = tm + a * TN;
+        int pt, qt;
+        fp4_tile_coords(p, tile, pt, qt);
+        const uint32_t q_col = qt * TN % 128 / 32;  // 0, or 2 where a tile starts in the middle of a tile of scales
         for (int kt = kt0; kt < kt1; ++kt) {
           if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kFull + s), parity, abort_flag)))) break;
           tc_fence_after();
@@ -356,7 +369,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
             if (kk < steps)
               umma_fp4_ss<FORMAT, PAIR>(acc, dp + 2 * kk, dq + 2 * kk,
                                         fp4_idesc(C::kRows, TN, FORMAT, kPer == 1 ? 0 : 2 * (kk % kPer)), tp + 4 * i,
-                                        tq + 4 * C::kQTiles * i, (kt > kt0 || kk > 0) ? 1u : 0u);
+                                        tq + 4 * C::kQTiles * i + q_col, (kt > kt0 || kk > 0) ? 1u : 0u);
           }
           fp4_commit<PAIR>(bar(C::kEmpty + s));
           sf_buf ^= 1;
@@ -419,16 +432,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         if constexpr (PAIR) mbar_arrive_cluster(acc_empty + a * 8);
         else mbar_arrive(acc_empty + a * 8);
       }
-      if (!PAIR && p.split > 1) {
-        // The ring is drained (its last MMAs have completed): it takes the
-        // partial tile, row by row.
-        float4* part = reinterpret_cast<float4*>(reinterpret_cast<float*>(smem) + row * C::kPartPitch + half * kCols);
+      if (C::kSplits && p.split > 1) {
+        const int rows = kGemmRows / p.split;
+        const uint32_t to = mapa_shared(smem_u32(staging), row / rows) +
+                            ((rank * rows + row % rows) * C::kPartPitch + half * kCols) * 4;
 #pragma unroll
-        for (int c = 0; c < kCols / 8; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            part[2 * c + i] = make_float4(__uint_as_float(r[c][4 * i]), __uint_as_float(r[c][4 * i + 1]),
-                                          __uint_as_float(r[c][4 * i + 2]), __uint_as_float(r[c][4 * i + 3]));
+        for (int c = 0; c < kCols / 4; ++c) st_shared_cluster(to + 16 * c, r[c / 2] + 4 * (c % 2));
         continue;
       }
       float v[kCols];
@@ -451,49 +460,36 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     }
   }
   tc_fence_before();
-  if (PAIR || p.split == 1) {
-    if constexpr (PAIR) cluster_sync();  // the pair's MMAs drained and every tensor-memory read done in both CTAs
-    else __syncthreads();
-  } else {
-    cluster_sync();  // every partial tile is in place
-    if (warp >= 2 && *abort_flag == 0) {
-      const float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
-      int pt, qt;
-      fp4_tile_coords(p, first_tile, pt, qt);
-      const int rows = kGemmRows / p.split;  // rows this CTA sums
-      constexpr int kFours = TN / 4;
-      for (int i = threadIdx.x - 64; i < rows * kFours; i += 256) {
-        // neighbouring lanes take neighbouring output columns
-        const int row = rank * rows + (p.q_is_tokens ? i % rows : i / kFours);
-        const int c = 4 * (p.q_is_tokens ? i / rows : i % kFours);
-        float4 part[8];
+  if (PAIR || (C::kSplits && p.split > 1)) cluster_sync();  // both CTAs' MMAs drained; or every partial sum is in place
+  else __syncthreads();
+  if (C::kSplits && p.split > 1 && warp >= 2 && *abort_flag == 0) {
+    const float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
+    int pt, qt;
+    fp4_tile_coords(p, first_tile, pt, qt);
+    const int rows = kGemmRows / p.split, pr0 = pt * kGemmRows + rank * rows, q0 = qt * TN;
+    const float* part = reinterpret_cast<const float*>(staging);
+    for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
+      // neighbouring lanes take neighbouring output columns
+      const int row = p.q_is_tokens ? i % rows : i / (TN / 4), c = 4 * (p.q_is_tokens ? i / rows : i % (TN / 4));
+      const int pr = pr0 + row, q = q0 + c;
+      if (pr >= p.p_rows || q >= p.q_rows) continue;
+      float4 sum = *reinterpret_cast<const float4*>(part + row * C::kPartPitch + c);
+      for (int k = 1; k < p.split; ++k) {
+        const float4 more = *reinterpret_cast<const float4*>(part + (k * rows + row) * C::kPartPitch + c);
+        sum.x += more.x;
+        sum.y += more.y;
+        sum.z += more.z;
+        sum.w += more.w;
+      }
+      const float v[4] = {sum.x * ga * gb, sum.y * ga * gb, sum.z * ga * gb, sum.w * ga * gb};
+      const float one = p.q_is_tokens && p.bias != nullptr ? fp4_gemm_bias(p, pr) : 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < p.split) part[k] = ld_shared_cluster4(mapa_shared(base, k) + (row * C::kPartPitch + c) * 4);
-        float4 sum = part[0];
-#pragma unroll
-        for (int k = 1; k < 8; ++k) {
-          if (k >= p.split) break;
-          sum.x += part[k].x;
-          sum.y += part[k].y;
-          sum.z += part[k].z;
-          sum.w += part[k].w;
-        }
-        const int pr = pt * kGemmRows + row;
-        const float v[4] = {sum.x * ga * gb, sum.y * ga * gb, sum.z * ga * gb, sum.w * ga * gb};
-        if (pr >= p.p_rows) continue;
-        const float one = p.q_is_tokens && p.bias != nullptr ? fp4_gemm_bias(p, pr) : 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int q = qt * TN + c + e;
-          if (q >= p.q_rows) break;
-          if (p.q_is_tokens) fp4_gemm_store(p, q * p.ld_out + pr, v[e] + one);
-          else fp4_gemm_store(p, pr * p.ld_out + q, v[e] + (p.bias != nullptr ? fp4_gemm_bias(p, q) : 0.f));
-        }
+      for (int e = 0; e < 4; ++e) {
+        if (q + e >= p.q_rows) break;
+        if (p.q_is_tokens) fp4_gemm_store(p, (q + e) * p.ld_out + pr, v[e] + one);
+        else fp4_gemm_store(p, pr * p.ld_out + q + e, v[e] + (p.bias != nullptr ? fp4_gemm_bias(p, q + e) : 0.f));
       }
     }
-    __syncwarp();
-    cluster_sync();  // no CTA leaves while a peer reads its partial tile
   }
   if (warp == 1) {
     tc_fence_after();
@@ -567,8 +563,49 @@ static int fp4_gemm_pick(Fp4GemmParams& p, const Fp4Operand& po, const Fp4Operan
     case 32: return fp4_gemm_launch<32, FORMAT, false>(p, po, qo, st);
     case 64: return fp4_gemm_launch<64, FORMAT, false>(p, po, qo, st);
     case 128: return fp4_gemm_launch<128, FORMAT, false>(p, po, qo, st);
+    case 192: return fp4_gemm_launch<192, FORMAT, false>(p, po, qo, st);
     default: return fp4_gemm_launch<256, FORMAT, true>(p, po, qo, st);
   }
+}
+
+// How a product is cut: the tile's columns (256: a CTA pair's 256 x 256),
+// into how many CTAs its K is split, which operand gives the tile's rows.
+struct Fp4Cut {
+  int tn, split;
+  bool q_is_tokens;
+};
+
+// The cut whose waves of tiles take the least time by what one tile took
+// (microseconds a stage of K and a tile, nvfp4, measured with K = 5120 and
+// 256 on products of one to nine waves): narrow tiles where only they fill
+// the SMs, wide ones, which load the least for what they compute, where those do too.
+static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
+  struct Kind {
+    int tn, rows, at_once;
+    double stage, tile;
+  };
+  static const Kind kinds[] = {{16, 128, 148, 0.13, 0.6}, {32, 128, 148, 0.15, 0.6}, {64, 128, 148, 0.26, 0.7},
+                               {128, 128, 148, 0.31, 1.0}, {192, 128, 148, 0.43, 1.2}, {256, 256, 74, 0.47, 1.4}};
+  Fp4Cut best{128, 1, false};
+  double least = 1e30;
+  const bool tokens = m <= n;  // with one tile of columns, the narrow side is Q
+  for (const Kind& kind : kinds) {
+    const int64_t narrow = m < n ? m : n;
+    const bool one = kind.tn <= 64 && narrow <= kind.tn;  // tiles of 16 and 32 columns only as one
+    if (kind.tn < 64 && !one) continue;
+    const int64_t p_rows = one && tokens ? n : m, q_rows = one && tokens ? m : n;
+    const int64_t tiles = (p_rows + kind.rows - 1) / kind.rows * ((q_rows + kind.tn - 1) / kind.tn);
+    for (int split = 1; split <= (kind.tn <= 64 ? 8 : 1) && split <= k_tiles; split *= 2) {
+      if (split > 1 && tiles * split > 148) break;
+      const int64_t waves = (tiles * split + kind.at_once - 1) / kind.at_once;
+      const double us = waves * ((k_tiles + split - 1) / split * kind.stage + kind.tile) + (split > 1 ? 0.8 : 0.0);
+      if (us < least) {
+        least = us;
+        best = {kind.tn, split, one && tokens};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace dgxm
@@ -602,25 +639,20 @@ extern "C" int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* d, const void* a_values
       (reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) % 4)
     return fail(DGXM_ERR_INVALID, "output, bias or scale is not aligned to its elements");
   const int64_t m = d->m, n = d->n;
-  if ((m + 127) / 128 * ((n + 127) / 128) > (1 << 28)) return fail(DGXM_ERR_UNSUPPORTED, "too many output tiles");
+  if ((m + 127) / 128 * ((n + 127) / 128) > (1 << 26)) return fail(DGXM_ERR_UNSUPPORTED, "too many output tiles");
   Fp4GemmParams p;
   memset(&p, 0, sizeof(p));
-  const int64_t narrow = m < n ? m : n;
-  p.q_is_tokens = narrow <= 64 && m <= n;
-  p.p_rows = static_cast<int>(p.q_is_tokens ? n : m);
-  p.q_rows = static_cast<int>(p.q_is_tokens ? m : n);
   p.k = static_cast<int>(d->k);
   p.k_tiles = static_cast<int>((d->k + kGemmK - 1) / kGemmK);
-  int tn = narrow <= 16 ? 16 : narrow <= 32 ? 32 : narrow <= 64 ? 64 : 128;
-  if (tn == 128 && (m + 255) / 256 * ((n + 255) / 256) >= 74) tn = 256;
-  p.split = 1;
-  const int64_t tiles = (int64_t(p.p_rows) + 127) / 128 * ((int64_t(p.q_rows) + tn - 1) / tn);
-  if (tn < 256)
-    while (p.split < 8 && p.split * 2 <= p.k_tiles && tiles * p.split * 2 <= 148) p.split *= 2;
+  Fp4Cut cut = fp4_cut(m, n, p.k_tiles);
 #ifdef FP4_TUNE
-  if (getenv("TN")) tn = atoi(getenv("TN"));
-  if (getenv("SPLIT")) p.split = atoi(getenv("SPLIT"));
+  if (getenv("TN")) cut.tn = atoi(getenv("TN"));
+  if (getenv("SPLIT")) cut.split = atoi(getenv("SPLIT"));
 #endif
+  p.q_is_tokens = cut.q_is_tokens;
+  p.split = cut.split;
+  p.p_rows = static_cast<int>(p.q_is_tokens ? n : m);
+  p.q_rows = static_cast<int>(p.q_is_tokens ? m : n);
   const Fp4Operand a{a_values, a_scales, m}, b{b_values, b_scales, n};
   const Fp4Operand &po = p.q_is_tokens ? b : a, &qo = p.q_is_tokens ? a : b;
   p.scale_a = a_scale;
@@ -632,5 +664,5 @@ extern "C" int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* d, const void* a_values
   p.bias_dtype = d->bias_dtype;
   p.vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && d->out_stride * out_elt % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return nv ? fp4_gemm_pick<DGXM_FP4_NVFP4>(p, po, qo, tn, st) : fp4_gemm_pick<DGXM_FP4_MXFP4>(p, po, qo, tn, st);
+  return nv ? fp4_gemm_pick<DGXM_FP4_NVFP4>(p, po, qo, cut.tn, st) : fp4_gemm_pick<DGXM_FP4_MXFP4>(p, po, qo, cut.tn, st);
 }
