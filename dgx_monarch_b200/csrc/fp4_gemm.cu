@@ -31,6 +31,7 @@ constexpr int kGemmStageRows = 32 * 128;  // a warp's staging: 32 rows of 128 by
 struct __align__(64) Fp4GemmParams {
   CUtensorMap tmap_p, tmap_q;    // codes: dims (pitch, 1, rows, 1), boxes (128, 1, 128 or TN, 1)
   CUtensorMap tmap_sp, tmap_sq;  // scale tiles of 128 words: dims (128, groups, row tiles)
+  CUtensorMap tmap_out;          // where `vec`: dims (n, 1, m, 1), boxes of 128 bytes x 32 rows
   const float* scale_a;          // the tensors' scales, or NULL
   const float* scale_b;
   const void* bias;              // n values of bias_dtype, or NULL
@@ -168,37 +169,55 @@ __device__ __forceinline__ void fp4_gemm_store(const Fp4GemmParams& p, int64_t a
   else static_cast<float*>(p.out)[at] = v;
 }
 
+// 16-byte piece i of a lane's row in words: four fp32, or eight of a 16-bit type.
+template <int ELT>
+__device__ __forceinline__ uint4 fp4_piece(const Fp4GemmParams& p, const float* f) {
+  if constexpr (ELT == 4)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else if (p.out_dtype == DGXM_DTYPE_BF16)
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  else
+    return make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
+}
+
 // A warp's 32 rows x NC columns of finished values (a row a lane) from row
-// pr0 and column q0 of the output, through its staging rows of 128 bytes, so
-// that neighbouring lanes store neighbouring pieces: 16-byte piece c of row
-// r lies at piece c ^ (r & 7).  ELT: bytes of an output element.
+// pr0 and column q0 of the output.  They pass through staging rows of 128
+// bytes, 16-byte piece i of row r at piece i ^ (r & 7): the 128-byte swizzle,
+// so that a whole chunk goes out as one bulk store (rows on 16 bytes), which
+// leaves the warp to its arithmetic (9450 x 5120 x 256: 47 us with stores of
+// the lanes, 23 us), or, otherwise, neighbouring lanes store neighbouring
+// elements.  ELT: bytes of an output element.
 template <int NC, int ELT>
 __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* stage, const float (&v)[NC], int pr0,
                                                int q0, int lane) {
-  constexpr int kEach = 16 / ELT;                         // elements of a piece
+  constexpr int kEach = 16 / ELT;  // elements of a piece
   constexpr int kMost = 128 / ELT;
   constexpr int kCols = NC % kMost == 0 ? kMost : NC % (kMost / 2) == 0 ? kMost / 2 : NC;  // columns staged at one time
   static_assert(kCols <= kMost && NC % kCols == 0, "whole chunks");
   constexpr int kPieces = kCols / kEach;
-  char* out = static_cast<char*>(p.out);
+  const bool bulk = kCols == kMost && p.vec;
 #pragma unroll
   for (int c0 = 0; c0 < NC; c0 += kCols) {
     if (q0 + c0 >= p.q_rows) return;  // uniform over the warp
+    if (bulk) {
+      if (lane == 0) tma_store_wait_read();  // the last chunk has left the staging rows
+      __syncwarp();
+    }
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const float* f = v + c0 + i * kEach;
-      uint4 piece;
-      if constexpr (ELT == 4) {
-        piece = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-      } else if (p.out_dtype == DGXM_DTYPE_BF16) {
-        piece = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-      } else {
-        piece = make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
+    for (int i = 0; i < kPieces; ++i)
+      *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = fp4_piece<ELT>(p, v + c0 + i * kEach);
+    if (bulk) {
+      tma_store_fence();
+      __syncwarp();
+      if (lane == 0) {
+        if (pr0 < p.p_rows) tma_store_4d(&p.tmap_out, smem_u32(stage), q0 + c0, 0, pr0, 0);
+        tma_store_commit();
       }
-      *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = piece;
+      continue;
     }
     __syncwarp();
     if (p.vec && q0 + c0 + kCols <= p.q_rows) {
+      char* out = static_cast<char*>(p.out);
       const int i = lane % kPieces;
 #pragma unroll
       for (int r = lane / kPieces; r < 32; r += 32 / kPieces)
@@ -395,7 +414,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;
     constexpr int kCols = TN / 2;  // this warp's columns
-    const float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
+    float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
+    if (const float both = ga * gb; fabsf(both) >= 0x1p-126f && fabsf(both) <= 0x1p126f) {
+      ga = 1.f;
+      gb = both;
+    }
+    const uint64_t gab = pk2(gb, gb);
     const uint32_t acc_empty = PAIR ? mapa_shared(bar(C::kAccEmpty), 0) : bar(C::kAccEmpty);
     uint8_t* stage = staging + (warp - 2) * kGemmStageRows;
     int u = 0;
@@ -429,7 +453,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster(acc_empty + a * 8);
+        // relaxed: the reads of tensor memory are done (wait::ld), and a release
+        // would first wait for the last tile's stores
+        if constexpr (PAIR) mbar_arrive_cluster_relaxed(acc_empty + a * 8);
         else mbar_arrive(acc_empty + a * 8);
       }
       if (C::kSplits && p.split > 1) {
@@ -442,7 +468,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
       }
       float v[kCols];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) v[c] = __uint_as_float(r[c / 8][c % 8]) * ga * gb;
+      for (int c = 0; c < kCols; ++c) v[c] = __uint_as_float(r[c / 8][c % 8]);
+      if (ga != 1.f) {  // g_a g_b leaves fp32's range: one after the other
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) v[c] *= ga;
+      }
+#pragma unroll
+      for (int c = 0; c < kCols; c += 2) upk2(fmul2(pk2(v[c], v[c + 1]), gab), v[c], v[c + 1]);
       if (p.q_is_tokens) {  // neighbouring lanes hold neighbouring output columns
         if (pr0 + lane < p.p_rows) {
 #pragma unroll
@@ -458,6 +490,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         else fp4_store_rows<kCols, 2>(p, stage, v, pr0, q0, lane);
       }
     }
+    if (lane == 0) tma_store_wait_all();  // the staging rows outlive the stores
+    __syncwarp();
   }
   tc_fence_before();
   if (PAIR || (C::kSplits && p.split > 1)) cluster_sync();  // both CTAs' MMAs drained; or every partial sum is in place
@@ -498,20 +532,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
   }
 }
 
-// Tensor map of packed scales: tiles of 128 words, `groups` of them in a row
-// of tiles; a box is one stage's tiles of `tiles` row tiles, zero out of bounds.
-static int fp4_scale_map(CUtensorMap* map, const void* scales, int64_t groups, int64_t row_tiles, int atoms, int tiles) {
+// A 3-D tensor map (strides in bytes), zero out of bounds.
+static int fp4_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const cuuint64_t (&dims)[3],
+                   const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(DGXM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[4] = {128, (cuuint64_t)groups, (cuuint64_t)row_tiles, 1};
-  cuuint64_t strides[3] = {512, (cuuint64_t)groups * 512, (cuuint64_t)(groups * row_tiles) * 512};
-  cuuint32_t box[4] = {128, (cuuint32_t)atoms, (cuuint32_t)tiles, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<void*>(scales), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], 1}, st[3] = {strides[0], strides[1], strides[1] * dims[2]};
+  const cuuint32_t bx[4] = {box[0], box[1], box[2], 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, dt, 4, const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(DGXM_ERR_INVALID, "cuTensorMapEncodeTiled returned %d", (int)r);
   return DGXM_OK;
+}
+
+// Packed scales: tiles of 128 words, `groups` of them in a row of tiles; a box
+// is one stage's tiles of `tiles` row tiles.
+static int fp4_scale_map(CUtensorMap* map, const void* scales, int64_t groups, int64_t row_tiles, int atoms, int tiles) {
+  return fp4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, {128, (cuuint64_t)groups, (cuuint64_t)row_tiles},
+                 {512, (cuuint64_t)groups * 512}, {128, (cuuint32_t)atoms, (cuuint32_t)tiles}, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 struct Fp4Operand {
@@ -533,6 +571,14 @@ static int fp4_gemm_launch(Fp4GemmParams& p, const Fp4Operand& po, const Fp4Oper
     return rc;
   if (int rc = fp4_scale_map(&p.tmap_sp, po.scales, groups, (po.rows + 127) / 128, C::kAtoms, 1)) return rc;
   if (int rc = fp4_scale_map(&p.tmap_sq, qo.scales, groups, (qo.rows + 127) / 128, C::kAtoms, C::kQTiles)) return rc;
+  if (p.vec && !p.q_is_tokens) {  // boxes of 128 bytes x 32 rows
+    const int elt = p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2;
+    const cuuint64_t row = static_cast<cuuint64_t>(p.ld_out) * elt;
+    if (int rc = fp4_map(&p.tmap_out, elt == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, p.out,
+                         {(cuuint64_t)p.q_rows, 1, (cuuint64_t)p.p_rows}, {row, row}, {(cuuint32_t)(128 / elt), 1, 32},
+                         CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
   p.p_tiles = (p.p_rows + C::kRows - 1) / C::kRows;
   p.q_tiles = (p.q_rows + TN - 1) / TN;
   const int tiles = p.p_tiles * p.q_tiles, share = PAIR ? 2 : p.split;
@@ -575,17 +621,19 @@ struct Fp4Cut {
   bool q_is_tokens;
 };
 
-// The cut whose waves of tiles take the least time by what one tile took
-// (microseconds a stage of K and a tile, nvfp4, measured with K = 5120 and
-// 256 on products of one to nine waves): narrow tiles where only they fill
-// the SMs, wide ones, which load the least for what they compute, where those do too.
+// The cut whose waves of tiles take the least time by what one wave took
+// (microseconds a stage of K, a tile, and at the least; nvfp4, 9450 x 5120 x
+// 256, 1024 and 5120, for the narrowest 16 x 1280 .. 5120 x 5120): narrow
+// tiles where only they fill the SMs, wide ones, which load the least for
+// what they compute, where those do too.
 static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
   struct Kind {
     int tn, rows, at_once;
-    double stage, tile;
+    double stage, tile, least;
   };
-  static const Kind kinds[] = {{16, 128, 148, 0.13, 0.6}, {32, 128, 148, 0.15, 0.6}, {64, 128, 148, 0.26, 0.7},
-                               {128, 128, 148, 0.31, 1.0}, {192, 128, 148, 0.43, 1.2}, {256, 256, 74, 0.47, 1.4}};
+  static const Kind kinds[] = {{16, 128, 148, 0.16, 1.0, 1.0},  {32, 128, 148, 0.17, 1.0, 1.0},
+                               {64, 128, 148, 0.24, 0.6, 1.0},  {128, 128, 148, 0.29, 0.8, 1.1},
+                               {192, 128, 148, 0.42, 1.1, 2.2}, {256, 256, 74, 0.42, 1.75, 2.2}};
   Fp4Cut best{128, 1, false};
   double least = 1e30;
   const bool tokens = m <= n;  // with one tile of columns, the narrow side is Q
@@ -598,7 +646,8 @@ static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
     for (int split = 1; split <= (kind.tn <= 64 ? 8 : 1) && split <= k_tiles; split *= 2) {
       if (split > 1 && tiles * split > 148) break;
       const int64_t waves = (tiles * split + kind.at_once - 1) / kind.at_once;
-      const double us = waves * ((k_tiles + split - 1) / split * kind.stage + kind.tile) + (split > 1 ? 0.8 : 0.0);
+      const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile, kind.least) +
+                        (split > 1 ? 0.4 : 0.0);
       if (us < least) {
         least = us;
         best = {kind.tn, split, one && tokens};
