@@ -78,25 +78,46 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t* r) {
                : "memory");
 }
 
-// The n <= N values at p (the rest zero).  VEC: p is 16-byte aligned, wide: 32-byte.
+// The n <= N values at p (the rest zero).  VEC: p is 16-byte aligned, wide:
+// 32-byte.  Otherwise, and for a row's last values, p's 16-byte words are
+// loaded -- those that hold one of the values, none else -- and shifted.
 template <typename T, int N, bool VEC>
 __device__ __forceinline__ Fp4Raw<T, N> fp4_load(const T* p, int n, bool wide) {
   Fp4Raw<T, N> r;
+  uint32_t* out = reinterpret_cast<uint32_t*>(&r);
+  constexpr int kWords = static_cast<int>(sizeof(r)) / 4;
   if (VEC && n >= N && wide) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(r) / 32); ++i) ld_global_32(p + i * (32 / sizeof(T)), reinterpret_cast<uint32_t*>(&r) + 8 * i);
-  } else if (VEC && n >= N) {
+    for (int i = 0; i < kWords / 8; ++i) ld_global_32(p + i * (32 / sizeof(T)), out + 8 * i);
+    return r;
+  }
+  if (VEC && n >= N) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i)
-      reinterpret_cast<uint4*>(&r)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  } else {
+    for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(out)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    return r;
+  }
+  const uint32_t off = reinterpret_cast<uintptr_t>(p) & 15u;  // bytes of the first word before p
+  const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+  const int bytes = n > 0 ? min(n, N) * static_cast<int>(sizeof(T)) : 0;
+  uint32_t w[kWords + 4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if constexpr (sizeof(T) == 4)
-        reinterpret_cast<uint32_t*>(&r)[i] = i < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0u;
-      else
-        reinterpret_cast<uint16_t*>(&r)[i] = i < n ? __ldg(reinterpret_cast<const uint16_t*>(p) + i) : uint16_t(0);
-    }
+  for (int i = 0; i < kWords / 4 + 1; ++i) {
+    const bool in = bytes > 0 && 16 * i < static_cast<int>(off) + bytes;
+    const uint4 v = in ? __ldg(from + i) : make_uint4(0u, 0u, 0u, 0u);
+    w[4 * i] = v.x;
+    w[4 * i + 1] = v.y;
+    w[4 * i + 2] = v.z;
+    w[4 * i + 3] = v.w;
+  }
+#pragma unroll
+  for (int i = 0; i < kWords + 2; ++i) w[i] = (off & 8u) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < kWords + 1; ++i) w[i] = (off & 4u) ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    const uint32_t v = __funnelshift_r(w[i], w[i + 1], 8 * (off & 3u));
+    const int left = bytes - 4 * i;  // bytes of this word that are values
+    out[i] = left >= 4 ? v : left == 2 ? v & 0xFFFFu : 0u;
   }
   return r;
 }
@@ -377,12 +398,18 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_dequantize_kernel(const __gri
   pdl_wait();
   const float g = FORMAT == DGXM_FP4_NVFP4 ? *static_cast<const float*>(p.scale) : 1.f;
   const uint64_t gg = pk2(g, g);
+  const int lane = threadIdx.x & 31;
   const uint32_t step = gridDim.x * kFp4Threads;
-  for (uint64_t i0 = blockIdx.x * kFp4Threads + threadIdx.x; i0 < p.items; i0 += step) {
-    const uint32_t item = static_cast<uint32_t>(i0);
+  for (uint64_t i0 = blockIdx.x * kFp4Threads + threadIdx.x - lane; i0 < p.items; i0 += step) {
+    const uint32_t item = static_cast<uint32_t>(i0) + lane;
+    const bool live = item < p.items;
     const uint32_t row = item / p.per_row, c16 = item - row * p.per_row;
-    const uint2 code = __ldg(reinterpret_cast<const uint2*>(p.values + row * p.pitch) + c16);
-    const uint32_t byte = __ldg(p.scales + fp4_scale_at(row, c16 * 16 / B, p.groups));
+    uint2 code = make_uint2(0u, 0u);
+    uint32_t byte = 0;
+    if (live) {
+      code = __ldg(reinterpret_cast<const uint2*>(p.values + row * p.pitch) + c16);
+      byte = __ldg(p.scales + fp4_scale_at(row, c16 * 16 / B, p.groups));
+    }
     __half2 h[2][4];
     fp4_decode8(code.x, h[0]);
     fp4_decode8(code.y, h[1]);
@@ -402,7 +429,7 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_dequantize_kernel(const __gri
       out.v[2 * i] = static_cast<T>(a);
       out.v[2 * i + 1] = static_cast<T>(b);
     }
-    const int n = p.cols - static_cast<int>(c16) * 16;
+    const int n = live ? p.cols - static_cast<int>(c16) * 16 : 0;
     T* dst = reinterpret_cast<T*>(const_cast<char*>(p.x)) + row * p.row_stride + int64_t(c16) * 16;
     if (VEC && n >= 16 && p.wide) {
 #pragma unroll
@@ -412,10 +439,28 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_dequantize_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(out) / 16); ++i)
         reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(&out)[i];
-    } else {
+    } else if (VEC) {  // a row's last values
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (i < n) dst[i] = out.v[i];
+    } else {
+      // Rows off 16 bytes: the warp's runs pass through shared memory, and
+      // neighbouring lanes store neighbouring values.
+      constexpr int kPitch = 16 * sizeof(T) + 16;  // 16 bytes on: neighbouring runs lie in other banks
+      __shared__ __align__(16) uint8_t runs[kFp4Threads * kPitch];
+      uint8_t* warp_runs = runs + (threadIdx.x - lane) * kPitch;
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(out) / 16); ++i)
+        reinterpret_cast<uint4*>(warp_runs + lane * kPitch)[i] = reinterpret_cast<const uint4*>(&out)[i];
+      __syncwarp();
+#pragma unroll 4
+      for (int k = 0; k < 16; ++k) {
+        const int run = 2 * k + lane / 16, e = lane % 16;
+        T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), run));
+        const int many = __shfl_sync(0xffffffffu, n, run);
+        if (e < many) to[e] = reinterpret_cast<const T*>(warp_runs + run * kPitch)[e];
+      }
+      __syncwarp();
     }
   }
 }
