@@ -38,6 +38,24 @@ def _check_format(format: str) -> int:
     return FORMATS[format]
 
 
+class _Layout:
+    """Where the parts of a packed tensor lie in one buffer, on 256 bytes each;
+    the scratch of its quantisation follows them."""
+
+    __slots__ = ("shape", "format", "rows", "cols", "scales", "scale", "scratch", "total", "devices")
+
+    def __init__(self, shape, format: str, index: int, scratch: int) -> None:
+        up = lambda n: (n + 255) // 256 * 256
+        self.shape, self.format = tuple(shape), format
+        self.rows, self.cols = math.prod(shape[:-1]), shape[-1]
+        self.scales = up(math.prod(values_shape(self.rows, self.cols)))
+        end = self.scales + up(math.prod(scales_shape(self.rows, self.cols, format)))
+        self.scale = end if format == "nvfp4" else None
+        self.scratch = end + (256 if format == "nvfp4" else 0)
+        self.total = max(self.scratch + scratch, 256)
+        self.devices = (index, index, index if format == "nvfp4" else None)
+
+
 class Fp4Tensor:
     """A (..., cols) tensor in 4 bits, its leading dimensions folded into rows.
 
@@ -47,7 +65,7 @@ class Fp4Tensor:
     None for mxfp4.  quantize_fp4 makes them; a weight kept in this layout is
     wrapped as it is."""
 
-    __slots__ = ("values", "scales", "shape", "format", "scale", "rows", "cols")
+    __slots__ = ("shape", "format", "rows", "cols", "_values", "_scales", "_scale", "_buffer", "_offsets", "_devices")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, shape, format: str,
                  scale: torch.Tensor | None = None) -> None:
@@ -66,23 +84,53 @@ class Fp4Tensor:
         if (scale is None) != (format == "mxfp4") or (scale is not None and (
                 scale.dtype != torch.float32 or scale.numel() != 1)):
             raise ValueError("an nvfp4 tensor has one fp32 scale, an mxfp4 tensor none")
-        self.values, self.scales, self.shape, self.format, self.scale = values, scales, shape, format, scale
-        self.rows, self.cols = rows, cols
+        self.shape, self.format, self.rows, self.cols = shape, format, rows, cols
+        self._values, self._scales, self._scale, self._buffer, self._offsets = values, scales, scale, None, None
+        self._devices = (values.get_device(), scales.get_device(), None if scale is None else scale.get_device())
 
     @classmethod
-    def _made(cls, values, scales, shape, format, scale, rows, cols) -> "Fp4Tensor":
-        """Of buffers that this module has just allocated."""
+    def _made(cls, buffer: torch.Tensor, layout: "_Layout") -> "Fp4Tensor":
+        """In one fresh buffer of layout.total bytes; its parts are views made on demand."""
         t = cls.__new__(cls)
-        t.values, t.scales, t.shape, t.format, t.scale, t.rows, t.cols = values, scales, shape, format, scale, rows, cols
+        t.shape, t.format, t.rows, t.cols = layout.shape, layout.format, layout.rows, layout.cols
+        t._values = t._scales = t._scale = None
+        t._buffer, t._offsets, t._devices = buffer, layout, layout.devices
         return t
 
     @property
-    def device(self) -> torch.device:
-        return self.values.device
+    def values(self) -> torch.Tensor:
+        if self._values is None:
+            shape = values_shape(self.rows, self.cols)
+            self._values = self._buffer[:math.prod(shape)].view(shape)
+        return self._values
 
-    def _devices(self):
-        return (self.values.get_device(), self.scales.get_device(),
-                None if self.scale is None else self.scale.get_device())
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            shape, at = scales_shape(self.rows, self.cols, self.format), self._offsets.scales
+            self._scales = self._buffer[at:at + math.prod(shape)].view(shape)
+        return self._scales
+
+    @property
+    def scale(self) -> torch.Tensor | None:
+        if self._scale is None and self._buffer is not None and self._offsets.scale is not None:
+            at = self._offsets.scale
+            self._scale = self._buffer[at:at + 4].view(torch.float32).view(())
+        return self._scale
+
+    @property
+    def device(self) -> torch.device:
+        return (self._values if self._buffer is None else self._buffer).device
+
+    def _tensors(self):
+        return (self._values, self._scales, self._scale) if self._buffer is None else (self._buffer,)
+
+    def _pointers(self):
+        """Addresses of the values, the scales and the scale."""
+        if self._buffer is None:
+            return self._values.data_ptr(), self._scales.data_ptr(), _ptr(self._scale)
+        base, at = self._buffer.data_ptr(), self._offsets
+        return base, base + at.scales, None if at.scale is None else base + at.scale
 
     def __repr__(self) -> str:
         return f"Fp4Tensor({self.shape}, {self.format}, {self.device})"
@@ -108,7 +156,7 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
     given = scale if isinstance(scale, torch.Tensor) else None
     key = ("q", x.shape, x.stride(), x.dtype, x.get_device(), format,
            scale if given is None else (given.dtype, given.get_device(), given.numel()),
-           None if out is None else (out.shape, out.format, out._devices()))
+           None if out is None else (out.shape, out.format, out._devices))
 
     def make():
         code = _check_format(format)
@@ -128,7 +176,7 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
         if out is not None:
             if out.shape != tuple(x.shape) or out.format != format:
                 raise ValueError(f"out is {out}, x is {tuple(x.shape)} for {format}")
-            _require_cuda(x, out.values, out.scales, out.scale)
+            _require_cuda(x, *out._tensors())
         desc = _lib.Fp4Desc()
         desc.rows, desc.cols, desc.format = math.prod(x.shape[:-1]), x.shape[-1], code
         desc.dtype = _dtype_code(x.dtype)
@@ -140,21 +188,21 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
         folds = x.numel() == 0 or (flat.data_ptr() == x.data_ptr()
                                    and (desc.rows == 1 or flat.stride(0) >= desc.cols))  # not overlapping or expanded
         desc.row_stride = flat.stride(0) if folds and desc.rows > 1 else desc.cols
-        shape = tuple(x.shape)
-        return (desc, folds, values_shape(desc.rows, desc.cols), scales_shape(desc.rows, desc.cols, format), shape,
-                _lib.load().dgxm_quantize_fp4_workspace() if format == "nvfp4" and scale is None else 0,
-                math.prod(shape[:-1]), shape[-1])
+        need = _lib.load().dgxm_quantize_fp4_workspace() if format == "nvfp4" and scale is None else 0
+        return desc, folds, need, _Layout(x.shape, format, x.get_device(), need)
 
-    desc, folds, vshape, sshape, shape, need, rows, cols = plan(key, make)
+    desc, folds, need, layout = plan(key, make)
     no_graph("", x, given)
     if not folds:
-        x = x.reshape(-1, cols).contiguous()
+        x = x.reshape(-1, layout.cols).contiguous()
     if out is None:
-        out = Fp4Tensor._made(x.new_empty(vshape, dtype=torch.uint8), x.new_empty(sshape, dtype=torch.uint8), shape,
-                              format, x.new_empty((), dtype=torch.float32) if format == "nvfp4" else None, rows, cols)
-    work = x.new_empty(need, dtype=torch.uint8) if need else None
-    launch("dgxm_quantize_fp4", x.get_device(), desc, x.data_ptr(), _ptr(given), out.values.data_ptr(),
-           out.scales.data_ptr(), _ptr(out.scale), _ptr(work), need)
+        buffer = x.new_empty(layout.total, dtype=torch.uint8)
+        out = Fp4Tensor._made(buffer, layout)
+        work = buffer.data_ptr() + layout.scratch
+    else:
+        buffer = x.new_empty(need, dtype=torch.uint8) if need else None
+        work = _ptr(buffer)
+    launch("dgxm_quantize_fp4", layout.devices[0], desc, x.data_ptr(), _ptr(given), *out._pointers(), work, need)
     return out
 
 
@@ -163,15 +211,14 @@ def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
     """The values that t stands for, in t.shape and dtype (dgxm_dequantize_fp4):
     code * block scale * scale in fp32, then rounded to dtype.  out: a
     contiguous tensor to write into."""
-    key = ("d", t.rows, t.cols, t.format, dtype, t._devices(),
+    key = ("d", t.shape, t.format, dtype, t._devices,
            None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
 
     def make():
-        _require_cuda(t.values, t.scales, t.scale, out)
+        _require_cuda(*t._tensors(), out)
         if dtype not in _FLOATS:
             raise TypeError(f"dtype {dtype} is not bf16, fp16 or fp32")
-        if out is not None and (math.prod(out.shape) != t.rows * t.cols or out.dtype != dtype
-                                or not out.is_contiguous()):
+        if out is not None and (out.shape != t.shape or out.dtype != dtype or not out.is_contiguous()):
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} is not a contiguous {t.shape} {dtype} tensor")
         desc = _lib.Fp4Desc()
         desc.rows, desc.cols, desc.row_stride, desc.format = t.rows, t.cols, t.cols, FORMATS[t.format]
@@ -180,11 +227,8 @@ def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
 
     desc = plan(key, make)
     if out is None:
-        out = t.values.new_empty(t.shape, dtype=dtype)
-    elif out.shape != t.shape:
-        raise ValueError(f"out {tuple(out.shape)} is not a {t.shape} tensor")
-    launch("dgxm_dequantize_fp4", t.values.get_device(), desc, t.values.data_ptr(), t.scales.data_ptr(),
-           _ptr(t.scale), out.data_ptr())
+        out = t._tensors()[0].new_empty(t.shape, dtype=dtype)
+    launch("dgxm_dequantize_fp4", t._devices[0], desc, *t._pointers(), out.data_ptr())
     return out
 
 
@@ -197,12 +241,12 @@ def fp4_matmul(a: Fp4Tensor, b: Fp4Tensor, *, bias: torch.Tensor | None = None,
     types.  fp32 accumulation on the block-scaled tensor cores, one rounding.
     out: a tensor of the result's shape and out_dtype to write into, with
     contiguous columns and rows that fold into one stride."""
-    key = ("m", a.shape, a.format, a._devices(), b.shape, b.format, b._devices(), out_dtype,
+    key = ("m", a.shape, a.format, a._devices, b.shape, b.format, b._devices, out_dtype,
            None if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.get_device()),
            None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
 
     def make():
-        _require_cuda(a.values, a.scales, a.scale, b.values, b.scales, b.scale, bias, out)
+        _require_cuda(*a._tensors(), *b._tensors(), bias, out)
         if a.format != b.format:
             raise ValueError(f"a product of {a.format} and {b.format}: both operands have one format")
         if a.cols != b.cols:
@@ -233,7 +277,6 @@ def fp4_matmul(a: Fp4Tensor, b: Fp4Tensor, *, bias: torch.Tensor | None = None,
     desc, shape = plan(key, make)
     no_graph("", bias)
     if out is None:
-        out = a.values.new_empty(shape, dtype=out_dtype)
-    launch("dgxm_fp4_matmul", a.values.get_device(), desc, a.values.data_ptr(), a.scales.data_ptr(), _ptr(a.scale),
-           b.values.data_ptr(), b.scales.data_ptr(), _ptr(b.scale), _ptr(bias), out.data_ptr())
+        out = a._tensors()[0].new_empty(shape, dtype=out_dtype)
+    launch("dgxm_fp4_matmul", a._devices[0], desc, *a._pointers(), *b._pointers(), _ptr(bias), out.data_ptr())
     return out

@@ -128,12 +128,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
     desc = plan(key, make)
     no_graph(_GRADS, q, k, norm_q_w, norm_k_w)
     if q_out is None:
-        q_out = q.new_empty(q.shape)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_in_place("q_out", q_out, q)
     if k is not None:
         if k_out is None:
-            k_out = k.new_empty(k.shape)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         else:
             _check_in_place("k_out", k_out, k)
     launch("dgxm_qk_norm_rope", q.get_device(), desc, q.data_ptr(), _ptr(k), _ptr(norm_q_w), _ptr(norm_k_w),
@@ -179,8 +179,8 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
 
     desc, need = plan(key, make)
     no_graph(_GRADS, dq, dk, q, k, norm_q_w, norm_k_w)
-    gq = q.new_empty(q.shape)
-    gk = None if k is None else k.new_empty(k.shape)
+    gq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    gk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     gwq = None if norm_q_w is None else torch.empty_like(norm_q_w)
     gwk = None if norm_k_w is None else torch.empty_like(norm_k_w)
     work = None if gwq is None else q.new_empty(need, dtype=torch.uint8)
