@@ -16,8 +16,10 @@
 // shared memory, where each lane finds its own values (and the halves order
 // its partners) again: loads in flight cost no registers, and the token's
 // cosines and sines and the head weight, which serve every row of the chunk,
-// are fetched and multiplied with one another meanwhile.  The arithmetic runs
-// on pairs of fp32, two rows at a time.
+// are fetched and multiplied with one another meanwhile.  The forward's
+// arithmetic runs on pairs of fp32, two rows at a time (72 us against 78 with
+// single values, 9450 x 80 heads of 128 in bf16, halves); the gradient's, on more
+// registers, on single values (108 us against 115 adjacent).
 //
 // Everything between the load and the store is fp32 and is rounded once, to
 // the tensors' type.  (The fused scatter of prologue.cu rounds after the
@@ -35,7 +37,7 @@ constexpr int kQkThreads = 128;
 constexpr int kQkWarps = kQkThreads / 32;
 constexpr int kQkRing = 4096;     // bytes of rows a warp has under way, of each tensor it reads
 constexpr int kQkFwdPerSm = 8;    // blocks of an SM: 64 registers a thread, 128 KB of rows under way
-constexpr int kQkBwdPerSm = 6;    // 80 registers a thread, 192 KB
+constexpr int kQkBwdPerSm = 6;    // 80 registers a thread, 192 KB (5 blocks of 96 registers: 113 us against 108 adjacent, 118 against 121 halves)
 constexpr int kQkBwdBlocks = 148 * kQkBwdPerSm;  // as many as run at one time, each with one partial sum of dw
 
 // Rows a lane group has under way.
@@ -277,19 +279,19 @@ __device__ __forceinline__ void qk_angles(const QkNormParams& p, const QkItem& i
 // A value that is not rotated gets itself.
 template <typename T, int ROT>
 __device__ __forceinline__ void qk_halves(const QkNormParams& p, int sub, int lane, uint8_t* ring, int u,
-                                          uint64_t (&q)[4]) {
+                                          float (&f)[8]) {
   const int e0 = 8 * sub, half = p.rot / 2;
   if constexpr (ROT == kQkHalves) {
     const int d = e0 < half ? half / 8 : e0 < p.rot ? -(half / 8) : 0;
-    qk_pairs_of<T>(qk_take<T>(ring, u, lane + d), q);
+    const Qk8<T> r = qk_take<T>(ring, u, lane + d);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = qk_widen<T>(r.v[i]);
   } else {
-    float f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = e0 + i, to = e < half ? e + half : e < p.rot ? e - half : e;
       f[i] = qk_widen<T>(qk_take1<T>(ring, u, lane - sub + to / 8, to % 8));
     }
-    qk_pair(f, q);
   }
 }
 
@@ -301,7 +303,9 @@ __device__ __forceinline__ void qk_rotate(const QkNormParams& p, int sub, int la
                                           uint64_t (&y)[4]) {
   uint64_t q[4];
   if constexpr (ROT != kQkAdjacent) {
-    qk_halves<T, ROT>(p, sub, lane, ring, u, q);
+    float f[8];
+    qk_halves<T, ROT>(p, sub, lane, ring, u, f);
+    qk_pair(f, q);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[j] = x[j ^ 1];
@@ -321,6 +325,24 @@ __device__ __forceinline__ void qk_rotate(const QkNormParams& p, int sub, int la
 #pragma unroll
     for (int i = 0; i < 8; ++i) yf[i] = 8 * sub + i < p.rot ? zf[i] : yf[i];
     qk_pair(yf, y);
+  }
+}
+
+// The same on single values.
+template <typename T, int ROT>
+__device__ __forceinline__ void qk_rotate(const QkNormParams& p, int sub, int lane, const float (&c)[8],
+                                          const float (&s)[8], uint8_t* ring, int u, float (&x)[8]) {
+  float q[8];
+  if constexpr (ROT != kQkAdjacent) {
+    qk_halves<T, ROT>(p, sub, lane, ring, u, q);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = x[i ^ 1];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = fmaf(q[i], s[i], x[i] * c[i]);
+    x[i] = p.rot == p.dim || 8 * sub + i < p.rot ? y : x[i];
   }
 }
 
@@ -468,13 +490,10 @@ __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kern
       qk_blank<T>(ring, lane);
       qk_blank<T>(xring, lane);
     }
-    uint64_t dw[4] = {0, 0, 0, 0};
-    uint64_t wv[4];
-    {
-      float w[8];
-      qk_weight<T>(p, t, sub, in, w);
-      qk_pair(w, wv);
-    }
+    float dw[8], w[8];
+    qk_weight<T>(p, t, sub, in, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[i] = 0.f;
     const uint32_t items = p.tokens * p.chunks[t];
     const int64_t step = p.os[t][2] * kGroups;
     for (uint32_t item = (blockIdx.x * kQkWarps + warp + warps - skip) % warps; item < items; item += warps) {
@@ -494,61 +513,49 @@ __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kern
           qk_blank_row<T>(xring, u, lane);
         }
       }
-      uint64_t a[4], b[4];
-      if constexpr (ROT != kQkNoTurn) {
-        float c[8], s[8];
-        qk_angles<ROT, -1>(p, it, sub, c, s);
-        qk_pair(c, a);
-        qk_pair(s, b);
-      }
+      float c[8], s[8];
+      if constexpr (ROT != kQkNoTurn) qk_angles<ROT, -1>(p, it, sub, c, s);
       cp_async_wait_all();
       __syncwarp();
       T* out = reinterpret_cast<T*>(p.out[t]) + it.b * p.os[t][0] + it.l * p.os[t][1] + (it.first + group) * p.os[t][2] + 8 * sub;
       const int n = (end - it.first + kGroups - 1) / kGroups;
       for (int u = 0; u < n; ++u, out += step) {
-        uint64_t g[4];
-        qk_pairs_of<T>(qk_take<T>(ring, u, lane), g);
-        if constexpr (ROT != kQkNoTurn) {
-          uint64_t y[4];
-          qk_rotate<T, ROT>(p, sub, lane, a, b, ring, u, g, y);
+        const Qk8<T> raw = qk_take<T>(ring, u, lane);
+        float g[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) g[j] = y[j];
-        }
+        for (int i = 0; i < 8; ++i) g[i] = qk_widen<T>(raw.v[i]);
+        if constexpr (ROT != kQkNoTurn) qk_rotate<T, ROT>(p, sub, lane, c, s, ring, u, g);
         if (p.norm) {
-          uint64_t x[4];
-          qk_pairs_of<T>(qk_take<T>(xring, u, lane), x);
-          uint64_t sx = fmul2(x[0], x[0]), sg = fmul2(fmul2(g[0], wv[0]), x[0]);
+          const Qk8<T> xraw = qk_take<T>(xring, u, lane);
+          float x[8], xx = 0.f, gx = 0.f;
 #pragma unroll
-          for (int j = 1; j < 4; ++j) {
-            sx = ffma2(x[j], x[j], sx);
-            sg = ffma2(fmul2(g[j], wv[j]), x[j], sg);
+          for (int i = 0; i < 8; ++i) {
+            x[i] = qk_widen<T>(xraw.v[i]);
+            xx = fmaf(x[i], x[i], xx);
+            gx = fmaf(g[i] * w[i], x[i], gx);
           }
-          const float xx = qk_group_sum<G>(qk_total(sx)), gx = qk_group_sum<G>(qk_total(sg));
+          xx = qk_group_sum<G>(xx);
+          gx = qk_group_sum<G>(gx);
           const float r = rsqrtf(fmaf(xx, p.inv_dim, p.eps));
           const float m = -gx * r * p.inv_dim;  // -mean(g w n); n and m stay in range however small x is
-          const uint64_t rr = pk2(r, r), mm = pk2(m, m);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint64_t nj = fmul2(x[j], rr);
-            dw[j] = ffma2(g[j], nj, dw[j]);
-            g[j] = fmul2(rr, ffma2(nj, mm, fmul2(g[j], wv[j])));
+          for (int i = 0; i < 8; ++i) {
+            const float n1 = x[i] * r;
+            dw[i] = fmaf(g[i], n1, dw[i]);
+            g[i] = r * fmaf(n1, m, g[i] * w[i]);
           }
         }
-        float gf[8];
-        qk_unpair(g, gf);
-        if (in && u < mine) qk_store<T, VEC>(out, gf);
+        if (in && u < mine) qk_store<T, VEC>(out, g);
       }
       __syncwarp();  // every lane has read its values and partners: the next item's may come
     }
     skip = items % warps;
     if (p.partial == nullptr) continue;  // uniform over the grid
-    float df[8];
-    qk_unpair(dw, df);
     __syncthreads();
     float* sums = reinterpret_cast<float*>(qk_smem);  // (warps, 256)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = df[i];
+      float v = dw[i];
 #pragma unroll
       for (int o = G; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (group == 0 && in) sums[warp * 256 + 8 * sub + i] = v;
