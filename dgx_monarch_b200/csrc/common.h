@@ -41,20 +41,25 @@ cudaError_t set_smem_limit_once(Kernel kern, int bytes, std::atomic<uint64_t>& d
 }
 
 // Launch a kernel whose prologue may overlap the end of the kernel before it
-// in the stream (it waits with pdl_wait before it touches global memory).
+// in the stream (it waits with pdl_wait before it touches global memory), in
+// clusters of `cluster` blocks.
 template <typename Params>
 cudaError_t launch_overlapped(void (*kernel)(Params), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
-                              const Params& params) {
+                              const Params& params, unsigned cluster = 1) {
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 

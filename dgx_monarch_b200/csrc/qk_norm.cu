@@ -38,6 +38,9 @@ constexpr int kQkWarps = kQkThreads / 32;
 constexpr int kQkRing = 4096;     // bytes of rows a warp has under way, of each tensor it reads
 constexpr int kQkFwdPerSm = 8;    // blocks of an SM: 64 registers a thread, 128 KB of rows under way
 constexpr int kQkBwdPerSm = 6;    // 80 registers a thread, 192 KB (5 blocks of 96 registers: 113 us against 108 adjacent, 118 against 121 halves)
+// Up to here a gradient with weights is one launch of a cluster, beyond a second launch adds the blocks (us at 8, 40, 80
+// and 160 warps of 128 bf16: 4.3, 5.3, 6.4, 8.6 against 4.9, 4.7, 4.7, 4.9; a launch and a workspace are 4.5 of host time).
+constexpr int kQkClusterWarps = 64;
 constexpr int kQkBwdBlocks = 148 * kQkBwdPerSm;  // as many as run at one time, each with one partial sum of dw
 
 // Rows a lane group has under way.
@@ -58,6 +61,8 @@ struct QkNormParams {
   const float* rope;  // (seq, rot / 2, 2) cosines and sines, or NULL
   int64_t rope_sb;    // floats between batch items (0: shared)
   float* partial;     // backward: (grid, 2, head_dim) sums of g n, or NULL
+  void* gw[2];        // backward on one cluster: the weights' gradients themselves
+  int gw_dtype, cluster;  // cluster: its blocks (the whole grid), or 0
   int heads[2], chunks[2];  // chunks: warps for one token's heads of the tensor
   uint32_t seq, tokens;     // tokens: batch * seq
   int rows;                 // rows of a chunk for each lane group of its warp
@@ -397,6 +402,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkFwdPerSm) qk_norm_rope_kernel(c
   extern __shared__ __align__(16) uint8_t qk_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = qk_smem + warp * kQkRing;
+  pdl_wait();
   uint32_t item = blockIdx.x * kQkWarps + warp;
   const uint32_t q_items = p.tokens * p.chunks[0];
   const int t = item >= q_items;
@@ -470,10 +476,18 @@ __global__ void __launch_bounds__(kQkThreads, kQkFwdPerSm) qk_norm_rope_kernel(c
   }
 }
 
+__device__ __forceinline__ void qk_store_weight_grad(void* out, int dtype, int e, float v) {
+  if (out == nullptr) return;
+  if (dtype == DGXM_DTYPE_F32) static_cast<float*>(out)[e] = v;
+  else if (dtype == DGXM_DTYPE_F16) static_cast<__half*>(out)[e] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(v);
+}
+
 // Gradients.  The blocks stride over q's items, then over k's; each lane adds
 // g n of its eight columns over all the rows it meets, the block sums its
-// warps in a fixed order, and qk_weight_grad_kernel sums the blocks: no
-// atomics, so the same call gives the same bits.
+// warps in a fixed order, and the blocks' sums are added in order by
+// qk_weight_grad_kernel, or, in a call small enough for one cluster, by the
+// cluster itself: no atomics, so the same call gives the same bits.
 template <typename T, int G, int ROT, bool VEC>
 __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kernel(const __grid_constant__ QkNormParams p) {
   constexpr int kGroups = 32 / G;
@@ -481,10 +495,14 @@ __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kern
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = qk_smem + warp * (2 * kQkRing);
   uint8_t* xring = ring + kQkRing;
+  pdl_wait();
   const int sub = lane % G, group = lane / G;
   const bool in = 8 * sub < p.dim;
   const uint32_t warps = gridDim.x * kQkWarps;
   uint32_t skip = 0;  // q's items taken: k's go on with the next warp
+  float total[2][256 / kQkThreads];  // this thread's columns of the block's sums
+#pragma unroll
+  for (int j = 0; j < 256 / kQkThreads; ++j) total[0][j] = total[1][j] = 0.f;
   for (int t = 0; t < 2; ++t) {
     if (!in) {
       qk_blank<T>(ring, lane);
@@ -550,7 +568,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kern
       __syncwarp();  // every lane has read its values and partners: the next item's may come
     }
     skip = items % warps;
-    if (p.partial == nullptr) continue;  // uniform over the grid
+    if (p.partial == nullptr && p.cluster == 0) continue;  // uniform over the grid
     __syncthreads();
     float* sums = reinterpret_cast<float*>(qk_smem);  // (warps, 256)
 #pragma unroll
@@ -561,14 +579,42 @@ __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kern
       if (group == 0 && in) sums[warp * 256 + 8 * sub + i] = v;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < p.dim; e += kQkThreads) {
+#pragma unroll
+    for (int j = 0; j < 256 / kQkThreads; ++j) {
+      const int e = threadIdx.x + j * kQkThreads;
+      if (e >= p.dim) break;
       float v = 0.f;
 #pragma unroll
       for (int k = 0; k < kQkWarps; ++k) v += sums[k * 256 + e];
-      p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + t) * p.dim + e] = v;
+      if (t == 0) total[0][j] = v;
+      else total[1][j] = v;
+      if (p.cluster == 0) p.partial[(static_cast<int64_t>(blockIdx.x) * 2 + t) * p.dim + e] = v;
     }
     __syncthreads();
   }
+  if (p.cluster == 0) return;  // uniform over the grid
+  // The blocks' sums in rank order, each block a share of the columns.
+  float* mine = reinterpret_cast<float*>(qk_smem);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int j = 0; j < 256 / kQkThreads; ++j)
+      if (threadIdx.x + j * kQkThreads < p.dim) mine[t * 256 + threadIdx.x + j * kQkThreads] = total[t][j];
+  cluster_sync();
+  for (int i = blockIdx.x * kQkThreads + threadIdx.x; i < 2 * p.dim; i += p.cluster * kQkThreads) {
+    const int t = i >= p.dim, e = i - t * p.dim;
+    float v = 0.f;
+    for (int r = 0; r < p.cluster; ++r) {
+      float other;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                   : "=f"(other)
+                   : "r"(mapa_shared(smem_u32(mine + t * 256 + e), r))
+                   : "memory");
+      v += other;
+    }
+    qk_store_weight_grad(p.gw[t], p.gw_dtype, e, v);
+  }
+  cluster_sync();  // no block leaves while another reads its sums
 }
 
 struct QkWeightGradParams {
@@ -595,10 +641,7 @@ __global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const __grid_const
 #pragma unroll
   for (int k = 0; k < 32; ++k) v += part[k][lane];
   const int t = col >= p.dim, e = col - t * p.dim;
-  if (p.out[t] == nullptr) return;
-  if (p.dtype == DGXM_DTYPE_F32) static_cast<float*>(p.out[t])[e] = v;
-  else if (p.dtype == DGXM_DTYPE_F16) static_cast<__half*>(p.out[t])[e] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p.out[t])[e] = __float2bfloat16_rn(v);
+  qk_store_weight_grad(p.out[t], p.dtype, e, v);
 }
 
 // How a call is cut into warps: chunks of as many rows as a warp has under
@@ -619,6 +662,9 @@ static QkCut qk_cut(const dgxm_qk_norm_desc* d, bool back, bool vec) {
   const int groups = 32 / c.group, most = d->dtype == DGXM_DTYPE_F32 ? kQkRows<float> : kQkRows<__half>;
   const int64_t tokens = static_cast<int64_t>(d->batch) * d->seq;
   const int longest = (std::max(d->q_heads, d->k_heads) + groups - 1) / groups;  // rows of the longer tensor
+  c.rows = c.chunks[0] = c.chunks[1] = c.blocks = 0;
+  c.warps = 0;
+  if (longest == 0 || tokens == 0) return c;
   for (int parts = (longest + most - 1) / most;; ++parts) {
     c.rows = (longest + parts - 1) / parts;
     c.chunks[0] = (d->q_heads + groups * c.rows - 1) / (groups * c.rows);
@@ -750,15 +796,21 @@ extern "C" int dgxm_qk_norm_rope(const dgxm_qk_norm_desc* d, const void* q, cons
   bool vec = false;
   if (int rc = qk_params(d, {q, k}, {nullptr, nullptr}, {q_out, k_out}, {norm_q_w, norm_k_w}, rope, &p, &cut, &vec))
     return rc;
-  qk_pick<false>(d->dtype, cut.group, p, vec)<<<cut.blocks, kQkThreads, kQkWarps * kQkRing, static_cast<cudaStream_t>(stream)>>>(p);
-  DGXM_CUDA_TRY(cudaGetLastError());
+  DGXM_CUDA_TRY(launch_overlapped(qk_pick<false>(d->dtype, cut.group, p, vec), cut.blocks, kQkThreads, kQkWarps * kQkRing,
+                                  static_cast<cudaStream_t>(stream), p));
   return DGXM_OK;
 }
 
 extern "C" int64_t dgxm_qk_norm_rope_backward_workspace(const dgxm_qk_norm_desc* d) {
   using namespace dgxm;
   if (qk_check(d)) return -1;
-  return int64_t(kQkBwdBlocks) * 2 * d->head_dim * 4;
+  // Whether the call is small enough for a cluster depends on the tensors' alignment too: both ways.
+  int64_t need = 0;
+  for (bool vec : {false, true}) {
+    const QkCut cut = qk_cut(d, true, vec);
+    if (cut.warps > kQkClusterWarps) need = std::max<int64_t>(need, int64_t(cut.blocks) * 2 * d->head_dim * 4);
+  }
+  return need;
 }
 
 extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void* dq, const void* dk, const void* q,
@@ -779,16 +831,22 @@ extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void
     QkCut cut;
     if (int rc = qk_params(d, {q, k}, {dq, dk}, {gq, gk}, {norm_q_w, norm_k_w}, rope, &p, &cut, &vec)) return rc;
     blocks = cut.blocks;
-    if (weights) {
-      if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 4 ||
-          workspace_bytes < dgxm_qk_norm_rope_backward_workspace(d))
-        return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes,
-                    (long long)dgxm_qk_norm_rope_backward_workspace(d));
+    if (weights && cut.warps <= kQkClusterWarps) {
+      p.cluster = blocks <= 1 ? 1 : blocks <= 2 ? 2 : blocks <= 4 ? 4 : 8;
+      blocks = p.cluster;
+      p.gw[0] = g_norm_q_w;
+      p.gw[1] = g_norm_k_w;
+      p.gw_dtype = d->weight_dtype;
+    } else if (weights) {
+      const int64_t need = int64_t(blocks) * 2 * d->head_dim * 4;
+      if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 4 || workspace_bytes < need)
+        return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes, (long long)need);
       p.partial = static_cast<float*>(workspace);
     }
-    qk_pick<true>(d->dtype, cut.group, p, vec)<<<blocks, kQkThreads, kQkWarps * 2 * kQkRing, st>>>(p);
-    DGXM_CUDA_TRY(cudaGetLastError());
+    DGXM_CUDA_TRY(launch_overlapped(qk_pick<true>(d->dtype, cut.group, p, vec), blocks, kQkThreads, kQkWarps * 2 * kQkRing,
+                                    st, p, p.cluster > 0 ? p.cluster : 1));
   }
+  if (p.cluster > 0) return DGXM_OK;
   if (!weights) return DGXM_OK;
   QkWeightGradParams wp;
   wp.partial = p.partial;
@@ -797,16 +855,6 @@ extern "C" int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* d, const void
   wp.blocks = blocks;
   wp.dim = d->head_dim;
   wp.dtype = d->weight_dtype;
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((2 * d->head_dim + 31) / 32);
-  cfg.blockDim = dim3(1024);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, qk_weight_grad_kernel, wp));
+  DGXM_CUDA_TRY(launch_overlapped(qk_weight_grad_kernel, (2 * d->head_dim + 31) / 32, 1024, 0, st, wp));
   return DGXM_OK;
 }

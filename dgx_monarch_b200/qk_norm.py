@@ -183,7 +183,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
     gk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     gwq = None if norm_q_w is None else torch.empty_like(norm_q_w)
     gwk = None if norm_k_w is None else torch.empty_like(norm_k_w)
-    work = None if gwq is None else q.new_empty(need, dtype=torch.uint8)
+    work = q.new_empty(need, dtype=torch.uint8) if need and gwq is not None else None
     launch("dgxm_qk_norm_rope_backward", q.get_device(), desc, dq.data_ptr(), _ptr(dk), q.data_ptr(), _ptr(k),
            _ptr(norm_q_w), _ptr(norm_k_w), _ptr(rope), gq.data_ptr(), _ptr(gk), _ptr(gwq), _ptr(gwk), _ptr(work),
            need if work is not None else 0)

@@ -66,12 +66,17 @@ def test_c_pointer_refusals(lib):
     assert lib.dgxm_qk_norm_rope(d, FAKE + 1, FAKE, None, None, None, FAKE, FAKE, None) == 1
     assert lib.dgxm_qk_norm_rope(d, FAKE, FAKE, FAKE + 1, None, None, FAKE, FAKE, None) == 1
     assert lib.dgxm_qk_norm_rope(d, FAKE, FAKE, None, None, FAKE + 2, FAKE, FAKE, None) == 1
+    # a call too large for one cluster: its weight gradients need the workspace
+    d = _desc(seq=4096)
     args = [FAKE] * 4 + [FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE]
     assert lib.dgxm_qk_norm_rope_backward(d, *args, None, 0, None) == 1
     assert "workspace" in lib.dgxm_last_error_message().decode()
     need = lib.dgxm_qk_norm_rope_backward_workspace(d)
     assert lib.dgxm_qk_norm_rope_backward(d, *args, FAKE, need - 1, None) == 1
     assert lib.dgxm_qk_norm_rope_backward(d, None, *args[1:], FAKE, need, None) == 1
+    assert lib.dgxm_qk_norm_rope_backward_workspace(_desc()) == 0
+    assert lib.dgxm_qk_norm_rope_backward_workspace(_desc(q_heads=0, k_heads=0)) == 0
+    assert lib.dgxm_qk_norm_rope_backward_workspace(_desc(seq=0)) == 0
     assert lib.dgxm_qk_norm_rope_backward_workspace(None) == -1
     assert lib.dgxm_qk_norm_rope_backward_workspace(_desc(head_dim=9)) == -1
 
