@@ -99,7 +99,7 @@ def _check(x, fmt, given=None, dtypes=(F32,)):
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 16), (3, 17), (127, 31), (128, 33), (129, 64), (5, 65), (300, 100),
-                                       (2, 5120), (33, 1023), (260, 128), (1, 13824)])
+                                       (2, 5120), (33, 1023), (260, 128), (1, 13824), (300, 1000), (257, 2050)])
 def test_sizes(fmt, dtype, rows, cols):
     g = torch.Generator(device="cuda").manual_seed(rows * 7 + cols)
     x = torch.randn(rows, cols, device="cuda", generator=g) * torch.exp(2 * torch.randn(rows, 1, device="cuda", generator=g))
