@@ -666,9 +666,11 @@ extern "C" int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* d, const void* a_values
   if (d == nullptr) return fail(DGXM_ERR_INVALID, "NULL 4-bit product descriptor");
   if (d->format != DGXM_FP4_NVFP4 && d->format != DGXM_FP4_MXFP4)
     return fail(DGXM_ERR_UNSUPPORTED, "4-bit format %d (nvfp4 or mxfp4)", d->format);
-  if (d->m < 0 || d->n < 0 || d->k <= 0 || d->m > (1 << 30) || d->n > (1 << 30) || d->k > (1 << 30))
+  if (d->m < 0 || d->n < 0 || d->k <= 0 || d->m > (1 << 30) || d->n > (1 << 30))
     return fail(DGXM_ERR_INVALID, "product of (%lld, %lld) and (%lld, %lld)", (long long)d->m, (long long)d->k,
                 (long long)d->n, (long long)d->k);
+  // One tile's K takes 0.5 us a stage at the most: 33 ms here, well within the bounded waits' second.
+  if (d->k > (1 << 24)) return fail(DGXM_ERR_UNSUPPORTED, "k %lld above 2^24", (long long)d->k);
   for (int t : {d->out_dtype, d->bias_dtype})
     if (t != DGXM_DTYPE_BF16 && t != DGXM_DTYPE_F16 && t != DGXM_DTYPE_F32)
       return fail(DGXM_ERR_UNSUPPORTED, "output or bias dtype %d (bf16, f16 or f32)", t);

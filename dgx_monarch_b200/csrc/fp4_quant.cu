@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
         const float s = fp4_scale_value<FORMAT>(byte);
         const bool on = s > 0.f;  // false for zero and NaN
         const float u = s * g, r = on ? rcp_approx(u) : 0.f;
-        if (few_bits) {
+        if (few_bits && amax * up * r < 0x1p100f) {  // (a residual of quotients beyond fp32's range is none)
 #pragma unroll
           for (int j = 0; j < B / 8; ++j) c[j] = fp4_codes_residual<T>(x + 8 * j, up, u, r);
         } else {
@@ -511,8 +511,7 @@ static int fp4_params(const dgxm_fp4_desc* d, const void* x, const void* values,
   if ((reinterpret_cast<uintptr_t>(values) | reinterpret_cast<uintptr_t>(scales)) % 16)
     return fail(DGXM_ERR_INVALID, "values and scales must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(x) % elt) return fail(DGXM_ERR_INVALID, "the matrix is not aligned to its elements");
-  const int64_t items = d->rows * per_row;
-  if (per_row > 0 && (d->rows > (int64_t(1) << 31) || items > (int64_t(1) << 31) - 1))
+  if (d->rows > (int64_t(1) << 31) || d->rows * per_row > (int64_t(1) << 31) - 1)
     return fail(DGXM_ERR_UNSUPPORTED, "%lld x %lld is more than 2^31 - 1 blocks", (long long)d->rows, (long long)d->cols);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | static_cast<uintptr_t>(d->rows == 1 ? 0 : d->row_stride * elt);
   *vec = bits % 16 == 0;
@@ -523,7 +522,7 @@ static int fp4_params(const dgxm_fp4_desc* d, const void* x, const void* values,
   p->scales = static_cast<uint8_t*>(const_cast<void*>(scales));
   p->pitch = fp4_pitch(d->cols);
   p->groups = fp4_groups(d->cols, d->format);
-  p->items = static_cast<uint32_t>(items);
+  p->items = static_cast<uint32_t>(d->rows * per_row);
   p->per_row = static_cast<uint32_t>(per_row);
   p->cols = static_cast<int>(d->cols);
   p->scale_dtype = d->scale_dtype;
@@ -571,11 +570,11 @@ static cudaError_t fp4_dequantize_typed(const Fp4Params& p, int format, bool vec
 }  // namespace dgxm
 
 extern "C" int64_t dgxm_fp4_values_bytes(int64_t rows, int64_t cols) {
-  return rows < 0 || cols <= 0 ? -1 : rows * dgxm::fp4_pitch(cols);
+  return rows < 0 || cols <= 0 || rows > (int64_t(1) << 31) || cols > (1 << 30) ? -1 : rows * dgxm::fp4_pitch(cols);
 }
 
 extern "C" int64_t dgxm_fp4_scales_bytes(int64_t rows, int64_t cols, int32_t format) {
-  if (rows < 0 || cols <= 0 || (format != DGXM_FP4_NVFP4 && format != DGXM_FP4_MXFP4)) return -1;
+  if (rows < 0 || cols <= 0 || rows > (int64_t(1) << 31) || cols > (1 << 30) || (format != DGXM_FP4_NVFP4 && format != DGXM_FP4_MXFP4)) return -1;
   return (rows + 127) / 128 * dgxm::fp4_groups(cols, format) * 512;
 }
 

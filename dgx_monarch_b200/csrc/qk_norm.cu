@@ -663,8 +663,8 @@ static QkCut qk_cut(const dgxm_qk_norm_desc* d, bool back, bool vec) {
   const int64_t tokens = static_cast<int64_t>(d->batch) * d->seq;
   const int longest = (std::max(d->q_heads, d->k_heads) + groups - 1) / groups;  // rows of the longer tensor
   c.rows = c.chunks[0] = c.chunks[1] = c.blocks = 0;
-  c.warps = 0;
-  if (longest == 0 || tokens == 0) return c;
+  c.warps = tokens;
+  if (longest == 0 || tokens == 0 || tokens > (int64_t(1) << 31) - 1) return c;  // nothing to do, or too much
   for (int parts = (longest + most - 1) / most;; ++parts) {
     c.rows = (longest + parts - 1) / parts;
     c.chunks[0] = (d->q_heads + groups * c.rows - 1) / (groups * c.rows);
@@ -682,6 +682,8 @@ static int qk_check(const dgxm_qk_norm_desc* d) {
   if (d->batch < 0 || d->seq < 0 || d->q_heads < 0 || d->k_heads < 0)
     return fail(DGXM_ERR_INVALID, "negative extents: batch %d, rows %d, heads %d / %d", d->batch, d->seq, d->q_heads,
                 d->k_heads);
+  if (d->q_heads > (1 << 20) || d->k_heads > (1 << 20))
+    return fail(DGXM_ERR_UNSUPPORTED, "%d / %d heads (up to 2^20)", d->q_heads, d->k_heads);
   if (d->head_dim <= 0 || d->head_dim % 8 || d->head_dim > 256)
     return fail(DGXM_ERR_UNSUPPORTED, "head_dim %d is not a multiple of 8 up to 256", d->head_dim);
   if (d->rot_dim < 0 || d->rot_dim % 2 || d->rot_dim > d->head_dim)

@@ -39,9 +39,13 @@ def _check_out(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
         raise ValueError(f"{name} is an expanded tensor: its rows share memory")
 
 
-def _check_in_place(name: str, out: torch.Tensor, src: torch.Tensor) -> None:
-    if out.data_ptr() == src.data_ptr() and out.stride() != src.stride() and src.numel():
+def _check_in_place(name: str, out: torch.Tensor, src: torch.Tensor, other: torch.Tensor | None) -> None:
+    if src.numel() == 0:
+        return
+    if out.data_ptr() == src.data_ptr() and out.stride() != src.stride():
         raise ValueError(f"{name} shares its input's memory with other strides")
+    if other is not None and other.numel() and out.data_ptr() == other.data_ptr():
+        raise ValueError(f"{name} is the memory of the other tensor")
 
 
 def _describe(q, k, norm_mode, wq, wk, eps, rope, rope_halves) -> _lib.QkNormDesc:
@@ -103,10 +107,11 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
     rope: fp32 (L, P, 2) or (B, L, P, 2) cosines and sines of P <= D / 2 pairs
     (prologue.rope_table); the first 2 P values of a head are rotated, values
     2i and 2i + 1 with each other, or i and P + i with rope_halves.  norm_mode
-    NORM_NONE rotates alone.  Sums and rotation are fp32, rounded once.
+    NORM_NONE rotates alone.  Sums and rotation are fp32, rounded once; a head
+    whose sum of squares leaves fp32's range (values above 1e18) comes out zero.
 
     q_out / k_out may be q / k themselves (same strides); they must not
-    overlap the inputs in any other way.  No autograd graph is recorded: see
+    overlap the inputs, or each other, in any other way.  No autograd graph is recorded: see
     qk_norm_rope_backward."""
     key = ("f", _meta(q), _meta(k), norm_mode, _meta(norm_q_w), _meta(norm_k_w), eps, _meta(rope), rope_halves,
            _meta(q_out), _meta(k_out))
@@ -126,16 +131,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
         return desc
 
     desc = plan(key, make)
-    no_graph(_GRADS, q, k, norm_q_w, norm_k_w)
+    no_graph(_GRADS, q, k, norm_q_w, norm_k_w, rope)
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _check_in_place("q_out", q_out, q)
+        _check_in_place("q_out", q_out, q, k)
     if k is not None:
         if k_out is None:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         else:
-            _check_in_place("k_out", k_out, k)
+            _check_in_place("k_out", k_out, k, q)
+            if k_out.data_ptr() == q_out.data_ptr() and k.numel() and q.numel():
+                raise ValueError("q_out and k_out share their memory")
     launch("dgxm_qk_norm_rope", q.get_device(), desc, q.data_ptr(), _ptr(k), _ptr(norm_q_w), _ptr(norm_k_w),
            _ptr(rope), q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
@@ -178,7 +185,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
         return desc, need
 
     desc, need = plan(key, make)
-    no_graph(_GRADS, dq, dk, q, k, norm_q_w, norm_k_w)
+    no_graph(_GRADS, dq, dk, q, k, norm_q_w, norm_k_w, rope)
     gq = torch.empty_like(q, memory_format=torch.contiguous_format)
     gk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     gwq = None if norm_q_w is None else torch.empty_like(norm_q_w)

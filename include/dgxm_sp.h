@@ -722,7 +722,7 @@ int dgxm_dequantize_fp4(const dgxm_fp4_desc* desc, const void* values, const voi
 
 /*
  * out[i, j] = g_a g_b sum_k a[i, k] b[j, k] + bias[j] over two packed
- * matrices of one format, (m, k) and (n, k): block-scaled tcgen05 products,
+ * matrices of one format, (m, k) and (n, k), k <= 2^24: block-scaled tcgen05 products,
  * fp32 accumulation, one rounding to out_dtype.  a_scale / b_scale: the
  * tensors' fp32 scales (nvfp4; NULL for mxfp4).  bias: n values of bias_dtype,
  * or NULL.  The same call gives the same bits.

@@ -170,6 +170,24 @@ def test_scales_over_the_whole_range(g):
     assert (got_byte == byte).all() and (got_code == code).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("g", [2.0 ** -12, 2.0 ** -60, 2.0 ** -140, 0.001, 1e-25, 1e-42, 1.0, 2.0 ** 20])
+def test_the_types_largest_values_keep_their_sign(dtype, g):
+    """Quotients beyond fp32's range saturate to 6 with the value's sign."""
+    big = torch.finfo(dtype).max
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    x = torch.randn(8, 64, device="cuda", generator=gen)
+    x[0, 5], x[1, 17], x[2, 40:44] = -big, big, -big
+    x[3, :16] = torch.where(torch.arange(16, device="cuda") % 2 == 0, big, -big)
+    x = x.to(dtype)
+    t = quantize_fp4(x, scale=torch.tensor(g, device="cuda"))
+    code, byte, _ = _reference(x.double().cpu().numpy(), "nvfp4", float(np.float32(g)))
+    got_code, got_byte = _unpack(t)
+    assert (got_byte == byte).all() and (got_code == code).all(), np.argwhere(got_code != code)[:5]
+    _check(x, "mxfp4")
+    _check(x, "nvfp4")
+
+
 def test_power_of_two_scales_over_the_whole_range():
     e = torch.arange(-149, 128, device="cuda")
     x = torch.ldexp(torch.ones(277, device="cuda", dtype=torch.float64), e)[:, None]

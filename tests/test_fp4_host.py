@@ -96,6 +96,7 @@ def test_quantisation_arguments(lib):
     ({"m": -1}, 1, "product"),
     ({"k": 0}, 1, "product"),
     ({"n": 2 ** 31}, 1, "product"),
+    ({"k": 2 ** 24 + 1}, 2, "k 16777217"),
     ({"out_dtype": 2}, 2, "dtype 2"),
     ({"bias_dtype": 9}, 2, "dtype 9"),
     ({"out_stride": 63}, 1, "row stride 63"),

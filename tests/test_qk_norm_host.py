@@ -44,6 +44,9 @@ def _desc(**kw):
     ({"eps": -1.0}, 1, "eps"),
     ({"eps": float("nan")}, 1, "eps"),
     ({"seq": 2 ** 31 - 1, "batch": 2}, 2, "head groups"),
+    ({"seq": 2 ** 31 - 1, "batch": 2 ** 31 - 1}, 2, "head groups"),
+    ({"seq": 2 ** 30}, 2, "head groups"),
+    ({"q_heads": 2 ** 20 + 1}, 2, "heads"),
     ({"seq": 0}, 0, ""),
     ({"batch": 0}, 0, ""),
     ({"q_heads": 0, "k_heads": 0}, 0, ""),
@@ -128,6 +131,12 @@ def test_output_and_gradient_checks():
         qk_norm._check_out("q_out", torch.zeros(1, 4, 2, 64), like)
     with pytest.raises(ValueError, match="expanded"):
         qk_norm._check_out("q_out", torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16).expand(1, 4, 2, 64), like)
+    q, k = torch.zeros(1, 4, 2, 64), torch.zeros(1, 4, 2, 64)
+    qk_norm._check_in_place("q_out", q, q, k)
+    with pytest.raises(ValueError, match="other strides"):
+        qk_norm._check_in_place("q_out", q.transpose(1, 2).reshape(1, 2, 4, 64)[:, :, :2], q[:, :2], k)
+    with pytest.raises(ValueError, match="other tensor"):
+        qk_norm._check_in_place("q_out", k, q, k)
     w = torch.zeros(3, requires_grad=True)
     with pytest.raises(RuntimeError, match="no_grad"):
         qk_norm.no_graph("", None, w)
