@@ -623,16 +623,18 @@ struct Fp4Cut {
 
 // The cut whose waves of tiles take the least time by what one wave took
 // (microseconds a stage of K, a tile, and at the least; nvfp4, 9450 x 5120 x
-// 256, 1024 and 5120, for the narrowest 16 x 1280 .. 5120 x 5120): narrow
-// tiles where only they fill the SMs, wide ones, which load the least for
-// what they compute, where those do too.
+// 256, 1024 and 5120, the narrow ones 1 .. 64 x 2560 .. 13824 x 256 .. 14336):
+// narrow tiles where only they fill the SMs or more are not needed (1 x 5120 x
+// 1024: 3.8 us with 16 columns, 4.9 with 64), wide ones, which load the least
+// for what they compute, where those do too, and K split where even those are
+// few (16 x 2560 x 5120: 8.0, 6.3, 5.5 us on 1, 2, 4 CTAs a tile).
 static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
   struct Kind {
     int tn, rows, at_once;
     double stage, tile, least;
   };
-  static const Kind kinds[] = {{16, 128, 148, 0.16, 1.0, 1.0},  {32, 128, 148, 0.17, 1.0, 1.0},
-                               {64, 128, 148, 0.24, 0.6, 1.0},  {128, 128, 148, 0.29, 0.8, 1.1},
+  static const Kind kinds[] = {{16, 128, 148, 0.26, 0.4, 0.4},  {32, 128, 148, 0.26, 0.6, 0.6},
+                               {64, 128, 148, 0.25, 0.8, 1.0},  {128, 128, 148, 0.29, 0.8, 1.1},
                                {192, 128, 148, 0.42, 1.1, 2.2}, {256, 256, 74, 0.42, 1.75, 2.2}};
   Fp4Cut best{128, 1, false};
   double least = 1e30;
@@ -647,7 +649,7 @@ static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
       if (split > 1 && tiles * split > 148) break;
       const int64_t waves = (tiles * split + kind.at_once - 1) / kind.at_once;
       const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile, kind.least) +
-                        (split > 1 ? 0.4 : 0.0);
+                        (split > 1 ? 1.3 : 0.0);  // exchange within the cluster
       if (us < least) {
         least = us;
         best = {kind.tn, split, one && tokens};

@@ -60,7 +60,9 @@ def _check(a, b, bias=None, out_dtype=BF16, out=None):
 
 SIZES = [(1, 1, 1), (1, 8, 16), (2, 256, 64), (16, 130, 100), (17, 300, 96), (33, 129, 257), (64, 640, 512),
          (65, 129, 320), (128, 256, 1024), (300, 77, 1000), (1000, 50, 320), (700, 20, 65), (500, 9, 2000),
-         (129, 1280, 5120), (257, 511, 127), (5, 5120, 2049), (1003, 777, 1000), (2560, 2304, 288), (3000, 4001, 33)]
+         (129, 1280, 5120), (257, 511, 127), (5, 5120, 2049), (1003, 777, 1000), (2560, 2304, 288), (3000, 4001, 33),
+         (4, 1000, 3000), (20, 900, 3000), (50, 600, 3000), (2300, 2700, 700), (2301, 2699, 700), (1100, 3100, 2000),
+         (1030, 3001, 2100)]  # narrow tiles with K split; 192 columns; CTA pairs, rows on and off 16 bytes
 
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
@@ -91,7 +93,7 @@ def test_exact_sums(fmt, m, n, k):
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("m,n,k", [(1, 700, 500), (3, 257, 5120), (40, 1000, 272), (200, 136, 768), (1500, 1000, 400),
-                                   (2300, 2600, 640)])
+                                   (2300, 2600, 640), (1100, 3100, 2000)])
 def test_random_tensors_with_bias(fmt, out_dtype, m, n, k):
     g = _gen(m + n)
     a, b = _random(g, m, k, fmt), _random(g, n, k, fmt)
