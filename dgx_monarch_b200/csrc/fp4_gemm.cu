@@ -11,7 +11,7 @@
 // that read them.
 //
 // Roles (10 warps): warp 0 loads (one thread), warp 1 copies scales and
-// issues MMAs (one thread), warps 2-9 run the epilogue, each a quarter of the
+// issues MMAs, warps 2-9 run the epilogue, each a quarter of the
 // tile's rows and half of its columns.
 #include <type_traits>
 
@@ -64,12 +64,16 @@ struct Fp4Tile {
   static constexpr int kStagingBytes = kPartBytes > 8 * kGemmStageRows ? kPartBytes : 8 * kGemmStageRows;
   static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes - kStagingBytes) / kStageBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kGemmCtrlBytes;
-  // Tensor memory: accumulators, then two buffers of scales (P's 4 columns a
-  // tile, Q's 4 columns a tile and 128 rows).
-  static constexpr int kAccs = TN <= 192 ? 2 : 1;
-  static constexpr int kSfP = 4 * kAtoms, kSfQ = 4 * kAtoms * kQTiles;
-  static constexpr int kSfCol = kAccs * TN;
-  static_assert(kSfCol + 2 * (kSfP + kSfQ) <= 512, "tensor memory");
+  // Tensor memory: accumulators, then scales, for each stage of the ring P's 4
+  // columns and Q's 4 a 128-row tile for four blocks of K.  A copy of scales is
+  // ordered before the MMAs that follow it, but not behind earlier ones that
+  // read the same columns; those of a stage have completed when the stage is
+  // filled again.  The room for that leaves 192 columns one accumulator, which
+  // its tiles do not feel, where two, and a wait of the MMA warp's for its fewer
+  // columns of scales, cost 5 % (512 x 5120 x 5120: 13.5 us, 14.2).
+  static constexpr int kAccs = TN <= 128 ? 2 : 1;
+  static constexpr int kSfCol = kAccs * TN, kSfCols = 4 * (1 + kQTiles);
+  static_assert(kSfCol + kStages * kAtoms * kSfCols <= 512, "tensor memory");
   static_assert(kStageBytes % 1024 == 0, "swizzle atoms stay aligned");
   // Barriers
   static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + kAccs,
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     // ------------------------------------------------------------ scales and MMAs
     if (cta == 0) {
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      int s = 0, parity = 0, sf_buf = 0, u = 0;
+      int s = 0, parity = 0, u = 0;
       bool ok = true;
       for (int tile = first_tile; ok && tile < tiles; tile += tile_step, ++u) {
         const int a = u % C::kAccs;
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
           if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kFull + s), parity, abort_flag)))) break;
           tc_fence_after();
           const uint32_t sp = base + s * C::kStageBytes, sq = sp + C::kPBytes, sf = sq + C::kQBytes;
-          const uint32_t tp = tm + C::kSfCol + sf_buf * (C::kSfP + C::kSfQ), tq = tp + C::kSfP;
+          const uint32_t tsf = tm + C::kSfCol + s * (C::kAtoms * C::kSfCols);
           const uint64_t dp = sdesc_sw128(sp, 16, 1024), dq = sdesc_sw128(sq, 16, 1024), df = fp4_sf_desc(sf);
           // K = 64 an MMA; the rest of the last tile is empty.
           const int steps = min(kGemmK, p.k - kt * kGemmK + 63) / 64;
@@ -379,19 +383,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
           for (int kk = 0; kk < kGemmK / 64; ++kk) {
             constexpr int kPer = 4 / C::kAtoms;  // MMAs a scale tile serves
             const int i = kk / kPer;
+            const uint32_t tp = tsf + i * C::kSfCols, tq = tp + 4;
             if (kk % kPer == 0) {
-              tmem_cp_scales<PAIR>(tp + 4 * i, df + 32 * i);
+              tmem_cp_scales<PAIR>(tp, df + 32 * i);
 #pragma unroll
               for (int j = 0; j < C::kQTiles; ++j)
-                tmem_cp_scales<PAIR>(tq + 4 * (C::kQTiles * i + j), df + ((1 + j) * C::kSfBytes + 512 * i) / 16);
+                tmem_cp_scales<PAIR>(tq + 4 * j, df + ((1 + j) * C::kSfBytes + 512 * i) / 16);
             }
             if (kk < steps)
               umma_fp4_ss<FORMAT, PAIR>(acc, dp + 2 * kk, dq + 2 * kk,
-                                        fp4_idesc(C::kRows, TN, FORMAT, kPer == 1 ? 0 : 2 * (kk % kPer)), tp + 4 * i,
-                                        tq + 4 * C::kQTiles * i + q_col, (kt > kt0 || kk > 0) ? 1u : 0u);
+                                        fp4_idesc(C::kRows, TN, FORMAT, kPer == 1 ? 0 : 2 * (kk % kPer)), tp,
+                                        tq + q_col, (kt > kt0 || kk > 0) ? 1u : 0u);
           }
           fp4_commit<PAIR>(bar(C::kEmpty + s));
-          sf_buf ^= 1;
           if (++s == C::kStages) {
             s = 0;
             parity ^= 1;
@@ -697,11 +701,7 @@ extern "C" int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* d, const void* a_values
   memset(&p, 0, sizeof(p));
   p.k = static_cast<int>(d->k);
   p.k_tiles = static_cast<int>((d->k + kGemmK - 1) / kGemmK);
-  Fp4Cut cut = fp4_cut(m, n, p.k_tiles);
-#ifdef FP4_TUNE
-  if (getenv("TN")) cut.tn = atoi(getenv("TN"));
-  if (getenv("SPLIT")) cut.split = atoi(getenv("SPLIT"));
-#endif
+  const Fp4Cut cut = fp4_cut(m, n, p.k_tiles);
   p.q_is_tokens = cut.q_is_tokens;
   p.split = cut.split;
   p.p_rows = static_cast<int>(p.q_is_tokens ? n : m);
