@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(kQkThreads, kQkBwdPerSm) qk_norm_rope_bwd_kern
           }
           xx = qk_group_sum<G>(xx);
           gx = qk_group_sum<G>(gx);
-          const float r = rsqrtf(fmaf(xx, p.inv_dim, p.eps));
+          // (a row that this group has not is blank: without an eps its r would be infinite, and dw NaN)
+          const float r = u < mine ? rsqrtf(fmaf(xx, p.inv_dim, p.eps)) : 0.f;
           const float m = -gx * r * p.inv_dim;  // -mean(g w n); n and m stay in range however small x is
 #pragma unroll
           for (int i = 0; i < 8; ++i) {

@@ -225,6 +225,23 @@ def test_zero_rows_infinities_and_nan_stay_in_their_row():
     assert torch.equal(y[0, 0, 0, 64:], x[0, 0, 0, 64:])
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_no_eps(d):
+    """Heads that do not fill a warp's lane groups, without an eps."""
+    g = _gen(17)
+    q, dq = (torch.randn(2, 5, 3, d, device="cuda", generator=g).bfloat16() for _ in range(2))
+    k, dk = (torch.randn(2, 5, 1, d, device="cuda", generator=g).bfloat16() for _ in range(2))
+    wq, wk = (torch.randn(d, device="cuda", generator=g) for _ in range(2))
+    rope = _table(5, d // 2, g)
+    how = {"norm_q_w": wq, "norm_k_w": wk, "eps": 0.0, "rope": rope}
+    yq, yk = qk_norm_rope(q, k, **how)
+    _check_forward(yq, q, wq, rope, False, 0.0, True)
+    _check_forward(yk, k, wk, rope, False, 0.0, True)
+    gq, gk, gwq, gwk = qk_norm_rope_backward(dq, dk, q, k, **how)
+    _check_backward(gq, gwq, dq, q, wq, rope, False, 0.0, True)
+    _check_backward(gk, gwk, dk, k, wk, rope, False, 0.0, True)
+
+
 def test_gradient_against_differences():
     """fp32 central differences of a 64-bit functional of the kernel's forward."""
     g = _gen(7)
