@@ -199,11 +199,13 @@ __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* 
   constexpr int kCols = NC % kMost == 0 ? kMost : NC % (kMost / 2) == 0 ? kMost / 2 : NC;  // columns staged at one time
   static_assert(kCols <= kMost && NC % kCols == 0, "whole chunks");
   constexpr int kPieces = kCols / kEach;
-  const bool bulk = kCols == kMost && p.vec;
 #pragma unroll
   for (int c0 = 0; c0 < NC; c0 += kCols) {
     if (q0 + c0 >= p.q_rows) return;  // uniform over the warp
-    if (bulk) {
+    const bool tma = kCols == kMost && p.vec;
+    // a row that ends inside 16 bytes would have the rest of them written too
+    const bool bulk = tma && (q0 + c0 + kCols <= p.q_rows || p.q_rows % kEach == 0);
+    if (tma) {
       if (lane == 0) tma_store_wait_read();  // the last chunk has left the staging rows
       __syncwarp();
     }

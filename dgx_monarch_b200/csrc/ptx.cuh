@@ -105,7 +105,8 @@ __device__ __forceinline__ void tma_load_4d_hint(uint32_t dst, const void* map, 
 }
 
 // 4-D tiled bulk tensor store from this CTA's shared memory; what lies out of
-// bounds is not written.  Generic writes to the source come before
+// bounds is not written, but a row that ends inside 16 bytes is filled up to
+// them.  Generic writes to the source come before
 // tma_store_fence; the source is free again after tma_store_wait_read.
 __device__ __forceinline__ void tma_store_4d(const void* map, uint32_t src, int c0, int c1, int c2, int c3) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(

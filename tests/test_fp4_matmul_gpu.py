@@ -126,6 +126,18 @@ def test_leading_dimensions_outputs_and_empty():
     assert fp4_matmul(empty, b).shape == (0, 40) and fp4_matmul(b, empty).shape == (40, 0)
 
 
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n", [(1, 57), (300, 57), (2475, 57), (2048, 513), (1024, 2041), (600, 1001), (2301, 2699)])
+def test_columns_behind_the_output_stay(m, n, out_dtype):
+    """Aligned output rows that end inside 16 bytes."""
+    g = _gen(m + n)
+    a, b = _random(g, m, 320, "nvfp4"), _random(g, n, 320, "nvfp4")
+    want = _check(a, b, None, out_dtype)
+    wide = torch.full((m + 1, (n + 15) // 8 * 8), 7.0, device="cuda", dtype=out_dtype)
+    assert torch.equal(fp4_matmul(a, b, out_dtype=out_dtype, out=wide[:m, :n]), want)
+    assert (wide[:, n:] == 7).all() and (wide[m:] == 7).all()
+
+
 def test_nan_scales_stay_in_their_row_and_column():
     g = _gen(2)
     x = torch.randn(200, 320, device="cuda", generator=g).bfloat16()
