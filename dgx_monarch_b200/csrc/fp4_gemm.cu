@@ -55,12 +55,11 @@ struct Fp4Tile {
   static constexpr int kQBytes = kQLoad * 128;
   static constexpr int kSfBytes = kAtoms * 512;
   static constexpr int kStageBytes = kPBytes + kQBytes + kSfBytes * (1 + kQTiles);
-  // A split tile's partial sums in the CTA that finishes their rows: (rank,
-  // row, column), rows 16 bytes off a multiple of 64, so that neighbouring
-  // ones lie in other banks.  They take the place of the staging rows.
+  // A split tile's partial sums in the CTA that finishes their rows, in the
+  // place of the staging rows: (rank, four columns, row), 16 bytes each, an odd
+  // number of rows apart (138 at the most for all ranks).
   static constexpr bool kSplits = !PAIR && TN <= 64;
-  static constexpr int kPartPitch = TN + 4;
-  static constexpr int kPartBytes = kSplits ? kGemmRows * kPartPitch * 4 : 0;
+  static constexpr int kPartBytes = kSplits ? (kGemmRows + 10) * TN * 4 : 0;
   static constexpr int kStagingBytes = kPartBytes > 8 * kGemmStageRows ? kPartBytes : 8 * kGemmStageRows;
   static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes - kStagingBytes) / kStageBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kGemmCtrlBytes;
@@ -167,12 +166,6 @@ __device__ __forceinline__ float fp4_gemm_bias(const Fp4GemmParams& p, int n) {
   return static_cast<const float*>(p.bias)[n];
 }
 
-__device__ __forceinline__ void fp4_gemm_store(const Fp4GemmParams& p, int64_t at, float v) {
-  if (p.out_dtype == DGXM_DTYPE_BF16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-  else if (p.out_dtype == DGXM_DTYPE_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-  else static_cast<float*>(p.out)[at] = v;
-}
-
 // 16-byte piece i of a lane's row in words: four fp32, or eight of a 16-bit type.
 template <int ELT>
 __device__ __forceinline__ uint4 fp4_piece(const Fp4GemmParams& p, const float* f) {
@@ -245,6 +238,57 @@ __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* 
       }
     }
     __syncwarp();
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T fp4_narrow(float v) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(v);
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return v;
+}
+
+// The finished values of one row of P, where that is a column of the output:
+// neighbouring lanes store neighbouring values.
+template <typename T, int NC>
+__device__ __forceinline__ void fp4_store_column(const Fp4GemmParams& p, const float (&v)[NC], float bias, int n, int q0) {
+  T* to = static_cast<T*>(p.out) + q0 * p.ld_out + n;
+#pragma unroll
+  for (int c = 0; c < NC; ++c, to += p.ld_out)
+    if (q0 + c < p.q_rows) *to = fp4_narrow<T>(v[c] + bias);
+}
+
+// A split tile: this CTA's share of the rows, `rows` from row pr0, out of the
+// partial sums.  A thread takes four columns of one row at a time; its bias
+// came before (row j's, where the rows of P are output columns, or column e's).
+template <typename T, int TN>
+__device__ __forceinline__ void fp4_store_split(const Fp4GemmParams& p, const float* part, int share, int rows, int pr0,
+                                                int q0, int thread, float ga, float gb, const float (&bias)[4]) {
+  const float4* part4 = reinterpret_cast<const float4*>(part);
+  const int pitch = share | 1;
+  constexpr int kTimes = kGemmRows / 2 * (TN / 4) / 256 > 1 ? kGemmRows / 2 * (TN / 4) / 256 : 1;
+#pragma unroll
+  for (int j = 0; j < kTimes; ++j) {
+    const int i = thread + 256 * j;
+    if (i >= rows * (TN / 4)) return;
+    // neighbouring lanes take neighbouring output columns
+    const int row = p.q_is_tokens ? i % rows : i / (TN / 4), c = 4 * (p.q_is_tokens ? i / rows : i % (TN / 4));
+    const int pr = pr0 + row, q = q0 + c;
+    if (pr >= p.p_rows || q >= p.q_rows) continue;
+    float4 sum = part4[c / 4 * pitch + row];
+    for (int k = 1; k < p.split; ++k) {
+      const float4 more = part4[(k * (TN / 4) + c / 4) * pitch + row];
+      sum.x += more.x;
+      sum.y += more.y;
+      sum.z += more.z;
+      sum.w += more.w;
+    }
+    const float v[4] = {sum.x * ga * gb, sum.y * ga * gb, sum.z * ga * gb, sum.w * ga * gb};
+    const int64_t step = p.q_is_tokens ? p.ld_out : 1;
+    T* to = static_cast<T*>(p.out) + (p.q_is_tokens ? q * p.ld_out + pr : pr * p.ld_out + q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (q + e < p.q_rows) to[e * step] = fp4_narrow<T>(v[e] + bias[p.q_is_tokens ? j : e]);
   }
 }
 
@@ -322,6 +366,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
   pdl_launch_dependents();
   pdl_wait();  // the operands are there
 
+  float ga = 1.f, gb = 1.f, split_bias[4] = {0.f, 0.f, 0.f, 0.f};  // the epilogue's
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
@@ -420,7 +465,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;
     constexpr int kCols = TN / 2;  // this warp's columns
-    float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
+    if (p.scale_a != nullptr) ga = *p.scale_a;
+    if (p.scale_b != nullptr) gb = *p.scale_b;
     if (const float both = ga * gb; fabsf(both) >= 0x1p-126f && fabsf(both) <= 0x1p126f) {
       ga = 1.f;
       gb = both;
@@ -435,6 +481,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
       fp4_tile_coords(p, tile, pt, qt);
       const int pr0 = pt * C::kRows + cta * kGemmRows + quarter * 32;  // this warp's first row
       const int q0 = qt * TN + half * kCols;
+      if (C::kSplits && p.split > 1) {
+        const int share = (kGemmRows + p.split - 1) / p.split, rows = min(share, kGemmRows - rank * share);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = threadIdx.x - 64 + 256 * j;
+          const int n = p.q_is_tokens ? pt * kGemmRows + rank * share + i % rows : qt * TN + 4 * (i % (TN / 4)) + j;
+          if (p.bias != nullptr && n < (p.q_is_tokens ? p.p_rows : p.q_rows)) split_bias[j] = fp4_gemm_bias(p, n);
+        }
+      }
       float bias[(kCols + 31) / 32];  // column 32 i + lane, or (tokens) this lane's row
 #pragma unroll
       for (int i = 0; i < (kCols + 31) / 32; ++i) {
@@ -465,11 +520,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
         else mbar_arrive(acc_empty + a * 8);
       }
       if (C::kSplits && p.split > 1) {
-        const int rows = kGemmRows / p.split;
-        const uint32_t to = mapa_shared(smem_u32(staging), row / rows) +
-                            ((rank * rows + row % rows) * C::kPartPitch + half * kCols) * 4;
+        const int share = (kGemmRows + p.split - 1) / p.split, pitch = share | 1;
+        const uint32_t to = mapa_shared(smem_u32(staging), row / share) +
+                            ((rank * (TN / 4) + half * (kCols / 4)) * pitch + row % share) * 16;
 #pragma unroll
-        for (int c = 0; c < kCols / 4; ++c) st_shared_cluster(to + 16 * c, r[c / 2] + 4 * (c % 2));
+        for (int c = 0; c < kCols / 4; ++c) st_shared_cluster(to + c * pitch * 16, r[c / 2] + 4 * (c % 2));
         continue;
       }
       float v[kCols];
@@ -482,10 +537,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
 #pragma unroll
       for (int c = 0; c < kCols; c += 2) upk2(fmul2(pk2(v[c], v[c + 1]), gab), v[c], v[c + 1]);
       if (p.q_is_tokens) {  // neighbouring lanes hold neighbouring output columns
-        if (pr0 + lane < p.p_rows) {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-            if (q0 + c < p.q_rows) fp4_gemm_store(p, (q0 + c) * p.ld_out + pr0 + lane, v[c] + bias[0]);
+        if (const int n = pr0 + lane; n < p.p_rows) {
+          if (p.out_dtype == DGXM_DTYPE_BF16) fp4_store_column<__nv_bfloat16>(p, v, bias[0], n, q0);
+          else if (p.out_dtype == DGXM_DTYPE_F16) fp4_store_column<__half>(p, v, bias[0], n, q0);
+          else fp4_store_column<float>(p, v, bias[0], n, q0);
         }
       } else {
         if (p.bias != nullptr) {
@@ -503,32 +558,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) fp4_gemm_kernel(const __grid_
   if (PAIR || (C::kSplits && p.split > 1)) cluster_sync();  // both CTAs' MMAs drained; or every partial sum is in place
   else __syncthreads();
   if (C::kSplits && p.split > 1 && warp >= 2 && *abort_flag == 0) {
-    const float ga = p.scale_a != nullptr ? *p.scale_a : 1.f, gb = p.scale_b != nullptr ? *p.scale_b : 1.f;
-    int pt, qt;
-    fp4_tile_coords(p, first_tile, pt, qt);
-    const int rows = kGemmRows / p.split, pr0 = pt * kGemmRows + rank * rows, q0 = qt * TN;
-    const float* part = reinterpret_cast<const float*>(staging);
-    for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
-      // neighbouring lanes take neighbouring output columns
-      const int row = p.q_is_tokens ? i % rows : i / (TN / 4), c = 4 * (p.q_is_tokens ? i / rows : i % (TN / 4));
-      const int pr = pr0 + row, q = q0 + c;
-      if (pr >= p.p_rows || q >= p.q_rows) continue;
-      float4 sum = *reinterpret_cast<const float4*>(part + row * C::kPartPitch + c);
-      for (int k = 1; k < p.split; ++k) {
-        const float4 more = *reinterpret_cast<const float4*>(part + (k * rows + row) * C::kPartPitch + c);
-        sum.x += more.x;
-        sum.y += more.y;
-        sum.z += more.z;
-        sum.w += more.w;
-      }
-      const float v[4] = {sum.x * ga * gb, sum.y * ga * gb, sum.z * ga * gb, sum.w * ga * gb};
-      const float one = p.q_is_tokens && p.bias != nullptr ? fp4_gemm_bias(p, pr) : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (q + e >= p.q_rows) break;
-        if (p.q_is_tokens) fp4_gemm_store(p, (q + e) * p.ld_out + pr, v[e] + one);
-        else fp4_gemm_store(p, pr * p.ld_out + q + e, v[e] + (p.bias != nullptr ? fp4_gemm_bias(p, q + e) : 0.f));
-      }
+    if constexpr (C::kSplits) {
+      const float* part = reinterpret_cast<const float*>(staging);
+      int pt, qt;
+      fp4_tile_coords(p, first_tile, pt, qt);
+      const int share = (kGemmRows + p.split - 1) / p.split, rows = min(share, kGemmRows - rank * share);
+      const int pr0 = pt * kGemmRows + rank * share, q0 = qt * TN, thread = threadIdx.x - 64;
+      if (p.out_dtype == DGXM_DTYPE_BF16)
+        fp4_store_split<__nv_bfloat16, TN>(p, part, share, rows, pr0, q0, thread, ga, gb, split_bias);
+      else if (p.out_dtype == DGXM_DTYPE_F16)
+        fp4_store_split<__half, TN>(p, part, share, rows, pr0, q0, thread, ga, gb, split_bias);
+      else
+        fp4_store_split<float, TN>(p, part, share, rows, pr0, q0, thread, ga, gb, split_bias);
     }
   }
   if (warp == 1) {
@@ -631,17 +672,21 @@ struct Fp4Cut {
 // (microseconds a stage of K, a tile, and at the least; nvfp4, 9450 x 5120 x
 // 256, 1024 and 5120, the narrow ones 1 .. 64 x 2560 .. 13824 x 256 .. 14336):
 // narrow tiles where only they fill the SMs or more are not needed (1 x 5120 x
-// 1024: 3.8 us with 16 columns, 4.9 with 64), wide ones, which load the least
+// 1024: 3.7 us with 16 columns, 4.1 with 64), wide ones, which load the least
 // for what they compute, where those do too, and K split where even those are
-// few (16 x 2560 x 5120: 8.0, 6.3, 5.5 us on 1, 2, 4 CTAs a tile).
+// few (16 x 5120 x 5120: 7.8 and 6.4 us on 1 and 3 CTAs a tile; 16 x 5120 x
+// 1024: 3.7 and 4.5).  A second tile of 16 or 32 columns would begin at an odd
+// column of scales in tensor memory, which the MMA cannot address.
 static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
   struct Kind {
     int tn, rows, at_once;
     double stage, tile, least;
   };
-  static const Kind kinds[] = {{16, 128, 148, 0.26, 0.4, 0.4},  {32, 128, 148, 0.26, 0.6, 0.6},
+  static const Kind kinds[] = {{16, 128, 148, 0.26, 0.4, 0.4},  {32, 128, 148, 0.26, 0.5, 0.5},
                                {64, 128, 148, 0.25, 0.8, 1.0},  {128, 128, 148, 0.29, 0.8, 1.1},
                                {192, 128, 148, 0.42, 1.1, 2.2}, {256, 256, 74, 0.42, 1.75, 2.2}};
+  // Clusters of a size that the SMs' groups hold at one time.
+  static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
   Fp4Cut best{128, 1, false};
   double least = 1e30;
   const bool tokens = m <= n;  // with one tile of columns, the narrow side is Q
@@ -651,11 +696,11 @@ static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
     if (kind.tn < 64 && !one) continue;
     const int64_t p_rows = one && tokens ? n : m, q_rows = one && tokens ? m : n;
     const int64_t tiles = (p_rows + kind.rows - 1) / kind.rows * ((q_rows + kind.tn - 1) / kind.tn);
-    for (int split = 1; split <= (kind.tn <= 64 ? 8 : 1) && split <= k_tiles; split *= 2) {
-      if (split > 1 && tiles * split > 148) break;
+    for (int split = 1; split <= (kind.tn <= 64 ? 8 : 1) && split <= k_tiles; ++split) {
+      if (split > 1 && tiles > clusters[split]) continue;
       const int64_t waves = (tiles * split + kind.at_once - 1) / kind.at_once;
       const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile, kind.least) +
-                        (split > 1 ? 1.3 : 0.0);  // exchange within the cluster
+                        (split > 1 ? 0.8 + 0.026 * kind.tn : 0.0);  // exchange within the cluster
       if (us < least) {
         least = us;
         best = {kind.tn, split, one && tokens};

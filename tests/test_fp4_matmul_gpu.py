@@ -62,7 +62,9 @@ SIZES = [(1, 1, 1), (1, 8, 16), (2, 256, 64), (16, 130, 100), (17, 300, 96), (33
          (65, 129, 320), (128, 256, 1024), (300, 77, 1000), (1000, 50, 320), (700, 20, 65), (500, 9, 2000),
          (129, 1280, 5120), (257, 511, 127), (5, 5120, 2049), (1003, 777, 1000), (2560, 2304, 288), (3000, 4001, 33),
          (4, 1000, 3000), (20, 900, 3000), (50, 600, 3000), (2300, 2700, 700), (2301, 2699, 700), (1100, 3100, 2000),
-         (1030, 3001, 2100)]  # narrow tiles with K split; 192 columns; CTA pairs, rows on and off 16 bytes
+         (1030, 3001, 2100), (3, 5000, 5120), (30, 3300, 5120), (10, 1900, 3600), (5000, 7, 2600), (2800, 64, 4000),
+         # narrow tiles, K split 2 .. 8 ways; 192 columns; CTA pairs, rows on and off 16 bytes
+         (5, 1900, 1700), (300, 100, 3000), (400, 200, 3500)]
 
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
