@@ -177,13 +177,27 @@ __device__ __forceinline__ uint4 fp4_piece(const Fp4GemmParams& p, const float* 
     return make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
 }
 
+// 16 bytes of the 32 in a and b from byte n on, n even and 16 at the most.
+__device__ __forceinline__ uint4 fp4_bytes_from(uint4 a, uint4 b, uint32_t n) {
+  uint32_t w[9] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, 0u};
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = (n & 16u) ? w[i + 4] : w[i];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) w[i] = (n & 8u) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = (n & 4u) ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (n & 3u));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A warp's 32 rows x NC columns of finished values (a row a lane) from row
 // pr0 and column q0 of the output.  They pass through staging rows of 128
 // bytes, 16-byte piece i of row r at piece i ^ (r & 7): the 128-byte swizzle,
 // so that a whole chunk goes out as one bulk store (rows on 16 bytes), which
 // leaves the warp to its arithmetic (9450 x 5120 x 256: 47 us with stores of
 // the lanes, 23 us), or, otherwise, neighbouring lanes store neighbouring
-// elements.  ELT: bytes of an output element.
+// words or elements.  ELT: bytes of an output element.
 template <int NC, int ELT>
 __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* stage, const float (&v)[NC], int pr0,
                                                int q0, int lane) {
@@ -192,6 +206,7 @@ __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* 
   constexpr int kCols = NC % kMost == 0 ? kMost : NC % (kMost / 2) == 0 ? kMost / 2 : NC;  // columns staged at one time
   static_assert(kCols <= kMost && NC % kCols == 0, "whole chunks");
   constexpr int kPieces = kCols / kEach;
+  using Elt = typename std::conditional<ELT == 4, uint32_t, uint16_t>::type;
 #pragma unroll
   for (int c0 = 0; c0 < NC; c0 += kCols) {
     if (q0 + c0 >= p.q_rows) return;  // uniform over the warp
@@ -223,9 +238,28 @@ __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* 
         if (pr0 + r < p.p_rows)
           *reinterpret_cast<uint4*>(out + ((pr0 + r) * p.ld_out + q0 + c0 + i * kEach) * ELT) =
               *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
+    } else if (kPieces >= 4 && q0 + c0 + kCols <= p.q_rows) {
+      // Rows off 16 bytes: whole aligned words, each from two neighbouring
+      // pieces, and by elements the bytes before the first word and behind
+      // the last, which are as many as one piece has (9450 x 5121 x 256: 102
+      // us by elements alone, 53).
+      const int i = lane % kPieces;
+#pragma unroll 4
+      for (int r = lane / kPieces; r < min(32, p.p_rows - pr0); r += 32 / kPieces) {
+        auto piece = [&](int k) { return stage + r * 128 + ((k ^ (r & 7)) << 4); };
+        char* row = static_cast<char*>(p.out) + ((pr0 + r) * p.ld_out + q0 + c0) * ELT;
+        const uint32_t head = 16u - (reinterpret_cast<uintptr_t>(row) & 15u);
+        if (i < kPieces - 1)
+          *reinterpret_cast<uint4*>(row + 16 * i + head) = fp4_bytes_from(
+              *reinterpret_cast<const uint4*>(piece(i)), *reinterpret_cast<const uint4*>(piece(i + 1)), head);
+#pragma unroll
+        for (int e = i; e < kEach; e += kPieces) {
+          const int k = e * ELT < head ? 0 : kPieces - 1;
+          *reinterpret_cast<Elt*>(row + 16 * k + e * ELT) = *reinterpret_cast<const Elt*>(piece(k) + e * ELT);
+        }
+      }
     } else {
       const int cols = min(kCols, p.q_rows - q0 - c0), rows = min(32, p.p_rows - pr0);
-      using Elt = typename std::conditional<ELT == 4, uint32_t, uint16_t>::type;
       Elt* to = reinterpret_cast<Elt*>(p.out) + pr0 * p.ld_out + q0 + c0;
 #pragma unroll
       for (int e = lane; e < kCols; e += 32) {

@@ -140,6 +140,21 @@ def test_columns_behind_the_output_stay(m, n, out_dtype):
     assert (wide[:, n:] == 7).all() and (wide[m:] == 7).all()
 
 
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,pad,first", [(300, 57, 0, 0), (40, 193, 5, 2), (2475, 300, 3, 1), (1024, 2041, 0, 0),
+                                           (2301, 2699, 2, 1), (500, 2048, 8, 3)])
+def test_output_rows_off_16_bytes(m, n, pad, first, out_dtype):
+    g = _gen(m * n)
+    a, b = _random(g, m, 320, "nvfp4"), _random(g, n, 320, "nvfp4")
+    want = _check(a, b, None, out_dtype)
+    wide = torch.full((m + 1, n + pad), 7.0, device="cuda", dtype=out_dtype).flatten()
+    out = wide[first:first + m * (n + pad)].view(m, n + pad)[:, :n]  # odd bases, strides, or both
+    assert torch.equal(fp4_matmul(a, b, out_dtype=out_dtype, out=out), want)
+    rest = torch.ones_like(wide, dtype=torch.bool)
+    rest[first:first + m * (n + pad)].view(m, n + pad)[:, :n] = False
+    assert (wide[rest] == 7).all()
+
+
 def test_nan_scales_stay_in_their_row_and_column():
     g = _gen(2)
     x = torch.randn(200, 320, device="cuda", generator=g).bfloat16()
