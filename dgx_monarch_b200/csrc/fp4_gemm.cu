@@ -177,13 +177,11 @@ __device__ __forceinline__ uint4 fp4_piece(const Fp4GemmParams& p, const float* 
     return make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
 }
 
-// 16 bytes of the 32 in a and b from byte n on, n even and 16 at the most.
+// 16 bytes of the 32 in a and b from byte n on, n even and below 16.
 __device__ __forceinline__ uint4 fp4_bytes_from(uint4 a, uint4 b, uint32_t n) {
-  uint32_t w[9] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, 0u};
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-  for (int i = 0; i < 5; ++i) w[i] = (n & 16u) ? w[i + 4] : w[i];
-#pragma unroll
-  for (int i = 0; i < 7; ++i) w[i] = (n & 8u) ? w[i + 2] : w[i];
+  for (int i = 0; i < 6; ++i) w[i] = (n & 8u) ? w[i + 2] : w[i];
 #pragma unroll
   for (int i = 0; i < 5; ++i) w[i] = (n & 4u) ? w[i + 1] : w[i];
 #pragma unroll
@@ -238,26 +236,40 @@ __device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* 
         if (pr0 + r < p.p_rows)
           *reinterpret_cast<uint4*>(out + ((pr0 + r) * p.ld_out + q0 + c0 + i * kEach) * ELT) =
               *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
-    } else if (kPieces >= 4 && q0 + c0 + kCols <= p.q_rows) {
-      // Rows off 16 bytes: whole aligned words, each from two neighbouring
-      // pieces, and by elements the bytes before the first word and behind
-      // the last, which are as many as one piece has (9450 x 5121 x 256: 102
-      // us by elements alone, 53).
-      const int i = lane % kPieces;
+    } else if (kPieces >= 4) {
+      // Rows off 16 bytes, or ending here: whole aligned words, each from two
+      // neighbouring pieces, and by elements the bytes before the first word
+      // and behind the last (9450 x 5121 x 256: 102 us by elements alone, 55;
+      // 100000 x 100 x 512, half a chunk at the end: 31, 23).
+      auto store = [&](auto whole, int bytes) {
+        constexpr bool kWhole = decltype(whole)::value;
+        const int i = lane % kPieces;
 #pragma unroll 4
-      for (int r = lane / kPieces; r < min(32, p.p_rows - pr0); r += 32 / kPieces) {
-        auto piece = [&](int k) { return stage + r * 128 + ((k ^ (r & 7)) << 4); };
-        char* row = static_cast<char*>(p.out) + ((pr0 + r) * p.ld_out + q0 + c0) * ELT;
-        const uint32_t head = 16u - (reinterpret_cast<uintptr_t>(row) & 15u);
-        if (i < kPieces - 1)
-          *reinterpret_cast<uint4*>(row + 16 * i + head) = fp4_bytes_from(
-              *reinterpret_cast<const uint4*>(piece(i)), *reinterpret_cast<const uint4*>(piece(i + 1)), head);
+        for (int r = lane / kPieces; r < min(32, p.p_rows - pr0); r += 32 / kPieces) {
+          auto piece = [&](int k) { return stage + r * 128 + ((k ^ (r & 7)) << 4); };
+          char* row = static_cast<char*>(p.out) + ((pr0 + r) * p.ld_out + q0 + c0) * ELT;
+          const int head = static_cast<int>(-reinterpret_cast<uintptr_t>(row) & 15u);
+          const int words = kWhole ? kPieces - (head > 0) : max(bytes - head, 0) / 16;
+          if (i < words)
+            *reinterpret_cast<uint4*>(row + head + 16 * i) =
+                fp4_bytes_from(*reinterpret_cast<const uint4*>(piece(i)),
+                               *reinterpret_cast<const uint4*>(piece(min(i + 1, kPieces - 1))), head);
+          auto element = [&](int at) {
+            *reinterpret_cast<Elt*>(row + at) = *reinterpret_cast<const Elt*>(piece(at / 16) + at % 16);
+          };
 #pragma unroll
-        for (int e = i; e < kEach; e += kPieces) {
-          const int k = e * ELT < head ? 0 : kPieces - 1;
-          *reinterpret_cast<Elt*>(row + 16 * k + e * ELT) = *reinterpret_cast<const Elt*>(piece(k) + e * ELT);
+          for (int e = i; e < kEach; e += kPieces) {
+            if (kWhole) {  // the bytes before and behind are none, or as many as a piece has
+              if (head > 0) element(e * ELT < head ? e * ELT : 16 * (kPieces - 1) + e * ELT);
+            } else {
+              if (e * ELT < min(head, bytes)) element(e * ELT);
+              if (head + 16 * words + e * ELT < bytes) element(head + 16 * words + e * ELT);
+            }
+          }
         }
-      }
+      };
+      if (q0 + c0 + kCols <= p.q_rows) store(std::true_type{}, kCols * ELT);
+      else store(std::false_type{}, (p.q_rows - q0 - c0) * ELT);
     } else {
       const int cols = min(kCols, p.q_rows - q0 - c0), rows = min(32, p.p_rows - pr0);
       Elt* to = reinterpret_cast<Elt*>(p.out) + pr0 * p.ld_out + q0 + c0;
