@@ -154,8 +154,9 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
     out: an Fp4Tensor of x's shape and the format to write into, its scale
     included."""
     given = scale if isinstance(scale, torch.Tensor) else None
-    key = ("q", x.shape, x.stride(), x.dtype, x.get_device(), format,
-           scale if given is None else (given.dtype, given.get_device(), given.numel()),
+    number = None if scale is None or given is not None else float(scale)
+    key = ("q", x.shape, x.stride(), x.dtype, x.get_device(), format, number is not None,
+           None if given is None else (given.dtype, given.get_device(), given.numel()),
            None if out is None else (out.shape, out.format, out._devices))
 
     def make():
@@ -171,8 +172,6 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
             raise ValueError("mxfp4 has no scale for the tensor")
         if given is not None and (given.dtype not in _FLOATS or given.numel() != 1):
             raise ValueError(f"scale {tuple(given.shape)} {given.dtype} is not one element of fp32, bf16 or fp16")
-        if scale is not None and given is None and not (0.0 < scale < 3.4e38):
-            raise ValueError(f"scale {scale} is not a positive finite number")
         if out is not None:
             if out.shape != tuple(x.shape) or out.format != format:
                 raise ValueError(f"out is {out}, x is {tuple(x.shape)} for {format}")
@@ -181,9 +180,6 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
         desc.rows, desc.cols, desc.format = math.prod(x.shape[:-1]), x.shape[-1], code
         desc.dtype = _dtype_code(x.dtype)
         desc.scale_dtype = _lib.DTYPE_F32 if given is None else _dtype_code(given.dtype)
-        desc.scale_value = 0.0 if given is not None or scale is None else scale
-        if scale is not None and given is None and desc.scale_value == 0.0:
-            raise ValueError(f"scale {scale} is zero in fp32")
         flat = x.reshape(-1, x.shape[-1]) if x.numel() else x
         folds = x.numel() == 0 or (flat.data_ptr() == x.data_ptr()
                                    and (desc.rows == 1 or flat.stride(0) >= desc.cols))  # not overlapping or expanded
@@ -193,6 +189,13 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
 
     desc, folds, need, layout = plan(key, make)
     no_graph("", x, given)
+    if number is not None:  # data, like a scale on the device: checked and set in each call
+        if not 0.0 < number < 3.4e38:
+            raise ValueError(f"scale {scale} is not a positive finite number")
+        desc = _lib.Fp4Desc.from_buffer_copy(desc)  # another thread may be using the plan's own
+        desc.scale_value = number
+        if desc.scale_value == 0.0:
+            raise ValueError(f"scale {scale} is zero in fp32")
     if not folds:
         x = x.reshape(-1, layout.cols).contiguous()
     if out is None:

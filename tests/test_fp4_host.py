@@ -211,6 +211,27 @@ def test_python_argument_checks(monkeypatch, make, error):
         make(fp4)
 
 
+def test_a_number_as_scale_is_no_part_of_the_plan(monkeypatch):
+    """Scales that change from call to call make one plan, and drop no other operator's; each call gets its own."""
+    from dgx_monarch_b200 import _call, fp4
+
+    got = []
+    monkeypatch.setattr(_call, "_PLANS", {"another operator's": object()})
+    monkeypatch.setattr(fp4, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(fp4, "launch", lambda name, index, desc, *a: got.append(desc))
+    x = torch.zeros(4, 64)
+    scales = [1.0 + i / 1024 for i in range(2 * _call._MOST_PLANS)]
+    for scale in scales:
+        fp4.quantize_fp4(x, scale=scale)
+    assert len(_call._PLANS) == 2 and "another operator's" in _call._PLANS
+    assert [d.scale_value for d in got] == scales  # exact in fp32
+    for bad in (0.0, -1.0, 1e-50, float("inf"), float("nan"), 1e39):  # with the plan there
+        with pytest.raises(ValueError, match="scale"):
+            fp4.quantize_fp4(x, scale=bad)
+    fp4.quantize_fp4(x, scale=torch.ones(()))
+    assert got[-1].scale_value == 0.0 and len(got) == len(scales) + 1
+
+
 def test_no_autograd_graph():
     from dgx_monarch_b200 import _call
 
