@@ -155,12 +155,18 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
     """Gradients of qk_norm_rope (dgxm_qk_norm_rope_backward): (gq, gk, gwq,
     gwk) from the upstream gradients dq, dk of its outputs and its inputs.
 
-    gq and gk have the full shape of q and k (an expanded input's gradient is
+    dq and dk may have any strides: one without a contiguous D (the expanded
+    ones that a sum passes back) is copied first, unlike q and k.  gq and gk
+    have the full shape of q and k (an expanded input's gradient is
     the caller's to sum) and gwq / gwk the weights' dtype, each summed over
     batch, rows and heads in fp32; gk, gwq and gwk are None where the
     corresponding argument is.  A weight that serves both q and k has the sum
     of gwq and gwk as its gradient.  The sums' order is fixed: the same call
     gives the same bits."""
+    if dq.ndim and dq.stride(-1) != 1:
+        dq = dq.contiguous()
+    if dk is not None and dk.ndim and dk.stride(-1) != 1:
+        dk = dk.contiguous()
     key = ("b", _meta(dq), _meta(dk), _meta(q), _meta(k), norm_mode, _meta(norm_q_w), _meta(norm_k_w), eps,
            _meta(rope), rope_halves)
 

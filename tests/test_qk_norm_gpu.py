@@ -170,6 +170,19 @@ def test_odd_alignment_and_transposed_strides(dtype, halves):
     _check_backward(gk, gwk, dk, k, wk, rope, halves, 1e-6, True)
 
 
+def test_upstream_gradients_of_a_sum_and_of_a_transposed_use():
+    g = _gen(18)
+    q = torch.randn(2, 9, 5, 64, device="cuda", generator=g).bfloat16()
+    k = torch.randn(2, 9, 2, 64, device="cuda", generator=g).bfloat16()
+    w = torch.randn(64, device="cuda", generator=g)
+    rope = _table(9, 32, g)
+    dq = torch.ones((), device="cuda", dtype=BF16).expand(q.shape)
+    dk = torch.randn(64, 2, 9, 2, device="cuda", generator=g).bfloat16().permute(1, 2, 3, 0)
+    gq, gk, gwq, gwk = qk_norm_rope_backward(dq, dk, q, k, norm_q_w=w, norm_k_w=w, rope=rope)
+    _check_backward(gq, gwq, dq, q, w, rope, False, 1e-6, True)
+    _check_backward(gk, gwk, dk, k, w, rope, False, 1e-6, True)
+
+
 @pytest.mark.parametrize("halves", [False, True])
 def test_in_place_is_the_same(halves):
     g = _gen(4)

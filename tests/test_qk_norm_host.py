@@ -142,3 +142,38 @@ def test_output_and_gradient_checks():
         qk_norm.no_graph("", None, w)
     with torch.no_grad():
         qk_norm.no_graph("", None, w)
+
+
+@pytest.mark.parametrize("layout", ["expanded", "head_dim first", "head_dim of a wider step"])
+def test_upstream_gradients_of_any_strides(lib, monkeypatch, layout):
+    """One that a sum passes back, and others without a contiguous head_dim, reach the kernel as whole tensors."""
+    from dgx_monarch_b200 import qk_norm
+
+    seen = []
+
+    def launch(name, index, desc, dq, dk, *rest):
+        seen.append((tuple(desc.dq_stride), tuple(desc.dk_stride), dq, dk))
+
+    monkeypatch.setattr(qk_norm, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(qk_norm, "launch", launch)
+
+    def upstream(heads):
+        if layout == "expanded":
+            return torch.ones(()).expand(2, 3, heads, 64)
+        if layout == "head_dim first":
+            return torch.zeros(64, 2, 3, heads).permute(1, 2, 3, 0)
+        return torch.zeros(2, 3, heads, 128)[..., ::2]
+
+    q, k = torch.zeros(2, 3, 4, 64), torch.zeros(2, 3, 2, 64)
+    dq, dk = upstream(4), upstream(2)
+    gq, gk, _, _ = qk_norm.qk_norm_rope_backward(dq, dk, q, k)
+    assert gq.shape == q.shape and gk.shape == k.shape
+    (qs, ks, pq, pk), = seen
+    assert qs == (3 * 4 * 64, 4 * 64, 64) and ks == (3 * 2 * 64, 2 * 64, 64)
+    assert pq != dq.data_ptr() and pk != dk.data_ptr()
+    qk_norm.qk_norm_rope_backward(q, k, q, k)  # whole ones as they are
+    assert seen[1][2:] == (q.data_ptr(), k.data_ptr())
+    with pytest.raises(ValueError, match="4-D"):
+        qk_norm.qk_norm_rope_backward(torch.ones(()), dk, q, k)
+    with pytest.raises(ValueError, match="contiguous head_dim"):
+        qk_norm.qk_norm_rope_backward(q, k, q, dk)
