@@ -188,7 +188,7 @@ def quantize_fp4(x: torch.Tensor, *, format: str = "nvfp4", scale: torch.Tensor 
         return desc, folds, need, _Layout(x.shape, format, x.get_device(), need)
 
     desc, folds, need, layout = plan(key, make)
-    no_graph("", x, given)
+    no_graph("", x, given, None if out is None else out._scale)
     if number is not None:  # data, like a scale on the device: checked and set in each call
         if not 0.0 < number < 3.4e38:
             raise ValueError(f"scale {scale} is not a positive finite number")
@@ -229,6 +229,7 @@ def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, *,
         return desc
 
     desc = plan(key, make)
+    no_graph("", t._scale, out)
     if out is None:
         out = t._tensors()[0].new_empty(t.shape, dtype=dtype)
     launch("dgxm_dequantize_fp4", t._devices[0], desc, *t._pointers(), out.data_ptr())
@@ -278,7 +279,7 @@ def fp4_matmul(a: Fp4Tensor, b: Fp4Tensor, *, bias: torch.Tensor | None = None,
         return desc, shape
 
     desc, shape = plan(key, make)
-    no_graph("", bias)
+    no_graph("", bias, a._scale, b._scale, out)
     if out is None:
         out = a._tensors()[0].new_empty(shape, dtype=out_dtype)
     launch("dgxm_fp4_matmul", a._devices[0], desc, *a._pointers(), *b._pointers(), _ptr(bias), out.data_ptr())

@@ -131,7 +131,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
         return desc
 
     desc = plan(key, make)
-    no_graph(_GRADS, q, k, norm_q_w, norm_k_w, rope)
+    no_graph(_GRADS, q, k, norm_q_w, norm_k_w, rope, q_out, k_out)
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:

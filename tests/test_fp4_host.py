@@ -242,6 +242,34 @@ def test_no_autograd_graph():
         _call.no_graph("", w)
 
 
+def test_every_tensor_that_requires_a_gradient_is_refused(monkeypatch):
+    """The scale of a packed tensor and an output to write into among them."""
+    from dgx_monarch_b200 import fp4, qk_norm
+
+    for module in (fp4, qk_norm):
+        monkeypatch.setattr(module, "_require_cuda", lambda *a: None)
+        monkeypatch.setattr(module, "launch", lambda *a: None)
+    x, bias = torch.zeros(4, 64), torch.zeros(4)
+    learned = _packed(scale=torch.ones((), requires_grad=True))
+    out, out_q = torch.zeros(4, 4, requires_grad=True), torch.zeros(1, 4, 2, 64, requires_grad=True)
+    q = torch.zeros(1, 4, 2, 64)
+    made = fp4.quantize_fp4(x)
+    made.scale.requires_grad_(True)
+    calls = [lambda: fp4.quantize_fp4(x, out=learned), lambda: fp4.dequantize_fp4(learned),
+             lambda: fp4.dequantize_fp4(made),
+             lambda: fp4.dequantize_fp4(_packed(), torch.float32, out=torch.zeros(4, 64, requires_grad=True)),
+             lambda: fp4.fp4_matmul(learned, _packed()), lambda: fp4.fp4_matmul(_packed(), learned),
+             lambda: fp4.fp4_matmul(_packed(), _packed(), out_dtype=torch.float32, out=out),
+             lambda: fp4.fp4_matmul(_packed(), _packed(), bias=bias.clone().requires_grad_()),
+             lambda: qk_norm.qk_norm_rope(q, q.clone(), q_out=out_q),
+             lambda: qk_norm.qk_norm_rope(q, q.clone(), k_out=out_q)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc is absent")
 def test_struct_layouts_match_the_header(tmp_path):
     from dgx_monarch_b200 import _lib
