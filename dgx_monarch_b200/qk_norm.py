@@ -113,6 +113,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
     q_out / k_out may be q / k themselves (same strides); they must not
     overlap the inputs, or each other, in any other way.  No autograd graph is recorded: see
     qk_norm_rope_backward."""
+    eps, rope_halves = float(eps), bool(rope_halves)  # values, never the identity of a number held in a tensor
     key = ("f", _meta(q), _meta(k), norm_mode, _meta(norm_q_w), _meta(norm_k_w), eps, _meta(rope), rope_halves,
            _meta(q_out), _meta(k_out))
 
@@ -163,6 +164,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
     corresponding argument is.  A weight that serves both q and k has the sum
     of gwq and gwk as its gradient.  The sums' order is fixed: the same call
     gives the same bits."""
+    eps, rope_halves = float(eps), bool(rope_halves)
     if dq.ndim and dq.stride(-1) != 1:
         dq = dq.contiguous()
     if dk is not None and dk.ndim and dk.stride(-1) != 1:

@@ -177,3 +177,20 @@ def test_upstream_gradients_of_any_strides(lib, monkeypatch, layout):
         qk_norm.qk_norm_rope_backward(torch.ones(()), dk, q, k)
     with pytest.raises(ValueError, match="contiguous head_dim"):
         qk_norm.qk_norm_rope_backward(q, k, q, dk)
+
+
+def test_numbers_held_in_tensors_are_read_in_each_call(lib, monkeypatch):
+    """An eps and an order of pairs that change in place between calls."""
+    from dgx_monarch_b200 import qk_norm
+
+    seen = []
+    monkeypatch.setattr(qk_norm, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(qk_norm, "launch", lambda name, index, desc, *a: seen.append((desc.eps, desc.rope_halves)))
+    q, rope = torch.zeros(1, 4, 2, 64), torch.zeros(4, 32, 2)
+    eps, halves = torch.tensor(0.25), torch.tensor(False)
+    for _ in range(2):
+        qk_norm.qk_norm_rope(q, q.clone(), eps=eps, rope=rope, rope_halves=halves)
+        qk_norm.qk_norm_rope_backward(q, q, q, q, eps=eps, rope=rope, rope_halves=halves)
+        eps.fill_(0.5)
+        halves.fill_(True)
+    assert seen == [(0.25, 0), (0.25, 0), (0.5, 1), (0.5, 1)]
