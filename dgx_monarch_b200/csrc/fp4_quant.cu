@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kFp4Threads) fp4_quantize_kernel(const __grid_
       g = p.scale != nullptr ? fp4_read_scale(p.scale, p.scale_dtype) : p.scale_value;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale_out = g;
-    bad = !(g >= 0.f) || __float_as_uint(g) >= 0x7F800000u;  // NaN, negative or infinite
+    bad = !(g >= 0.f && g < INFINITY);  // NaN, negative or infinite; -0 is a zero
     up = g < 0x1p-64f ? 0x1p64f : g > 0x1p64f ? 0x1p-64f : 1.f;
     g *= up;
     inv6g = g > 0.f ? __frcp_rn(6.f * g) : 0.f;

@@ -218,6 +218,13 @@ def test_zeros_infinities_and_nan(fmt, dtype):
         assert (dequantize_fp4(quantize_fp4(torch.ones_like(zero), scale=torch.zeros((), device="cuda"))) == 0).all()
 
 
+@pytest.mark.parametrize("scale_dtype", [BF16, F16, F32])
+def test_a_scale_of_minus_zero_is_zero(scale_dtype):
+    x = torch.ones(3, 40, device="cuda")
+    t = _check(x, "nvfp4", torch.tensor(-0.0, device="cuda", dtype=scale_dtype))
+    assert (dequantize_fp4(t) == 0).all()
+
+
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_strides_alignment_and_leading_dimensions(fmt, dtype):
