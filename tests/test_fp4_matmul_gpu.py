@@ -155,6 +155,95 @@ def test_output_rows_off_16_bytes(m, n, pad, first, out_dtype):
     assert (wide[rest] == 7).all()
 
 
+# More tiles than CTAs (or CTA pairs) at one time: 320 and 256 tiles on 74 pairs, in the first with rows on 16 bytes
+# whatever the type; 157 and 313 of 16, 32 and 64 columns on 148 CTAs, either operand's rows as the tile's; 216 of 192.
+MANY_TILES = [(4000, 5000, 2000), (4000, 4097, 1500), (9, 20000, 300), (20000, 9, 300), (30, 20001, 300),
+              (20000, 30, 300), (50, 40000, 300), (20000, 60, 300), (3000, 1600, 2100)]
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", MANY_TILES)
+def test_many_tiles_exact_sums(fmt, m, n, k):
+    test_exact_sums(fmt, m, n, k)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,k", [(4000, 5000, 2000), (4000, 4097, 1500), (9, 20000, 300), (20000, 30, 300),
+                                   (3000, 1600, 2100)])
+def test_many_tiles_with_bias(fmt, out_dtype, m, n, k):
+    """_check's bound, for sums that may also leave a 16-bit type: the border
+    between its largest value and infinity is half a step above that value
+    (fp16: 65504 + 16).  A sum above it by more than the fp32 error has to be
+    infinite, with its sign, and none below it by more may be."""
+    g = _gen(m + n)
+    a, b = _random(g, m, k, fmt), _random(g, n, k, fmt)
+    bias = torch.randn(n, device="cuda", generator=g)
+    got = fp4_matmul(a, b, bias=bias, out_dtype=out_dtype)
+    x, w = _exact_values(a), _exact_values(b)
+    want, size = x @ w.T + bias.double(), x.abs() @ w.abs().T + bias.double().abs()
+    info = torch.finfo(out_dtype)
+    fp32_error = ((k + 15) // 16 + 8) * 2.0 ** -23 * size + 3 * 2.0 ** -24 * size
+    border = info.max * (1 + info.eps / 2 / (2 - info.eps))  # max = (2 - eps) 2^e, half its step = eps / 2 2^e
+    over = got.isinf()
+    assert not got.isnan().any()
+    assert (want.abs() + fp32_error >= border)[over].all() and (got[over].double().sign() == want[over].sign()).all()
+    assert not (want.abs() - fp32_error > border)[~over].any()
+    tol = fp32_error + info.eps / 2 * 1.001 * want.abs() + info.tiny
+    assert ((got.double() - want).abs() <= tol)[~over].all()
+    assert torch.equal(got, fp4_matmul(a, b, bias=bias, out_dtype=out_dtype))
+
+
+@pytest.mark.parametrize("out_dtype", [BF16, F32])
+def test_many_tiles_leave_the_rest_of_the_output(out_dtype):
+    """CTA pairs with several tiles each, rows on 16 bytes in a wider matrix: nothing before, behind or below is touched."""
+    g = _gen(11)
+    m, n = 4000, 4100
+    a, b = _random(g, m, 600, "nvfp4"), _random(g, n, 600, "nvfp4")
+    want = _check(a, b, None, out_dtype)
+    wide = torch.full((m + 1, n + 44), 7.0, device="cuda", dtype=out_dtype)
+    assert torch.equal(fp4_matmul(a, b, out_dtype=out_dtype, out=wide[:m, 16:16 + n]), want)
+    assert (wide[:, :16] == 7).all() and (wide[:, 16 + n:] == 7).all() and (wide[m] == 7).all()
+
+
+def test_one_plan_on_another_alignment_and_from_two_threads():
+    """Sizes and strides of the output alike, bases on 16 bytes and off them; and threads that call at the same time."""
+    import threading
+
+    g = _gen(12)
+    a, b = _random(g, 90, 512, "nvfp4"), _random(g, 256, 512, "nvfp4")
+    x = torch.randn(90 * 512 + 8, device="cuda", generator=g).bfloat16()
+    want = _check(a, b)
+    flat = torch.empty(90 * 256 + 8, device="cuda", dtype=BF16)
+    for first in (0, 1, 8, 5):
+        assert torch.equal(fp4_matmul(a, b, out=flat[first:first + 90 * 256].view(90, 256)), want)
+    chains = {}
+    for first in (0, 1, 8, 5):
+        rows = x[first:first + 90 * 512].view(90, 512)
+        chains[first] = rows, fp4_matmul(quantize_fp4(rows), b), fp4_matmul(quantize_fp4(rows, scale=0.01), b)
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(first):
+        try:
+            rows = chains[first][0]
+            with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                got[first] = [(fp4_matmul(quantize_fp4(rows), b), fp4_matmul(quantize_fp4(rows, scale=0.01), b))
+                              for _ in range(50)]
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 - shown below, from the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(first,)) for first in chains]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for first, calls in got.items():
+        assert all(torch.equal(u, chains[first][1]) and torch.equal(v, chains[first][2]) for u, v in calls)
+
+
 def test_nan_scales_stay_in_their_row_and_column():
     g = _gen(2)
     x = torch.randn(200, 320, device="cuda", generator=g).bfloat16()

@@ -170,6 +170,40 @@ def test_odd_alignment_and_transposed_strides(dtype, halves):
     _check_backward(gk, gwk, dk, k, wk, rope, halves, 1e-6, True)
 
 
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("b,l,hq,hk,d,rot,dtype,pad", [
+    (1, 4000, 20, 4, 96, 96, F16, 0),    # two chunks of five rows a lane group, and one that two rows fill
+    (1, 4000, 13, 3, 128, 128, BF16, 0),  # seven rows, six in the other lane group
+    (2, 2000, 13, 3, 128, 64, F32, 0),   # a full ring of four, the last chunk shorter
+    (1, 4001, 30, 10, 64, 64, BF16, 0),  # a full ring of eight, four lane groups
+    (4, 1000, 5, 2, 256, 256, BF16, 0),  # one lane group
+    (2, 2000, 13, 3, 72, 36, F16, 0),    # halves off the lanes' vectors
+    (1, 4000, 13, 3, 96, 96, BF16, 1),   # rows off 16 bytes
+    (1, 4001, 13, 3, 96, 36, F32, 1),
+])
+def test_many_tokens(b, l, hq, hk, d, rot, dtype, pad, halves):
+    """Calls large enough that a warp keeps several heads' rows under way (from
+    148 * 48 warps on) and, in the gradient, takes several chunks (from 888
+    blocks of four warps on): at most 6 chunks of 8 rows a lane, so dw's longest
+    chain is 48 + 2 (lane groups) + 4 (warps) + 28 + 32 (blocks) additions."""
+    g = _gen(l + d)
+    qkv = (torch.randn(b, l, hq + 2 * hk, d + pad, device="cuda", generator=g)
+           * torch.exp(torch.randn(b, l, 1, 1, device="cuda", generator=g))).to(dtype)[..., pad:]
+    q, k = qkv[:, :, :hq], qkv[:, :, hq + hk:]
+    wq, wk = (torch.randn(d, device="cuda", generator=g).to(dtype) for _ in range(2))
+    rope = _table(l, rot // 2, g, b)
+    how = {"norm_q_w": wq, "norm_k_w": wk, "rope": rope, "rope_halves": halves}
+    yq, yk = qk_norm_rope(q, k, **how)
+    _check_forward(yq, q, wq, rope, halves, 1e-6, True)
+    _check_forward(yk, k, wk, rope, halves, 1e-6, True)
+    dq, dk = (torch.randn(b, l, h, d + pad, device="cuda", generator=g).to(dtype)[..., pad:] for h in (hq, hk))
+    gq, gk, gwq, gwk = qk_norm_rope_backward(dq, dk, q, k, **how)
+    _check_backward(gq, gwq, dq, q, wq, rope, halves, 1e-6, True)
+    _check_backward(gk, gwk, dk, k, wk, rope, halves, 1e-6, True)
+    again = qk_norm_rope_backward(dq, dk, q, k, **how)
+    assert all(torch.equal(x, y) for x, y in zip((gq, gk, gwq, gwk), again))
+
+
 def test_upstream_gradients_of_a_sum_and_of_a_transposed_use():
     g = _gen(18)
     q = torch.randn(2, 9, 5, 64, device="cuda", generator=g).bfloat16()
@@ -313,6 +347,54 @@ def test_streams_graphs_and_two_calls_at_once():
     torch.cuda.synchronize()
     for _, outs in graphs:
         assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+def test_one_plan_on_another_alignment_and_from_two_threads():
+    """Sizes and strides alike, bases on 16 bytes and 2 past them; and two threads that call at the same time."""
+    import threading
+
+    g = _gen(19)
+    w = torch.randn(64, device="cuda", generator=g).bfloat16()
+    rope = _table(50, 32, g)
+    how = {"norm_q_w": w, "norm_k_w": w, "rope": rope}
+    flat = torch.randn(2 * 50 * 6 * 64 + 8, device="cuda", generator=g).bfloat16()
+    up = torch.randn(2 * 50 * 6 * 64 + 8, device="cuda", generator=g).bfloat16()
+
+    def at(t, first):
+        return t[first:first + 2 * 50 * 6 * 64].view(2, 50, 6, 64)
+
+    def call(first):
+        q, dq = at(flat, first), at(up, first)
+        return (*qk_norm_rope(q[:, :, :4], q[:, :, 4:], **how),
+                *qk_norm_rope_backward(dq[:, :, :4], dq[:, :, 4:], q[:, :, :4], q[:, :, 4:], **how))
+
+    want = {}
+    for first in (0, 1, 8, 3):
+        yq, yk, gq, gk, gwq, gwk = want[first] = call(first)
+        q, dq = at(flat, first), at(up, first)
+        _check_forward(yq, q[:, :, :4], w, rope, False, 1e-6, True)
+        _check_forward(yk, q[:, :, 4:], w, rope, False, 1e-6, True)
+        _check_backward(gq, gwq, dq[:, :, :4], q[:, :, :4], w, rope, False, 1e-6, True)
+        _check_backward(gk, gwk, dq[:, :, 4:], q[:, :, 4:], w, rope, False, 1e-6, True)
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(first):
+        try:
+            with torch.no_grad(), torch.cuda.stream(torch.cuda.Stream()):
+                got[first] = [call(first) for _ in range(50)]
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 - shown below, from the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(first,)) for first in want]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for first, calls in got.items():
+        assert all(torch.equal(x, y) for outs in calls for x, y in zip(outs, want[first]))
 
 
 def test_matches_the_fused_prologue_up_to_its_roundings():
