@@ -2,11 +2,14 @@
 position embedding in the same pass, on this rank's own tensors, and its
 gradient.
 
-The reference's block forwards run these as separate modules before the
-attention seam (Q/K norm and RoPE, adapters/wan_family.py:70-73).  prologue.py
-fuses them with the Ulysses scatter; the calls here serve where nothing is
-scattered (one rank, ring attention, cross attention) and where the block is
-trained.  There is no CPU path.
+The norm is the QKNorm of the Flux and Krea2 blocks, over each head's values,
+which those blocks run with RoPE before the attention seam (inside the forwards
+of adapters/flux_family.py:108-265 and adapters/krea2.py:130-246).  Wan's
+norm_q / norm_k go over all heads of a row (adapters/wan_family.py:70-71) and
+are not this norm; its rotation (adapters/wan_family.py:73) is NORM_NONE here.
+prologue.py fuses both norms with the Ulysses scatter; the calls here serve
+where nothing is scattered (one rank, ring attention, cross attention) and
+where the block is trained.  There is no CPU path.
 """
 from __future__ import annotations
 

@@ -635,8 +635,11 @@ int dgxm_cfg_combine(const void* cond, const void* uncond, int64_t n, int32_t dt
  * are head_dim values of weight_dtype (dtype, or F32), or NULL.  fp32 inside,
  * rounded once.  The outputs may be the inputs themselves (same strides).
  *
- * Serves the reference's Q/K norm and RoPE (adapters/wan_family.py:70-73)
- * where no scatter follows.
+ * Serves the per-head QKNorm and RoPE of the Flux and Krea2 blocks (inside the
+ * forwards of adapters/flux_family.py:108-265, adapters/krea2.py:130-246) where
+ * no scatter follows, and under DGXM_NORM_NONE Wan's apply_rope1
+ * (adapters/wan_family.py:73).  Wan's own norm over all heads of a row
+ * (adapters/wan_family.py:70-71, DGXM_NORM_HIDDEN) is refused here.
  */
 typedef struct dgxm_qk_norm_desc {
   int32_t batch, seq, q_heads, k_heads, head_dim, rot_dim;
