@@ -15,8 +15,9 @@
 
 namespace dgxm {
 
-// About one second at the B200 boost clock.  A correct kernel never waits
-// longer than a few microseconds on any single barrier phase.
+// About one second at the B200 boost clock.  A correct kernel waits a few
+// microseconds on a barrier phase, or as long as one tile's products take: at
+// the most 33 ms, behind the 4-bit product's longest K (2^24 columns).
 constexpr long long kWaitBudgetCycles = 2000000000LL;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
