@@ -23,14 +23,14 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _GRADS = " and take the gradients from qk_norm_rope_backward"
 
 
-def _check_rows(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
+def _check_rows(name: str, t: torch.Tensor, q: torch.Tensor, whole: bool = True) -> None:
     if t.ndim != 4:
         raise ValueError(f"{name} must be 4-D (batch, rows, heads, head_dim), got {tuple(t.shape)}")
     if t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3]:
         raise ValueError(f"{name} {tuple(t.shape)} does not share (batch, rows, head_dim) with q {tuple(q.shape)}")
     if t.dtype != q.dtype:
         raise TypeError(f"{name} is {t.dtype}, q is {q.dtype}: they must share one dtype")
-    if t.shape[3] > 1 and t.stride(3) != 1:
+    if whole and t.shape[3] > 1 and t.stride(3) != 1:
         raise ValueError(f"{name} must have a contiguous head_dim")
 
 
@@ -168,10 +168,6 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
     of gwq and gwk as its gradient.  The sums' order is fixed: the same call
     gives the same bits."""
     eps, rope_halves = float(eps), bool(rope_halves)
-    if dq.ndim and dq.stride(-1) != 1:
-        dq = dq.contiguous()
-    if dk is not None and dk.ndim and dk.stride(-1) != 1:
-        dk = dk.contiguous()
     key = ("b", _meta(dq), _meta(dk), _meta(q), _meta(k), norm_mode, _meta(norm_q_w), _meta(norm_k_w), eps,
            _meta(rope), rope_halves)
 
@@ -184,19 +180,23 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor | None, q: torch.Te
                                          (dk, k, desc.dk_stride, desc.k_out_stride, "dk")):
             if src is None:
                 continue
-            _check_rows(name, up, q)
+            _check_rows(name, up, q, whole=False)
             if up.shape != src.shape:
                 raise ValueError(f"{name} {tuple(up.shape)} is not the gradient of a {tuple(src.shape)} tensor")
-            ups[:] = up.stride()[:3]
             h, d = src.shape[2], src.shape[3]
             outs[:] = [src.shape[1] * h * d, h * d, d]
+            ups[:] = outs if up.stride(3) != 1 else up.stride()[:3]
         need = _lib.load().dgxm_qk_norm_rope_backward_workspace(desc)
         if need < 0:
             _lib.check(_lib.DGXM_ERR_INVALID, "dgxm_qk_norm_rope_backward_workspace")
-        return desc, need
+        scattered = dq.stride(3) != 1 or (dk is not None and dk.stride(3) != 1)
+        return desc, need, scattered
 
-    desc, need = plan(key, make)
+    desc, need, scattered = plan(key, make)
     no_graph(_GRADS, dq, dk, q, k, norm_q_w, norm_k_w, rope)
+    if scattered:
+        dq = dq if dq.stride(3) == 1 else dq.contiguous()
+        dk = dk if dk is None or dk.stride(3) == 1 else dk.contiguous()
     gq = torch.empty_like(q, memory_format=torch.contiguous_format)
     gk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     gwq = None if norm_q_w is None else torch.empty_like(norm_q_w)
