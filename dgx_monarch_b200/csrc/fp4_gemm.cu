@@ -721,7 +721,11 @@ struct Fp4Cut {
 // 1024: 3.7 us with 16 columns, 4.1 with 64), wide ones, which load the least
 // for what they compute, where those do too, and K split where even those are
 // few (16 x 5120 x 5120: 7.8 and 6.4 us on 1 and 3 CTAs a tile; 16 x 5120 x
-// 1024: 3.7 and 4.5).  A second tile of 16 or 32 columns would begin at an odd
+// 1024: 3.7 and 4.5).  The sums order the cuts and are not the times of calls:
+// launches in a row took 10.1 us where they say 5.8 (65 x 5120 x 5120), 12.0
+// for 6.6 (300 rows), 11.8 for 9.5 (512), 17.3 for 19.0 (1024), and 117 for 147
+// (40000 x 5120 x 1024).  mxfp4, with half the copies of scales, takes the same
+// cuts and 0.1 to 2.4 us less at K = 5120.  A second tile of 16 or 32 columns would begin at an odd
 // column of scales in tensor memory, which the MMA cannot address.
 static Fp4Cut fp4_cut(int64_t m, int64_t n, int k_tiles) {
   struct Kind {
