@@ -61,8 +61,8 @@ class Fp4Tensor:
 
     values: uint8 of values_shape, zero past the last column; scales: uint8 of
     scales_shape, zero past a row's last block (bytes of rows past the last are not
-    read); scale: the fp32 scale of an nvfp4 tensor (one element on the device),
-    None for mxfp4.  quantize_fp4 makes them; a weight kept in this layout is
+    read; e4m3 ones have no sign, 0x7F at the most); scale: the fp32 scale of an
+    nvfp4 tensor (one element on the device), None for mxfp4.  quantize_fp4 makes them; a weight kept in this layout is
     wrapped as it is."""
 
     __slots__ = ("shape", "format", "rows", "cols", "_values", "_scales", "_scale", "_buffer", "_offsets", "_devices")

@@ -111,7 +111,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None = None, *, norm_mode: i
     (prologue.rope_table); the first 2 P values of a head are rotated, values
     2i and 2i + 1 with each other, or i and P + i with rope_halves.  norm_mode
     NORM_NONE rotates alone.  Sums and rotation are fp32, rounded once; a head
-    whose sum of squares leaves fp32's range (values above 1e18) comes out zero.
+    whose sum of squares leaves fp32's range comes out zero (values above 1e18)
+    or, with an eps of zero, loses digits and ends infinite or NaN (values below
+    1e-18).
 
     q_out / k_out may be q / k themselves (same strides); they must not
     overlap the inputs, or each other, in any other way.  No autograd graph is recorded: see

@@ -633,7 +633,9 @@ int dgxm_cfg_combine(const void* cond, const void* uncond, int64_t n, int32_t dt
  * sines, rope_batch_stride floats apart by batch item (0: one table).  Pair i
  * is values 2i and 2i + 1, or i and rot_dim / 2 + i with rope_halves.  Weights
  * are head_dim values of weight_dtype (dtype, or F32), or NULL.  fp32 inside,
- * rounded once.  The outputs may be the inputs themselves (same strides).
+ * rounded once; a head whose sum of squares leaves fp32's range comes out zero,
+ * or, below it and without an eps, not finite.  The outputs may be the inputs
+ * themselves (same strides).
  *
  * Serves the per-head QKNorm and RoPE of the Flux and Krea2 blocks (inside the
  * forwards of adapters/flux_family.py:108-265, adapters/krea2.py:130-246) where
@@ -684,6 +686,8 @@ int dgxm_qk_norm_rope_backward(const dgxm_qk_norm_desc* desc, const void* dq, co
  * ceil(cols / (4 block)) of them), row r and block b of a tile at
  * (r % 32) * 16 + (r / 32) * 4 + b; bytes past the last block of a row are
  * zero, those of rows past the last are not read.  Both 16-byte aligned.
+ * A scale has no sign: e4m3 bytes are 0x00 .. 0x7F, those with the top bit are
+ * not defined.
  */
 #define DGXM_FP4_NVFP4 0
 #define DGXM_FP4_MXFP4 1
