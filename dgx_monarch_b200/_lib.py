@@ -234,6 +234,41 @@ class Fp4GemmDesc(ctypes.Structure):
     ]
 
 
+BLOCK_NORM_NONE, BLOCK_NORM_LAYER, BLOCK_NORM_RMS = 0, 1, 2
+MOD_NONE, MOD_SHARED, MOD_SAMPLE, MOD_TOKEN = 0, 1, 2, 3
+
+
+class BlockNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("seq", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("mod_dtype", ctypes.c_int32),
+        ("norm_mode", ctypes.c_int32),
+        ("branch_norm", ctypes.c_int32),
+        ("gate_form", ctypes.c_int32),
+        ("mod_form", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64 * 2),
+        ("branch_stride", ctypes.c_int64 * 2),
+        ("x_out_stride", ctypes.c_int64 * 2),
+        ("out_stride", ctypes.c_int64 * 2),
+        ("gate_stride", ctypes.c_int64 * 2),
+        ("scale_stride", ctypes.c_int64 * 2),
+        ("shift_stride", ctypes.c_int64 * 2),
+        ("dy_stride", ctypes.c_int64 * 2),
+        ("dx_out_stride", ctypes.c_int64 * 2),
+    ]
+
+
+class BlockNormGradPointers(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p)
+                for name in ("x", "branch", "gate", "scale", "shift", "norm_w", "norm_b", "branch_w")]
+
+
 # Every symbol include/dgxm_sp.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -308,6 +343,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dgxm_quantize_fp4_workspace": (ctypes.c_int64, []),
     "dgxm_quantize_fp4": (ctypes.c_int, [ctypes.POINTER(Fp4Desc), _P, _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
     "dgxm_dequantize_fp4": (ctypes.c_int, [ctypes.POINTER(Fp4Desc), _P, _P, _P, _P, _P]),
+    "dgxm_block_norm": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "dgxm_block_norm_backward_workspace": (ctypes.c_int64, [ctypes.POINTER(BlockNormDesc)]),
+    "dgxm_block_norm_backward": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), ctypes.POINTER(BlockNormGradPointers),
+                                                _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
     "dgxm_fp4_matmul": (ctypes.c_int, [ctypes.POINTER(Fp4GemmDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 

@@ -19,3 +19,4 @@
 #include "qk_norm.cu"
 #include "fp4_quant.cu"
 #include "fp4_gemm.cu"
+#include "block_norm.cu"

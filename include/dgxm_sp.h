@@ -750,6 +750,83 @@ int dgxm_fp4_matmul(const dgxm_fp4_gemm_desc* desc, const void* a_values, const 
                     const float* a_scale, const void* b_values, const void* b_scales,
                     const float* b_scale, const void* bias, void* out, void* stream);
 
+/* ------------------------------------------------------------ between two branches of a block */
+/*
+ * The residual addition of a branch and the next norm with its modulation, in
+ * one pass over (batch, seq, width) tensors of dtype, any strides (elements:
+ * batch, row) with contiguous values, width up to 8192:
+ *   m = branch, or with branch_norm branch / sqrt(mean(branch^2) + eps) * branch_w
+ *   r = x + gate * m                                    -> x_out, with a branch
+ *   n = (r - mean(r)) / sqrt(var(r) + eps)              LAYER
+ *       r / sqrt(mean(r^2) + eps)                       RMS
+ *   y = (n * norm_w + norm_b) * (1 + scale) + shift     -> out, not under NONE
+ * norm_w, norm_b (LAYER only) and branch_w are width values of weight_dtype
+ * (dtype or F32), or NULL.  gate, scale and shift are of mod_dtype (dtype or
+ * F32), or NULL, and hold width values for all rows (SHARED), each sample
+ * (SAMPLE; stride [0]) or each token (TOKEN; both strides): gate by gate_form,
+ * scale and shift by mod_form.  fp32 inside, each output rounded once; the
+ * norm is of the sum before its rounding.  x_out and out may each be x or
+ * branch (same strides), not both the same.
+ *
+ * Serves the modulation, gate and residual of the blocks around the attention
+ * seam (inside the forwards of adapters/flux_family.py:108-265,
+ * adapters/krea2.py:130-246 and adapters/wan_family.py:64-162).
+ */
+#define DGXM_BLOCK_NORM_NONE 0
+#define DGXM_BLOCK_NORM_LAYER 1
+#define DGXM_BLOCK_NORM_RMS 2
+
+#define DGXM_MOD_NONE 0
+#define DGXM_MOD_SHARED 1
+#define DGXM_MOD_SAMPLE 2
+#define DGXM_MOD_TOKEN 3
+
+typedef struct dgxm_block_norm_desc {
+  int32_t batch, seq, width;
+  int32_t dtype;                 /* of the tensors: BF16, F16 or F32 */
+  int32_t weight_dtype;
+  int32_t mod_dtype;
+  int32_t norm_mode;
+  int32_t branch_norm;           /* 1: RMSNorm of the branch */
+  int32_t gate_form, mod_form;
+  float eps;
+  int32_t reserved;              /* 0 */
+  int64_t x_stride[2];           /* backward: of x_out, the sum */
+  int64_t branch_stride[2];
+  int64_t x_out_stride[2];       /* backward: of the gradient of x */
+  int64_t out_stride[2];         /* backward: of the gradient of branch */
+  int64_t gate_stride[2], scale_stride[2], shift_stride[2];
+  int64_t dy_stride[2], dx_out_stride[2];  /* backward: of the upstream gradients */
+} dgxm_block_norm_desc;
+
+int dgxm_block_norm(const dgxm_block_norm_desc* desc, const void* x, const void* branch,
+                    const void* gate, const void* scale, const void* shift, const void* norm_w,
+                    const void* norm_b, const void* branch_w, void* x_out, void* out, void* stream);
+
+/*
+ * Its gradients; NULL ones are not computed.  Those of gate, scale and shift
+ * are contiguous (width), (batch, width) or (batch, seq, width) of mod_dtype
+ * by form, those of the weights width values of weight_dtype, each summed
+ * over its rows in fp32 in a fixed order.  Without a gate and a branch norm
+ * the branch's gradient is that of x: branch must be NULL in both.
+ */
+typedef struct dgxm_block_norm_grads {
+  void *x, *branch, *gate, *scale, *shift, *norm_w, *norm_b, *branch_w;
+} dgxm_block_norm_grads;
+
+/*
+ * From the upstream gradients dy of y (not under NONE) and dx_out of x_out
+ * (or NULL: none), and the forward's x_out (without a branch: its x).
+ * `workspace` holds dgxm_block_norm_backward_workspace(desc) bytes (-1: a bad
+ * descriptor) where a gradient is summed over rows.
+ */
+int64_t dgxm_block_norm_backward_workspace(const dgxm_block_norm_desc* desc);
+int dgxm_block_norm_backward(const dgxm_block_norm_desc* desc, const dgxm_block_norm_grads* grads,
+                             const void* dy, const void* dx_out, const void* x_out,
+                             const void* branch, const void* gate, const void* scale,
+                             const void* norm_w, const void* norm_b, const void* branch_w,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
