@@ -18,7 +18,7 @@ LIB_PATH = PKG_DIR / LIB_NAME
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
+    "--split-compile=0", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
 ]
 
 

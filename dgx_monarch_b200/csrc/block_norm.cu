@@ -14,12 +14,21 @@
 //   dx = R,  dg = sum R m,  dm = R g,  dw2 = sum dm n2,
 //   dbranch = dm, or k2 (dm w2 - n2 mean(dm w2 n2)).
 //
-// Every value is moved once and takes a few operations, so DRAM bounds both.
-// A block holds a row, a thread the same columns of every row it sees: the
-// modulation of a sample and the weights stay in its registers, and so do the
-// sums over rows, which a second kernel adds in the order of the blocks.
-// Means and variances are fp32 and the variance is that of the deviations, a
-// second sum over the row; every output is rounded once.
+// Every value is moved once and takes a few operations, so DRAM bounds both as
+// long as no warp waits for another's sums.  So the warps of a block share the
+// work out by kind, a ring of rows in shared memory between them:
+//   one fetches, a bulk copy a row and tensor, so that rows under way cost
+//     neither registers nor instructions of the others;
+//   three to eight take the rows' statistics, a row each at a time;
+//   the rest make the outputs.  A thread of theirs holds the same columns of
+//     every row, so the modulation of a sample and the weights stay in its
+//     registers, and so do the sums over rows, which a second kernel adds in
+//     the order of the blocks.
+// Means and variances are fp32, gathered a chunk at a time from deviations
+// (never as a difference of squares); every output is rounded once.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.h"
 #include "ptx.cuh"
 
@@ -27,6 +36,7 @@ namespace dgxm {
 
 constexpr int kBnMaxWidth = 8192;  // six fp32 rows fit the shared memory of a block
 constexpr int kBnMaxIn = 6;
+constexpr int kBnMaxSlots = 16;
 // Streams of rows that a block reads: forward (x, branch, gate, scale, shift),
 // backward (dy, dr, r, branch, gate, scale); the modulations where each token
 // has its own.
@@ -36,10 +46,10 @@ enum { kBnDy = 0, kBnDr = 1, kBnR = 2, kBnBranchB = 3, kBnGateB = 4, kBnScaleB =
 struct BlockNormParams {
   const char* in[kBnMaxIn];  // streams, NULL: absent
   int64_t in_sb[kBnMaxIn], in_sr[kBnMaxIn];  // bytes between samples, rows
-  int in_f32[kBnMaxIn];      // a modulation of fp32 beside 16-bit tensors
+  int in_elt[kBnMaxIn];      // bytes of a value: 4 for a modulation of fp32 beside 16-bit tensors
   int in_off[kBnMaxIn];      // bytes into the stage
   int in_pitch[kBnMaxIn];    // bytes of a row in the stage, a multiple of 16
-  int n_in, stage_bytes;
+  int n_in, slot_bytes, slots, param_bytes;  // the ring, behind the statistics' copy of a column vector
   // Values of a column that serve every row of a sample (gate, scale, shift), or all rows; NULL: absent
   const char *gate, *scale, *shift, *norm_w, *norm_b, *branch_w;
   int64_t gate_sb, scale_sb, shift_sb;  // bytes between samples
@@ -49,31 +59,73 @@ struct BlockNormParams {
   char *g_gate, *g_scale, *g_shift;  // backward, a row each token: contiguous
   float* partial;            // backward: (block + sample, 3, width)
   int want;                  // which of the three sums are wanted, a bit each
-  int batch, seq, width, mode, branch_norm, gated;
-  int64_t rows;
+  int batch, seq, width, mode, branch_norm;
+  int64_t rows, rows_each;
+  int rows_more;
   float eps, inv_width;
 };
 
+// A thread works on pairs of fp32 (sm_100 f32x2 arithmetic); a chunk, the 16
+// bytes of the tensors' type that it takes at a time, is kPairs of them.
 template <typename T>
-struct __align__(16) BnChunk {
-  static constexpr int kN = 16 / static_cast<int>(sizeof(T));
-  T v[kN];
-};
+constexpr int kBnChunk = 16 / static_cast<int>(sizeof(T));
 
-// CH values from 16 bytes of T, or from fp32 (a modulation of fp32 beside 16-bit tensors).
-template <typename T, int CH>
-__device__ __forceinline__ void bn_read(const uint8_t* row, int chunk, int f32, float (&v)[CH]) {
-  if (sizeof(T) == 4 || f32) {
-    const float4* p = reinterpret_cast<const float4*>(row + static_cast<int64_t>(chunk) * CH * 4);
+template <typename T>
+__device__ __forceinline__ uint64_t bn_widen2(uint32_t w);
+template <>
+__device__ __forceinline__ uint64_t bn_widen2<__nv_bfloat16>(uint32_t w) {
+  return pk2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ uint64_t bn_widen2<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pk2(f.x, f.y);
+}
+
+__device__ __forceinline__ uint64_t bn_both(float v) { return pk2(v, v); }
+
+__device__ __forceinline__ float bn_total(uint64_t v) {
+  float lo, hi;
+  upk2(v, lo, hi);
+  return lo + hi;
+}
+
+// 16 bytes global -> this CTA's shared memory and on, `bytes` a multiple of
+// 16, both ends aligned; completion counted on `bar`.
+__device__ __forceinline__ void bn_bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// N pairs of chunk q (2 N values of T) of a staged row.  Rows off 16 bytes
+// (!VEC) lie in the stage as they do in memory: `off` bytes behind a 16-byte
+// border; values past the row's end read as zeros.
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void bn_read(const uint8_t* row, int off, int q, int width, uint64_t (&v)[N]) {
+  constexpr int kWords = 2 * N / kBnChunk<T>;
+  const uint4* p = reinterpret_cast<const uint4*>(row) + q * kWords;
 #pragma unroll
-    for (int i = 0; i < CH / 4; ++i) {
-      const float4 a = p[i];
-      v[4 * i] = a.x, v[4 * i + 1] = a.y, v[4 * i + 2] = a.z, v[4 * i + 3] = a.w;
+  for (int k = 0; k < kWords; ++k) {
+    uint4 w = p[k];
+    if (!VEC && off) w = fp4_bytes_from(w, p[k + 1], off);
+    if constexpr (sizeof(T) == 4) {
+      v[2 * k] = pk2(__uint_as_float(w.x), __uint_as_float(w.y));
+      v[2 * k + 1] = pk2(__uint_as_float(w.z), __uint_as_float(w.w));
+    } else {
+      v[4 * k] = bn_widen2<T>(w.x);
+      v[4 * k + 1] = bn_widen2<T>(w.y);
+      v[4 * k + 2] = bn_widen2<T>(w.z);
+      v[4 * k + 3] = bn_widen2<T>(w.w);
     }
-  } else {
-    const BnChunk<T> c = *reinterpret_cast<const BnChunk<T>*>(row + chunk * 16);
+  }
+  if (!VEC && (q + 1) * 2 * N > width) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) v[i] = qk_widen(c.v[i]);
+    for (int i = 0; i < N; ++i) {
+      float lo, hi;
+      upk2(v[i], lo, hi);
+      v[i] = pk2(q * 2 * N + 2 * i < width ? lo : 0.f, q * 2 * N + 2 * i + 1 < width ? hi : 0.f);
+    }
   }
 }
 
@@ -83,175 +135,668 @@ __device__ __forceinline__ float bn_value(const char* base, int f32, int col) {
   return f32 ? reinterpret_cast<const float*>(base)[col] : qk_widen(reinterpret_cast<const T*>(base)[col]);
 }
 
-template <typename T, int CH>
-__device__ __forceinline__ void bn_vector(const char* base, int f32, int col, int width, float fill, float (&v)[CH]) {
+// 2 N values from column `col` on, `fill` without a vector or past its end, in
+// whole 16-byte words; value by value only at the ends of a vector off 16 bytes.
+template <typename V, int N>
+__device__ __forceinline__ void bn_vector_of(const char* base, int col, int width, float fill, uint64_t (&v)[N]) {
+  constexpr int kElt = static_cast<int>(sizeof(V)), kWords = 2 * N * kElt / 16 > 0 ? 2 * N * kElt / 16 : 1;
+  const char* at = base + static_cast<int64_t>(col) * kElt;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+  const bool whole = 2 * N * kElt % 16 == 0 && col + 2 * N <= width;
+  if (whole && (off == 0 || (col * kElt >= off && (col + 2 * N) * kElt + 16 - off <= width * kElt))) {
+    const uint4* p = reinterpret_cast<const uint4*>(at - off);
+    uint4 w[kWords + 1];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) v[i] = base != nullptr && col + i < width ? bn_value<T>(base, f32, col + i) : fill;
-}
-
-// Store CH values of a row from column `col` on.
-template <typename T, int CH>
-__device__ __forceinline__ void bn_store(char* row, int col, int width, const float (&v)[CH]) {
+    for (int k = 0; k < kWords; ++k) w[k] = __ldg(p + k);
+    if (off) {
+      w[kWords] = __ldg(p + kWords);
 #pragma unroll
-  for (int i = 0; i < CH; ++i)
-    if (col + i < width) reinterpret_cast<T*>(row)[col + i] = qk_narrow<T>(v[i]);
-}
-
-template <typename T, int CH>
-__device__ __forceinline__ void bn_store_mod(char* row, int f32, int col, int width, const float (&v)[CH]) {
-  if (f32) bn_store<float, CH>(row, col, width, v);
-  else bn_store<T, CH>(row, col, width, v);
-}
-
-// Sums over the block, the same in every thread.  `red` alternates between
-// two halves of N x 32 floats, so one barrier a sum is enough.
-template <int N>
-__device__ __forceinline__ void bn_block_sum(float (&v)[N], float* red, int& turn) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+      for (int k = 0; k < kWords; ++k) w[k] = fp4_bytes_from(w[k], w[k + 1], off);
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+      if constexpr (kElt == 4) {
+        v[2 * k] = pk2(__uint_as_float(u[0]), __uint_as_float(u[1]));
+        if (N > 1) v[2 * k + 1] = pk2(__uint_as_float(u[2]), __uint_as_float(u[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 && 4 * k + i < N; ++i) v[4 * k + i] = bn_widen2<V>(u[i]);
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i)
+    v[i] = pk2(col + 2 * i < width ? bn_value<V>(base, 0, col + 2 * i) : fill,
+               col + 2 * i + 1 < width ? bn_value<V>(base, 0, col + 2 * i + 1) : fill);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void bn_vector(const char* base, int f32, int col, int width, float fill, uint64_t (&v)[N]) {
+  if (base == nullptr) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  float* half = red + (turn ^= 1) * (4 * 32);
-  if (lane == 0)
+    for (int i = 0; i < N; ++i) v[i] = bn_both(fill);
+  } else if (f32) {
+    bn_vector_of<float>(base, col, width, fill, v);
+  } else {
+    bn_vector_of<T>(base, col, width, fill, v);
+  }
+}
+
+// Store N pairs of a row from column `col` on.  Off 16 bytes (!VEC) and with
+// neighbouring chunks in neighbouring lanes (NEXT), a lane stores the aligned
+// word that its chunk shares with the next lane's, and single values only
+// where there is none: at the ends of the warp's chunks and of the row.
+template <typename T, bool VEC, bool NEXT, int N>
+__device__ __forceinline__ void bn_store(char* row, int col, int width, const uint64_t (&v)[N]) {
+  float f[2 * N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) half[i * 32 + (threadIdx.x >> 5)] = v[i];
+  for (int i = 0; i < N; ++i) upk2(v[i], f[2 * i], f[2 * i + 1]);
+  constexpr int CH = kBnChunk<T>;
+  if constexpr (!VEC && !(NEXT && 2 * N == CH)) {
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i)
+      if (col + i < width) reinterpret_cast<T*>(row)[col + i] = qk_narrow<T>(f[i]);
+  } else if constexpr (sizeof(T) == 4 && VEC) {
+#pragma unroll
+    for (int i = 0; i < 2 * N; i += 4)
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(row) + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  } else {
+    uint4 w;
+    if constexpr (sizeof(T) == 4) {
+      w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    } else {
+      constexpr bool kHalf = std::is_same<T, __half>::value;
+      static_assert(2 * N == CH, "one chunk");
+      w = make_uint4(pack16<kHalf>(f[0], f[1]), pack16<kHalf>(f[2], f[3]), pack16<kHalf>(f[4], f[5]), pack16<kHalf>(f[6], f[7]));
+    }
+    T* to = reinterpret_cast<T*>(row) + col;
+    const uint32_t off = VEC ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) & 15u;
+    if (VEC || (off == 0 && col + CH <= width)) {
+      *reinterpret_cast<uint4*>(to) = w;
+      if (VEC) return;
+    }
+    // The lanes with a chunk of the row are the first ones of the warp.
+    const int lane = threadIdx.x & 31, lanes = min(32, (width - (col - lane * CH) + CH - 1) / CH);
+    const uint32_t mask = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u;
+    const uint4 n = make_uint4(__shfl_down_sync(mask, w.x, 1), __shfl_down_sync(mask, w.y, 1),
+                               __shfl_down_sync(mask, w.z, 1), __shfl_down_sync(mask, w.w, 1));
+    if (off == 0 && col + CH <= width) return;
+    const int head = off == 0 ? CH : static_cast<int>((16u - off) / sizeof(T));  // values before the aligned word
+    const bool before = off != 0 && lane > 0 && col + head <= width;  // they are the lane before's
+    const bool shared = off != 0 && lane < 31 && col + CH + head <= width;
+    if (shared) *reinterpret_cast<uint4*>(to + head) = fp4_bytes_from(w, n, 16u - off);
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      if (col + i < width && (i < head ? !before : !shared)) to[i] = qk_narrow<T>(f[i]);
+  }
+}
+
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void bn_store_mod(char* base, int64_t row, int f32, int col, int width, const uint64_t (&v)[N]) {
+  if (f32) bn_store<float, VEC, false>(base + row * width * 4, col, width, v);
+  else bn_store<T, VEC, true>(base + row * width * static_cast<int>(sizeof(T)), col, width, v);
+}
+
+// A block's rows: contiguous, one after the other.
+struct BnWalk {
+  int64_t row, last;
+  int b, l, seq;
+  int slot = 0, parity = 0, slots;
+  __device__ __forceinline__ BnWalk(const BlockNormParams& p) : seq(p.seq), slots(p.slots) {
+    // the first `rows_more` blocks have a row more than the others
+    const int more = min(static_cast<int>(blockIdx.x), p.rows_more);
+    row = static_cast<int64_t>(blockIdx.x) * p.rows_each + more;
+    last = row + p.rows_each + (static_cast<int>(blockIdx.x) < p.rows_more);
+    b = static_cast<int>(last <= 0xffffffffLL ? static_cast<uint32_t>(row) / static_cast<uint32_t>(seq) : row / seq);
+    l = static_cast<int>(row - static_cast<int64_t>(b) * seq);
+  }
+  __device__ __forceinline__ bool more() const { return row < last; }
+  __device__ __forceinline__ void next() {
+    ++row;
+    if (++l == seq) {
+      l = 0;
+      ++b;
+    }
+    if (++slot == slots) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// A row's statistics.  n = (r - mean) root.
+struct __align__(16) BnStats {
+  float mean, root, root2, m1, m2, m3, spare[2];
+};
+
+struct BnShared {
+  uint64_t full[kBnMaxSlots], ready[kBnMaxSlots], empty[kBnMaxSlots];
+  BnStats stats[kBnMaxSlots];
+};
+
+// Every wait is bounded; after one that ran out, a warp waits no more.
+__device__ __forceinline__ void bn_wait(uint64_t* bar, int parity, bool& dead) {
+  if (!dead) dead = !mbar_wait(smem_u32(bar), parity, nullptr);
+}
+
+__device__ __forceinline__ void bn_start(const BlockNormParams& p, BnShared& sh, int out_warps) {
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.slots; ++s) {
+      mbar_init(smem_u32(&sh.full[s]), 1);
+      mbar_init(smem_u32(&sh.ready[s]), 1);
+      mbar_init(smem_u32(&sh.empty[s]), out_warps);
+    }
+    mbar_fence_init();
+  }
   __syncthreads();
+  pdl_launch_dependents();
+  pdl_wait();
+}
+
+// The fetching warp: lane i takes stream i.
+template <bool VEC>
+__device__ __forceinline__ void bn_fetch(const BlockNormParams& p, uint8_t* ring, BnShared& sh) {
+  const int lane = threadIdx.x & 31;
+  const bool mine = lane < p.n_in && p.in[lane < kBnMaxIn ? lane : 0] != nullptr;
+  bool dead = false;
+  for (BnWalk w(p); w.more(); w.next()) {
+    bn_wait(&sh.empty[w.slot], w.parity ^ 1, dead);
+    const uint32_t full = smem_u32(&sh.full[w.slot]);
+    uint8_t* to = ring + w.slot * p.slot_bytes;
+    const char* from = nullptr;
+    uint32_t bytes = 0;
+    if (mine) {
+      to += p.in_off[lane];
+      from = p.in[lane] + w.b * p.in_sb[lane] + w.l * p.in_sr[lane];
+      bytes = p.width * p.in_elt[lane];
+    }
+    if constexpr (!VEC) {
+      // Whole 16-byte words by the bulk copy; the ends value by value, lanes 0 .. 7
+      // the first and 8 .. 15 the last of the first half of the streams, the others the second's.
+      constexpr int kHalf = kBnMaxIn / 2;
+      const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) & 15u;
+      const uint32_t head = min((16u - off) & 15u, bytes), tail = (bytes - head) & 15u;
+      uint16_t end[kHalf];
+      uint32_t at[kHalf];
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) {
+        const int s = i + (lane >= 16 ? kHalf : 0);
+        const uint64_t f = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), s);
+        const uint32_t n = __shfl_sync(0xffffffffu, bytes, s), h = __shfl_sync(0xffffffffu, head, s);
+        const uint32_t e = __shfl_sync(0xffffffffu, tail, s), unit = 2 * (lane & 7);
+        at[i] = (lane & 8) == 0 ? (unit < h ? unit : ~0u) : (unit < e ? n - e + unit : ~0u);
+        if (at[i] != ~0u) end[i] = *reinterpret_cast<const uint16_t*>(f + at[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) {
+        const int s = i + (lane >= 16 ? kHalf : 0);
+        const uint32_t dst = __shfl_sync(0xffffffffu, smem_u32(to) + off, s);
+        if (at[i] != ~0u) asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + at[i]), "h"(end[i]) : "memory");
+      }
+      to += off + head;
+      from += head;
+      bytes -= head + tail;
+    }
+    const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
+    __syncwarp();  // the ends' stores come before lane 0's arrival
+    if (lane == 0) {
+      if (sum > 0) mbar_expect_tx(full, sum);
+      else mbar_arrive(full);
+    }
+    __syncwarp();
+    if (bytes > 0) bn_bulk_load(smem_u32(to), from, bytes, full);
+  }
+  if (dead) report_device_error(kErrProducerTimeout);
+}
+
+// Bytes that a row of stream s lies behind a 16-byte border.
+template <bool VEC>
+__device__ __forceinline__ int bn_offset(const BlockNormParams& p, int s, const BnWalk& w) {
+  if (VEC) return 0;
+  return static_cast<int>(reinterpret_cast<uintptr_t>(p.in[s] + w.b * p.in_sb[s] + w.l * p.in_sr[s]) & 15);
+}
+
+// Chunk q of stream s of the row in `slot`: the tensors, and the modulations of each token.
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void bn_get(const BlockNormParams& p, const uint8_t* slot, int s, const BnWalk& w, int q,
+                                       uint64_t (&v)[N]) {
+  bn_read<T, VEC>(slot + p.in_off[s], bn_offset<VEC>(p, s, w), q, p.width, v);
+}
+
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void bn_get_mod(const BlockNormParams& p, const uint8_t* slot, int s, const BnWalk& w, int q,
+                                           uint64_t (&v)[N]) {
+  if (p.mod_f32) bn_get<float, VEC>(p, slot, s, w, q, v);
+  else bn_get<T, VEC>(p, slot, s, w, q, v);
+}
+
+// ------------------------------------------------------------ the statistics' warps
+// A row is one warp's: its sums are shuffles, and several rows' latencies overlap.
+template <int N>
+__device__ __forceinline__ void bn_warp_sum(float (&v)[N]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+}
+
+// Count, mean and sum of squared deviations of a set, and of two sets
+// together: every term of the sum is positive, so nothing cancels.
+struct BnMoments {
+  float n = 0.f, mean = 0.f, m2 = 0.f;
+  __device__ __forceinline__ void add(float on, float omean, float om2) {
+    const float all = n + on, share = all > 0.f ? __fdividef(on, all) : 0.f, delta = omean - mean;
+    mean = fmaf(delta, share, mean);
+    m2 += fmaf(delta * delta, n * share, om2);
+    n = all;
+  }
+};
+
+// The moments of a chunk's first `count` values (the rest are zeros).
+template <int N>
+__device__ __forceinline__ void bn_add_chunk(BnMoments& all, uint64_t (&v)[N], int count) {
+  uint64_t s = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) s = fadd2(s, v[i]);
+  const float mean = bn_total(s) * (count == 2 * N ? 1.f / (2 * N) : 1.f / count);
+  uint64_t ss = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    v[i] = lane < warps ? half[i * 32 + lane] : 0.f;
+    uint64_t d = fadd2(v[i], bn_both(-mean));
+    if (count < 2 * N) {
+      float lo, hi;
+      upk2(d, lo, hi);
+      d = pk2(2 * i < count ? lo : 0.f, 2 * i + 1 < count ? hi : 0.f);
+    }
+    ss = ffma2(d, d, ss);
+  }
+  all.add(static_cast<float>(count), mean, bn_total(ss));
+}
+
+// Mean and mean squared deviation over the warp.
+__device__ __forceinline__ float2 bn_warp_moments(BnMoments v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  for (int o = 16; o > 0; o >>= 1) {
+    const float n = __shfl_down_sync(0xffffffffu, v.n, o), mean = __shfl_down_sync(0xffffffffu, v.mean, o);
+    const float m2 = __shfl_down_sync(0xffffffffu, v.m2, o);
+    v.add(n, mean, m2);
+  }
+  return make_float2(__shfl_sync(0xffffffffu, v.mean, 0), __shfl_sync(0xffffffffu, __fdividef(v.m2, v.n), 0));
+}
+
+// The statistics' copy of a column vector of the row's sample: loaded when the
+// sample changes, which every one of their warps sees at the same row.
+template <int WARPS, typename Make>
+__device__ __forceinline__ void bn_param(const BlockNormParams& p, float* param, int t, Make&& make) {
+  if (p.param_bytes == 0) return;
+  named_barrier_sync(1, WARPS * 32);
+#pragma unroll 8
+  for (int c = t; c < p.param_bytes / 4; c += WARPS * 32) param[c] = c < p.width ? make(c) : 0.f;
+  named_barrier_sync(1, WARPS * 32);
+}
+
+template <int N>
+__device__ __forceinline__ void bn_param_get(const float* param, int q, uint64_t (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float4 f = *reinterpret_cast<const float4*>(param + q * 2 * N + 2 * i);
+    v[i] = pk2(f.x, f.y);
+    v[i + 1] = pk2(f.z, f.w);
   }
 }
 
-// Copy one row of every stream into the stage, value by value, and zeros up
-// to whole chunks.
-template <typename T>
-__device__ __forceinline__ void bn_fill(const BlockNormParams& p, uint8_t* stage, int64_t b, int64_t l) {
-  for (int s = 0; s < p.n_in; ++s) {
-    if (p.in[s] == nullptr) continue;
-    const char* from = p.in[s] + b * p.in_sb[s] + l * p.in_sr[s];
-    uint8_t* to = stage + p.in_off[s];
-    if (p.in_f32[s] || sizeof(T) == 4) {
-      for (int c = threadIdx.x; c < p.in_pitch[s] / 4; c += blockDim.x)
-        reinterpret_cast<float*>(to)[c] = c < p.width ? reinterpret_cast<const float*>(from)[c] : 0.f;
-    } else {
-      for (int c = threadIdx.x; c < p.in_pitch[s] / 2; c += blockDim.x)
-        reinterpret_cast<uint16_t*>(to)[c] = c < p.width ? reinterpret_cast<const uint16_t*>(from)[c] : uint16_t(0);
+template <typename T, bool VEC, bool FULL, int STAT>
+__device__ __forceinline__ void bn_forward_stats(const BlockNormParams& p, float* param, const uint8_t* ring, BnShared& sh,
+                                                 int t) {
+  constexpr int CH = kBnChunk<T>, N = CH / 2;
+  const int lane = t & 31;
+  // Rows in turn, by no more warps than there are slots: none waits for a phase
+  // of a slot whose last one is still open.
+  const int warps = min(STAT, p.slots);
+  int turn = t >> 5 < warps ? t >> 5 : 0x7fffffff;  // rows until this warp's next
+  const bool branch = p.in[kBnBranch] != nullptr, layer = p.mode == DGXM_BLOCK_NORM_LAYER;
+  const bool norm = p.mode != DGXM_BLOCK_NORM_NONE, tok = FULL && p.in[kBnGate] != nullptr;
+  int sample = -1;
+  bool dead = false;
+  for (BnWalk w(p); w.more(); w.next()) {
+    if (w.b != sample) {
+      sample = w.b;
+      bn_param<STAT>(p, param, t, [&](int c) { return bn_value<T>(p.gate + sample * p.gate_sb, p.mod_f32, c); });
     }
-  }
-}
-
-// Thread t holds chunks t, t + blockDim, ... of each row, NV of them.
-template <typename T, int NV>
-__global__ void __launch_bounds__(1024) block_norm_kernel(const __grid_constant__ BlockNormParams p) {
-  constexpr int CH = BnChunk<T>::kN;
-  extern __shared__ __align__(16) uint8_t stage[];
-  __shared__ float red[2 * 4 * 32];
-  const int64_t first = blockIdx.x * p.rows / gridDim.x, last = (blockIdx.x + 1) * p.rows / gridDim.x;
-  float g[NV][CH], a[NV][CH], c[NV][CH];
-  int64_t sample = -1;
-  int turn = 0;
-  for (int64_t row = first; row < last; ++row) {
-    const int64_t b = row / p.seq, l = row - b * p.seq;
-    if (b != sample) {
-      sample = b;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int col = (threadIdx.x + k * blockDim.x) * CH;
-        float w[CH], bias[CH], t[CH];
-        bn_vector<T, CH>(p.gate ? p.gate + b * p.gate_sb : nullptr, p.mod_f32, col, p.width, 1.f, g[k]);
-        bn_vector<T, CH>(p.scale ? p.scale + b * p.scale_sb : nullptr, p.mod_f32, col, p.width, 0.f, a[k]);
-        bn_vector<T, CH>(p.shift ? p.shift + b * p.shift_sb : nullptr, p.mod_f32, col, p.width, 0.f, t);
-        bn_vector<T, CH>(p.norm_w, p.w_f32, col, p.width, 1.f, w);
-        bn_vector<T, CH>(p.norm_b, p.w_f32, col, p.width, 0.f, bias);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {  // y = n a + c
-          a[k][i] += 1.f;
-          c[k][i] = fmaf(bias[i], a[k][i], t[i]);
-          a[k][i] *= w[i];
-        }
-      }
-    }
-    __syncthreads();
-    bn_fill<T>(p, stage, b, l);
-    __syncthreads();
+    if (turn-- > 0) continue;
+    turn = warps - 1;
+    bn_wait(&sh.full[w.slot], w.parity, dead);
+    const uint8_t* slot = ring + w.slot * p.slot_bytes;
     float root2 = 1.f;
-    if (p.branch_norm) {
-      float ss[1] = {0.f};
+    if (FULL && p.branch_norm) {
+      uint64_t ss = 0;
+#pragma unroll 2
+    for (int q = lane; q * CH < p.width; q += 32) {
+        uint64_t m[N];
+        bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = threadIdx.x + k * blockDim.x;
-        if (q * CH >= p.width) continue;
-        float m[CH];
-        bn_read<T, CH>(stage + p.in_off[kBnBranch], q, 0, m);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) ss[0] = fmaf(m[i], m[i], ss[0]);
+        for (int i = 0; i < N; ++i) ss = ffma2(m[i], m[i], ss);
       }
-      bn_block_sum<1>(ss, red, turn);
-      root2 = rsqrtf(fmaf(ss[0], p.inv_width, p.eps));
+      float sum[1] = {bn_total(ss)};
+      bn_warp_sum(sum);
+      root2 = rsqrtf(fmaf(sum[0], p.inv_width, p.eps));
     }
-    float r[NV][CH], sum[1] = {0.f};
+    BnMoments moments;
+    uint64_t ss = 0;
+#pragma unroll 2
+    for (int q = lane; norm && q * CH < p.width; q += 32) {
+      uint64_t r[N];
+      bn_get<T, VEC>(p, slot, kBnX, w, q, r);
+      if (branch) {
+        uint64_t m[N], g[N];
+        bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
+        if (FULL && p.branch_norm) {
+          bn_vector<T>(p.branch_w, p.w_f32, q * CH, p.width, 1.f, g);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * blockDim.x, col = q * CH;
-      if (col >= p.width) continue;
-      bn_read<T, CH>(stage + p.in_off[kBnX], q, 0, r[k]);
-      if (p.in[kBnBranch] != nullptr) {
-        float m[CH];
-        bn_read<T, CH>(stage + p.in_off[kBnBranch], q, 0, m);
-        if (p.branch_norm) {
-          float w2[CH];
-          bn_vector<T, CH>(p.branch_w, p.w_f32, col, p.width, 1.f, w2);
-#pragma unroll
-          for (int i = 0; i < CH; ++i) m[i] *= root2 * w2[i];
+          for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], fmul2(bn_both(root2), g[i]));
         }
-        if (p.in[kBnGate] != nullptr) bn_read<T, CH>(stage + p.in_off[kBnGate], q, p.in_f32[kBnGate], g[k]);
+        if (tok) bn_get_mod<T, VEC>(p, slot, kBnGate, w, q, g);
+        else if (p.param_bytes > 0) bn_param_get(param, q, g);
+        else bn_vector<T>(p.gate ? p.gate + sample * p.gate_sb : nullptr, p.mod_f32, q * CH, p.width, 1.f, g);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) r[k][i] = fmaf(g[k][i], m[i], r[k][i]);
-        bn_store<T, CH>(p.x_out + b * p.x_out_sb + l * p.x_out_sr, col, p.width, r[k]);
+        for (int i = 0; i < N; ++i) r[i] = ffma2(g[i], m[i], r[i]);
       }
+      if (layer) {
+        bn_add_chunk(moments, r, VEC ? CH : min(CH, p.width - q * CH));
+      } else {
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (col + i < p.width) sum[0] += p.mode == DGXM_BLOCK_NORM_LAYER ? r[k][i] : r[k][i] * r[k][i];
+        for (int i = 0; i < N; ++i) ss = ffma2(r[i], r[i], ss);
+      }
     }
-    if (p.mode == DGXM_BLOCK_NORM_NONE) continue;
-    bn_block_sum<1>(sum, red, turn);
-    float mean = 0.f;
-    if (p.mode == DGXM_BLOCK_NORM_LAYER) {
-      mean = sum[0] * p.inv_width;
-      sum[0] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if ((threadIdx.x + k * blockDim.x) * CH + i < p.width) sum[0] = fmaf(r[k][i] - mean, r[k][i] - mean, sum[0]);
-      bn_block_sum<1>(sum, red, turn);
+    float mean = 0.f, square = 0.f;
+    if (layer) {
+      const float2 v = bn_warp_moments(moments);
+      mean = v.x;
+      square = v.y;
+    } else if (norm) {
+      float sum[1] = {bn_total(ss)};
+      bn_warp_sum(sum);
+      square = sum[0] * p.inv_width;
     }
-    const float root = rsqrtf(fmaf(sum[0], p.inv_width, p.eps));
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * blockDim.x, col = q * CH;
-      if (col >= p.width) continue;
-      float y[CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) y[i] = fmaf((r[k][i] - mean) * root, a[k][i], c[k][i]);
-      if (p.in[kBnScale] != nullptr) {
-        float s[CH];
-        bn_read<T, CH>(stage + p.in_off[kBnScale], q, p.in_f32[kBnScale], s);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) y[i] = fmaf(y[i], s[i], y[i]);
-      }
-      if (p.in[kBnShift] != nullptr) {
-        float t[CH];
-        bn_read<T, CH>(stage + p.in_off[kBnShift], q, p.in_f32[kBnShift], t);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) y[i] += t[i];
-      }
-      bn_store<T, CH>(p.out + b * p.out_sb + l * p.out_sr, col, p.width, y);
+    if (lane == 0) {
+      sh.stats[w.slot].mean = mean;
+      sh.stats[w.slot].root = rsqrtf(square + p.eps);
+      sh.stats[w.slot].root2 = root2;
+      mbar_arrive(smem_u32(&sh.ready[w.slot]));
     }
   }
+  if (dead) report_device_error(kErrSoftmaxTimeout);
+}
+
+// ------------------------------------------------------------ the kernels
+// The warps that make the outputs hold E values a thread, chunks of 16 bytes
+// t, t + threads, ... of each row.  FULL: with a branch norm, or modulations
+// of each token.
+template <typename T, int E, bool VEC, bool FULL, int MAXT, int STAT, int PER_SM>
+__global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kernel(const __grid_constant__ BlockNormParams p) {
+  constexpr int CH = kBnChunk<T>, NV = E / CH, N = CH / 2;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ BnShared sh;
+  const int threads = blockDim.x - 32 * STAT - 32, t = threadIdx.x;
+  uint8_t* ring = smem + p.param_bytes;
+  bn_start(p, sh, threads >> 5);
+  if (t >= threads + 32 * STAT) {
+    bn_fetch<VEC>(p, ring, sh);
+    return;
+  }
+  if (t >= threads) {
+    bn_forward_stats<T, VEC, FULL, STAT>(p, reinterpret_cast<float*>(smem), ring, sh, t - threads);
+    return;
+  }
+  const bool branch = p.in[kBnBranch] != nullptr, norm = p.mode != DGXM_BLOCK_NORM_NONE;
+  uint64_t g[NV][N], a[NV][N], c[NV][N];
+  int sample = -1;
+  bool dead = false;
+  for (BnWalk w(p); w.more(); w.next()) {
+    if (w.b != sample) {
+      sample = w.b;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int col = (t + k * threads) * CH;
+        uint64_t wt[N], bias[N];
+        bn_vector<T>(p.gate ? p.gate + sample * p.gate_sb : nullptr, p.mod_f32, col, p.width, 1.f, g[k]);
+        bn_vector<T>(p.scale ? p.scale + sample * p.scale_sb : nullptr, p.mod_f32, col, p.width, 0.f, a[k]);
+        bn_vector<T>(p.shift ? p.shift + sample * p.shift_sb : nullptr, p.mod_f32, col, p.width, 0.f, c[k]);
+        bn_vector<T>(p.norm_w, p.w_f32, col, p.width, 1.f, wt);
+        bn_vector<T>(p.norm_b, p.w_f32, col, p.width, 0.f, bias);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {  // y = n a + c
+          a[k][i] = fadd2(a[k][i], bn_both(1.f));
+          c[k][i] = ffma2(bias[i], a[k][i], c[k][i]);
+          a[k][i] = fmul2(a[k][i], wt[i]);
+        }
+      }
+    }
+    bn_wait(&sh.full[w.slot], w.parity, dead);
+    bn_wait(&sh.ready[w.slot], w.parity, dead);
+    const uint8_t* slot = ring + w.slot * p.slot_bytes;
+    const BnStats st = sh.stats[w.slot];
+    char* const to_r = p.x_out + w.b * p.x_out_sb + w.l * p.x_out_sr;
+    char* const to_y = p.out + w.b * p.out_sb + w.l * p.out_sr;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int q = t + k * threads, col = q * CH;
+      if (col >= p.width) continue;
+      uint64_t r[N];
+      bn_get<T, VEC>(p, slot, kBnX, w, q, r);
+      if (branch) {
+        uint64_t m[N];
+        bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
+        if constexpr (FULL) {
+          if (p.branch_norm) {
+            uint64_t w2[N];
+            bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, w2);
+#pragma unroll
+            for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], fmul2(bn_both(st.root2), w2[i]));
+          }
+          if (p.in[kBnGate] != nullptr) bn_get_mod<T, VEC>(p, slot, kBnGate, w, q, g[k]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = ffma2(g[k][i], m[i], r[i]);
+        bn_store<T, VEC, true>(to_r, col, p.width, r);
+      }
+      if (!norm) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        r[i] = ffma2(fmul2(fadd2(r[i], bn_both(-st.mean)), bn_both(st.root)), a[k][i], c[k][i]);
+      if constexpr (FULL) {
+        uint64_t s[N];
+        if (p.in[kBnScale] != nullptr) {
+          bn_get_mod<T, VEC>(p, slot, kBnScale, w, q, s);
+#pragma unroll
+          for (int i = 0; i < N; ++i) r[i] = ffma2(r[i], s[i], r[i]);
+        }
+        if (p.in[kBnShift] != nullptr) {
+          bn_get_mod<T, VEC>(p, slot, kBnShift, w, q, s);
+#pragma unroll
+          for (int i = 0; i < N; ++i) r[i] = fadd2(r[i], s[i]);
+        }
+      }
+      bn_store<T, VEC, true>(to_y, col, p.width, r);
+    }
+    __syncwarp();
+    if ((t & 31) == 0) mbar_arrive(smem_u32(&sh.empty[w.slot]));
+  }
+  if (dead) report_device_error(kErrEpilogueTimeout);
+}
+
+// The gradient's row of one chunk: e = dy, under a scale of each token dh, and n.
+template <typename T, bool VEC, bool FULL, int N>
+__device__ __forceinline__ void bn_normed(const BlockNormParams& p, const uint8_t* slot, const BnWalk& w, const BnStats& st,
+                                          int q, uint64_t (&e)[N], uint64_t (&n)[N]) {
+  bn_get<T, VEC>(p, slot, kBnDy, w, q, e);
+  bn_get<T, VEC>(p, slot, kBnR, w, q, n);
+#pragma unroll
+  for (int i = 0; i < N; ++i) n[i] = fmul2(fadd2(n[i], bn_both(-st.mean)), bn_both(st.root));
+  if (!VEC && (q + 1) * 2 * N > p.width) {  // zeros past the row's end
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float lo, hi;
+      upk2(n[i], lo, hi);
+      n[i] = pk2(q * 2 * N + 2 * i < p.width ? lo : 0.f, q * 2 * N + 2 * i + 1 < p.width ? hi : 0.f);
+    }
+  }
+}
+
+template <typename T, bool VEC, bool FULL, int N>
+__device__ __forceinline__ void bn_modulate(const BlockNormParams& p, const uint8_t* slot, const BnWalk& w, int q,
+                                            uint64_t (&e)[N]) {
+  if (!FULL || p.in[kBnScaleB] == nullptr) return;
+  uint64_t s[N];
+  bn_get_mod<T, VEC>(p, slot, kBnScaleB, w, q, s);
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = ffma2(e[i], s[i], e[i]);
+}
+
+// R, the stream's gradient; dn = e a.
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void bn_stream_grad(const BlockNormParams& p, const uint8_t* slot, const BnWalk& w,
+                                               const BnStats& st, int q, const uint64_t (&e)[N], const uint64_t (&n)[N],
+                                               const uint64_t (&a)[N], uint64_t (&big)[N]) {
+  if (p.in[kBnDr] != nullptr) {
+    bn_get<T, VEC>(p, slot, kBnDr, w, q, big);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) big[i] = 0;
+  }
+  if (p.mode == DGXM_BLOCK_NORM_NONE) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint64_t inner = ffma2(e[i], a[i], ffma2(n[i], bn_both(-st.m2), bn_both(-st.m1)));
+    big[i] = ffma2(bn_both(st.root), inner, big[i]);
+  }
+}
+
+template <typename T, bool VEC, bool FULL, int STAT>
+__device__ __forceinline__ void bn_backward_stats(const BlockNormParams& p, float* param, const uint8_t* ring, BnShared& sh,
+                                                  int t) {
+  constexpr int CH = kBnChunk<T>, N = CH / 2;
+  const int lane = t & 31;
+  // Rows in turn, by no more warps than there are slots: none waits for a phase
+  // of a slot whose last one is still open.
+  const int warps = min(STAT, p.slots);
+  int turn = t >> 5 < warps ? t >> 5 : 0x7fffffff;  // rows until this warp's next
+  const bool norm = p.mode != DGXM_BLOCK_NORM_NONE, layer = p.mode == DGXM_BLOCK_NORM_LAYER;
+  int sample = -1;
+  bool dead = false;
+  for (BnWalk w(p); w.more(); w.next()) {
+    const char* const scale = p.scale ? p.scale + w.b * p.scale_sb : nullptr;
+    if (w.b != sample) {
+      sample = w.b;
+      bn_param<STAT>(p, param, t, [&](int c) {
+        const float up = scale ? 1.f + bn_value<T>(scale, p.mod_f32, c) : 1.f;
+        return p.norm_w ? up * bn_value<T>(p.norm_w, p.w_f32, c) : up;
+      });
+    }
+    if (turn-- > 0) continue;
+    turn = warps - 1;
+    bn_wait(&sh.full[w.slot], w.parity, dead);
+    const uint8_t* slot = ring + w.slot * p.slot_bytes;
+    auto factor = [&](int q, uint64_t (&a)[N]) {  // dn = e a
+      if (p.param_bytes > 0) {
+        bn_param_get(param, q, a);
+        return;
+      }
+      uint64_t wt[N];
+      bn_vector<T>(scale, p.mod_f32, q * CH, p.width, 0.f, a);
+      bn_vector<T>(p.norm_w, p.w_f32, q * CH, p.width, 1.f, wt);
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] = fmul2(fadd2(a[i], bn_both(1.f)), wt[i]);
+    };
+    BnStats st;
+    st.mean = st.root = st.m1 = st.m2 = st.m3 = 0.f;
+    st.root2 = 1.f;
+    if (norm) {
+      BnMoments moments;
+      uint64_t ss = 0;
+#pragma unroll 2
+    for (int q = lane; q * CH < p.width; q += 32) {
+        uint64_t r[N];
+        bn_get<T, VEC>(p, slot, kBnR, w, q, r);
+        if (layer) {
+          bn_add_chunk(moments, r, VEC ? CH : min(CH, p.width - q * CH));
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) ss = ffma2(r[i], r[i], ss);
+        }
+      }
+      if (layer) {
+        const float2 v = bn_warp_moments(moments);
+        st.mean = v.x;
+        st.root = rsqrtf(v.y + p.eps);
+      } else {
+        float sum[1] = {bn_total(ss)};
+        bn_warp_sum(sum);
+        st.root = rsqrtf(fmaf(sum[0], p.inv_width, p.eps));
+      }
+    }
+    float sums[3];
+    uint64_t s1 = 0, s2 = 0, s3 = 0;
+#pragma unroll 2
+    for (int q = lane; q * CH < p.width; q += 32) {
+      if (norm) {
+        uint64_t e[N], n[N], a[N];
+        bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
+        bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
+        factor(q, a);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint64_t dn = fmul2(e[i], a[i]);
+          s1 = fadd2(s1, dn);
+          s2 = ffma2(dn, n[i], s2);
+        }
+      }
+      if (FULL && p.branch_norm) {
+        uint64_t m[N];
+        bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s3 = ffma2(m[i], m[i], s3);
+      }
+    }
+    sums[0] = bn_total(s1);
+    sums[1] = bn_total(s2);
+    sums[2] = bn_total(s3);
+    bn_warp_sum(sums);
+    st.m1 = layer ? sums[0] * p.inv_width : 0.f;
+    st.m2 = sums[1] * p.inv_width;
+    if (FULL && p.branch_norm) {
+      st.root2 = rsqrtf(fmaf(sums[2], p.inv_width, p.eps));
+      uint64_t part = 0;
+#pragma unroll 2
+    for (int q = lane; q * CH < p.width; q += 32) {
+        uint64_t e[N], n[N], a[N], big[N], m[N], v[N];
+        if (norm) {
+          bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
+          bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
+          factor(q, a);
+        }
+        bn_stream_grad<T, VEC>(p, slot, w, st, q, e, n, a, big);
+        bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
+        if (p.in[kBnGateB] != nullptr) bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, v);
+        else bn_vector<T>(p.gate ? p.gate + w.b * p.gate_sb : nullptr, p.mod_f32, q * CH, p.width, 1.f, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) big[i] = fmul2(fmul2(big[i], v[i]), m[i]);
+        bn_vector<T>(p.branch_w, p.w_f32, q * CH, p.width, 1.f, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) part = ffma2(fmul2(big[i], v[i]), bn_both(st.root2), part);
+      }
+      float inner[1] = {bn_total(part)};
+      bn_warp_sum(inner);
+      st.m3 = inner[0] * p.inv_width;
+    }
+    if (lane == 0) {
+      sh.stats[w.slot] = st;
+      mbar_arrive(smem_u32(&sh.ready[w.slot]));
+    }
+  }
+  if (dead) report_device_error(kErrSoftmaxTimeout);
 }
 
 // The gradient.  The sums over rows that a thread keeps for its columns are
@@ -259,171 +804,128 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const __grid_constant_
 // with e = dy and f = R where the modulation serves a sample, so that the
 // gradients of weights and modulations both follow from them, and e = dh,
 // f = dm where each token has its own (n2 = branch without a branch norm).
-template <typename T, int NV>
-__global__ void __launch_bounds__(1024) block_norm_backward_kernel(const __grid_constant__ BlockNormParams p) {
-  constexpr int CH = BnChunk<T>::kN;
-  extern __shared__ __align__(16) uint8_t stage[];
-  __shared__ float red[2 * 4 * 32];
-  const int64_t first = blockIdx.x * p.rows / gridDim.x, last = (blockIdx.x + 1) * p.rows / gridDim.x;
-  float g[NV][CH], a[NV][CH], w2[NV][CH], acc[3][NV][CH];
-  int64_t sample = -1;
-  int turn = 0;
+template <typename T, int E, bool VEC, bool FULL, int MAXT, int STAT, int PER_SM>
+__global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_backward_kernel(const __grid_constant__ BlockNormParams p) {
+  constexpr int CH = kBnChunk<T>, NV = E / CH, N = CH / 2;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ BnShared sh;
+  const int threads = blockDim.x - 32 * STAT - 32, t = threadIdx.x;
+  uint8_t* ring = smem + p.param_bytes;
+  bn_start(p, sh, threads >> 5);
+  if (t >= threads + 32 * STAT) {
+    bn_fetch<VEC>(p, ring, sh);
+    return;
+  }
+  if (t >= threads) {
+    bn_backward_stats<T, VEC, FULL, STAT>(p, reinterpret_cast<float*>(smem), ring, sh, t - threads);
+    return;
+  }
+  const bool branch = p.in[kBnBranchB] != nullptr, norm = p.mode != DGXM_BLOCK_NORM_NONE;
+  uint64_t g[NV][N], a[NV][N], acc[3][NV][N];
+  int sample = -1;
+  bool dead = false;
   auto flush = [&]() {
     if (sample < 0 || p.partial == nullptr) return;
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
       if (!(p.want >> j & 1)) continue;
-      float* to = p.partial + ((blockIdx.x + sample) * 3 + j) * p.width;
+      char* to = reinterpret_cast<char*>(p.partial + ((blockIdx.x + static_cast<int64_t>(sample)) * 3 + j) * p.width);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (const int col = (threadIdx.x + k * blockDim.x) * CH + i; col < p.width) to[col] = acc[j][k][i];
+        if (const int col = (t + k * threads) * CH; col < p.width) bn_store<float, VEC, false>(to, col, p.width, acc[j][k]);
     }
   };
-  for (int64_t row = first; row < last; ++row) {
-    const int64_t b = row / p.seq, l = row - b * p.seq;
-    if (b != sample) {
+  for (BnWalk w(p); w.more(); w.next()) {
+    if (w.b != sample) {
       flush();
-      sample = b;
+      sample = w.b;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int col = (threadIdx.x + k * blockDim.x) * CH;
-        float w[CH];
-        bn_vector<T, CH>(p.gate ? p.gate + b * p.gate_sb : nullptr, p.mod_f32, col, p.width, 1.f, g[k]);
-        bn_vector<T, CH>(p.scale ? p.scale + b * p.scale_sb : nullptr, p.mod_f32, col, p.width, 0.f, a[k]);
-        bn_vector<T, CH>(p.norm_w, p.w_f32, col, p.width, 1.f, w);
-        bn_vector<T, CH>(p.branch_w, p.w_f32, col, p.width, 1.f, w2[k]);
+        const int col = (t + k * threads) * CH;
+        uint64_t wt[N];
+        bn_vector<T>(p.gate ? p.gate + sample * p.gate_sb : nullptr, p.mod_f32, col, p.width, 1.f, g[k]);
+        bn_vector<T>(p.scale ? p.scale + sample * p.scale_sb : nullptr, p.mod_f32, col, p.width, 0.f, a[k]);
+        bn_vector<T>(p.norm_w, p.w_f32, col, p.width, 1.f, wt);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          a[k][i] = (1.f + a[k][i]) * w[i];  // dh w = dy a
-          acc[0][k][i] = acc[1][k][i] = acc[2][k][i] = 0.f;
+        for (int i = 0; i < N; ++i) {
+          a[k][i] = fmul2(fadd2(a[k][i], bn_both(1.f)), wt[i]);
+          acc[0][k][i] = acc[1][k][i] = acc[2][k][i] = 0;
         }
       }
     }
-    __syncthreads();
-    bn_fill<T>(p, stage, b, l);
-    __syncthreads();
-    float n[NV][CH], dn[NV][CH];
-    float sums[2] = {0.f, 0.f};
+    bn_wait(&sh.full[w.slot], w.parity, dead);
+    bn_wait(&sh.ready[w.slot], w.parity, dead);
+    const uint8_t* slot = ring + w.slot * p.slot_bytes;
+    const BnStats st = sh.stats[w.slot];
+    char* const to_x = p.x_out + w.b * p.x_out_sb + w.l * p.x_out_sr;
+    char* const to_m = p.out + w.b * p.out_sb + w.l * p.out_sr;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * blockDim.x, col = q * CH;
+      const int q = t + k * threads, col = q * CH;
       if (col >= p.width) continue;
-      if (p.mode != DGXM_BLOCK_NORM_NONE) {
-        bn_read<T, CH>(stage + p.in_off[kBnR], q, 0, n[k]);
+      uint64_t e[N], n[N], big[N];
+      if (norm) {
+        bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
+        if constexpr (FULL) {
+          if (p.g_scale != nullptr) {  // a token's own: dy h
+            uint64_t h[N], bias[N];
+            bn_vector<T>(p.norm_w, p.w_f32, col, p.width, 1.f, h);
+            bn_vector<T>(p.norm_b, p.w_f32, col, p.width, 0.f, bias);
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
-          sums[0] += p.mode == DGXM_BLOCK_NORM_LAYER ? n[k][i] : n[k][i] * n[k][i];
-      }
-      if (p.branch_norm) {
-        float m[CH];
-        bn_read<T, CH>(stage + p.in_off[kBnBranchB], q, 0, m);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) sums[1] = fmaf(m[i], m[i], sums[1]);
-      }
-    }
-    bn_block_sum<2>(sums, red, turn);
-    const float root2 = p.branch_norm ? rsqrtf(fmaf(sums[1], p.inv_width, p.eps)) : 1.f;
-    float mean = 0.f, root = 0.f, m1 = 0.f, m2 = 0.f;
-    if (p.mode != DGXM_BLOCK_NORM_NONE) {
-      if (p.mode == DGXM_BLOCK_NORM_LAYER) {
-        mean = sums[0] * p.inv_width;
-        float ss[1] = {0.f};
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-          for (int i = 0; i < CH; ++i)
-            if ((threadIdx.x + k * blockDim.x) * CH + i < p.width) ss[0] = fmaf(n[k][i] - mean, n[k][i] - mean, ss[0]);
-        bn_block_sum<1>(ss, red, turn);
-        sums[0] = ss[0];
-      }
-      root = rsqrtf(fmaf(sums[0], p.inv_width, p.eps));
-      sums[0] = sums[1] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int q = threadIdx.x + k * blockDim.x, col = q * CH;
-        if (col >= p.width) continue;
-        float dy[CH], e[CH], s[CH];
-        bn_read<T, CH>(stage + p.in_off[kBnDy], q, 0, dy);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) n[k][i] = (n[k][i] - mean) * root;
-        if (p.in[kBnScaleB] != nullptr) bn_read<T, CH>(stage + p.in_off[kBnScaleB], q, p.in_f32[kBnScaleB], s);
-        if (p.g_scale != nullptr) {  // a token's own: dy h
-          float h[CH], bias[CH];
-          bn_vector<T, CH>(p.norm_w, p.w_f32, col, p.width, 1.f, h);
-          bn_vector<T, CH>(p.norm_b, p.w_f32, col, p.width, 0.f, bias);
-#pragma unroll
-          for (int i = 0; i < CH; ++i) h[i] = dy[i] * fmaf(n[k][i], h[i], bias[i]);
-          bn_store_mod<T, CH>(p.g_scale + row * p.width * (p.mod_f32 ? 4 : sizeof(T)), p.mod_f32, col, p.width, h);
+            for (int i = 0; i < N; ++i) h[i] = fmul2(e[i], ffma2(n[i], h[i], bias[i]));
+            bn_store_mod<T, VEC>(p.g_scale, w.row, p.mod_f32, col, p.width, h);
+          }
+          if (p.g_shift != nullptr) bn_store_mod<T, VEC>(p.g_shift, w.row, p.mod_f32, col, p.width, e);
         }
-        if (p.g_shift != nullptr)
-          bn_store_mod<T, CH>(p.g_shift + row * p.width * (p.mod_f32 ? 4 : sizeof(T)), p.mod_f32, col, p.width, dy);
+        bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          e[i] = p.in[kBnScaleB] != nullptr ? dy[i] * (1.f + s[i]) : dy[i];
-          dn[k][i] = e[i] * a[k][i];
-          acc[0][k][i] += e[i];
-          acc[1][k][i] = fmaf(e[i], n[k][i], acc[1][k][i]);
-          if (col + i < p.width) {
-            sums[0] += dn[k][i];
-            sums[1] = fmaf(dn[k][i], n[k][i], sums[1]);
+        for (int i = 0; i < N; ++i) {
+          acc[0][k][i] = fadd2(acc[0][k][i], e[i]);
+          acc[1][k][i] = ffma2(e[i], n[i], acc[1][k][i]);
+        }
+      }
+      bn_stream_grad<T, VEC>(p, slot, w, st, q, e, n, a[k], big);
+      if (p.x_out != nullptr) bn_store<T, VEC, true>(to_x, col, p.width, big);
+      if (!branch) continue;
+      uint64_t m[N];
+      bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
+      bool own = false;  // f = dm
+      if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], bn_both(st.root2));
+        if (p.in[kBnGateB] != nullptr) {
+          own = true;
+          bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, g[k]);
+          if (p.g_gate != nullptr) {
+            uint64_t dg[N];
+            bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, dg);
+#pragma unroll
+            for (int i = 0; i < N; ++i) dg[i] = fmul2(fmul2(big[i], m[i]), dg[i]);
+            bn_store_mod<T, VEC>(p.g_gate, w.row, p.mod_f32, col, p.width, dg);
           }
         }
       }
-      bn_block_sum<2>(sums, red, turn);
-      m1 = p.mode == DGXM_BLOCK_NORM_LAYER ? sums[0] * p.inv_width : 0.f;
-      m2 = sums[1] * p.inv_width;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint64_t dm = fmul2(big[i], g[k][i]);
+        acc[2][k][i] = ffma2(own ? dm : big[i], m[i], acc[2][k][i]);
+        big[i] = dm;
+      }
+      if (p.out == nullptr) continue;
+      if (FULL && p.branch_norm) {
+        uint64_t w2[N];
+        bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, w2);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          big[i] = fmul2(bn_both(st.root2), ffma2(m[i], bn_both(-st.m3), fmul2(big[i], w2[i])));
+      }
+      bn_store<T, VEC, true>(to_m, col, p.width, big);
     }
-    float inner[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int q = threadIdx.x + k * blockDim.x, col = q * CH;
-      if (col >= p.width) continue;
-      float big[CH];
-      if (p.in[kBnDr] != nullptr) bn_read<T, CH>(stage + p.in_off[kBnDr], q, 0, big);
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (p.in[kBnDr] == nullptr) big[i] = 0.f;
-        if (p.mode != DGXM_BLOCK_NORM_NONE) big[i] = fmaf(root, dn[k][i] - m1 - n[k][i] * m2, big[i]);
-      }
-      if (p.x_out != nullptr) bn_store<T, CH>(p.x_out + b * p.x_out_sb + l * p.x_out_sr, col, p.width, big);
-      if (p.in[kBnBranchB] == nullptr) continue;
-      float m[CH];
-      bn_read<T, CH>(stage + p.in_off[kBnBranchB], q, 0, m);
-      if (p.in[kBnGateB] != nullptr) bn_read<T, CH>(stage + p.in_off[kBnGateB], q, p.in_f32[kBnGateB], g[k]);
-      if (p.g_gate != nullptr) {
-        float dg[CH];
-#pragma unroll
-        for (int i = 0; i < CH; ++i) dg[i] = big[i] * m[i] * root2 * w2[k][i];
-        bn_store_mod<T, CH>(p.g_gate + row * p.width * (p.mod_f32 ? 4 : sizeof(T)), p.mod_f32, col, p.width, dg);
-      }
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        m[i] *= root2;
-        const float dm = big[i] * g[k][i];
-        acc[2][k][i] = fmaf(p.in[kBnGateB] != nullptr ? dm : big[i], m[i], acc[2][k][i]);
-        n[k][i] = m[i];
-        dn[k][i] = dm * w2[k][i];
-        if (col + i < p.width) inner[0] = fmaf(dn[k][i], m[i], inner[0]);
-      }
-      if (!p.branch_norm && p.out != nullptr)
-        bn_store<T, CH>(p.out + b * p.out_sb + l * p.out_sr, col, p.width, dn[k]);
-    }
-    if (p.branch_norm) {
-      bn_block_sum<1>(inner, red, turn);
-      const float m3 = inner[0] * p.inv_width;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int col = (threadIdx.x + k * blockDim.x) * CH;
-        if (col >= p.width) continue;
-#pragma unroll
-        for (int i = 0; i < CH; ++i) dn[k][i] = root2 * (dn[k][i] - n[k][i] * m3);
-        if (p.out != nullptr) bn_store<T, CH>(p.out + b * p.out_sb + l * p.out_sr, col, p.width, dn[k]);
-      }
-    }
+    __syncwarp();
+    if ((t & 31) == 0) mbar_arrive(smem_u32(&sh.empty[w.slot]));
   }
   flush();
+  if (dead) report_device_error(kErrEpilogueTimeout);
 }
 
 // The gradients of weights and modulations from the blocks' sums.
@@ -459,6 +961,8 @@ constexpr int kBnSumWarps = 32;
 // order.
 __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const __grid_constant__ BlockNormSumParams p) {
   __shared__ float part[kBnSumWarps][6][32];
+  pdl_launch_dependents();
+  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * 32 + lane;
   const bool in = col < p.width;
@@ -486,12 +990,13 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
   };
   for (int b = many ? warp : 0; b < p.batch; b += many ? kBnSumWarps : 1) {
     float s[3] = {0.f, 0.f, 0.f};
-    // The blocks that hold rows of this sample: block i has rows [i rows / blocks, (i + 1) rows / blocks).
+    // The blocks that hold rows of this sample.
     int64_t lo = 0, hi = 0;
     if (p.rows > 0) {
-      const int64_t r0 = static_cast<int64_t>(b) * p.seq, r1 = r0 + p.seq - 1;
-      lo = ((r0 + 1) * p.blocks - 1) / p.rows;
-      hi = ((r1 + 1) * p.blocks - 1) / p.rows + 1;
+      const int64_t each = p.rows / p.blocks, more = p.rows % p.blocks, longer = more * (each + 1);
+      auto block = [&](int64_t row) { return row < longer ? row / (each + 1) : more + (row - longer) / each; };
+      lo = block(static_cast<int64_t>(b) * p.seq);
+      hi = block(static_cast<int64_t>(b) * p.seq + p.seq - 1) + 1;
     }
     const int64_t i0 = many ? lo : lo + (hi - lo) * warp / kBnSumWarps;
     const int64_t i1 = many ? hi : lo + (hi - lo) * (warp + 1) / kBnSumWarps;
@@ -564,24 +1069,44 @@ static int bn_check(const dgxm_block_norm_desc* d) {
 
 static int64_t bn_rows(const dgxm_block_norm_desc* d) { return static_cast<int64_t>(d->batch) * d->seq; }
 
-// How a call is cut: chunks a thread, threads of a block, blocks.
-struct BnCut {
-  int chunks, threads, blocks;
+// How a call is cut: sixteen values a thread that makes outputs; for narrow
+// (0), middle (1) and wide (2) rows, how many of those a block has at the most
+// and how many warps for the statistics.
+constexpr int kBnEach = 16;
+
+template <bool BACK, int SIZE>
+struct BnKind {
+  static constexpr int kThreads = SIZE == 0 ? 128 : SIZE == 1 ? 320 : 512;
+  static constexpr int kStat = SIZE == 1 ? (BACK ? 5 : 8) : 3;
+  static constexpr int kMost = kThreads + 32 * kStat + 32;
+  // blocks of an SM by the registers of its warps, which come in fours
+  static constexpr int kPerSm = SIZE == 0 ? (BACK ? 2 : 3) : 1;
 };
 
-static BnCut bn_cut(const dgxm_block_norm_desc* d, bool back) {
-  const int ch = d->dtype == DGXM_DTYPE_F32 ? 4 : 8;
-  const int total = (d->width + ch - 1) / ch;
+struct BnCut {
+  int threads, blocks, per_sm;
+};
+
+static int bn_size(const dgxm_block_norm_desc* d) { return d->width <= 2048 ? 0 : d->width <= 5120 ? 1 : 2; }
+
+template <bool BACK, int SIZE>
+static BnCut bn_cut_of(const dgxm_block_norm_desc* d) {
+  using K = BnKind<BACK, SIZE>;
   BnCut cut;
-  cut.chunks = total <= 1024 ? 1 : 2;
-  cut.threads = ((total + cut.chunks - 1) / cut.chunks + 31) / 32 * 32;
-  const int per_sm = std::max(1, (back ? 1024 : 2048) / cut.threads);
-  cut.blocks = static_cast<int>(std::min<int64_t>(bn_rows(d), 148 * std::min(per_sm, 16)));
+  cut.threads = ((d->width + kBnEach - 1) / kBnEach + 31) / 32 * 32;
+  cut.per_sm = K::kPerSm;
+  cut.blocks = static_cast<int>(std::min<int64_t>(bn_rows(d), 148 * cut.per_sm));
   return cut;
 }
 
+template <bool BACK>
+static BnCut bn_cut(const dgxm_block_norm_desc* d) {
+  const int size = bn_size(d);
+  return size == 0 ? bn_cut_of<BACK, 0>(d) : size == 1 ? bn_cut_of<BACK, 1>(d) : bn_cut_of<BACK, 2>(d);
+}
+
 static int64_t bn_partial_bytes(const dgxm_block_norm_desc* d) {
-  return (bn_cut(d, true).blocks + static_cast<int64_t>(d->batch)) * 3 * d->width * 4;
+  return (bn_cut<true>(d).blocks + static_cast<int64_t>(d->batch)) * 3 * d->width * 4;
 }
 
 // What both directions share of the parameters.
@@ -605,22 +1130,38 @@ static void bn_stream(BlockNormParams* p, int s, const void* base, const int64_t
   p->in[s] = static_cast<const char*>(base);
   p->in_sb[s] = stride[0] * bn_elt(dtype);
   p->in_sr[s] = stride[1] * bn_elt(dtype);
-  p->in_f32[s] = dtype == DGXM_DTYPE_F32;
+  p->in_elt[s] = bn_elt(dtype);
 }
 
-// Place the streams in the stage; whole chunks of the widest.
-static void bn_layout(const dgxm_block_norm_desc* d, BlockNormParams* p, int n_in) {
+// Place the streams of a row in a slot of the ring, and as many slots as the
+// block's share of the shared memory holds.  `slack`: 16 bytes each for rows
+// off 16 bytes.  `param`: the statistics want a copy of a column vector.
+static void bn_layout(const dgxm_block_norm_desc* d, const BnCut& cut, BlockNormParams* p, bool param, bool slack) {
   const int ch = d->dtype == DGXM_DTYPE_F32 ? 4 : 8;
-  const int padded = (d->width + ch - 1) / ch * ch;
-  p->n_in = n_in;
+  const int padded = (d->width + ch - 1) / ch * ch, room = (224 / cut.per_sm - 4) * 1024;  // beside the static part
   int at = 0;
-  for (int s = 0; s < n_in; ++s) {
-    if (p->in[s] == nullptr) continue;
+  for (int s = 0; s < p->n_in; ++s) {
     p->in_off[s] = at;
-    p->in_pitch[s] = padded * (p->in_f32[s] ? 4 : 2);
+    if (p->in[s] == nullptr) continue;
+    p->in_pitch[s] = padded * p->in_elt[s] + (slack ? 16 : 0);
     at += p->in_pitch[s];
   }
-  p->stage_bytes = at;
+  p->slot_bytes = at;
+  // the copy only where it leaves three slots (its reader can do without)
+  p->param_bytes = param && 3 * at + padded * 4 <= room ? padded * 4 : 0;
+  p->slots = std::max(1, std::min(kBnMaxSlots, (room - p->param_bytes) / at));
+}
+
+// Every row of every stream and output on 16 bytes.
+static bool bn_vec(const dgxm_block_norm_desc* d, const BlockNormParams& p) {
+  uint64_t bits = 0;
+  for (int s = 0; s < p.n_in; ++s)
+    if (p.in[s] != nullptr) bits |= reinterpret_cast<uintptr_t>(p.in[s]) | p.in_sb[s] | p.in_sr[s];
+  bits |= reinterpret_cast<uintptr_t>(p.out) | p.out_sb | p.out_sr;
+  if (p.x_out != nullptr) bits |= reinterpret_cast<uintptr_t>(p.x_out) | p.x_out_sb | p.x_out_sr;
+  for (char* q : {p.g_gate, p.g_scale, p.g_shift}) bits |= reinterpret_cast<uintptr_t>(q);
+  bits |= reinterpret_cast<uintptr_t>(p.partial);
+  return bits % 16 == 0 && d->width % (d->dtype == DGXM_DTYPE_F32 ? 4 : 8) == 0;
 }
 
 static int bn_aligned(std::initializer_list<const void*> ptrs, int elt, const char* what) {
@@ -629,27 +1170,44 @@ static int bn_aligned(std::initializer_list<const void*> ptrs, int elt, const ch
   return DGXM_OK;
 }
 
-template <typename T, int NV>
-static int bn_launch_as(bool back, const BnCut& cut, const BlockNormParams& p, cudaStream_t st) {
-  static std::atomic<uint64_t> done[2] = {};
-  auto kernel = back ? block_norm_backward_kernel<T, NV> : block_norm_kernel<T, NV>;
-  if (p.stage_bytes > 48 * 1024) DGXM_CUDA_TRY(set_smem_limit_once(kernel, 224 * 1024, done[back]));
-  kernel<<<cut.blocks, cut.threads, p.stage_bytes, st>>>(p);
-  DGXM_CUDA_TRY(cudaGetLastError());
+template <bool BACK, typename T, int SIZE, bool VEC, bool FULL>
+static int bn_launch_as(const dgxm_block_norm_desc* d, BlockNormParams& p, cudaStream_t st) {
+  using K = BnKind<BACK, SIZE>;
+  static std::atomic<uint64_t> done{0};
+  void (*kernel)(BlockNormParams);
+  if constexpr (BACK) kernel = block_norm_backward_kernel<T, kBnEach, VEC, FULL, K::kThreads, K::kStat, K::kPerSm>;
+  else kernel = block_norm_kernel<T, kBnEach, VEC, FULL, K::kThreads, K::kStat, K::kPerSm>;
+  const BnCut cut = bn_cut<BACK>(d);
+  p.rows_each = p.rows / cut.blocks;
+  p.rows_more = static_cast<int>(p.rows % cut.blocks);
+  bn_layout(d, cut, &p, BACK ? p.scale != nullptr || p.norm_w != nullptr : p.gate != nullptr, !VEC);
+  DGXM_CUDA_TRY(set_smem_limit_once(kernel, 220 * 1024, done));
+  DGXM_CUDA_TRY(launch_overlapped(kernel, cut.blocks, cut.threads + 32 * K::kStat + 32,
+                                  p.param_bytes + p.slots * p.slot_bytes, st, p));
   return DGXM_OK;
 }
 
-template <typename T>
-static int bn_launch(bool back, const BnCut& cut, const BlockNormParams& p, cudaStream_t st) {
-  if (cut.chunks == 1) return bn_launch_as<T, 1>(back, cut, p, st);
-  return bn_launch_as<T, 2>(back, cut, p, st);
-
+template <bool BACK, typename T, int SIZE>
+static int bn_launch_size(const dgxm_block_norm_desc* d, BlockNormParams& p, cudaStream_t st) {
+  const bool full = p.branch_norm || d->gate_form == DGXM_MOD_TOKEN || d->mod_form == DGXM_MOD_TOKEN;
+  if (bn_vec(d, p))
+    return full ? bn_launch_as<BACK, T, SIZE, true, true>(d, p, st) : bn_launch_as<BACK, T, SIZE, true, false>(d, p, st);
+  return bn_launch_as<BACK, T, SIZE, false, true>(d, p, st);
 }
 
-static int bn_run(const dgxm_block_norm_desc* d, bool back, const BnCut& cut, const BlockNormParams& p, cudaStream_t st) {
-  if (d->dtype == DGXM_DTYPE_BF16) return bn_launch<__nv_bfloat16>(back, cut, p, st);
-  if (d->dtype == DGXM_DTYPE_F16) return bn_launch<__half>(back, cut, p, st);
-  return bn_launch<float>(back, cut, p, st);
+template <bool BACK, typename T>
+static int bn_launch(const dgxm_block_norm_desc* d, BlockNormParams& p, cudaStream_t st) {
+  const int size = bn_size(d);
+  return size == 0   ? bn_launch_size<BACK, T, 0>(d, p, st)
+         : size == 1 ? bn_launch_size<BACK, T, 1>(d, p, st)
+                     : bn_launch_size<BACK, T, 2>(d, p, st);
+}
+
+template <bool BACK>
+static int bn_run(const dgxm_block_norm_desc* d, BlockNormParams& p, cudaStream_t st) {
+  if (d->dtype == DGXM_DTYPE_BF16) return bn_launch<BACK, __nv_bfloat16>(d, p, st);
+  if (d->dtype == DGXM_DTYPE_F16) return bn_launch<BACK, __half>(d, p, st);
+  return bn_launch<BACK, float>(d, p, st);
 }
 
 }  // namespace dgxm
@@ -707,8 +1265,8 @@ extern "C" int dgxm_block_norm(const dgxm_block_norm_desc* d, const void* x, con
   p.x_out_sr = d->x_out_stride[1] * e;
   p.out_sb = d->out_stride[0] * e;
   p.out_sr = d->out_stride[1] * e;
-  bn_layout(d, &p, 5);
-  return bn_run(d, false, bn_cut(d, false), p, static_cast<cudaStream_t>(stream));
+  p.n_in = 5;
+  return bn_run<false>(d, p, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t dgxm_block_norm_backward_workspace(const dgxm_block_norm_desc* d) {
@@ -795,10 +1353,9 @@ extern "C" int dgxm_block_norm_backward(const dgxm_block_norm_desc* d, const dgx
     p.out_sb = d->out_stride[0] * e;
     p.out_sr = d->out_stride[1] * e;
     if (!apart && g->branch != nullptr) return fail(DGXM_ERR_INVALID, "the branch's gradient is that of x: pass NULL");
-    bn_layout(d, &p, 6);
-    const BnCut cut = bn_cut(d, true);
-    blocks = cut.blocks;
-    if (int rc = bn_run(d, true, cut, p, st)) return rc;
+    p.n_in = 6;
+    blocks = bn_cut<true>(d).blocks;
+    if (int rc = bn_run<true>(d, p, st)) return rc;
   }
   if (!p.want) return DGXM_OK;
   BlockNormSumParams sp;
@@ -828,7 +1385,6 @@ extern "C" int dgxm_block_norm_backward(const dgxm_block_norm_desc* d, const dgx
   sp.width = d->width;
   sp.blocks = blocks;
   sp.rows = rows;
-  block_norm_sum_kernel<<<(d->width + 31) / 32, kBnSumWarps * 32, 0, st>>>(sp);
-  DGXM_CUDA_TRY(cudaGetLastError());
+  DGXM_CUDA_TRY(launch_overlapped(block_norm_sum_kernel, (d->width + 31) / 32, kBnSumWarps * 32, 0, st, sp));
   return DGXM_OK;
 }
