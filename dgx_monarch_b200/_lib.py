@@ -269,6 +269,34 @@ class BlockNormGradPointers(ctypes.Structure):
                 for name in ("x", "branch", "gate", "scale", "shift", "norm_w", "norm_b", "branch_w")]
 
 
+ACT_NONE, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2, 3
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("w_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("pre_stride", ctypes.c_int64),
+        ("gate_stride", ctypes.c_int64 * 2),
+        ("sample_rows", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32),
+        ("gate_dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("gate_form", ctypes.c_int32),
+    ]
+
+
+class LinearGradPointers(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "w", "bias", "gate")]
+
+
 # Every symbol include/dgxm_sp.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -347,6 +375,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dgxm_block_norm_backward_workspace": (ctypes.c_int64, [ctypes.POINTER(BlockNormDesc)]),
     "dgxm_block_norm_backward": (ctypes.c_int, [ctypes.POINTER(BlockNormDesc), ctypes.POINTER(BlockNormGradPointers),
                                                 _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
+    "dgxm_linear_workspace": (ctypes.c_int64, [ctypes.POINTER(LinearDesc), _P, _P]),
+    "dgxm_linear": (ctypes.c_int, [ctypes.POINTER(LinearDesc), _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int64, _P]),
+    "dgxm_linear_backward_workspace": (ctypes.c_int64, [ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearGradPointers),
+                                                        _P, _P, _P]),
+    "dgxm_linear_backward": (ctypes.c_int, [ctypes.POINTER(LinearDesc), ctypes.POINTER(LinearGradPointers), _P, _P, _P, _P,
+                                            _P, _P, ctypes.c_int64, _P]),
     "dgxm_fp4_matmul": (ctypes.c_int, [ctypes.POINTER(Fp4GemmDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 

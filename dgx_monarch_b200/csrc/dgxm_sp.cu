@@ -20,3 +20,4 @@
 #include "fp4_quant.cu"
 #include "fp4_gemm.cu"
 #include "block_norm.cu"
+#include "linear.cu"

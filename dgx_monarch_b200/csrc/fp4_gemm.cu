@@ -167,8 +167,8 @@ __device__ __forceinline__ float fp4_gemm_bias(const Fp4GemmParams& p, int n) {
 }
 
 // 16-byte piece i of a lane's row in words: four fp32, or eight of a 16-bit type.
-template <int ELT>
-__device__ __forceinline__ uint4 fp4_piece(const Fp4GemmParams& p, const float* f) {
+template <int ELT, typename P>
+__device__ __forceinline__ uint4 fp4_piece(const P& p, const float* f) {
   if constexpr (ELT == 4)
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   else if (p.out_dtype == DGXM_DTYPE_BF16)
@@ -196,8 +196,8 @@ __device__ __forceinline__ uint4 fp4_bytes_from(uint4 a, uint4 b, uint32_t n) {
 // leaves the warp to its arithmetic (9450 x 5120 x 256: 47 us with stores of
 // the lanes, 23 us), or, otherwise, neighbouring lanes store neighbouring
 // words or elements.  ELT: bytes of an output element.
-template <int NC, int ELT>
-__device__ __forceinline__ void fp4_store_rows(const Fp4GemmParams& p, uint8_t* stage, const float (&v)[NC], int pr0,
+template <int NC, int ELT, typename P>
+__device__ __forceinline__ void fp4_store_rows(const P& p, uint8_t* stage, const float (&v)[NC], int pr0,
                                                int q0, int lane) {
   constexpr int kEach = 16 / ELT;  // elements of a piece
   constexpr int kMost = 128 / ELT;
@@ -340,7 +340,8 @@ __device__ __forceinline__ void fp4_store_split(const Fp4GemmParams& p, const fl
 
 // Tiles run in groups of eight P tiles, Q outermost within a group, so that
 // the CTAs resident at one time share a few panels of both operands.
-__device__ __forceinline__ void fp4_tile_coords(const Fp4GemmParams& p, int tile, int& pt, int& qt) {
+template <typename P>
+__device__ __forceinline__ void fp4_tile_coords(const P& p, int tile, int& pt, int& qt) {
   const int per_group = 8 * p.q_tiles;
   const int g = tile / per_group, r = tile - g * per_group;
   const int rows = min(8, p.p_tiles - g * 8);

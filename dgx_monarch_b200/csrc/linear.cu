@@ -1,0 +1,1093 @@
+// A 16-bit Linear with everything that follows it in a block in its epilogue,
+// and its gradients:
+//   pre = x W^T + bias,   out = residual + gate * act(pre)
+//   dz = dout * gate * act'(pre),   dx = dz W,   dW = dz^T x,
+//   dbias = sum dz,   dgate = sum dout * act(pre).
+//
+// All three products run in one kernel, D[p, q] = sum_k A[p, k] B[q, k], on
+// tcgen05 with fp32 accumulators in tensor memory.  Either operand is K-major
+// (contiguous in k) or MN-major (contiguous in its rows, as W is to dx and dz
+// and x are to dW): only the TMA boxes and the descriptors' strides differ, so
+// no operand is transposed in memory.
+//
+// Roles (10 warps), tile order, stores and the exchange of a split K are those
+// of the 4-bit product (fp4_gemm.cu): warp 0 loads, warp 1 issues the MMAs,
+// warps 2-9 run the epilogue.  Large products run on CTA pairs (256 x 256,
+// M256 MMAs that read both CTAs' operands), others on single CTAs, and with
+// few rows the weight gives the rows of a tile.
+#include <type_traits>
+
+#include "common.h"
+#include "ptx.cuh"
+
+namespace dgxm {
+
+constexpr int kLinK = 64;  // K a stage: one swizzle atom of 128 bytes
+
+struct __align__(64) LinearParams {
+  CUtensorMap tmap_a, tmap_b;  // K-major: dims (k, 1, rows), boxes (64, 1, 128 ..); MN-major: dims (rows, 1, k), boxes (64, 1, 64)
+  CUtensorMap tmap_out;        // where `vec`: dims (q_rows, 1, p_rows), boxes of 128 bytes x 32 rows
+  CUtensorMap tmap_res;        // where `res_bulk`: the same of the residual
+  const void *bias, *gate, *residual;
+  void *out, *pre;
+  int64_t ld_out, ld_res, ld_pre;         // elements
+  int64_t gate_sample, gate_row;          // elements between samples, rows
+  int p_rows, q_rows, k_tiles, k;
+  int p_tiles, q_tiles, split;
+  int q_is_tokens;                        // the rows of A are output columns: the tile is the output transposed
+  int out_dtype, bias_dtype, gate_dtype, pre_dtype, vec, res_bulk;
+  int act, sample_rows, f16;
+};
+
+template <int TN, bool PAIR>
+struct LinTile {
+  static constexpr int kRows = PAIR ? 256 : 128;
+  static constexpr int kQLoad = PAIR ? TN / 2 : TN;  // rows of B this CTA loads
+  static constexpr int kABytes = 128 * 128, kBBytes = kQLoad * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr bool kSplits = !PAIR;
+  static constexpr int kPartBytes = kSplits ? (128 + 10) * TN * 4 : 0;  // as in Fp4Tile
+  static constexpr int kStage2 = 2 * kGemmStageRows;  // two staging buffers an epilogue warp
+  static constexpr int kStagingBytes = kPartBytes > 8 * kStage2 ? kPartBytes : 8 * kStage2;
+  static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes - kStagingBytes) / kStageBytes;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kGemmCtrlBytes;
+  static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + 2,
+                       kDrain = kAccEmpty + 2, kRes = kDrain + 1, kBars = kRes + 16;
+  static_assert(kBars * 8 + 16 <= kGemmCtrlBytes, "control block");
+  static_assert(kStageBytes % 1024 == 0, "swizzle atoms stay aligned");
+  static constexpr int kTmem = TN < 32 ? 64 : 2 * TN;  // columns: a power of two, two accumulators
+};
+
+template <bool PAIR>
+__device__ __forceinline__ void lin_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  if constexpr (PAIR)
+    asm volatile(DGXM_ELECT
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+                 "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+  else
+    asm volatile(DGXM_ELECT
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+                 "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// 1 / (1 + e^-v)
+__device__ __forceinline__ float lin_sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
+constexpr float kGeluTanhA = 1.5957691216057308f;  // 2 sqrt(2 / pi): 1 + tanh(u) = 2 / (1 + e^-2u)
+constexpr float kGeluTanhB = 0.044715f;
+
+__device__ __forceinline__ float lin_act(float z, int act) {
+  if (act == DGXM_ACT_SILU) return z * lin_sigmoid(z);
+  if (act == DGXM_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (act == DGXM_ACT_GELU_TANH) return z * lin_sigmoid(kGeluTanhA * fmaf(kGeluTanhB * z * z, z, z));
+  return z;
+}
+
+__device__ __forceinline__ float lin_slope(float z, int act) {
+  if (act == DGXM_ACT_SILU) {
+    const float s = lin_sigmoid(z);
+    return s * fmaf(z, 1.f - s, 1.f);
+  }
+  if (act == DGXM_ACT_GELU)
+    return fmaf(z * 0.39894228040143268f, __expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+  if (act == DGXM_ACT_GELU_TANH) {
+    const float s = lin_sigmoid(kGeluTanhA * fmaf(kGeluTanhB * z * z, z, z));
+    return s * fmaf(z * (1.f - s), kGeluTanhA * fmaf(3.f * kGeluTanhB * z, z, 1.f), 1.f);
+  }
+  return 1.f;
+}
+
+__device__ __forceinline__ float lin_value(const void* base, int dtype, int64_t at) {
+  if (dtype == DGXM_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
+  if (dtype == DGXM_DTYPE_F16) return __half2float(static_cast<const __half*>(base)[at]);
+  return static_cast<const float*>(base)[at];
+}
+
+__device__ __forceinline__ void lin_put(void* base, int dtype, int64_t at, float v) {
+  if (dtype == DGXM_DTYPE_BF16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(v);
+  else if (dtype == DGXM_DTYPE_F16) static_cast<__half*>(base)[at] = __float2half_rn(v);
+  else static_cast<float*>(base)[at] = v;
+}
+
+// The epilogue of one value, of token m and output n.
+__device__ __forceinline__ void lin_finish(const LinearParams& p, int m, int n, float v, float bias) {
+  v += bias;
+  if (p.pre != nullptr) lin_put(p.pre, p.pre_dtype, m * p.ld_pre + n, v);
+  v = lin_act(v, p.act);
+  if (p.gate != nullptr)
+    v *= lin_value(p.gate, p.gate_dtype, m / p.sample_rows * p.gate_sample + m % p.sample_rows * p.gate_row + n);
+  if (p.residual != nullptr) v += lin_value(p.residual, p.out_dtype, m * p.ld_res + n);
+  lin_put(p.out, p.out_dtype, m * p.ld_out + n, v);
+}
+
+// One operand's rows of a stage.  K-major: `rows` rows of 64 k.  MN-major:
+// blocks of 64 rows, each 64 k of 128 bytes.
+template <bool PAIR, bool MN, int ROWS>
+__device__ __forceinline__ void lin_load(uint32_t dst, const void* map, uint32_t bar, int kt, int row) {
+  if constexpr (MN) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 64; ++i) fp4_tma<PAIR>(dst + i * 8192, map, bar, row + i * 64, 0, kt * kLinK);
+  } else {
+    fp4_tma<PAIR>(dst, map, bar, kt * kLinK, 0, row);
+  }
+}
+
+// Descriptor of an operand's K step kk (16 k): K-major 32 bytes on in each row;
+// MN-major 16 rows of 128 bytes on, blocks of 64 rows 8 KB apart.
+template <bool MN>
+__device__ __forceinline__ uint64_t lin_desc(uint32_t addr) {
+  return MN ? sdesc_sw128(addr, 8192, 1024) : sdesc_sw128(addr, 16, 1024);
+}
+template <bool MN>
+constexpr uint32_t kLinStep = MN ? 2048 / 16 : 32 / 16;
+
+// The epilogue of a warp's 32 rows x kCols columns of a tile from row pr0 and
+// column q0, rows being tokens: chunks of 128 output bytes, or all of them.
+template <int TN, bool PAIR, int ELT>
+__device__ __forceinline__ void lin_epilogue(const LinearParams& p, uint8_t* stage, uint32_t res_bar, int& res_phase,
+                                             uint32_t tmem, uint32_t acc_empty, int pr0, int q0, int lane,
+                                             const float (&bias)[(TN / 2 + 31) / 32]) {
+  constexpr int kCols = TN / 2, kMost = 128 / ELT, CC = kCols < kMost ? kCols : kMost, kChunks = kCols / CC;
+  const int m = pr0 + lane;
+  const int sample = min(m, p.p_rows - 1) / p.sample_rows, in_sample = m - sample * p.sample_rows;
+  const char* const gate = static_cast<const char*>(p.gate);
+  const bool one = p.gate_row == 0 && __all_sync(0xffffffffu, sample == __shfl_sync(0xffffffffu, sample, 0));
+  float gates[(kCols + 31) / 32];
+  if (gate != nullptr && one) {
+#pragma unroll
+    for (int i = 0; i < (kCols + 31) / 32; ++i) {
+      const int n = q0 + 32 * i + lane;
+      gates[i] = n < p.q_rows ? lin_value(gate, p.gate_dtype, sample * p.gate_sample + n) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int ch = 0; ch < kChunks; ++ch) {
+    const int c0 = ch * CC;
+    uint32_t r[CC / 8][8];
+#pragma unroll
+    for (int c = 0; c < CC / 8; ++c) tmem_ld8(tmem + c0 + 8 * c, r[c]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < CC / 8; ++c) reg_fence8(r[c]);
+    if (ch == kChunks - 1) {  // the accumulator is in registers: the next tile's MMAs may start
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster_relaxed(acc_empty);
+        else mbar_arrive(acc_empty);
+      }
+    }
+    if (q0 + c0 >= p.q_rows) continue;  // uniform over the warp; no residual is under way
+    float v[CC];
+#pragma unroll
+    for (int c = 0; c < CC; ++c) v[c] = __uint_as_float(r[c / 8][c % 8]);
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int c = 0; c < CC; ++c) v[c] += __shfl_sync(0xffffffffu, bias[(c0 + c) / 32], (c0 + c) % 32);
+    }
+    if (p.pre != nullptr && m < p.p_rows) {
+      if (ELT == 2 && q0 + c0 + CC <= p.q_rows && p.ld_pre % 8 == 0 && reinterpret_cast<uintptr_t>(p.pre) % 16 == 0) {
+        uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.pre) + m * p.ld_pre + q0 + c0);
+#pragma unroll
+        for (int c = 0; c < CC / 8; ++c) to[c] = fp4_piece<2>(p, v + 8 * c);
+      } else {
+        for (int c = 0; c < CC; ++c)
+          if (q0 + c0 + c < p.q_rows) lin_put(p.pre, p.pre_dtype, m * p.ld_pre + q0 + c0 + c, v[c]);
+      }
+    }
+    if (p.act == DGXM_ACT_SILU) {
+#pragma unroll
+      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], DGXM_ACT_SILU);
+    } else if (p.act == DGXM_ACT_GELU) {
+#pragma unroll
+      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], DGXM_ACT_GELU);
+    } else if (p.act == DGXM_ACT_GELU_TANH) {
+#pragma unroll
+      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], DGXM_ACT_GELU_TANH);
+    }
+    if (gate != nullptr) {
+      if (one) {
+#pragma unroll
+        for (int c = 0; c < CC; ++c) v[c] *= __shfl_sync(0xffffffffu, gates[(c0 + c) / 32], (c0 + c) % 32);
+      } else if (m < p.p_rows) {
+        const int64_t at = sample * p.gate_sample + in_sample * p.gate_row + q0 + c0;
+#pragma unroll 8
+        for (int c = 0; c < CC; ++c)
+          if (q0 + c0 + c < p.q_rows) v[c] *= lin_value(gate, p.gate_dtype, at + c);
+      }
+    }
+    uint8_t* const buffer = stage + (ch & 1) * kGemmStageRows;
+    if (p.residual != nullptr) {
+      if (CC == kMost && p.res_bulk) {
+        const int b = ch & 1;
+        if (!mbar_wait(res_bar + 8 * b, (res_phase >> b) & 1, nullptr)) report_device_error(kErrEpilogueTimeout);
+        res_phase ^= 1 << b;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4*>(buffer + lane * 128 + ((i ^ (lane & 7)) << 4));
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (ELT == 4) {
+              v[4 * i + k] += __uint_as_float(u[k]);
+            } else {
+              float2 f;
+              if (p.out_dtype == DGXM_DTYPE_BF16)
+                f = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xFFFF0000u));
+              else
+                f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+              v[8 * i + 2 * k] += f.x;
+              v[8 * i + 2 * k + 1] += f.y;
+            }
+          }
+        }
+        __syncwarp();
+      } else if (m < p.p_rows) {
+#pragma unroll 8
+        for (int c = 0; c < CC; ++c)
+          if (q0 + c0 + c < p.q_rows) v[c] += lin_value(p.residual, p.out_dtype, m * p.ld_res + q0 + c0 + c);
+      }
+    }
+    fp4_store_rows<CC, ELT>(p, buffer, v, pr0, q0 + c0, lane);
+    if (CC == kMost && p.res_bulk && ch + 2 < kChunks && q0 + c0 + 2 * CC < p.q_rows && lane == 0) {
+      tma_store_wait_read();
+      mbar_expect_tx(res_bar + 8 * (ch & 1), kGemmStageRows);
+      tma_load_4d(smem_u32(buffer), &p.tmap_res, res_bar + 8 * (ch & 1), q0 + c0 + 2 * CC, 0, pr0, 0);
+    }
+  }
+}
+
+template <int TN, bool PAIR, bool AMN, bool BMN>
+__global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_constant__ LinearParams p) {
+  using C = LinTile<TN, PAIR>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  uint8_t* staging = smem + C::kStages * C::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + C::kStagingBytes);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int cta = PAIR ? rank : 0;
+  const int share = PAIR ? 2 : p.split;  // CTAs of a tile
+  const int first_tile = blockIdx.x / share, tile_step = gridDim.x / share;
+  const int tiles = p.p_tiles * p.q_tiles;
+  const int kt0 = PAIR ? 0 : static_cast<int>(static_cast<int64_t>(rank) * p.k_tiles / p.split);  // this CTA's share of K
+  const int kt1 = PAIR ? p.k_tiles : static_cast<int>(static_cast<int64_t>(rank + 1) * p.k_tiles / p.split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(bar(C::kFull + s), 1);
+      mbar_init(bar(C::kEmpty + s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(bar(C::kAccFull + a), 1);
+      mbar_init(bar(C::kAccEmpty + a), PAIR ? 16 : 8);  // every epilogue warp
+    }
+    mbar_init(bar(C::kDrain), 1);
+    for (int i = 0; i < 16; ++i) mbar_init(bar(C::kRes + i), 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&p.tmap_a);
+    tma_prefetch_desc(&p.tmap_b);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), C::kTmem);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::kTmem);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if (PAIR || (C::kSplits && p.split > 1)) cluster_sync();  // the peers' barriers, and their shared memory, are there
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();  // the operands are there
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < tiles; tile += tile_step) {
+        int pt, qt;
+        fp4_tile_coords(p, tile, pt, qt);
+        for (int kt = kt0; kt < kt1; ++kt, ++it) {
+          const int s = it % C::kStages;
+          if (!mbar_wait(bar(C::kEmpty + s), ((it / C::kStages) & 1) ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = base + s * C::kStageBytes;
+          const uint32_t full = PAIR ? mapa_shared(bar(C::kFull + s), 0) : bar(C::kFull + s);
+          if (cta == 0) mbar_expect_tx(bar(C::kFull + s), (PAIR ? 2 : 1) * C::kStageBytes);
+          lin_load<PAIR, AMN, 128>(dst, &p.tmap_a, full, kt, pt * C::kRows + cta * 128);
+          lin_load<PAIR, BMN, C::kQLoad>(dst + C::kABytes, &p.tmap_b, full, kt, qt * TN + cta * C::kQLoad);
+        }
+      }
+      if (!ok) {
+        report_device_error(kErrProducerTimeout);
+        *abort_flag = 1;
+        // Let the loads already issued land before the CTA can exit.
+        if (cta == 0) {
+          const int first = it > C::kStages ? it - C::kStages : 0;
+          for (int i = first; i < it; ++i) mbar_wait(bar(C::kFull + i % C::kStages), (i / C::kStages) & 1, nullptr);
+        } else {
+          for (int i = 0; i < 50; ++i) __nanosleep(1000);  // the odd CTA cannot test the even one's barriers
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs
+    if (cta == 0) {
+      // idesc: fp32 accumulator, one format for both operands, their majors
+      const uint32_t idesc = __shfl_sync(0xffffffffu, idesc_make(C::kRows, TN, p.f16 ? 0u : 1u, BMN) | (AMN ? 1u << 15 : 0u), 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      int s = 0, parity = 0, u = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < tiles; tile += tile_step, ++u) {
+        const int a = u & 1;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kAccEmpty + a), ((u >> 1) & 1) ^ 1, abort_flag)))) break;
+        tc_fence_after();
+        const uint32_t acc = tm + a * TN;
+        for (int kt = kt0; kt < kt1; ++kt) {
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kFull + s), parity, abort_flag)))) break;
+          tc_fence_after();
+          const uint32_t sa = base + s * C::kStageBytes;
+          const uint64_t da = lin_desc<AMN>(sa), db = lin_desc<BMN>(sa + C::kABytes);
+#pragma unroll
+          for (int kk = 0; kk < kLinK / 16; ++kk)
+            lin_umma<PAIR>(acc, da + kk * kLinStep<AMN>, db + kk * kLinStep<BMN>, idesc, (kt > kt0 || kk > 0) ? 1u : 0u);
+          fp4_commit<PAIR>(bar(C::kEmpty + s));
+          if (++s == C::kStages) {
+            s = 0;
+            parity ^= 1;
+          }
+        }
+        if (ok) fp4_commit<PAIR>(bar(C::kAccFull + a));
+      }
+      if (!ok) {
+        report_device_error(kErrMmaTimeout);
+        *abort_flag = 1;
+      }
+      // Every MMA issued has completed before tensor memory is released.
+      fp4_commit<PAIR>(bar(C::kDrain));
+      mbar_wait(bar(C::kDrain), 0, nullptr);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const int row = quarter * 32 + lane;
+    constexpr int kCols = TN / 2;  // this warp's columns
+    constexpr int kBias = (kCols + 31) / 32;
+    const uint32_t acc_empty = PAIR ? mapa_shared(bar(C::kAccEmpty), 0) : bar(C::kAccEmpty);
+    uint8_t* stage = staging + (warp - 2) * C::kStage2;
+    const uint32_t res_bar = bar(C::kRes + 2 * (warp - 2));
+    int u = 0, res_phase = 0;
+    for (int tile = first_tile; tile < tiles; tile += tile_step, ++u) {
+      const int a = u & 1;
+      int pt, qt;
+      fp4_tile_coords(p, tile, pt, qt);
+      const int pr0 = pt * C::kRows + cta * 128 + quarter * 32;  // this warp's first row
+      const int q0 = qt * TN + half * kCols;
+      float bias[kBias];  // column 32 i + lane, or (tokens) this lane's row
+#pragma unroll
+      for (int i = 0; i < kBias; ++i) {
+        const int n = p.q_is_tokens ? pr0 + lane : q0 + 32 * i + lane;
+        bias[i] = p.bias != nullptr && n < (p.q_is_tokens ? p.p_rows : p.q_rows) ? lin_value(p.bias, p.bias_dtype, n) : 0.f;
+      }
+      // The residual's first two chunks come while the MMAs run.
+      if (p.res_bulk && lane == 0) {
+        const int chunk = 128 / (p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2);
+        tma_store_wait_read();
+        for (int b = 0; b < 2 && b * chunk < kCols; ++b) {
+          if (q0 + b * chunk >= p.q_rows) break;
+          mbar_expect_tx(res_bar + 8 * b, kGemmStageRows);
+          tma_load_4d(smem_u32(stage + b * kGemmStageRows), &p.tmap_res, res_bar + 8 * b, q0 + b * chunk, 0, pr0, 0);
+        }
+      }
+      __syncwarp();
+      const bool got = __all_sync(0xffffffffu, mbar_wait(bar(C::kAccFull + a), (u >> 1) & 1, abort_flag));
+      if (!got) {
+        report_device_error(kErrEpilogueTimeout);
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t from = tmem + lane_off + a * TN + half * kCols;
+      if constexpr (TN > 64) {
+        if (PAIR || p.split == 1) {
+          if (p.out_dtype == DGXM_DTYPE_F32)
+            lin_epilogue<TN, PAIR, 4>(p, stage, res_bar, res_phase, from, acc_empty + a * 8, pr0, q0, lane, bias);
+          else
+            lin_epilogue<TN, PAIR, 2>(p, stage, res_bar, res_phase, from, acc_empty + a * 8, pr0, q0, lane, bias);
+          continue;
+        }
+      }
+      if constexpr (!PAIR) {
+        uint32_t r[kCols / 8][8];
+#pragma unroll
+        for (int c = 0; c < kCols / 8; ++c) tmem_ld8(from + 8 * c, r[c]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < kCols / 8; ++c) reg_fence8(r[c]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + a * 8);
+        if (p.split > 1) {
+          const int rows = (128 + p.split - 1) / p.split, pitch = rows | 1;
+          const uint32_t to = mapa_shared(smem_u32(staging), row / rows) +
+                              ((rank * (TN / 4) + half * (kCols / 4)) * pitch + row % rows) * 16;
+#pragma unroll
+          for (int c = 0; c < kCols / 4; ++c) st_shared_cluster(to + c * pitch * 16, r[c / 2] + 4 * (c % 2));
+        } else if (const int n = pr0 + lane; n < p.p_rows) {  // the rows are output columns
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            if (q0 + c < p.q_rows) lin_finish(p, q0 + c, n, __uint_as_float(r[c / 8][c % 8]), bias[0]);
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait_all();  // the staging rows outlive the stores
+    __syncwarp();
+  }
+  tc_fence_before();
+  if (PAIR || (C::kSplits && p.split > 1)) cluster_sync();  // both CTAs' MMAs drained; or every partial sum is in place
+  else __syncthreads();
+  if constexpr (C::kSplits) {
+    if (p.split > 1 && warp >= 2 && *abort_flag == 0) {
+      // A split tile: this CTA's share of its rows, four columns of a row a thread.
+      const float4* part = reinterpret_cast<const float4*>(staging);
+      int pt, qt;
+      fp4_tile_coords(p, first_tile, pt, qt);
+      const int most = (128 + p.split - 1) / p.split, rows = min(most, 128 - rank * most), pitch = most | 1;
+      for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
+        // neighbouring lanes take neighbouring output columns
+        const int r = p.q_is_tokens ? i % rows : i / (TN / 4), c = 4 * (p.q_is_tokens ? i / rows : i % (TN / 4));
+        const int pr = pt * 128 + rank * most + r, q = qt * TN + c;
+        if (pr >= p.p_rows || q >= p.q_rows) continue;
+        float4 sum = part[c / 4 * pitch + r];
+        for (int k = 1; k < p.split; ++k) {
+          const float4 more = part[(k * (TN / 4) + c / 4) * pitch + r];
+          sum.x += more.x;
+          sum.y += more.y;
+          sum.z += more.z;
+          sum.w += more.w;
+        }
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (q + e >= p.q_rows) continue;
+          const int m = p.q_is_tokens ? q + e : pr, n = p.q_is_tokens ? pr : q + e;
+          lin_finish(p, m, n, v[e], p.bias != nullptr ? lin_value(p.bias, p.bias_dtype, n) : 0.f);
+        }
+      }
+    }
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, C::kTmem);
+    else tmem_dealloc(tmem, C::kTmem);
+  }
+}
+
+// One operand of a product: rows x k, contiguous in k, or (mn) in its rows.
+struct LinOperand {
+  const void* ptr;
+  int64_t rows, ld;
+  bool mn;
+};
+
+static int lin_map(CUtensorMap* map, const LinOperand& o, int64_t k, int box_rows) {
+  const cuuint64_t row = static_cast<cuuint64_t>(o.ld) * 2;
+  if (o.mn)
+    return fp4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.ptr, {(cuuint64_t)o.rows, 1, (cuuint64_t)k}, {row, row},
+                   {64, 1, kLinK}, CU_TENSOR_MAP_SWIZZLE_128B);
+  return fp4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.ptr, {(cuuint64_t)k, 1, (cuuint64_t)o.rows}, {row, row},
+                 {kLinK, 1, (cuuint32_t)box_rows}, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+static int lin_out_map(CUtensorMap* map, const void* base, int64_t ld, const LinearParams& p) {
+  const int elt = p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2;
+  const cuuint64_t row = static_cast<cuuint64_t>(ld) * elt;
+  return fp4_map(map, elt == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, base,
+                 {(cuuint64_t)p.q_rows, 1, (cuuint64_t)p.p_rows}, {row, row}, {(cuuint32_t)(128 / elt), 1, 32},
+                 CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int TN, bool PAIR, bool AMN, bool BMN>
+static int lin_launch(LinearParams& p, const LinOperand& a, const LinOperand& b, cudaStream_t st) {
+  using C = LinTile<TN, PAIR>;
+  static std::atomic<uint64_t> configured{0};
+  DGXM_CUDA_TRY(set_smem_limit_once(linear_kernel<TN, PAIR, AMN, BMN>, C::kSmemBytes, configured));
+  if (int rc = lin_map(&p.tmap_a, a, p.k, 128)) return rc;
+  if (int rc = lin_map(&p.tmap_b, b, p.k, C::kQLoad)) return rc;
+  const int elt = p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2;
+  const bool rows = !p.q_is_tokens && p.split == 1;
+  p.vec = p.vec && rows;
+  p.res_bulk = p.vec && p.residual != nullptr && TN / 2 >= 128 / elt && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0 &&
+               p.ld_res > 0 && p.ld_res * elt % 16 == 0;
+  if (p.vec)
+    if (int rc = lin_out_map(&p.tmap_out, p.out, p.ld_out, p)) return rc;
+  if (p.res_bulk)
+    if (int rc = lin_out_map(&p.tmap_res, p.residual, p.ld_res, p)) return rc;
+  p.p_tiles = (p.p_rows + C::kRows - 1) / C::kRows;
+  p.q_tiles = (p.q_rows + TN - 1) / TN;
+  const int tiles = p.p_tiles * p.q_tiles, share = PAIR ? 2 : p.split;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = share;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  // One tile at a time; a split tile's cluster has one tile.
+  cfg.gridDim = dim3(PAIR ? 2 * std::min(tiles, 74) : p.split > 1 ? tiles * p.split : std::min(tiles, 148));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_kernel<TN, PAIR, AMN, BMN>, p));
+  return DGXM_OK;
+}
+
+// How a product is cut: the tile's columns (256: a CTA pair's 256 x 256), into
+// how many CTAs its K is split, and whether the tile is transposed.
+struct LinCut {
+  int tn, split;
+  bool q_is_tokens;  // with at most 64 columns
+};
+
+// Tiles of up to 64 columns are transposed: the few rows (m) are B's, which is
+// K-major then.
+static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn) {
+  struct Kind {
+    int tn, rows, at_once;
+    double stage, tile, least;
+  };
+  static const Kind kinds[] = {{16, 128, 148, 0.26, 0.4, 0.4},  {32, 128, 148, 0.26, 0.5, 0.5},
+                               {64, 128, 148, 0.25, 0.8, 1.0},  {128, 128, 148, 0.29, 0.8, 1.1},
+                               {256, 256, 74, 0.42, 1.75, 2.2}};
+  static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};  // that the SMs hold at one time
+  LinCut best{128, 1, false};
+  double least = 1e30;
+  for (const Kind& kind : kinds) {
+    const bool swapped = kind.tn <= 64;
+    if (swapped && (a_mn || (kind.tn < 64 && m > kind.tn))) continue;
+    const int64_t p_rows = swapped ? n : m, q_rows = swapped ? m : n;
+    const int64_t tiles = (p_rows + kind.rows - 1) / kind.rows * ((q_rows + kind.tn - 1) / kind.tn);
+    for (int split = 1; split <= (kind.tn <= 128 ? 8 : 1) && split <= k_tiles; ++split) {
+      if (split > 1 && tiles > clusters[split]) continue;
+      const int64_t waves = (tiles * split + kind.at_once - 1) / kind.at_once;
+      const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile, kind.least) +
+                        (split > 1 ? 0.8 + 0.026 * kind.tn : 0.0);
+      if (us < least) {
+        least = us;
+        best = {kind.tn, split, swapped};
+      }
+    }
+  }
+  return best;
+}
+
+// D (m x n) = A B^T with the epilogue in p; a gives the tokens' side.
+static int lin_product(LinearParams& p, const LinOperand& a, const LinOperand& b, int64_t k, cudaStream_t st) {
+  p.k = static_cast<int>(k);
+  p.k_tiles = static_cast<int>((k + kLinK - 1) / kLinK);
+  const LinCut cut = lin_cut(a.rows, b.rows, p.k_tiles, a.mn);
+  p.split = cut.split;
+  p.q_is_tokens = cut.q_is_tokens;
+  const LinOperand &po = p.q_is_tokens ? b : a, &qo = p.q_is_tokens ? a : b;
+  p.p_rows = static_cast<int>(po.rows);
+  p.q_rows = static_cast<int>(qo.rows);
+  p.vec = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ld_out * (p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2) % 16 == 0;
+  const bool amn = po.mn, bmn = qo.mn;
+  switch (cut.tn) {
+    case 16: return amn ? lin_launch<16, false, true, false>(p, po, qo, st) : lin_launch<16, false, false, false>(p, po, qo, st);
+    case 32: return amn ? lin_launch<32, false, true, false>(p, po, qo, st) : lin_launch<32, false, false, false>(p, po, qo, st);
+    case 64: return amn ? lin_launch<64, false, true, false>(p, po, qo, st) : lin_launch<64, false, false, false>(p, po, qo, st);
+    case 128:
+      return amn   ? lin_launch<128, false, true, true>(p, po, qo, st)
+             : bmn ? lin_launch<128, false, false, true>(p, po, qo, st)
+                   : lin_launch<128, false, false, false>(p, po, qo, st);
+    default:
+      return amn   ? lin_launch<256, true, true, true>(p, po, qo, st)
+             : bmn ? lin_launch<256, true, false, true>(p, po, qo, st)
+                   : lin_launch<256, true, false, false>(p, po, qo, st);
+  }
+}
+
+// ------------------------------------------------------------ matrices off 16 bytes
+// Rows that no TMA box can start at are copied to a pitch of whole 16 bytes first.
+struct LinPackParams {
+  const uint16_t* from;
+  uint16_t* to;
+  int64_t rows, ld, pitch;
+  int cols;
+};
+
+__global__ void __launch_bounds__(256) linear_pack_kernel(const __grid_constant__ LinPackParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int words = static_cast<int>(p.pitch / 8);
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < p.rows * words; i += gridDim.x * 256LL) {
+    const int64_t row = i / words;
+    const int col = static_cast<int>(i - row * words) * 8;
+    const uint16_t* from = p.from + row * p.ld + col;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = col + 2 * k < p.cols ? from[2 * k] : 0u, hi = col + 2 * k + 1 < p.cols ? from[2 * k + 1] : 0u;
+      w[k] = lo | hi << 16;
+    }
+    *reinterpret_cast<uint4*>(p.to + row * p.pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+static int64_t lin_pitch(int64_t cols) { return (cols + 7) / 8 * 8; }
+static bool lin_on_words(const void* ptr, int64_t ld) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && ld % 8 == 0; }
+static int64_t lin_packed_bytes(const void* ptr, int64_t ld, int64_t rows, int64_t cols) {
+  return lin_on_words(ptr, ld) ? 0 : (rows * lin_pitch(cols) * 2 + 255) / 256 * 256;
+}
+
+// o with its rows on 16 bytes, from the workspace where they are not.
+static int lin_pack(const void** ptr, int64_t* ld, int64_t rows, int64_t cols, char** work, cudaStream_t st) {
+  const int64_t bytes = lin_packed_bytes(*ptr, *ld, rows, cols);
+  if (bytes == 0) return DGXM_OK;
+  LinPackParams p{static_cast<const uint16_t*>(*ptr), reinterpret_cast<uint16_t*>(*work), rows, *ld, lin_pitch(cols),
+                  static_cast<int>(cols)};
+  const int64_t blocks = std::min<int64_t>((rows * (p.pitch / 8) + 255) / 256, 148 * 16);
+  DGXM_CUDA_TRY(launch_overlapped(linear_pack_kernel, static_cast<unsigned>(blocks), 256, 0, st, p));
+  *ptr = *work;
+  *ld = p.pitch;
+  *work += bytes;
+  return DGXM_OK;
+}
+
+// ------------------------------------------------------------ dz and the sums over rows
+// A thread takes eight columns of a run of rows of one sample; its sums go to
+// (run, 2, n) partial sums of dz and dout act(pre), which a second kernel adds
+// in the order of the runs.
+constexpr int kDzRows = 32;  // rows of a run
+
+struct LinDzParams {
+  const void *dout, *pre, *gate;
+  void *dz, *g_gate;  // g_gate: a token's own, contiguous
+  float* partial;     // (runs, 2, n), or NULL
+  int64_t ld_dout, ld_pre, ld_dz, gate_sample, gate_row;
+  int64_t runs;
+  int n, sample_rows, sample_runs, act, sum_bias, sum_gate;
+  int dtype, dout_dtype, gate_dtype, vec;
+};
+
+// Eight values from column `col`, zeros past the last.
+__device__ __forceinline__ void lin_read8(const void* base, int dtype, int64_t at, int col, int n, int vec, float (&v)[8]) {
+  if (vec && col + 8 <= n) {
+    if (dtype == DGXM_DTYPE_F32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+      const float4 a = p[0], b = p[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 f;
+        if (dtype == DGXM_DTYPE_BF16) f = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xFFFF0000u));
+        else f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = col + i < n ? lin_value(base, dtype, at + i) : 0.f;
+  }
+}
+
+__global__ void __launch_bounds__(128) linear_dz_kernel(const __grid_constant__ LinDzParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
+  if (col >= p.n) return;
+  for (int64_t run = blockIdx.x; run < p.runs; run += gridDim.x) {
+    const int64_t sample = run / p.sample_runs;
+    const int first = static_cast<int>(run - sample * p.sample_runs) * kDzRows, rows = min(kDzRows, p.sample_rows - first);
+    float gate[8], sum[8], sum_gate[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      gate[i] = 1.f;
+      sum[i] = sum_gate[i] = 0.f;
+    }
+    if (p.gate != nullptr && p.gate_row == 0) lin_read8(p.gate, p.gate_dtype, sample * p.gate_sample + col, col, p.n, 0, gate);
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const int64_t m = sample * p.sample_rows + first + r;
+      float d[8], z[8];
+      lin_read8(p.dout, p.dout_dtype, m * p.ld_dout + col, col, p.n, p.vec, d);
+      if (p.pre != nullptr) lin_read8(p.pre, p.dtype, m * p.ld_pre + col, col, p.n, p.vec, z);
+      if (p.gate != nullptr && p.gate_row != 0)
+        lin_read8(p.gate, p.gate_dtype, sample * p.gate_sample + (first + r) * p.gate_row + col, col, p.n, 0, gate);
+      if (p.sum_gate || p.g_gate != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = d[i] * lin_act(z[i], p.act);
+          sum_gate[i] += v;
+          if (p.g_gate != nullptr && col + i < p.n) lin_put(p.g_gate, p.gate_dtype, m * p.n + col + i, v);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        d[i] *= gate[i];
+        if (p.act != DGXM_ACT_NONE) d[i] *= lin_slope(z[i], p.act);
+        sum[i] += d[i];
+      }
+      if (p.dz != nullptr) {
+        const bool f16 = p.dtype == DGXM_DTYPE_F16;
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = f16 ? pack_f16x2(d[2 * k], d[2 * k + 1]) : pack_bf16x2(d[2 * k], d[2 * k + 1]);
+        // (columns past the last, up to the pitch, are zeros)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dz) + m * p.ld_dz + col) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (p.partial != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (col + i >= p.n) continue;
+        if (p.sum_bias) p.partial[run * 2 * p.n + col + i] = sum[i];
+        if (p.sum_gate) p.partial[(run * 2 + 1) * p.n + col + i] = sum_gate[i];
+      }
+    }
+  }
+}
+
+struct LinSumParams {
+  const float* partial;
+  void *g_bias, *g_gate;
+  int64_t samples;
+  int n, sample_runs, bias_dtype, gate_dtype, gate_form;
+};
+
+// A block takes 32 columns.  Its warps take the samples in turn where there
+// are many, or else share out the runs of each; warp 0 adds their sums in order.
+__global__ void __launch_bounds__(1024) linear_sum_kernel(const __grid_constant__ LinSumParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ float part[32][2][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
+  const bool in = col < p.n, gates = p.g_gate != nullptr, many = p.samples >= 32;
+  float bias = 0.f, shared = 0.f;
+  auto own = [&](int64_t s, float g) {
+    if (in && gates && p.gate_form == DGXM_MOD_SAMPLE) lin_put(p.g_gate, p.gate_dtype, s * p.n + col, g);
+  };
+  auto join = [&](float& b, float& g) {  // for warp 0
+    part[warp][0][lane] = b;
+    part[warp][1][lane] = g;
+    __syncthreads();
+    if (warp == 0) {
+      b = g = 0.f;
+      for (int k = 0; k < 32; ++k) {
+        b += part[k][0][lane];
+        g += part[k][1][lane];
+      }
+    }
+    __syncthreads();
+  };
+  for (int64_t s = many ? warp : 0; s < p.samples; s += many ? 32 : 1) {
+    float b = 0.f, g = 0.f;
+    const int64_t r0 = s * p.sample_runs + (many ? 0 : static_cast<int64_t>(p.sample_runs) * warp / 32);
+    const int64_t r1 = s * p.sample_runs + (many ? p.sample_runs : static_cast<int64_t>(p.sample_runs) * (warp + 1) / 32);
+    if (in) {
+#pragma unroll 4
+      for (int64_t r = r0; r < r1; ++r) {
+        if (p.g_bias != nullptr) b += p.partial[r * 2 * p.n + col];
+        if (gates) g += p.partial[(r * 2 + 1) * p.n + col];
+      }
+    }
+    if (!many) join(b, g);
+    if (many || warp == 0) own(s, g);
+    bias += b;
+    shared += g;
+  }
+  if (many) join(bias, shared);
+  if (warp != 0 || !in) return;
+  if (gates && p.gate_form == DGXM_MOD_SHARED) lin_put(p.g_gate, p.gate_dtype, col, shared);
+  if (p.g_bias != nullptr) lin_put(p.g_bias, p.bias_dtype, col, bias);
+}
+
+// ------------------------------------------------------------ the C entries
+static int lin_check(const dgxm_linear_desc* d) {
+  if (d == nullptr) return fail(DGXM_ERR_INVALID, "NULL linear descriptor");
+  const int64_t most = int64_t(1) << 30;
+  if (d->m < 0 || d->n < 0 || d->k <= 0 || d->m > most || d->n > most)
+    return fail(DGXM_ERR_INVALID, "product of (%lld, %lld) and (%lld, %lld)", (long long)d->m, (long long)d->k,
+                (long long)d->n, (long long)d->k);
+  // A stage of K takes 0.5 us at the most: the longest K waits well within the bounded waits' second.
+  if (d->k > (1 << 24) || d->n > (1 << 24)) return fail(DGXM_ERR_UNSUPPORTED, "k %lld or n %lld above 2^24", (long long)d->k, (long long)d->n);
+  if (d->dtype != DGXM_DTYPE_BF16 && d->dtype != DGXM_DTYPE_F16)
+    return fail(DGXM_ERR_UNSUPPORTED, "dtype %d (bf16 or f16)", d->dtype);
+  for (int t : {d->out_dtype, d->bias_dtype, d->gate_dtype})
+    if (t != d->dtype && t != DGXM_DTYPE_F32)
+      return fail(DGXM_ERR_UNSUPPORTED, "output, bias or gate dtype %d (the operands' or f32)", t);
+  if (d->activation < DGXM_ACT_NONE || d->activation > DGXM_ACT_GELU_TANH)
+    return fail(DGXM_ERR_UNSUPPORTED, "activation %d", d->activation);
+  if (d->gate_form < DGXM_MOD_NONE || d->gate_form > DGXM_MOD_TOKEN)
+    return fail(DGXM_ERR_INVALID, "modulation form %d", d->gate_form);
+  if (d->gate_form != DGXM_MOD_NONE && (d->sample_rows <= 0 || (d->m > 0 && d->m % d->sample_rows != 0)))
+    return fail(DGXM_ERR_INVALID, "%lld rows are no whole samples of %lld", (long long)d->m, (long long)d->sample_rows);
+  if ((d->m > 1 && d->x_stride < d->k) || (d->n > 1 && d->w_stride < d->k) || (d->m > 1 && d->out_stride < d->n))
+    return fail(DGXM_ERR_INVALID, "a row stride is below its row");
+  if ((d->m + 127) / 128 * ((d->n + 127) / 128) > (1 << 26) || (d->m + 127) / 128 * ((d->k + 127) / 128) > (1 << 26) ||
+      (d->n + 127) / 128 * ((d->k + 127) / 128) > (1 << 26))
+    return fail(DGXM_ERR_UNSUPPORTED, "too many output tiles");
+  return DGXM_OK;
+}
+
+static int lin_elt(int dtype) { return dtype == DGXM_DTYPE_F32 ? 4 : 2; }
+
+static int lin_aligned(const void* ptr, int dtype, const char* what) {
+  if (reinterpret_cast<uintptr_t>(ptr) % lin_elt(dtype)) return fail(DGXM_ERR_INVALID, "%s is not aligned to its elements", what);
+  return DGXM_OK;
+}
+
+static void lin_gate_strides(const dgxm_linear_desc* d, int64_t* sample, int64_t* row) {
+  *sample = d->gate_form == DGXM_MOD_SAMPLE || d->gate_form == DGXM_MOD_TOKEN ? d->gate_stride[0] : 0;
+  *row = d->gate_form == DGXM_MOD_TOKEN ? d->gate_stride[1] : 0;
+}
+
+}  // namespace dgxm
+
+extern "C" int64_t dgxm_linear_workspace(const dgxm_linear_desc* d, const void* x, const void* w) {
+  using namespace dgxm;
+  if (lin_check(d)) return -1;
+  if (d->m == 0 || d->n == 0) return 0;
+  return lin_packed_bytes(x, d->x_stride, d->m, d->k) + lin_packed_bytes(w, d->w_stride, d->n, d->k);
+}
+
+extern "C" int dgxm_linear(const dgxm_linear_desc* d, const void* x, const void* w, const void* bias, const void* gate,
+                           const void* residual, void* out, void* pre, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+  using namespace dgxm;
+  if (int rc = lin_check(d)) return rc;
+  if (d->m == 0 || d->n == 0) return DGXM_OK;
+  if (x == nullptr || w == nullptr || out == nullptr) return fail(DGXM_ERR_INVALID, "NULL operand or output");
+  if ((gate != nullptr) != (d->gate_form != DGXM_MOD_NONE)) return fail(DGXM_ERR_INVALID, "gate and gate_form do not match");
+  if ((residual != nullptr && d->m > 1 && d->residual_stride < d->n && d->residual_stride != 0) ||
+      (pre != nullptr && d->m > 1 && d->pre_stride < d->n))
+    return fail(DGXM_ERR_INVALID, "a row stride is below its row");
+  if (int rc = lin_aligned(x, d->dtype, "x")) return rc;
+  if (int rc = lin_aligned(w, d->dtype, "w")) return rc;
+  if (int rc = lin_aligned(bias, d->bias_dtype, "bias")) return rc;
+  if (int rc = lin_aligned(gate, d->gate_dtype, "gate")) return rc;
+  if (int rc = lin_aligned(residual, d->out_dtype, "residual")) return rc;
+  if (int rc = lin_aligned(out, d->out_dtype, "out")) return rc;
+  if (int rc = lin_aligned(pre, d->dtype, "pre")) return rc;
+  const int64_t need = dgxm_linear_workspace(d, x, w);
+  if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
+    return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes, (long long)need);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* work = static_cast<char*>(workspace);
+  int64_t ldx = d->m > 1 ? d->x_stride : lin_pitch(d->k), ldw = d->n > 1 ? d->w_stride : lin_pitch(d->k);
+  if (d->m == 1 && !lin_on_words(x, d->x_stride)) ldx = d->x_stride;
+  if (d->n == 1 && !lin_on_words(w, d->w_stride)) ldw = d->w_stride;
+  if (int rc = lin_pack(&x, &ldx, d->m, d->k, &work, st)) return rc;
+  if (int rc = lin_pack(&w, &ldw, d->n, d->k, &work, st)) return rc;
+  LinearParams p;
+  memset(&p, 0, sizeof(p));
+  p.bias = bias;
+  p.gate = gate;
+  p.residual = residual;
+  p.out = out;
+  p.pre = pre;
+  p.ld_out = d->m > 1 ? d->out_stride : lin_pitch(d->n);  // (of one row unused)
+  p.ld_res = d->m > 1 ? d->residual_stride : lin_pitch(d->n);
+  p.ld_pre = d->m > 1 ? d->pre_stride : lin_pitch(d->n);
+  lin_gate_strides(d, &p.gate_sample, &p.gate_row);
+  p.out_dtype = d->out_dtype;
+  p.bias_dtype = d->bias_dtype;
+  p.gate_dtype = d->gate_dtype;
+  p.pre_dtype = d->dtype;
+  p.act = d->activation;
+  p.sample_rows = static_cast<int>(d->gate_form != DGXM_MOD_NONE ? d->sample_rows : d->m);
+  p.f16 = d->dtype == DGXM_DTYPE_F16;
+  return lin_product(p, {x, d->m, ldx, false}, {w, d->n, ldw, false}, d->k, st);
+}
+
+namespace dgxm {
+
+// Where the gradient's intermediates lie in the workspace.
+struct LinBackPlan {
+  bool dz;      // dz is not dout itself
+  bool sums;
+  int64_t runs, sample_runs, sample_rows, dz_bytes, part_bytes, x_bytes, w_bytes, dout_bytes;
+  int64_t total() const { return dz_bytes + part_bytes + x_bytes + w_bytes + dout_bytes; }
+};
+
+static LinBackPlan lin_back_plan(const dgxm_linear_desc* d, const dgxm_linear_grads* g, const void* dout, const void* x,
+                                 const void* w) {
+  LinBackPlan b;
+  memset(&b, 0, sizeof(b));
+  const bool products = g->x != nullptr || g->w != nullptr;
+  b.dz = products && (d->activation != DGXM_ACT_NONE || d->gate_form != DGXM_MOD_NONE || d->out_dtype != d->dtype);
+  b.sums = g->bias != nullptr || (g->gate != nullptr && d->gate_form != DGXM_MOD_TOKEN);
+  b.sample_rows = d->gate_form != DGXM_MOD_NONE ? d->sample_rows : d->m;
+  b.sample_runs = (b.sample_rows + kDzRows - 1) / kDzRows;
+  b.runs = b.sample_rows > 0 ? d->m / b.sample_rows * b.sample_runs : 0;
+  if (b.dz) b.dz_bytes = (d->m * lin_pitch(d->n) * 2 + 255) / 256 * 256;
+  else if (products) b.dout_bytes = lin_packed_bytes(dout, d->out_stride, d->m, d->n);
+  if (b.sums) b.part_bytes = (b.runs * 2 * d->n * 4 + 255) / 256 * 256;
+  if (g->w != nullptr) b.x_bytes = lin_packed_bytes(x, d->x_stride, d->m, d->k);
+  if (g->x != nullptr) b.w_bytes = lin_packed_bytes(w, d->w_stride, d->n, d->k);
+  return b;
+}
+
+}  // namespace dgxm
+
+extern "C" int64_t dgxm_linear_backward_workspace(const dgxm_linear_desc* d, const dgxm_linear_grads* g, const void* dout,
+                                                  const void* x, const void* w) {
+  using namespace dgxm;
+  if (lin_check(d)) return -1;
+  if (g == nullptr) return fail(DGXM_ERR_INVALID, "NULL gradients"), -1;
+  if (d->m == 0 || d->n == 0) return 0;
+  return lin_back_plan(d, g, dout, x, w).total();
+}
+
+extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear_grads* g, const void* dout, const void* x,
+                                    const void* w, const void* gate, const void* pre, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  using namespace dgxm;
+  if (int rc = lin_check(d)) return rc;
+  if (g == nullptr) return fail(DGXM_ERR_INVALID, "NULL gradients");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d->m == 0 || d->n == 0) {  // sums of nothing
+    if (g->x != nullptr && d->m > 0) DGXM_CUDA_TRY(cudaMemsetAsync(g->x, 0, d->m * d->k * 2, st));
+    if (g->w != nullptr && d->n > 0) DGXM_CUDA_TRY(cudaMemsetAsync(g->w, 0, d->n * d->k * 2, st));
+    if (g->bias != nullptr && d->n > 0) DGXM_CUDA_TRY(cudaMemsetAsync(g->bias, 0, d->n * lin_elt(d->bias_dtype), st));
+    if (g->gate != nullptr && d->n > 0 && d->gate_form == DGXM_MOD_SHARED)
+      DGXM_CUDA_TRY(cudaMemsetAsync(g->gate, 0, d->n * lin_elt(d->gate_dtype), st));
+    return DGXM_OK;
+  }
+  if (dout == nullptr) return fail(DGXM_ERR_INVALID, "NULL upstream gradient");
+  if ((g->x != nullptr && w == nullptr) || (g->w != nullptr && x == nullptr)) return fail(DGXM_ERR_INVALID, "NULL operand");
+  if ((gate != nullptr) != (d->gate_form != DGXM_MOD_NONE) || (gate == nullptr && g->gate != nullptr))
+    return fail(DGXM_ERR_INVALID, "gate, gate_form and the gate's gradient do not match");
+  if (pre == nullptr && (d->activation != DGXM_ACT_NONE || g->gate != nullptr))
+    return fail(DGXM_ERR_INVALID, "an activation's or a gate's gradient without pre");
+  if (pre != nullptr && d->m > 1 && d->pre_stride < d->n) return fail(DGXM_ERR_INVALID, "a row stride is below its row");
+  for (const void* q : {x, w, pre, static_cast<const void*>(g->x), static_cast<const void*>(g->w)})
+    if (int rc = lin_aligned(q, d->dtype, "a tensor")) return rc;
+  if (int rc = lin_aligned(dout, d->out_dtype, "dout")) return rc;
+  if (int rc = lin_aligned(g->bias, d->bias_dtype, "the bias' gradient")) return rc;
+  for (const void* q : {gate, static_cast<const void*>(g->gate)})
+    if (int rc = lin_aligned(q, d->gate_dtype, "the gate or its gradient")) return rc;
+  const LinBackPlan plan = lin_back_plan(d, g, dout, x, w);
+  if (plan.total() > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < plan.total()))
+    return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes, (long long)plan.total());
+  char* work = static_cast<char*>(workspace);
+  const void* dz = dout;
+  int64_t ld_dz = d->out_stride;
+  const bool tok = d->gate_form == DGXM_MOD_TOKEN;
+  if (plan.dz || plan.sums || (g->gate != nullptr && tok)) {
+    LinDzParams q;
+    memset(&q, 0, sizeof(q));
+    q.dout = dout;
+    q.pre = pre;
+    q.gate = gate;
+    if (plan.dz) {
+      q.dz = work;
+      q.ld_dz = lin_pitch(d->n);
+      work += plan.dz_bytes;
+    }
+    if (plan.sums) {
+      q.partial = reinterpret_cast<float*>(work);
+      work += plan.part_bytes;
+    }
+    q.g_gate = tok ? g->gate : nullptr;
+    q.ld_dout = d->out_stride;
+    q.ld_pre = d->pre_stride;
+    lin_gate_strides(d, &q.gate_sample, &q.gate_row);
+    q.runs = plan.runs;
+    q.n = static_cast<int>(d->n);
+    q.sample_rows = static_cast<int>(plan.sample_rows);
+    q.sample_runs = static_cast<int>(plan.sample_runs);
+    q.act = d->activation;
+    q.sum_bias = g->bias != nullptr;
+    q.sum_gate = g->gate != nullptr && !tok;
+    q.dtype = d->dtype;
+    q.dout_dtype = d->out_dtype;
+    q.gate_dtype = d->gate_dtype;
+    q.vec = reinterpret_cast<uintptr_t>(dout) % 16 == 0 && d->out_stride * lin_elt(d->out_dtype) % 16 == 0 &&
+            (pre == nullptr || (reinterpret_cast<uintptr_t>(pre) % 16 == 0 && d->pre_stride % 8 == 0));
+    const unsigned across = static_cast<unsigned>((lin_pitch(d->n) / 8 + 127) / 128);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(plan.runs, 1 << 20)), across);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_dz_kernel, q));
+    if (plan.sums) {
+      LinSumParams s;
+      s.partial = q.partial;
+      s.g_bias = g->bias;
+      s.g_gate = tok ? nullptr : g->gate;
+      s.samples = d->m / plan.sample_rows;
+      s.n = q.n;
+      s.sample_runs = q.sample_runs;
+      s.bias_dtype = d->bias_dtype;
+      s.gate_dtype = d->gate_dtype;
+      s.gate_form = d->gate_form;
+      DGXM_CUDA_TRY(launch_overlapped(linear_sum_kernel, (q.n + 31) / 32, 1024, 0, st, s));
+    }
+    if (plan.dz) {
+      dz = q.dz;
+      ld_dz = q.ld_dz;
+    }
+  }
+  if (g->x == nullptr && g->w == nullptr) return DGXM_OK;
+  if (!plan.dz)
+    if (int rc = lin_pack(&dz, &ld_dz, d->m, d->n, &work, st)) return rc;
+  LinearParams p;
+  memset(&p, 0, sizeof(p));
+  p.out_dtype = p.bias_dtype = p.gate_dtype = p.pre_dtype = d->dtype;
+  p.f16 = d->dtype == DGXM_DTYPE_F16;
+  p.ld_out = d->k;
+  if (g->x != nullptr) {
+    int64_t ldw = d->w_stride;
+    if (int rc = lin_pack(&w, &ldw, d->n, d->k, &work, st)) return rc;
+    p.out = g->x;
+    p.sample_rows = static_cast<int>(d->m);
+    if (int rc = lin_product(p, {dz, d->m, ld_dz, false}, {w, d->k, ldw, true}, d->n, st)) return rc;
+  }
+  if (g->w != nullptr) {
+    int64_t ldx = d->x_stride;
+    if (int rc = lin_pack(&x, &ldx, d->m, d->k, &work, st)) return rc;
+    p.out = g->w;
+    p.sample_rows = static_cast<int>(d->n);
+    if (int rc = lin_product(p, {dz, d->n, ld_dz, true}, {x, d->k, ldx, true}, d->m, st)) return rc;
+  }
+  return DGXM_OK;
+}

@@ -827,6 +827,68 @@ int dgxm_block_norm_backward(const dgxm_block_norm_desc* desc, const dgxm_block_
                              const void* norm_w, const void* norm_b, const void* branch_w,
                              void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------ 16-bit Linear */
+/*
+ *   pre = x w^T + bias,   out = residual + gate * act(pre)
+ * of x (m, k) and w (n, k) in dtype (BF16 or F16), fp32 accumulation and
+ * epilogue, one rounding of each output.  Rows may have any stride (elements);
+ * columns are contiguous.  bias: n values of bias_dtype; gate: of gate_dtype,
+ * n values for all rows (SHARED), for each run of sample_rows rows (SAMPLE;
+ * gate_stride[0]) or for each row (TOKEN; gate_stride: between samples and
+ * between rows of a sample); residual: (m, n) of out_dtype, which may be out
+ * itself; pre (dtype): written where not NULL, for the gradient.  Each may be
+ * NULL.  out_dtype, bias_dtype and gate_dtype are dtype or F32.  `workspace`
+ * (16-byte aligned) holds dgxm_linear_workspace() bytes: copies of operands
+ * whose rows are not on 16 bytes.  k and n up to 2^24.  The same call gives
+ * the same bits.
+ *
+ * Serves the 16-bit Linears of the blocks around the attention seam (inside
+ * the forwards of adapters/flux_family.py:108-265, adapters/krea2.py:130-246
+ * and adapters/wan_family.py:64-162) with what follows them.
+ */
+#define DGXM_ACT_NONE 0
+#define DGXM_ACT_SILU 1
+#define DGXM_ACT_GELU 2       /* x Phi(x) */
+#define DGXM_ACT_GELU_TANH 3  /* its tanh form */
+
+typedef struct dgxm_linear_desc {
+  int64_t m, n, k;
+  int64_t x_stride, w_stride;
+  int64_t out_stride;      /* backward: of dout */
+  int64_t residual_stride, pre_stride;
+  int64_t gate_stride[2];
+  int64_t sample_rows;
+  int32_t dtype;
+  int32_t out_dtype;       /* of out and residual; backward: of dout */
+  int32_t bias_dtype, gate_dtype;
+  int32_t activation;
+  int32_t gate_form;       /* DGXM_MOD_* */
+} dgxm_linear_desc;
+
+int64_t dgxm_linear_workspace(const dgxm_linear_desc* desc, const void* x, const void* w);
+int dgxm_linear(const dgxm_linear_desc* desc, const void* x, const void* w, const void* bias,
+                const void* gate, const void* residual, void* out, void* pre, void* workspace,
+                int64_t workspace_bytes, void* stream);
+
+/*
+ * Its gradients; NULL ones are not computed.  x (m, k) and w (n, k) in dtype,
+ * bias in bias_dtype, gate in gate_dtype and by its form (n), (m / sample_rows,
+ * n) or (m, n), all contiguous.  With dz = dout * gate * act'(pre):
+ *   x: dz w,   w: dz^T x,   bias: sum dz,   gate: sum dout * act(pre)
+ * The residual's gradient is dout.  pre is the forward's, or NULL without an
+ * activation and a gradient of the gate.  dz is rounded to dtype before the
+ * products, not in the sums, which are fp32 in a fixed order.
+ */
+typedef struct dgxm_linear_grads {
+  void *x, *w, *bias, *gate;
+} dgxm_linear_grads;
+
+int64_t dgxm_linear_backward_workspace(const dgxm_linear_desc* desc, const dgxm_linear_grads* grads,
+                                       const void* dout, const void* x, const void* w);
+int dgxm_linear_backward(const dgxm_linear_desc* desc, const dgxm_linear_grads* grads,
+                         const void* dout, const void* x, const void* w, const void* gate,
+                         const void* pre, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
