@@ -189,13 +189,95 @@ __device__ __forceinline__ uint4 fp4_bytes_from(uint4 a, uint4 b, uint32_t n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Whether a chunk of kCols columns goes out as one bulk store.
+template <int kCols, int ELT, typename P>
+__device__ __forceinline__ bool fp4_by_bulk(const P& p, int q0) {
+  // a row that ends inside 16 bytes would have the rest of them written too
+  return kCols == 128 / ELT && p.vec && (q0 + kCols <= p.q_rows || p.q_rows % (16 / ELT) == 0);
+}
+
+// Store a warp's 32 rows x kCols columns from staging rows of 128 bytes,
+// 16-byte piece i of row r at piece i ^ (r & 7): the 128-byte swizzle, so that
+// a whole chunk goes out as one bulk store (rows on 16 bytes), which leaves
+// the warp to its arithmetic (9450 x 5120 x 256: 47 us with stores of the
+// lanes, 23 us), or, otherwise, neighbouring lanes store neighbouring words or
+// elements.  ELT: bytes of an output element.
+template <int kCols, int ELT, typename P>
+__device__ __forceinline__ void fp4_flush_rows(const P& p, uint8_t* stage, int pr0, int q0, int lane) {
+  constexpr int kEach = 16 / ELT;  // elements of a piece
+  constexpr int kPieces = kCols / kEach;
+  using Elt = typename std::conditional<ELT == 4, uint32_t, uint16_t>::type;
+  const bool bulk = fp4_by_bulk<kCols, ELT>(p, q0);
+  if (bulk) {
+    tma_store_fence();
+    __syncwarp();
+    if (lane == 0) {
+      if (pr0 < p.p_rows) tma_store_4d(&p.tmap_out, smem_u32(stage), q0, 0, pr0, 0);
+      tma_store_commit();
+    }
+    return;
+  }
+  __syncwarp();
+  if (p.vec && q0 + kCols <= p.q_rows) {
+    char* out = static_cast<char*>(p.out);
+    const int i = lane % kPieces;
+#pragma unroll
+    for (int r = lane / kPieces; r < 32; r += 32 / kPieces)
+      if (pr0 + r < p.p_rows)
+        *reinterpret_cast<uint4*>(out + ((pr0 + r) * p.ld_out + q0 + i * kEach) * ELT) =
+            *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
+  } else if (kPieces >= 4) {
+    // Rows off 16 bytes, or ending here: whole aligned words, each from two
+    // neighbouring pieces, and by elements the bytes before the first word
+    // and behind the last (9450 x 5121 x 256: 102 us by elements alone, 55;
+    // 100000 x 100 x 512, half a chunk at the end: 31, 23).
+    auto store = [&](auto whole, int bytes) {
+      constexpr bool kWhole = decltype(whole)::value;
+      const int i = lane % kPieces;
+#pragma unroll 4
+      for (int r = lane / kPieces; r < min(32, p.p_rows - pr0); r += 32 / kPieces) {
+        auto piece = [&](int k) { return stage + r * 128 + ((k ^ (r & 7)) << 4); };
+        char* row = static_cast<char*>(p.out) + ((pr0 + r) * p.ld_out + q0) * ELT;
+        const int head = static_cast<int>(-reinterpret_cast<uintptr_t>(row) & 15u);
+        const int words = kWhole ? kPieces - (head > 0) : max(bytes - head, 0) / 16;
+        if (i < words)
+          *reinterpret_cast<uint4*>(row + head + 16 * i) =
+              fp4_bytes_from(*reinterpret_cast<const uint4*>(piece(i)),
+                             *reinterpret_cast<const uint4*>(piece(min(i + 1, kPieces - 1))), head);
+        auto element = [&](int at) {
+          *reinterpret_cast<Elt*>(row + at) = *reinterpret_cast<const Elt*>(piece(at / 16) + at % 16);
+        };
+#pragma unroll
+        for (int e = i; e < kEach; e += kPieces) {
+          if (kWhole) {  // the bytes before and behind are none, or as many as a piece has
+            if (head > 0) element(e * ELT < head ? e * ELT : 16 * (kPieces - 1) + e * ELT);
+          } else {
+            if (e * ELT < min(head, bytes)) element(e * ELT);
+            if (head + 16 * words + e * ELT < bytes) element(head + 16 * words + e * ELT);
+          }
+        }
+      }
+    };
+    if (q0 + kCols <= p.q_rows) store(std::true_type{}, kCols * ELT);
+    else store(std::false_type{}, (p.q_rows - q0) * ELT);
+  } else {
+    const int cols = min(kCols, p.q_rows - q0), rows = min(32, p.p_rows - pr0);
+    Elt* to = reinterpret_cast<Elt*>(p.out) + pr0 * p.ld_out + q0;
+#pragma unroll
+    for (int e = lane; e < kCols; e += 32) {
+      if (e >= cols) break;
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r)
+        if (r < rows)
+          to[r * p.ld_out + e] =
+              *reinterpret_cast<const Elt*>(stage + r * 128 + (((e / kEach) ^ (r & 7)) << 4) + (e % kEach) * ELT);
+    }
+  }
+  __syncwarp();
+}
+
 // A warp's 32 rows x NC columns of finished values (a row a lane) from row
-// pr0 and column q0 of the output.  They pass through staging rows of 128
-// bytes, 16-byte piece i of row r at piece i ^ (r & 7): the 128-byte swizzle,
-// so that a whole chunk goes out as one bulk store (rows on 16 bytes), which
-// leaves the warp to its arithmetic (9450 x 5120 x 256: 47 us with stores of
-// the lanes, 23 us), or, otherwise, neighbouring lanes store neighbouring
-// words or elements.  ELT: bytes of an output element.
+// pr0 and column q0 of the output.
 template <int NC, int ELT, typename P>
 __device__ __forceinline__ void fp4_store_rows(const P& p, uint8_t* stage, const float (&v)[NC], int pr0,
                                                int q0, int lane) {
@@ -204,86 +286,17 @@ __device__ __forceinline__ void fp4_store_rows(const P& p, uint8_t* stage, const
   constexpr int kCols = NC % kMost == 0 ? kMost : NC % (kMost / 2) == 0 ? kMost / 2 : NC;  // columns staged at one time
   static_assert(kCols <= kMost && NC % kCols == 0, "whole chunks");
   constexpr int kPieces = kCols / kEach;
-  using Elt = typename std::conditional<ELT == 4, uint32_t, uint16_t>::type;
 #pragma unroll
   for (int c0 = 0; c0 < NC; c0 += kCols) {
     if (q0 + c0 >= p.q_rows) return;  // uniform over the warp
-    const bool tma = kCols == kMost && p.vec;
-    // a row that ends inside 16 bytes would have the rest of them written too
-    const bool bulk = tma && (q0 + c0 + kCols <= p.q_rows || p.q_rows % kEach == 0);
-    if (tma) {
+    if (kCols == kMost && p.vec) {
       if (lane == 0) tma_store_wait_read();  // the last chunk has left the staging rows
       __syncwarp();
     }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
       *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = fp4_piece<ELT>(p, v + c0 + i * kEach);
-    if (bulk) {
-      tma_store_fence();
-      __syncwarp();
-      if (lane == 0) {
-        if (pr0 < p.p_rows) tma_store_4d(&p.tmap_out, smem_u32(stage), q0 + c0, 0, pr0, 0);
-        tma_store_commit();
-      }
-      continue;
-    }
-    __syncwarp();
-    if (p.vec && q0 + c0 + kCols <= p.q_rows) {
-      char* out = static_cast<char*>(p.out);
-      const int i = lane % kPieces;
-#pragma unroll
-      for (int r = lane / kPieces; r < 32; r += 32 / kPieces)
-        if (pr0 + r < p.p_rows)
-          *reinterpret_cast<uint4*>(out + ((pr0 + r) * p.ld_out + q0 + c0 + i * kEach) * ELT) =
-              *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
-    } else if (kPieces >= 4) {
-      // Rows off 16 bytes, or ending here: whole aligned words, each from two
-      // neighbouring pieces, and by elements the bytes before the first word
-      // and behind the last (9450 x 5121 x 256: 102 us by elements alone, 55;
-      // 100000 x 100 x 512, half a chunk at the end: 31, 23).
-      auto store = [&](auto whole, int bytes) {
-        constexpr bool kWhole = decltype(whole)::value;
-        const int i = lane % kPieces;
-#pragma unroll 4
-        for (int r = lane / kPieces; r < min(32, p.p_rows - pr0); r += 32 / kPieces) {
-          auto piece = [&](int k) { return stage + r * 128 + ((k ^ (r & 7)) << 4); };
-          char* row = static_cast<char*>(p.out) + ((pr0 + r) * p.ld_out + q0 + c0) * ELT;
-          const int head = static_cast<int>(-reinterpret_cast<uintptr_t>(row) & 15u);
-          const int words = kWhole ? kPieces - (head > 0) : max(bytes - head, 0) / 16;
-          if (i < words)
-            *reinterpret_cast<uint4*>(row + head + 16 * i) =
-                fp4_bytes_from(*reinterpret_cast<const uint4*>(piece(i)),
-                               *reinterpret_cast<const uint4*>(piece(min(i + 1, kPieces - 1))), head);
-          auto element = [&](int at) {
-            *reinterpret_cast<Elt*>(row + at) = *reinterpret_cast<const Elt*>(piece(at / 16) + at % 16);
-          };
-#pragma unroll
-          for (int e = i; e < kEach; e += kPieces) {
-            if (kWhole) {  // the bytes before and behind are none, or as many as a piece has
-              if (head > 0) element(e * ELT < head ? e * ELT : 16 * (kPieces - 1) + e * ELT);
-            } else {
-              if (e * ELT < min(head, bytes)) element(e * ELT);
-              if (head + 16 * words + e * ELT < bytes) element(head + 16 * words + e * ELT);
-            }
-          }
-        }
-      };
-      if (q0 + c0 + kCols <= p.q_rows) store(std::true_type{}, kCols * ELT);
-      else store(std::false_type{}, (p.q_rows - q0 - c0) * ELT);
-    } else {
-      const int cols = min(kCols, p.q_rows - q0 - c0), rows = min(32, p.p_rows - pr0);
-      Elt* to = reinterpret_cast<Elt*>(p.out) + pr0 * p.ld_out + q0 + c0;
-#pragma unroll
-      for (int e = lane; e < kCols; e += 32) {
-        if (e >= cols) break;
-#pragma unroll 8
-        for (int r = 0; r < 32; ++r)
-          if (r < rows)
-            to[r * p.ld_out + e] =
-                *reinterpret_cast<const Elt*>(stage + r * 128 + (((e / kEach) ^ (r & 7)) << 4) + (e % kEach) * ELT);
-      }
-    }
-    __syncwarp();
+    fp4_flush_rows<kCols, ELT>(p, stage, pr0, q0 + c0, lane);
   }
 }
 

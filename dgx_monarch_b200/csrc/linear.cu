@@ -28,14 +28,16 @@ struct __align__(64) LinearParams {
   CUtensorMap tmap_a, tmap_b;  // K-major: dims (k, 1, rows), boxes (64, 1, 128 ..); MN-major: dims (rows, 1, k), boxes (64, 1, 64)
   CUtensorMap tmap_out;        // where `vec`: dims (q_rows, 1, p_rows), boxes of 128 bytes x 32 rows
   CUtensorMap tmap_res;        // where `res_bulk`: the same of the residual
+  CUtensorMap tmap_pre;        // where `pre_vec`: the same of pre
   const void *bias, *gate, *residual;
   void *out, *pre;
   int64_t ld_out, ld_res, ld_pre;         // elements
   int64_t gate_sample, gate_row;          // elements between samples, rows
   int p_rows, q_rows, k_tiles, k;
   int p_tiles, q_tiles, split;
+  int step, tn;                           // rows of A a tile takes, 128 (256) at the most, and rows of B
   int q_is_tokens;                        // the rows of A are output columns: the tile is the output transposed
-  int out_dtype, bias_dtype, gate_dtype, pre_dtype, vec, res_bulk;
+  int out_dtype, bias_dtype, gate_dtype, pre_dtype, vec, res_bulk, pre_vec;
   int act, sample_rows, f16;
 };
 
@@ -45,14 +47,15 @@ struct LinTile {
   static constexpr int kQLoad = PAIR ? TN / 2 : TN;  // rows of B this CTA loads
   static constexpr int kABytes = 128 * 128, kBBytes = kQLoad * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr bool kSplits = !PAIR;
-  static constexpr int kPartBytes = kSplits ? (128 + 10) * TN * 4 : 0;  // as in Fp4Tile
-  static constexpr int kStage2 = 2 * kGemmStageRows;  // two staging buffers an epilogue warp
-  static constexpr int kStagingBytes = kPartBytes > 8 * kStage2 ? kPartBytes : 8 * kStage2;
+  static constexpr bool kSplits = TN <= 64;           // transposed tiles, stored by the lanes
+  // Partial sums as in Fp4Tile, or a staging buffer for each epilogue warp.  (A
+  // sixth stage of the ring is worth more than a second buffer: the loads'
+  // latency bounds a stage.)
+  static constexpr int kStagingBytes = kSplits ? (128 + 10) * TN * 4 : 8 * kGemmStageRows;
   static constexpr int kStages = (kGemmSmemMax - 1024 - kGemmCtrlBytes - kStagingBytes) / kStageBytes;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kGemmCtrlBytes;
   static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + 2,
-                       kDrain = kAccEmpty + 2, kRes = kDrain + 1, kBars = kRes + 16;
+                       kDrain = kAccEmpty + 2, kRes = kDrain + 1, kBars = kRes + 8;
   static_assert(kBars * 8 + 16 <= kGemmCtrlBytes, "control block");
   static_assert(kStageBytes % 1024 == 0, "swizzle atoms stay aligned");
   static constexpr int kTmem = TN < 32 ? 64 : 2 * TN;  // columns: a power of two, two accumulators
@@ -108,6 +111,46 @@ __device__ __forceinline__ float lin_value(const void* base, int dtype, int64_t 
   return static_cast<const float*>(base)[at];
 }
 
+__device__ __forceinline__ void lin_widen8(uint4 w, int dtype, float (&v)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float2 f;
+    if (dtype == DGXM_DTYPE_BF16) f = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xFFFF0000u));
+    else f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+    v[2 * k] = f.x;
+    v[2 * k + 1] = f.y;
+  }
+}
+
+// The first `count` of N neighbouring values.
+template <int N, typename Use>
+__device__ __forceinline__ void lin_each(const void* base, int dtype, int64_t at, int count, Use&& use) {
+  if (dtype == DGXM_DTYPE_F32) {
+    const float* from = static_cast<const float*>(base) + at;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < count) use(c, from[c]);
+  } else if (const uint16_t* from = static_cast<const uint16_t*>(base) + at;
+             count >= N && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i) {
+      float f[8];
+      lin_widen8(reinterpret_cast<const uint4*>(from)[i], dtype, f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) use(8 * i + k, f[k]);
+    }
+  } else {
+    const bool bf16 = dtype == DGXM_DTYPE_BF16;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < count) {
+        const uint16_t u = from[c];
+        use(c, bf16 ? __uint_as_float(static_cast<uint32_t>(u) << 16) : __half2float(*reinterpret_cast<const __half*>(&u)));
+      }
+  }
+}
+
 __device__ __forceinline__ void lin_put(void* base, int dtype, int64_t at, float v) {
   if (dtype == DGXM_DTYPE_BF16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(v);
   else if (dtype == DGXM_DTYPE_F16) static_cast<__half*>(base)[at] = __float2half_rn(v);
@@ -146,123 +189,242 @@ __device__ __forceinline__ uint64_t lin_desc(uint32_t addr) {
 template <bool MN>
 constexpr uint32_t kLinStep = MN ? 2048 / 16 : 32 / 16;
 
-// The epilogue of a warp's 32 rows x kCols columns of a tile from row pr0 and
-// column q0, rows being tokens: chunks of 128 output bytes, or all of them.
-template <int TN, bool PAIR, int ELT>
-__device__ __forceinline__ void lin_epilogue(const LinearParams& p, uint8_t* stage, uint32_t res_bar, int& res_phase,
-                                             uint32_t tmem, uint32_t acc_empty, int pr0, int q0, int lane,
-                                             const float (&bias)[(TN / 2 + 31) / 32]) {
-  constexpr int kCols = TN / 2, kMost = 128 / ELT, CC = kCols < kMost ? kCols : kMost, kChunks = kCols / CC;
-  const int m = pr0 + lane;
-  const int sample = min(m, p.p_rows - 1) / p.sample_rows, in_sample = m - sample * p.sample_rows;
-  const char* const gate = static_cast<const char*>(p.gate);
-  const bool one = p.gate_row == 0 && __all_sync(0xffffffffu, sample == __shfl_sync(0xffffffffu, sample, 0));
-  float gates[(kCols + 31) / 32];
-  if (gate != nullptr && one) {
+// What fp4_store_rows is told of `pre`.
+struct LinPreOut {
+  const CUtensorMap& tmap_out;
+  void* out;
+  int64_t ld_out;
+  int p_rows, q_rows, out_dtype, vec;
+};
+
+// The residual of a warp's 32 rows x 128 bytes from row pr0 and column q0 into
+// its staging rows as a bulk load leaves them, where its rows are off 16
+// bytes: neighbouring lanes load neighbouring values.
+template <int ELT>
+__device__ __forceinline__ void lin_stage_residual(const LinearParams& p, uint8_t* buffer, int pr0, int q0, int lane) {
+  using Elt = typename std::conditional<ELT == 4, uint32_t, uint16_t>::type;
+  constexpr int kMost = 128 / ELT, kEach = 16 / ELT;
+  const int rows = min(32, p.p_rows - pr0);
+  const Elt* from = static_cast<const Elt*>(p.residual) + pr0 * p.ld_res + q0;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r)
 #pragma unroll
-    for (int i = 0; i < (kCols + 31) / 32; ++i) {
-      const int n = q0 + 32 * i + lane;
-      gates[i] = n < p.q_rows ? lin_value(gate, p.gate_dtype, sample * p.gate_sample + n) : 0.f;
-    }
+    for (int c = lane; c < kMost; c += 32)
+      if (q0 + c < p.q_rows)
+        *reinterpret_cast<Elt*>(buffer + r * 128 + (((c / kEach) ^ (r & 7)) << 4) + (c % kEach) * ELT) = from[r * p.ld_res + c];
+  __syncwarp();
+}
+
+// Column chunks of 128 output bytes of a tile, the even ones for the warps of
+// half 0, the odd ones for half 1; a warp's own are numbered here.
+template <int TN, int ELT>
+struct LinChunks {
+  static constexpr int kCols = 128 / ELT, kOwn = TN / kCols / 2 > 0 ? TN / kCols / 2 : 1;
+  static __device__ __forceinline__ int column(int half, int i) { return (2 * i + half) * kCols; }
+};
+
+template <bool PAIR>
+__device__ __forceinline__ void lin_release(uint32_t acc_empty, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) {
+    if constexpr (PAIR) mbar_arrive_cluster_relaxed(acc_empty);
+    else mbar_arrive(acc_empty);
   }
+}
+
+// The epilogue of a warp's 32 rows of a tile from row pr0, rows being tokens:
+// bias and activation alone.  What else there can be stands apart
+// (lin_epilogue_full, in kernels of its own): with those ways between them, the few instructions
+// here miss the instruction cache at every jump (2000 cycles a chunk of 64
+// columns instead of 300).
+template <int TN, bool PAIR, int ELT, int ACT>
+__device__ __forceinline__ void lin_epilogue(const LinearParams& p, uint8_t* stage, uint32_t tmem,
+                                             uint32_t acc_empty, int pr0, int q_tile, int half, int lane,
+                                             const float (&bias)[LinChunks<TN, ELT>::kOwn * LinChunks<TN, ELT>::kCols / 32]) {
+  using K = LinChunks<TN, ELT>;
+  constexpr int CC = K::kCols;
 #pragma unroll
-  for (int ch = 0; ch < kChunks; ++ch) {
-    const int c0 = ch * CC;
+  for (int ch = 0; ch < K::kOwn; ++ch) {
+    const int c0 = K::column(half, ch), q0 = q_tile + c0;
+    const bool mine = c0 < p.tn && q0 < p.q_rows;  // uniform over the warp
     uint32_t r[CC / 8][8];
+    if (mine) {
 #pragma unroll
-    for (int c = 0; c < CC / 8; ++c) tmem_ld8(tmem + c0 + 8 * c, r[c]);
-    tmem_wait_ld();
+      for (int c = 0; c < CC / 8; ++c) tmem_ld8(tmem + c0 + 8 * c, r[c]);
+      tmem_wait_ld();
 #pragma unroll
-    for (int c = 0; c < CC / 8; ++c) reg_fence8(r[c]);
-    if (ch == kChunks - 1) {  // the accumulator is in registers: the next tile's MMAs may start
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster_relaxed(acc_empty);
-        else mbar_arrive(acc_empty);
-      }
+      for (int c = 0; c < CC / 8; ++c) reg_fence8(r[c]);
     }
-    if (q0 + c0 >= p.q_rows) continue;  // uniform over the warp; no residual is under way
+    if (ch == K::kOwn - 1) lin_release<PAIR>(acc_empty, lane);  // the accumulator is in registers
+    if (!mine) continue;
     float v[CC];
 #pragma unroll
     for (int c = 0; c < CC; ++c) v[c] = __uint_as_float(r[c / 8][c % 8]);
     if (p.bias != nullptr) {
 #pragma unroll
-      for (int c = 0; c < CC; ++c) v[c] += __shfl_sync(0xffffffffu, bias[(c0 + c) / 32], (c0 + c) % 32);
+      for (int c = 0; c < CC; ++c) v[c] += __shfl_sync(0xffffffffu, bias[(ch * CC + c) / 32], c % 32);
     }
-    if (p.pre != nullptr && m < p.p_rows) {
-      if (ELT == 2 && q0 + c0 + CC <= p.q_rows && p.ld_pre % 8 == 0 && reinterpret_cast<uintptr_t>(p.pre) % 16 == 0) {
-        uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.pre) + m * p.ld_pre + q0 + c0);
+    if (ACT != DGXM_ACT_NONE) {
 #pragma unroll
-        for (int c = 0; c < CC / 8; ++c) to[c] = fp4_piece<2>(p, v + 8 * c);
-      } else {
-        for (int c = 0; c < CC; ++c)
-          if (q0 + c0 + c < p.q_rows) lin_put(p.pre, p.pre_dtype, m * p.ld_pre + q0 + c0 + c, v[c]);
-      }
+      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], ACT);
     }
-    if (p.act == DGXM_ACT_SILU) {
+    if (lane == 0) tma_store_wait_read();  // the last chunk has left the staging rows
+    __syncwarp();
+    uint8_t* const row_out = stage + lane * 128;
 #pragma unroll
-      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], DGXM_ACT_SILU);
-    } else if (p.act == DGXM_ACT_GELU) {
-#pragma unroll
-      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], DGXM_ACT_GELU);
-    } else if (p.act == DGXM_ACT_GELU_TANH) {
-#pragma unroll
-      for (int c = 0; c < CC; ++c) v[c] = lin_act(v[c], DGXM_ACT_GELU_TANH);
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<uint4*>(row_out + ((i ^ (lane & 7)) << 4)) = fp4_piece<ELT>(p, v + i * (16 / ELT));
+    fp4_flush_rows<CC, ELT>(p, stage, pr0, q0, lane);
+  }
+}
+
+// The same with a gate, a residual or pre, sixteen columns at a time.
+template <int TN, bool PAIR, int ELT>
+__device__ __forceinline__ void lin_epilogue_full(const LinearParams& p, uint8_t* stage, uint32_t res_bar, int& res_phase,
+                                               uint32_t tmem, uint32_t acc_empty, int pr0, int q_tile, int half, int lane) {
+  using K = LinChunks<TN, ELT>;
+  constexpr int CC = K::kCols;
+  const int m = pr0 + lane;
+  const int sample = min(m, p.p_rows - 1) / p.sample_rows, in_sample = m - sample * p.sample_rows;
+  const char* const gate = static_cast<const char*>(p.gate);
+  const bool one = p.gate_row == 0 && __all_sync(0xffffffffu, sample == __shfl_sync(0xffffffffu, sample, 0));
+  const bool pre_staged = p.pre != nullptr && p.residual == nullptr;
+  const LinPreOut to_pre{p.tmap_pre, p.pre, p.ld_pre, p.p_rows, p.q_rows, p.pre_dtype, p.pre_vec};
+#pragma unroll 1
+  for (int ch = 0; ch < K::kOwn; ++ch) {
+    const int c0 = K::column(half, ch), q0 = q_tile + c0;
+    if (!(c0 < p.tn && q0 < p.q_rows)) {  // uniform over the warp
+      if (ch == K::kOwn - 1) lin_release<PAIR>(acc_empty, lane);
+      continue;
     }
-    if (gate != nullptr) {
-      if (one) {
+    float bias[2], gates[2];  // of column 32 i + lane
 #pragma unroll
-        for (int c = 0; c < CC; ++c) v[c] *= __shfl_sync(0xffffffffu, gates[(c0 + c) / 32], (c0 + c) % 32);
-      } else if (m < p.p_rows) {
-        const int64_t at = sample * p.gate_sample + in_sample * p.gate_row + q0 + c0;
-#pragma unroll 8
-        for (int c = 0; c < CC; ++c)
-          if (q0 + c0 + c < p.q_rows) v[c] *= lin_value(gate, p.gate_dtype, at + c);
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int n = q0 + 32 * i + lane;
+      const bool in = 32 * i < CC && n < p.q_rows;
+      bias[i] = p.bias != nullptr && in ? lin_value(p.bias, p.bias_dtype, n) : 0.f;
+      gates[i] = gate == nullptr ? 1.f : one && in ? lin_value(gate, p.gate_dtype, sample * p.gate_sample + n) : 0.f;
     }
-    uint8_t* const buffer = stage + (ch & 1) * kGemmStageRows;
+    uint8_t* const row_out = stage + lane * 128;
     if (p.residual != nullptr) {
-      if (CC == kMost && p.res_bulk) {
-        const int b = ch & 1;
-        if (!mbar_wait(res_bar + 8 * b, (res_phase >> b) & 1, nullptr)) report_device_error(kErrEpilogueTimeout);
-        res_phase ^= 1 << b;
+      if (p.res_bulk) {
+        if (!mbar_wait(res_bar, res_phase, nullptr)) report_device_error(kErrEpilogueTimeout);
+        res_phase ^= 1;
+      } else if (ch > 0) {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+        lin_stage_residual<ELT>(p, stage, pr0, q0, lane);
+      }
+    } else {
+      if (lane == 0) tma_store_wait_read();  // the last chunk has left the staging rows
+      __syncwarp();
+    }
+    if (pre_staged) {  // pre by itself first
+#pragma unroll 1
+      for (int i = 0; i < CC / 16; ++i) {
+        uint32_t r[2][8];
+        tmem_ld8(tmem + c0 + 16 * i, r[0]);
+        tmem_ld8(tmem + c0 + 16 * i + 8, r[1]);
+        tmem_wait_ld();
+        reg_fence8(r[0]);
+        reg_fence8(r[1]);
+        float v[16];
+        const float b = i < 2 ? bias[0] : bias[1];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(buffer + lane * 128 + ((i ^ (lane & 7)) << 4));
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        for (int k = 0; k < 16; ++k)
+          v[k] = __uint_as_float(r[k / 8][k % 8]) + __shfl_sync(0xffffffffu, b, (16 * i & 16) + k);
+        *reinterpret_cast<uint4*>(row_out + (((2 * i) ^ (lane & 7)) << 4)) = fp4_piece<2>(to_pre, v);
+        *reinterpret_cast<uint4*>(row_out + (((2 * i + 1) ^ (lane & 7)) << 4)) = fp4_piece<2>(to_pre, v + 8);
+      }
+      fp4_flush_rows<CC, 2>(to_pre, stage, pr0, q0, lane);
+      if (lane == 0) tma_store_wait_read();
+      __syncwarp();
+    }
+#pragma unroll 1
+    for (int i = 0; i < CC / 16; ++i) {
+      uint32_t r[2][8];
+      tmem_ld8(tmem + c0 + 16 * i, r[0]);
+      tmem_ld8(tmem + c0 + 16 * i + 8, r[1]);
+      tmem_wait_ld();
+      reg_fence8(r[0]);
+      reg_fence8(r[1]);
+      if (ch == K::kOwn - 1 && i == CC / 16 - 1) lin_release<PAIR>(acc_empty, lane);
+      float v[16];
+      const float b = i < 2 ? bias[0] : bias[1], g = i < 2 ? gates[0] : gates[1];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (ELT == 4) {
-              v[4 * i + k] += __uint_as_float(u[k]);
-            } else {
-              float2 f;
-              if (p.out_dtype == DGXM_DTYPE_BF16)
-                f = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xFFFF0000u));
-              else
-                f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-              v[8 * i + 2 * k] += f.x;
-              v[8 * i + 2 * k + 1] += f.y;
-            }
+      for (int k = 0; k < 16; ++k)
+        v[k] = __uint_as_float(r[k / 8][k % 8]) + __shfl_sync(0xffffffffu, b, (16 * i & 16) + k);
+      if (p.pre != nullptr && !pre_staged && m < p.p_rows) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 piece = fp4_piece<2>(to_pre, v + 8 * h);
+          const int n = q0 + 16 * i + 8 * h;
+          uint16_t* at = static_cast<uint16_t*>(p.pre) + m * p.ld_pre + n;
+          if (p.pre_vec && n + 8 <= p.q_rows) {
+            *reinterpret_cast<uint4*>(at) = piece;
+          } else {
+            const uint32_t u[4] = {piece.x, piece.y, piece.z, piece.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (n + k < p.q_rows) at[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k % 2)));
           }
         }
-        __syncwarp();
+      }
+      if (p.act == DGXM_ACT_SILU) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = lin_act(v[k], DGXM_ACT_SILU);
+      } else if (p.act == DGXM_ACT_GELU) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = lin_act(v[k], DGXM_ACT_GELU);
+      } else if (p.act == DGXM_ACT_GELU_TANH) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = lin_act(v[k], DGXM_ACT_GELU_TANH);
+      }
+      if (gate == nullptr || one) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] *= __shfl_sync(0xffffffffu, g, (16 * i & 16) + k);
       } else if (m < p.p_rows) {
-#pragma unroll 8
-        for (int c = 0; c < CC; ++c)
-          if (q0 + c0 + c < p.q_rows) v[c] += lin_value(p.residual, p.out_dtype, m * p.ld_res + q0 + c0 + c);
+        lin_each<16>(gate, p.gate_dtype, sample * p.gate_sample + in_sample * p.gate_row + q0 + 16 * i,
+                     p.q_rows - q0 - 16 * i, [&](int k, float f) { v[k] *= f; });
+      }
+#pragma unroll
+      for (int j = 0; j < ELT; ++j) {
+        constexpr int kEach = 16 / ELT;
+        uint4* const at = reinterpret_cast<uint4*>(row_out + (((i * ELT + j) ^ (lane & 7)) << 4));
+        if (p.residual != nullptr) {
+          const uint4 w = *at;
+          if constexpr (ELT == 4) {
+            v[4 * j] += __uint_as_float(w.x);
+            v[4 * j + 1] += __uint_as_float(w.y);
+            v[4 * j + 2] += __uint_as_float(w.z);
+            v[4 * j + 3] += __uint_as_float(w.w);
+          } else {
+            float f[8];
+            lin_widen8(w, p.out_dtype, f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[8 * j + k] += f[k];
+          }
+        }
+        *at = fp4_piece<ELT>(p, v + kEach * j);
       }
     }
-    fp4_store_rows<CC, ELT>(p, buffer, v, pr0, q0 + c0, lane);
-    if (CC == kMost && p.res_bulk && ch + 2 < kChunks && q0 + c0 + 2 * CC < p.q_rows && lane == 0) {
+    fp4_flush_rows<CC, ELT>(p, stage, pr0, q0, lane);
+    const int next = K::column(half, ch + 1);
+    if (p.res_bulk && ch + 1 < K::kOwn && next < p.tn && q_tile + next < p.q_rows && lane == 0) {
       tma_store_wait_read();
-      mbar_expect_tx(res_bar + 8 * (ch & 1), kGemmStageRows);
-      tma_load_4d(smem_u32(buffer), &p.tmap_res, res_bar + 8 * (ch & 1), q0 + c0 + 2 * CC, 0, pr0, 0);
+      mbar_expect_tx(res_bar, kGemmStageRows);
+      tma_load_4d(smem_u32(stage), &p.tmap_res, res_bar, q_tile + next, 0, pr0, 0);
     }
   }
 }
 
-template <int TN, bool PAIR, bool AMN, bool BMN>
+// What follows a product by rows: ELT bytes of an output, the activation, or
+// (kActFull) any of them with a gate, a residual or pre.  Kernels of their own:
+// together in one they spill, and miss the instruction cache.
+constexpr int kActFull = -1;
+
+template <int TN, bool PAIR, bool AMN, bool BMN, int ELT, int ACT>
 __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_constant__ LinearParams p) {
   using C = LinTile<TN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
@@ -293,7 +455,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
       mbar_init(bar(C::kAccEmpty + a), PAIR ? 16 : 8);  // every epilogue warp
     }
     mbar_init(bar(C::kDrain), 1);
-    for (int i = 0; i < 16; ++i) mbar_init(bar(C::kRes + i), 1);
+    for (int i = 0; i < 8; ++i) mbar_init(bar(C::kRes + i), 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -323,6 +485,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
     if (lane == 0) {
       int it = 0;
       bool ok = true;
+      const int q_load = PAIR ? p.tn / 2 : TN;  // rows of B that this CTA multiplies
+      // (MN-major B comes in whole blocks of 64 rows)
+      const uint32_t bytes = PAIR ? 2 * (C::kABytes + (BMN ? C::kQLoad : q_load) * 128) : (AMN ? 128 : p.step) * 128 + C::kBBytes;
       for (int tile = first_tile; ok && tile < tiles; tile += tile_step) {
         int pt, qt;
         fp4_tile_coords(p, tile, pt, qt);
@@ -334,9 +499,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
           }
           const uint32_t dst = base + s * C::kStageBytes;
           const uint32_t full = PAIR ? mapa_shared(bar(C::kFull + s), 0) : bar(C::kFull + s);
-          if (cta == 0) mbar_expect_tx(bar(C::kFull + s), (PAIR ? 2 : 1) * C::kStageBytes);
-          lin_load<PAIR, AMN, 128>(dst, &p.tmap_a, full, kt, pt * C::kRows + cta * 128);
-          lin_load<PAIR, BMN, C::kQLoad>(dst + C::kABytes, &p.tmap_b, full, kt, qt * TN + cta * C::kQLoad);
+          if (cta == 0) mbar_expect_tx(bar(C::kFull + s), bytes);
+          lin_load<PAIR, AMN, 128>(dst, &p.tmap_a, full, kt, pt * p.step + cta * 128);
+          lin_load<PAIR, BMN, C::kQLoad>(dst + C::kABytes, &p.tmap_b, full, kt, qt * p.tn + cta * q_load);
         }
       }
       if (!ok) {
@@ -356,7 +521,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
     // ------------------------------------------------------------ MMAs
     if (cta == 0) {
       // idesc: fp32 accumulator, one format for both operands, their majors
-      const uint32_t idesc = __shfl_sync(0xffffffffu, idesc_make(C::kRows, TN, p.f16 ? 0u : 1u, BMN) | (AMN ? 1u << 15 : 0u), 0);
+      const uint32_t idesc = __shfl_sync(0xffffffffu, idesc_make(C::kRows, PAIR ? p.tn : TN, p.f16 ? 0u : 1u, BMN) | (AMN ? 1u << 15 : 0u), 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       int s = 0, parity = 0, u = 0;
       bool ok = true;
@@ -396,34 +561,40 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;
     constexpr int kCols = TN / 2;  // this warp's columns
-    constexpr int kBias = (kCols + 31) / 32;
     const uint32_t acc_empty = PAIR ? mapa_shared(bar(C::kAccEmpty), 0) : bar(C::kAccEmpty);
-    uint8_t* stage = staging + (warp - 2) * C::kStage2;
-    const uint32_t res_bar = bar(C::kRes + 2 * (warp - 2));
+    uint8_t* stage = staging + (warp - 2) * kGemmStageRows;  // (not of a transposed tile)
+    const uint32_t res_bar = bar(C::kRes + warp - 2);
+    const bool by_rows = TN > 64;
     int u = 0, res_phase = 0;
     for (int tile = first_tile; tile < tiles; tile += tile_step, ++u) {
       const int a = u & 1;
       int pt, qt;
       fp4_tile_coords(p, tile, pt, qt);
-      const int pr0 = pt * C::kRows + cta * 128 + quarter * 32;  // this warp's first row
-      const int q0 = qt * TN + half * kCols;
-      float bias[kBias];  // column 32 i + lane, or (tokens) this lane's row
-#pragma unroll
-      for (int i = 0; i < kBias; ++i) {
-        const int n = p.q_is_tokens ? pr0 + lane : q0 + 32 * i + lane;
-        bias[i] = p.bias != nullptr && n < (p.q_is_tokens ? p.p_rows : p.q_rows) ? lin_value(p.bias, p.bias_dtype, n) : 0.f;
+      const int pr0 = pt * p.step + cta * 128 + quarter * 32;  // this warp's first row
+      if (ACT == kActFull && by_rows && p.residual != nullptr) {  // the residual's first chunk comes while the MMAs run
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+        if (const int c0 = LinChunks<TN, ELT>::column(half, 0), q0 = qt * p.tn + c0; c0 < p.tn && q0 < p.q_rows) {
+          if (!p.res_bulk) {
+            lin_stage_residual<ELT>(p, stage, pr0, q0, lane);
+          } else if (lane == 0) {
+            mbar_expect_tx(res_bar, kGemmStageRows);
+            tma_load_4d(smem_u32(stage), &p.tmap_res, res_bar, q0, 0, pr0, 0);
+          }
+        }
+        __syncwarp();
       }
-      // The residual's first two chunks come while the MMAs run.
-      if (p.res_bulk && lane == 0) {
-        const int chunk = 128 / (p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2);
-        tma_store_wait_read();
-        for (int b = 0; b < 2 && b * chunk < kCols; ++b) {
-          if (q0 + b * chunk >= p.q_rows) break;
-          mbar_expect_tx(res_bar + 8 * b, kGemmStageRows);
-          tma_load_4d(smem_u32(stage + b * kGemmStageRows), &p.tmap_res, res_bar + 8 * b, q0 + b * chunk, 0, pr0, 0);
+      // Bias of column 32 i + lane of this warp's chunks, one after the other.
+      constexpr int kBias = LinChunks<TN, ELT>::kOwn * LinChunks<TN, ELT>::kCols / 32;
+      float bias[kBias];
+      if (ACT != kActFull && by_rows) {
+        constexpr int kOwn = LinChunks<TN, ELT>::kCols;
+#pragma unroll
+        for (int i = 0; i < kBias; ++i) {
+          const int n = qt * p.tn + LinChunks<TN, ELT>::column(half, 32 * i / kOwn) + 32 * i % kOwn + lane;
+          bias[i] = p.bias != nullptr && n < p.q_rows ? lin_value(p.bias, p.bias_dtype, n) : 0.f;
         }
       }
-      __syncwarp();
       const bool got = __all_sync(0xffffffffu, mbar_wait(bar(C::kAccFull + a), (u >> 1) & 1, abort_flag));
       if (!got) {
         report_device_error(kErrEpilogueTimeout);
@@ -431,17 +602,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
         break;
       }
       tc_fence_after();
-      const uint32_t from = tmem + lane_off + a * TN + half * kCols;
       if constexpr (TN > 64) {
-        if (PAIR || p.split == 1) {
-          if (p.out_dtype == DGXM_DTYPE_F32)
-            lin_epilogue<TN, PAIR, 4>(p, stage, res_bar, res_phase, from, acc_empty + a * 8, pr0, q0, lane, bias);
+        if (by_rows) {
+          const uint32_t from = tmem + lane_off + a * TN;
+          const uint32_t to = acc_empty + a * 8;
+          if constexpr (ACT == kActFull)
+            lin_epilogue_full<TN, PAIR, ELT>(p, stage, res_bar, res_phase, from, to, pr0, qt * p.tn, half, lane);
           else
-            lin_epilogue<TN, PAIR, 2>(p, stage, res_bar, res_phase, from, acc_empty + a * 8, pr0, q0, lane, bias);
+            lin_epilogue<TN, PAIR, ELT, ACT>(p, stage, from, to, pr0, qt * p.tn, half, lane, bias);
           continue;
         }
       }
-      if constexpr (!PAIR) {
+      if constexpr (TN <= 64) {  // transposed, maybe a share of K
+        const int q0 = qt * TN + half * kCols;
+        const uint32_t from = tmem + lane_off + a * TN + half * kCols;
         uint32_t r[kCols / 8][8];
 #pragma unroll
         for (int c = 0; c < kCols / 8; ++c) tmem_ld8(from + 8 * c, r[c]);
@@ -457,10 +631,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
                               ((rank * (TN / 4) + half * (kCols / 4)) * pitch + row % rows) * 16;
 #pragma unroll
           for (int c = 0; c < kCols / 4; ++c) st_shared_cluster(to + c * pitch * 16, r[c / 2] + 4 * (c % 2));
-        } else if (const int n = pr0 + lane; n < p.p_rows) {  // the rows are output columns
+        } else if (const int n = pr0 + lane; n < p.p_rows && row < p.step) {  // the rows are output columns
 #pragma unroll
           for (int c = 0; c < kCols; ++c)
-            if (q0 + c < p.q_rows) lin_finish(p, q0 + c, n, __uint_as_float(r[c / 8][c % 8]), bias[0]);
+            if (q0 + c < p.q_rows)
+              lin_finish(p, q0 + c, n, __uint_as_float(r[c / 8][c % 8]), p.bias != nullptr ? lin_value(p.bias, p.bias_dtype, n) : 0.f);
         }
       }
     }
@@ -476,11 +651,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
       const float4* part = reinterpret_cast<const float4*>(staging);
       int pt, qt;
       fp4_tile_coords(p, first_tile, pt, qt);
-      const int most = (128 + p.split - 1) / p.split, rows = min(most, 128 - rank * most), pitch = most | 1;
+      const int most = (128 + p.split - 1) / p.split, rows = min(most, p.step - rank * most), pitch = most | 1;
       for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
         // neighbouring lanes take neighbouring output columns
         const int r = p.q_is_tokens ? i % rows : i / (TN / 4), c = 4 * (p.q_is_tokens ? i / rows : i % (TN / 4));
-        const int pr = pt * 128 + rank * most + r, q = qt * TN + c;
+        const int pr = pt * p.step + rank * most + r, q = qt * TN + c;
         if (pr >= p.p_rows || q >= p.q_rows) continue;
         float4 sum = part[c / 4 * pitch + r];
         for (int k = 1; k < p.split; ++k) {
@@ -523,32 +698,35 @@ static int lin_map(CUtensorMap* map, const LinOperand& o, int64_t k, int box_row
                  {kLinK, 1, (cuuint32_t)box_rows}, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-static int lin_out_map(CUtensorMap* map, const void* base, int64_t ld, const LinearParams& p) {
-  const int elt = p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2;
+static int lin_out_map(CUtensorMap* map, const void* base, int64_t ld, int elt, const LinearParams& p) {
   const cuuint64_t row = static_cast<cuuint64_t>(ld) * elt;
   return fp4_map(map, elt == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, base,
                  {(cuuint64_t)p.q_rows, 1, (cuuint64_t)p.p_rows}, {row, row}, {(cuuint32_t)(128 / elt), 1, 32},
                  CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int TN, bool PAIR, bool AMN, bool BMN>
+template <int TN, bool PAIR, bool AMN, bool BMN, int ELT = 2, int ACT = DGXM_ACT_NONE>
 static int lin_launch(LinearParams& p, const LinOperand& a, const LinOperand& b, cudaStream_t st) {
   using C = LinTile<TN, PAIR>;
   static std::atomic<uint64_t> configured{0};
-  DGXM_CUDA_TRY(set_smem_limit_once(linear_kernel<TN, PAIR, AMN, BMN>, C::kSmemBytes, configured));
-  if (int rc = lin_map(&p.tmap_a, a, p.k, 128)) return rc;
-  if (int rc = lin_map(&p.tmap_b, b, p.k, C::kQLoad)) return rc;
+  DGXM_CUDA_TRY(set_smem_limit_once(linear_kernel<TN, PAIR, AMN, BMN, ELT, ACT>, C::kSmemBytes, configured));
+  if (int rc = lin_map(&p.tmap_a, a, p.k, PAIR ? 128 : p.step)) return rc;
+  if (int rc = lin_map(&p.tmap_b, b, p.k, PAIR ? p.tn / 2 : TN)) return rc;
   const int elt = p.out_dtype == DGXM_DTYPE_F32 ? 4 : 2;
   const bool rows = !p.q_is_tokens && p.split == 1;
   p.vec = p.vec && rows;
-  p.res_bulk = p.vec && p.residual != nullptr && TN / 2 >= 128 / elt && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0 &&
-               p.ld_res > 0 && p.ld_res * elt % 16 == 0;
+  p.res_bulk = rows && p.residual != nullptr && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0 && p.ld_res > 0 &&
+               p.ld_res * elt % 16 == 0;
+  // (a chunk of pre is 128 bytes of its own beside a 16-bit output only)
+  p.pre_vec = rows && p.pre != nullptr && reinterpret_cast<uintptr_t>(p.pre) % 16 == 0 && p.ld_pre % 8 == 0;
   if (p.vec)
-    if (int rc = lin_out_map(&p.tmap_out, p.out, p.ld_out, p)) return rc;
+    if (int rc = lin_out_map(&p.tmap_out, p.out, p.ld_out, elt, p)) return rc;
   if (p.res_bulk)
-    if (int rc = lin_out_map(&p.tmap_res, p.residual, p.ld_res, p)) return rc;
-  p.p_tiles = (p.p_rows + C::kRows - 1) / C::kRows;
-  p.q_tiles = (p.q_rows + TN - 1) / TN;
+    if (int rc = lin_out_map(&p.tmap_res, p.residual, p.ld_res, elt, p)) return rc;
+  if (p.pre_vec)
+    if (int rc = lin_out_map(&p.tmap_pre, p.pre, p.ld_pre, 2, p)) return rc;
+  p.p_tiles = (p.p_rows + p.step - 1) / p.step;
+  p.q_tiles = (p.q_rows + p.tn - 1) / p.tn;
   const int tiles = p.p_tiles * p.q_tiles, share = PAIR ? 2 : p.split;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -566,45 +744,71 @@ static int lin_launch(LinearParams& p, const LinOperand& a, const LinOperand& b,
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_kernel<TN, PAIR, AMN, BMN>, p));
+  DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_kernel<TN, PAIR, AMN, BMN, ELT, ACT>, p));
   return DGXM_OK;
 }
 
-// How a product is cut: the tile's columns (256: a CTA pair's 256 x 256), into
-// how many CTAs its K is split, and whether the tile is transposed.
+template <int TN, bool PAIR, int ELT>
+static int lin_launch_act(LinearParams& p, const LinOperand& a, const LinOperand& b, cudaStream_t st) {
+  if (p.gate != nullptr || p.residual != nullptr || p.pre != nullptr)
+    return lin_launch<TN, PAIR, false, false, ELT, kActFull>(p, a, b, st);
+  switch (p.act) {
+    case DGXM_ACT_SILU: return lin_launch<TN, PAIR, false, false, ELT, DGXM_ACT_SILU>(p, a, b, st);
+    case DGXM_ACT_GELU: return lin_launch<TN, PAIR, false, false, ELT, DGXM_ACT_GELU>(p, a, b, st);
+    case DGXM_ACT_GELU_TANH: return lin_launch<TN, PAIR, false, false, ELT, DGXM_ACT_GELU_TANH>(p, a, b, st);
+    default: return lin_launch<TN, PAIR, false, false, ELT, DGXM_ACT_NONE>(p, a, b, st);
+  }
+}
+
+// How a product is cut: the tile's columns, whether a CTA pair has it, into how
+// many CTAs its K is split, and whether the tile is transposed.
 struct LinCut {
-  int tn, split;
+  int tn;
+  bool pair;
+  int split;
   bool q_is_tokens;  // with at most 64 columns
+  int step;          // rows of a tile
 };
 
 // Tiles of up to 64 columns are transposed: the few rows (m) are B's, which is
-// K-major then.
-static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn) {
+// K-major then.  (b_mn: B is MN-major, and comes in blocks of 64 rows.)
+static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn, bool b_mn) {
   struct Kind {
-    int tn, rows, at_once;
+    int tn;
+    bool pair;
     double stage, tile, least;
   };
-  static const Kind kinds[] = {{16, 128, 148, 0.26, 0.4, 0.4},  {32, 128, 148, 0.26, 0.5, 0.5},
-                               {64, 128, 148, 0.25, 0.8, 1.0},  {128, 128, 148, 0.29, 0.8, 1.1},
-                               {256, 256, 74, 0.42, 1.75, 2.2}};
+  // Microseconds a stage of K, a tile, and at the least, as measured with all SMs at work (1024 and 2048 x 5120 x 5120 by rows,
+  // 1 .. 64 x 5120 x 5120 transposed); the sums order the cuts and are not the times of calls.
+  static const Kind kinds[] = {{16, false, 0.18, 0.4, 0.4},  {32, false, 0.19, 0.5, 0.5},  {64, false, 0.20, 0.8, 1.0},
+                               {128, false, 0.24, 1.3, 1.6}, {128, true, 0.245, 1.5, 2.0}, {192, true, 0.285, 1.7, 2.2},
+                               {256, true, 0.315, 2.0, 2.5}};
   static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};  // that the SMs hold at one time
-  LinCut best{128, 1, false};
+  LinCut best{128, false, 1, false, 128};
   double least = 1e30;
   for (const Kind& kind : kinds) {
     const bool swapped = kind.tn <= 64;
-    if (swapped && (a_mn || (kind.tn < 64 && m > kind.tn))) continue;
+    if ((swapped && (a_mn || m > kind.tn)) || (b_mn && kind.pair && kind.tn % 128 != 0)) continue;
     const int64_t p_rows = swapped ? n : m, q_rows = swapped ? m : n;
-    const int64_t tiles = (p_rows + kind.rows - 1) / kind.rows * ((q_rows + kind.tn - 1) / kind.tn);
-    for (int split = 1; split <= (kind.tn <= 128 ? 8 : 1) && split <= k_tiles; ++split) {
+    const int rows = kind.pair ? 256 : 128, at_once = kind.pair ? 74 : 148;
+    const int64_t tiles = (p_rows + rows - 1) / rows * ((q_rows + kind.tn - 1) / kind.tn);
+    for (int split = 1; split <= (swapped ? 8 : 1) && split <= k_tiles; ++split) {
       if (split > 1 && tiles > clusters[split]) continue;
-      const int64_t waves = (tiles * split + kind.at_once - 1) / kind.at_once;
+      const int64_t waves = (tiles * split + at_once - 1) / at_once;
       const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile, kind.least) +
                         (split > 1 ? 0.8 + 0.026 * kind.tn : 0.0);
       if (us < least) {
         least = us;
-        best = {kind.tn, split, swapped};
+        best = {kind.tn, kind.pair, split, swapped, rows};
       }
     }
+  }
+  // A transposed product reads the weight once and DRAM bounds it: tiles of
+  // fewer rows, so that every SM has as many as the others (2 x 30720 x 5120:
+  // 240 tiles of 128 rows or 296 of 104 on 148 SMs).
+  if (best.q_is_tokens && best.split == 1) {
+    const int64_t waves = ((n + 127) / 128 + 147) / 148;
+    best.step = static_cast<int>(std::min<int64_t>(128, ((n + 148 * waves - 1) / (148 * waves) + 7) / 8 * 8));
   }
   return best;
 }
@@ -613,9 +817,12 @@ static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn) {
 static int lin_product(LinearParams& p, const LinOperand& a, const LinOperand& b, int64_t k, cudaStream_t st) {
   p.k = static_cast<int>(k);
   p.k_tiles = static_cast<int>((k + kLinK - 1) / kLinK);
-  const LinCut cut = lin_cut(a.rows, b.rows, p.k_tiles, a.mn);
+  const LinCut cut = lin_cut(a.rows, b.rows, p.k_tiles, a.mn, b.mn);
   p.split = cut.split;
   p.q_is_tokens = cut.q_is_tokens;
+  p.step = cut.step;
+  p.tn = cut.tn;
+  if (p.q_is_tokens && b.mn) p.step = 128;  // whole blocks of 64 rows are loaded there
   const LinOperand &po = p.q_is_tokens ? b : a, &qo = p.q_is_tokens ? a : b;
   p.p_rows = static_cast<int>(po.rows);
   p.q_rows = static_cast<int>(qo.rows);
@@ -625,41 +832,47 @@ static int lin_product(LinearParams& p, const LinOperand& a, const LinOperand& b
     case 16: return amn ? lin_launch<16, false, true, false>(p, po, qo, st) : lin_launch<16, false, false, false>(p, po, qo, st);
     case 32: return amn ? lin_launch<32, false, true, false>(p, po, qo, st) : lin_launch<32, false, false, false>(p, po, qo, st);
     case 64: return amn ? lin_launch<64, false, true, false>(p, po, qo, st) : lin_launch<64, false, false, false>(p, po, qo, st);
-    case 128:
-      return amn   ? lin_launch<128, false, true, true>(p, po, qo, st)
-             : bmn ? lin_launch<128, false, false, true>(p, po, qo, st)
-                   : lin_launch<128, false, false, false>(p, po, qo, st);
-    default:
-      return amn   ? lin_launch<256, true, true, true>(p, po, qo, st)
-             : bmn ? lin_launch<256, true, false, true>(p, po, qo, st)
-                   : lin_launch<256, true, false, false>(p, po, qo, st);
+    default: break;
   }
+  if (amn || bmn) {  // the gradients' products: 16-bit outputs and nothing more
+    if (cut.pair) return amn ? lin_launch<256, true, true, true>(p, po, qo, st) : lin_launch<256, true, false, true>(p, po, qo, st);
+    return amn ? lin_launch<128, false, true, true>(p, po, qo, st) : lin_launch<128, false, false, true>(p, po, qo, st);
+  }
+  const bool wide = p.out_dtype == DGXM_DTYPE_F32;
+  if (cut.pair) return wide ? lin_launch_act<256, true, 4>(p, po, qo, st) : lin_launch_act<256, true, 2>(p, po, qo, st);
+  return wide ? lin_launch_act<128, false, 4>(p, po, qo, st) : lin_launch_act<128, false, 2>(p, po, qo, st);
 }
 
 // ------------------------------------------------------------ matrices off 16 bytes
-// Rows that no TMA box can start at are copied to a pitch of whole 16 bytes first.
+// Rows that no TMA box can start at are copied to a pitch of whole 16 bytes
+// first, up to two matrices in one launch.
 struct LinPackParams {
-  const uint16_t* from;
-  uint16_t* to;
-  int64_t rows, ld, pitch;
-  int cols;
+  struct {
+    const uint16_t* from;
+    uint16_t* to;
+    int64_t ld, words;  // of the whole copy, 16 bytes each
+    int cols, pitch;
+  } of[2];
+  int n;
 };
 
 __global__ void __launch_bounds__(256) linear_pack_kernel(const __grid_constant__ LinPackParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int words = static_cast<int>(p.pitch / 8);
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < p.rows * words; i += gridDim.x * 256LL) {
-    const int64_t row = i / words;
-    const int col = static_cast<int>(i - row * words) * 8;
-    const uint16_t* from = p.from + row * p.ld + col;
-    uint32_t w[4];
+  for (int j = 0; j < p.n; ++j) {
+    const auto& o = p.of[j];
+    const int across = o.pitch / 8;
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < o.words; i += gridDim.x * 256LL) {
+      const int64_t row = o.words <= 0xffffffffLL ? static_cast<uint32_t>(i) / static_cast<uint32_t>(across) : i / across;
+      const int col = static_cast<int>(i - row * across) * 8;
+      const uint16_t* from = o.from + row * o.ld + col;
+      uint32_t v[8], w[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t lo = col + 2 * k < p.cols ? from[2 * k] : 0u, hi = col + 2 * k + 1 < p.cols ? from[2 * k + 1] : 0u;
-      w[k] = lo | hi << 16;
+      for (int k = 0; k < 8; ++k) v[k] = col + k < o.cols ? from[k] : 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = v[2 * k] | v[2 * k + 1] << 16;
+      *reinterpret_cast<uint4*>(o.to + row * o.pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(p.to + row * p.pitch + col) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -669,34 +882,51 @@ static int64_t lin_packed_bytes(const void* ptr, int64_t ld, int64_t rows, int64
   return lin_on_words(ptr, ld) ? 0 : (rows * lin_pitch(cols) * 2 + 255) / 256 * 256;
 }
 
-// o with its rows on 16 bytes, from the workspace where they are not.
-static int lin_pack(const void** ptr, int64_t* ld, int64_t rows, int64_t cols, char** work, cudaStream_t st) {
-  const int64_t bytes = lin_packed_bytes(*ptr, *ld, rows, cols);
-  if (bytes == 0) return DGXM_OK;
-  LinPackParams p{static_cast<const uint16_t*>(*ptr), reinterpret_cast<uint16_t*>(*work), rows, *ld, lin_pitch(cols),
-                  static_cast<int>(cols)};
-  const int64_t blocks = std::min<int64_t>((rows * (p.pitch / 8) + 255) / 256, 148 * 16);
-  DGXM_CUDA_TRY(launch_overlapped(linear_pack_kernel, static_cast<unsigned>(blocks), 256, 0, st, p));
-  *ptr = *work;
-  *ld = p.pitch;
-  *work += bytes;
-  return DGXM_OK;
-}
+// Matrices to be copied so that their rows lie on 16 bytes.
+struct LinPacker {
+  LinPackParams p;
+  char* work;
+  explicit LinPacker(char* w) : work(w) { memset(&p, 0, sizeof(p)); }
+  void add(const void** ptr, int64_t* ld, int64_t rows, int64_t cols) {
+    const int64_t bytes = lin_packed_bytes(*ptr, *ld, rows, cols);
+    if (bytes == 0) return;
+    auto& o = p.of[p.n++];
+    o.from = static_cast<const uint16_t*>(*ptr);
+    o.to = reinterpret_cast<uint16_t*>(work);
+    o.ld = *ld;
+    o.cols = static_cast<int>(cols);
+    o.pitch = static_cast<int>(lin_pitch(cols));
+    o.words = rows * (o.pitch / 8);
+    *ptr = work;
+    *ld = o.pitch;
+    work += bytes;
+  }
+  int run(cudaStream_t st) {
+    if (p.n == 0) return DGXM_OK;
+    const int64_t words = std::max(p.of[0].words, p.n > 1 ? p.of[1].words : 0);
+    DGXM_CUDA_TRY(launch_overlapped(linear_pack_kernel, static_cast<unsigned>(std::min<int64_t>((words + 255) / 256, 148 * 8)),
+                                    256, 0, st, p));
+    p.n = 0;
+    return DGXM_OK;
+  }
+};
 
 // ------------------------------------------------------------ dz and the sums over rows
-// A thread takes eight columns of a run of rows of one sample; its sums go to
-// (run, 2, n) partial sums of dz and dout act(pre), which a second kernel adds
-// in the order of the runs.
-constexpr int kDzRows = 32;  // rows of a run
+// A thread takes eight columns of a run of rows of one sample, four rows'
+// loads at a time; its sums go to (run, 2, n) partial sums of dz and dout
+// act(pre), which a second kernel adds in the order of the runs.  DRAM bounds
+// it: dout and pre read, dz written.
+constexpr int kDzBatch = 4;
 
 struct LinDzParams {
   const void *dout, *pre, *gate;
   void *dz, *g_gate;  // g_gate: a token's own, contiguous
-  float* partial;     // (runs, 2, n), or NULL
+  float* partial;     // (runs, 2, pitch), or NULL
+  int64_t pitch;
   int64_t ld_dout, ld_pre, ld_dz, gate_sample, gate_row;
   int64_t runs;
-  int n, sample_rows, sample_runs, act, sum_bias, sum_gate;
-  int dtype, dout_dtype, gate_dtype, vec;
+  int n, sample_rows, sample_runs, run_rows, sum_bias, sum_gate;
+  int dtype, dout_dtype, gate_dtype, vec, gate_vec;
 };
 
 // Eight values from column `col`, zeros past the last.
@@ -707,16 +937,7 @@ __device__ __forceinline__ void lin_read8(const void* base, int dtype, int64_t a
       const float4 a = p[0], b = p[1];
       v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float2 f;
-        if (dtype == DGXM_DTYPE_BF16) f = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xFFFF0000u));
-        else f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
-        v[2 * k] = f.x;
-        v[2 * k + 1] = f.y;
-      }
+      lin_widen8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at), dtype, v);
     }
   } else {
 #pragma unroll
@@ -724,68 +945,101 @@ __device__ __forceinline__ void lin_read8(const void* base, int dtype, int64_t a
   }
 }
 
-__global__ void __launch_bounds__(128) linear_dz_kernel(const __grid_constant__ LinDzParams p) {
+// GATES: a gate's gradient is wanted.
+template <int ACT, bool GATES>
+__global__ void __launch_bounds__(128, GATES ? 5 : 6) linear_dz_kernel(const __grid_constant__ LinDzParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int col = (blockIdx.y * 128 + threadIdx.x) * 8;
   if (col >= p.n) return;
   for (int64_t run = blockIdx.x; run < p.runs; run += gridDim.x) {
     const int64_t sample = run / p.sample_runs;
-    const int first = static_cast<int>(run - sample * p.sample_runs) * kDzRows, rows = min(kDzRows, p.sample_rows - first);
+    const int first = static_cast<int>(run - sample * p.sample_runs) * p.run_rows;
+    const int rows = min(p.run_rows, p.sample_rows - first);
     float gate[8], sum[8], sum_gate[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       gate[i] = 1.f;
       sum[i] = sum_gate[i] = 0.f;
     }
-    if (p.gate != nullptr && p.gate_row == 0) lin_read8(p.gate, p.gate_dtype, sample * p.gate_sample + col, col, p.n, 0, gate);
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      const int64_t m = sample * p.sample_rows + first + r;
-      float d[8], z[8];
-      lin_read8(p.dout, p.dout_dtype, m * p.ld_dout + col, col, p.n, p.vec, d);
-      if (p.pre != nullptr) lin_read8(p.pre, p.dtype, m * p.ld_pre + col, col, p.n, p.vec, z);
-      if (p.gate != nullptr && p.gate_row != 0)
-        lin_read8(p.gate, p.gate_dtype, sample * p.gate_sample + (first + r) * p.gate_row + col, col, p.n, 0, gate);
-      if (p.sum_gate || p.g_gate != nullptr) {
+    if (p.gate != nullptr && p.gate_row == 0) lin_read8(p.gate, p.gate_dtype, sample * p.gate_sample + col, col, p.n, p.gate_vec, gate);
+    const int64_t m0 = sample * p.sample_rows + first;
+    constexpr bool kPre = ACT != DGXM_ACT_NONE || GATES;
+    const bool whole = p.vec && col + 8 <= p.n && p.dout_dtype == p.dtype;
+    for (int r0 = 0; r0 < rows; r0 += kDzBatch) {
+      uint4 raw_d[kDzBatch], raw_z[kDzBatch];
+      if (whole) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = d[i] * lin_act(z[i], p.act);
-          sum_gate[i] += v;
-          if (p.g_gate != nullptr && col + i < p.n) lin_put(p.g_gate, p.gate_dtype, m * p.n + col + i, v);
+        for (int j = 0; j < kDzBatch; ++j) {
+          const int64_t m = m0 + min(r0 + j, rows - 1);
+          raw_d[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dout) + m * p.ld_dout + col);
+          if (kPre) raw_z[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.pre) + m * p.ld_pre + col);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        d[i] *= gate[i];
-        if (p.act != DGXM_ACT_NONE) d[i] *= lin_slope(z[i], p.act);
-        sum[i] += d[i];
-      }
-      if (p.dz != nullptr) {
-        const bool f16 = p.dtype == DGXM_DTYPE_F16;
-        uint32_t w[4];
+      for (int j = 0; j < kDzBatch; ++j) {
+        if (r0 + j >= rows) break;
+        const int64_t m = m0 + r0 + j;
+        float d[8], z[8];
+        if (whole) {
+          lin_widen8(raw_d[j], p.dtype, d);
+          if (kPre) lin_widen8(raw_z[j], p.dtype, z);
+        } else {
+          lin_read8(p.dout, p.dout_dtype, m * p.ld_dout + col, col, p.n, p.vec, d);
+          if (kPre) lin_read8(p.pre, p.dtype, m * p.ld_pre + col, col, p.n, p.vec, z);
+        }
+        if (p.gate != nullptr && p.gate_row != 0)
+          lin_read8(p.gate, p.gate_dtype, sample * p.gate_sample + (first + r0 + j) * p.gate_row + col, col, p.n, p.gate_vec, gate);
+        if constexpr (GATES) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = f16 ? pack_f16x2(d[2 * k], d[2 * k + 1]) : pack_bf16x2(d[2 * k], d[2 * k + 1]);
-        // (columns past the last, up to the pitch, are zeros)
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dz) + m * p.ld_dz + col) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int i = 0; i < 8; ++i) {
+            const float v = d[i] * lin_act(z[i], ACT);
+            sum_gate[i] += v;
+            if (p.g_gate != nullptr && col + i < p.n) lin_put(p.g_gate, p.gate_dtype, m * p.n + col + i, v);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          d[i] *= gate[i];
+          if (ACT != DGXM_ACT_NONE) d[i] *= lin_slope(z[i], ACT);
+          sum[i] += d[i];
+        }
+        if (p.dz != nullptr) {
+          const bool f16 = p.dtype == DGXM_DTYPE_F16;
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = f16 ? pack_f16x2(d[2 * k], d[2 * k + 1]) : pack_bf16x2(d[2 * k], d[2 * k + 1]);
+          // (columns past the last, up to the pitch, are zeros)
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dz) + m * p.ld_dz + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
     }
     if (p.partial != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (col + i >= p.n) continue;
-        if (p.sum_bias) p.partial[run * 2 * p.n + col + i] = sum[i];
-        if (p.sum_gate) p.partial[(run * 2 + 1) * p.n + col + i] = sum_gate[i];
-      }
+      auto put = [&](int64_t row, const float (&v)[8]) {  // the pitch is whole eights
+        float4* to = reinterpret_cast<float4*>(p.partial + row * p.pitch + col);
+        to[0] = make_float4(v[0], v[1], v[2], v[3]);
+        to[1] = make_float4(v[4], v[5], v[6], v[7]);
+      };
+      if (p.sum_bias) put(run * 2, sum);
+      if (GATES && p.sum_gate) put(run * 2 + 1, sum_gate);
     }
   }
+}
+
+template <bool GATES>
+static auto lin_dz_pick(int act) {
+  return act == DGXM_ACT_SILU   ? linear_dz_kernel<DGXM_ACT_SILU, GATES>
+         : act == DGXM_ACT_GELU ? linear_dz_kernel<DGXM_ACT_GELU, GATES>
+         : act == DGXM_ACT_NONE ? linear_dz_kernel<DGXM_ACT_NONE, GATES>
+                                : linear_dz_kernel<DGXM_ACT_GELU_TANH, GATES>;
 }
 
 struct LinSumParams {
   const float* partial;
   void *g_bias, *g_gate;
   int64_t samples;
-  int n, sample_runs, bias_dtype, gate_dtype, gate_form;
+  int n, pitch, sample_runs, bias_dtype, gate_dtype, gate_form;
 };
 
 // A block takes 32 columns.  Its warps take the samples in turn where there
@@ -820,8 +1074,8 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const __grid_constant_
     if (in) {
 #pragma unroll 4
       for (int64_t r = r0; r < r1; ++r) {
-        if (p.g_bias != nullptr) b += p.partial[r * 2 * p.n + col];
-        if (gates) g += p.partial[(r * 2 + 1) * p.n + col];
+        if (p.g_bias != nullptr) b += p.partial[r * 2 * p.pitch + col];
+        if (gates) g += p.partial[(r * 2 + 1) * p.pitch + col];
       }
     }
     if (!many) join(b, g);
@@ -906,12 +1160,13 @@ extern "C" int dgxm_linear(const dgxm_linear_desc* d, const void* x, const void*
   if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need))
     return fail(DGXM_ERR_INVALID, "workspace of %lld bytes (%lld needed)", (long long)workspace_bytes, (long long)need);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  char* work = static_cast<char*>(workspace);
   int64_t ldx = d->m > 1 ? d->x_stride : lin_pitch(d->k), ldw = d->n > 1 ? d->w_stride : lin_pitch(d->k);
   if (d->m == 1 && !lin_on_words(x, d->x_stride)) ldx = d->x_stride;
   if (d->n == 1 && !lin_on_words(w, d->w_stride)) ldw = d->w_stride;
-  if (int rc = lin_pack(&x, &ldx, d->m, d->k, &work, st)) return rc;
-  if (int rc = lin_pack(&w, &ldw, d->n, d->k, &work, st)) return rc;
+  LinPacker pack(static_cast<char*>(workspace));
+  pack.add(&x, &ldx, d->m, d->k);
+  pack.add(&w, &ldw, d->n, d->k);
+  if (int rc = pack.run(st)) return rc;
   LinearParams p;
   memset(&p, 0, sizeof(p));
   p.bias = bias;
@@ -939,7 +1194,7 @@ namespace dgxm {
 struct LinBackPlan {
   bool dz;      // dz is not dout itself
   bool sums;
-  int64_t runs, sample_runs, sample_rows, dz_bytes, part_bytes, x_bytes, w_bytes, dout_bytes;
+  int64_t runs, sample_runs, sample_rows, run_rows, dz_bytes, part_bytes, x_bytes, w_bytes, dout_bytes;
   int64_t total() const { return dz_bytes + part_bytes + x_bytes + w_bytes + dout_bytes; }
 };
 
@@ -951,11 +1206,14 @@ static LinBackPlan lin_back_plan(const dgxm_linear_desc* d, const dgxm_linear_gr
   b.dz = products && (d->activation != DGXM_ACT_NONE || d->gate_form != DGXM_MOD_NONE || d->out_dtype != d->dtype);
   b.sums = g->bias != nullptr || (g->gate != nullptr && d->gate_form != DGXM_MOD_TOKEN);
   b.sample_rows = d->gate_form != DGXM_MOD_NONE ? d->sample_rows : d->m;
-  b.sample_runs = (b.sample_rows + kDzRows - 1) / kDzRows;
+  // Runs of 64 rows, or shorter ones where those would leave the SMs without work.
+  const int64_t across = (lin_pitch(d->n) / 8 + 127) / 128;
+  b.run_rows = std::max<int64_t>(kDzBatch, std::min<int64_t>(64, d->m * across / (148 * 4) / kDzBatch * kDzBatch));
+  b.sample_runs = (b.sample_rows + b.run_rows - 1) / b.run_rows;
   b.runs = b.sample_rows > 0 ? d->m / b.sample_rows * b.sample_runs : 0;
   if (b.dz) b.dz_bytes = (d->m * lin_pitch(d->n) * 2 + 255) / 256 * 256;
   else if (products) b.dout_bytes = lin_packed_bytes(dout, d->out_stride, d->m, d->n);
-  if (b.sums) b.part_bytes = (b.runs * 2 * d->n * 4 + 255) / 256 * 256;
+  if (b.sums) b.part_bytes = (b.runs * 2 * lin_pitch(d->n) * 4 + 255) / 256 * 256;
   if (g->w != nullptr) b.x_bytes = lin_packed_bytes(x, d->x_stride, d->m, d->k);
   if (g->x != nullptr) b.w_bytes = lin_packed_bytes(w, d->w_stride, d->n, d->k);
   return b;
@@ -1022,6 +1280,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
       q.partial = reinterpret_cast<float*>(work);
       work += plan.part_bytes;
     }
+    q.pitch = lin_pitch(d->n);
     q.g_gate = tok ? g->gate : nullptr;
     q.ld_dout = d->out_stride;
     q.ld_pre = d->pre_stride;
@@ -1030,7 +1289,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
     q.n = static_cast<int>(d->n);
     q.sample_rows = static_cast<int>(plan.sample_rows);
     q.sample_runs = static_cast<int>(plan.sample_runs);
-    q.act = d->activation;
+    q.run_rows = static_cast<int>(plan.run_rows);
     q.sum_bias = g->bias != nullptr;
     q.sum_gate = g->gate != nullptr && !tok;
     q.dtype = d->dtype;
@@ -1038,6 +1297,8 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
     q.gate_dtype = d->gate_dtype;
     q.vec = reinterpret_cast<uintptr_t>(dout) % 16 == 0 && d->out_stride * lin_elt(d->out_dtype) % 16 == 0 &&
             (pre == nullptr || (reinterpret_cast<uintptr_t>(pre) % 16 == 0 && d->pre_stride % 8 == 0));
+    const int ge = lin_elt(d->gate_dtype);
+    q.gate_vec = reinterpret_cast<uintptr_t>(gate) % 16 == 0 && q.gate_sample * ge % 16 == 0 && q.gate_row * ge % 16 == 0;
     const unsigned across = static_cast<unsigned>((lin_pitch(d->n) / 8 + 127) / 128);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -1048,7 +1309,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_dz_kernel, q));
+    DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, g->gate != nullptr ? lin_dz_pick<true>(d->activation) : lin_dz_pick<false>(d->activation), q));
     if (plan.sums) {
       LinSumParams s;
       s.partial = q.partial;
@@ -1056,6 +1317,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
       s.g_gate = tok ? nullptr : g->gate;
       s.samples = d->m / plan.sample_rows;
       s.n = q.n;
+      s.pitch = static_cast<int>(q.pitch);
       s.sample_runs = q.sample_runs;
       s.bias_dtype = d->bias_dtype;
       s.gate_dtype = d->gate_dtype;
@@ -1068,23 +1330,25 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
     }
   }
   if (g->x == nullptr && g->w == nullptr) return DGXM_OK;
-  if (!plan.dz)
-    if (int rc = lin_pack(&dz, &ld_dz, d->m, d->n, &work, st)) return rc;
+  LinPacker pack(work);
+  int64_t ldw = d->w_stride, ldx = d->x_stride;
+  if (!plan.dz) pack.add(&dz, &ld_dz, d->m, d->n);
+  if (g->x != nullptr) pack.add(&w, &ldw, d->n, d->k);
+  if (pack.p.n == 2)
+    if (int rc = pack.run(st)) return rc;
+  if (g->w != nullptr) pack.add(&x, &ldx, d->m, d->k);
+  if (int rc = pack.run(st)) return rc;
   LinearParams p;
   memset(&p, 0, sizeof(p));
   p.out_dtype = p.bias_dtype = p.gate_dtype = p.pre_dtype = d->dtype;
   p.f16 = d->dtype == DGXM_DTYPE_F16;
   p.ld_out = d->k;
   if (g->x != nullptr) {
-    int64_t ldw = d->w_stride;
-    if (int rc = lin_pack(&w, &ldw, d->n, d->k, &work, st)) return rc;
     p.out = g->x;
     p.sample_rows = static_cast<int>(d->m);
     if (int rc = lin_product(p, {dz, d->m, ld_dz, false}, {w, d->k, ldw, true}, d->n, st)) return rc;
   }
   if (g->w != nullptr) {
-    int64_t ldx = d->x_stride;
-    if (int rc = lin_pack(&x, &ldx, d->m, d->k, &work, st)) return rc;
     p.out = g->w;
     p.sample_rows = static_cast<int>(d->n);
     if (int rc = lin_product(p, {dz, d->n, ld_dz, true}, {x, d->k, ldx, true}, d->m, st)) return rc;
