@@ -59,7 +59,7 @@ struct BlockNormParams {
   char *g_gate, *g_scale, *g_shift;  // backward, a row each token: contiguous
   float* partial;            // backward: (block + sample, 3, width)
   int want;                  // which of the three sums are wanted, a bit each
-  int batch, seq, width, mode, branch_norm;
+  int batch, seq, width, mode, branch_norm, factor;  // factor: backward, dn = e a with other than ones
   int64_t rows, rows_each;
   int rows_more;
   float eps, inv_width;
@@ -426,14 +426,16 @@ __device__ __forceinline__ float2 bn_warp_moments(BnMoments v) {
   return make_float2(__shfl_sync(0xffffffffu, v.mean, 0), __shfl_sync(0xffffffffu, __fdividef(v.m2, v.n), 0));
 }
 
-// The statistics' copy of a column vector of the row's sample: loaded when the
-// sample changes, which every one of their warps sees at the same row.
+// The statistics' copy of column vectors of the row's sample, `each` values
+// one: loaded when the sample changes, which every one of their warps sees at
+// the same row.
 template <int WARPS, typename Make>
-__device__ __forceinline__ void bn_param(const BlockNormParams& p, float* param, int t, Make&& make) {
+__device__ __forceinline__ void bn_param(const BlockNormParams& p, float* param, int t, int each, Make&& make) {
   if (p.param_bytes == 0) return;
   named_barrier_sync(1, WARPS * 32);
+  for (int which = 0; which * each < p.param_bytes / 4; ++which)
 #pragma unroll 8
-  for (int c = t; c < p.param_bytes / 4; c += WARPS * 32) param[c] = c < p.width ? make(c) : 0.f;
+    for (int c = t; c < each; c += WARPS * 32) param[which * each + c] = c < p.width ? make(c, which) : 0.f;
   named_barrier_sync(1, WARPS * 32);
 }
 
@@ -447,82 +449,121 @@ __device__ __forceinline__ void bn_param_get(const float* param, int q, uint64_t
   }
 }
 
+// What a row's values are made of, for its mean and squares: one stream
+// (kBnAlone); x plus a branch as it is, times a vector of the statistics' copy,
+// or times a gate of each token; or (kBnAny) whatever the parameters say.  Each
+// has a loop of its own: ways not taken between the few instructions of one
+// cost more than the instructions (250 cycles a chunk instead of 100).
+enum { kBnAlone, kBnPlain, kBnScaled, kBnToken, kBnAny };
+
+// Sum (of deviations from the mean, in LAYER) of squares, and the mean, over a row: one warp's.
+template <typename T, bool VEC, bool FULL, bool LAYER, int SRC>
+__device__ __forceinline__ float2 bn_row_sums(const BlockNormParams& p, const uint8_t* slot, int s, const BnWalk& w,
+                                              const float* param, float root2) {
+  constexpr int CH = kBnChunk<T>, N = CH / 2;
+  const int lane = threadIdx.x & 31;
+  BnMoments moments;
+  uint64_t ss = 0;
+#pragma unroll 2
+  for (int q = lane; q * CH < p.width; q += 32) {
+    uint64_t r[N];
+    bn_get<T, VEC>(p, slot, s, w, q, r);
+    if constexpr (SRC != kBnAlone) {
+      uint64_t m[N], g[N];
+      bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
+      if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], bn_both(root2));
+      }
+      if constexpr (SRC == kBnToken || SRC == kBnAny) {
+        if (SRC == kBnToken || p.in[kBnGate] != nullptr) {
+          bn_get_mod<T, VEC>(p, slot, kBnGate, w, q, g);
+#pragma unroll
+          for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], g[i]);
+        }
+      }
+      if constexpr (SRC == kBnAny) {
+        bn_vector<T>(p.gate ? p.gate + w.b * p.gate_sb : nullptr, p.mod_f32, q * CH, p.width, 1.f, g);
+#pragma unroll
+        for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], g[i]);
+        bn_vector<T>(p.branch_w, p.w_f32, q * CH, p.width, 1.f, g);
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = ffma2(g[i], m[i], r[i]);
+      } else if (SRC == kBnScaled || (SRC == kBnToken && p.param_bytes > 0)) {
+        bn_param_get(param, q, g);
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = ffma2(g[i], m[i], r[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = fadd2(r[i], m[i]);
+      }
+    }
+    if constexpr (LAYER) {
+      bn_add_chunk(moments, r, VEC ? CH : min(CH, p.width - q * CH));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) ss = ffma2(r[i], r[i], ss);
+    }
+  }
+  if constexpr (LAYER) {
+    return bn_warp_moments(moments);
+  } else {
+    float sum[1] = {bn_total(ss)};
+    bn_warp_sum(sum);
+    return make_float2(0.f, sum[0] * p.inv_width);
+  }
+}
+
+template <typename T, bool VEC, bool FULL, int SRC>
+__device__ __forceinline__ float2 bn_row_stats(const BlockNormParams& p, const uint8_t* slot, int s, const BnWalk& w,
+                                               const float* param, float root2) {
+  return p.mode == DGXM_BLOCK_NORM_LAYER ? bn_row_sums<T, VEC, FULL, true, SRC>(p, slot, s, w, param, root2)
+                                         : bn_row_sums<T, VEC, FULL, false, SRC>(p, slot, s, w, param, root2);
+}
+
 template <typename T, bool VEC, bool FULL, int STAT>
 __device__ __forceinline__ void bn_forward_stats(const BlockNormParams& p, float* param, const uint8_t* ring, BnShared& sh,
                                                  int t) {
-  constexpr int CH = kBnChunk<T>, N = CH / 2;
   const int lane = t & 31;
-  // Rows in turn, by no more warps than there are slots: none waits for a phase
-  // of a slot whose last one is still open.
+  // Rows in turn, by no more warps than there are slots, whose number is a
+  // multiple: all rows of a slot are one warp's, so that none waits for a phase
+  // of a slot whose last one may still be open (rows land in any order).
   const int warps = min(STAT, p.slots);
   int turn = t >> 5 < warps ? t >> 5 : 0x7fffffff;  // rows until this warp's next
-  const bool branch = p.in[kBnBranch] != nullptr, layer = p.mode == DGXM_BLOCK_NORM_LAYER;
-  const bool norm = p.mode != DGXM_BLOCK_NORM_NONE, tok = FULL && p.in[kBnGate] != nullptr;
+  const bool wanted = p.gate != nullptr || p.branch_w != nullptr;
+  const int src = p.in[kBnBranch] == nullptr          ? kBnAlone
+                  : wanted && p.param_bytes == 0      ? kBnAny
+                  : FULL && p.in[kBnGate] != nullptr  ? kBnToken
+                  : wanted                            ? kBnScaled
+                                                      : kBnPlain;
   int sample = -1;
   bool dead = false;
   for (BnWalk w(p); w.more(); w.next()) {
     if (w.b != sample) {
       sample = w.b;
-      bn_param<STAT>(p, param, t, [&](int c) { return bn_value<T>(p.gate + sample * p.gate_sb, p.mod_f32, c); });
+      bn_param<STAT>(p, param, t, p.param_bytes / 4, [&](int c, int) {
+        const float g = p.gate ? bn_value<T>(p.gate + sample * p.gate_sb, p.mod_f32, c) : 1.f;
+        return FULL && p.branch_w ? g * bn_value<T>(p.branch_w, p.w_f32, c) : g;
+      });
     }
     if (turn-- > 0) continue;
     turn = warps - 1;
     bn_wait(&sh.full[w.slot], w.parity, dead);
     const uint8_t* slot = ring + w.slot * p.slot_bytes;
     float root2 = 1.f;
-    if (FULL && p.branch_norm) {
-      uint64_t ss = 0;
-#pragma unroll 2
-    for (int q = lane; q * CH < p.width; q += 32) {
-        uint64_t m[N];
-        bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss = ffma2(m[i], m[i], ss);
-      }
-      float sum[1] = {bn_total(ss)};
-      bn_warp_sum(sum);
-      root2 = rsqrtf(fmaf(sum[0], p.inv_width, p.eps));
-    }
-    BnMoments moments;
-    uint64_t ss = 0;
-#pragma unroll 2
-    for (int q = lane; norm && q * CH < p.width; q += 32) {
-      uint64_t r[N];
-      bn_get<T, VEC>(p, slot, kBnX, w, q, r);
-      if (branch) {
-        uint64_t m[N], g[N];
-        bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
-        if (FULL && p.branch_norm) {
-          bn_vector<T>(p.branch_w, p.w_f32, q * CH, p.width, 1.f, g);
-#pragma unroll
-          for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], fmul2(bn_both(root2), g[i]));
-        }
-        if (tok) bn_get_mod<T, VEC>(p, slot, kBnGate, w, q, g);
-        else if (p.param_bytes > 0) bn_param_get(param, q, g);
-        else bn_vector<T>(p.gate ? p.gate + sample * p.gate_sb : nullptr, p.mod_f32, q * CH, p.width, 1.f, g);
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = ffma2(g[i], m[i], r[i]);
-      }
-      if (layer) {
-        bn_add_chunk(moments, r, VEC ? CH : min(CH, p.width - q * CH));
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss = ffma2(r[i], r[i], ss);
-      }
-    }
-    float mean = 0.f, square = 0.f;
-    if (layer) {
-      const float2 v = bn_warp_moments(moments);
-      mean = v.x;
-      square = v.y;
-    } else if (norm) {
-      float sum[1] = {bn_total(ss)};
-      bn_warp_sum(sum);
-      square = sum[0] * p.inv_width;
+    if (FULL && p.branch_norm)
+      root2 = rsqrtf(bn_row_sums<T, VEC, FULL, false, kBnAlone>(p, slot, kBnBranch, w, param, 1.f).y + p.eps);
+    float2 v = make_float2(0.f, 0.f);
+    if (p.mode != DGXM_BLOCK_NORM_NONE) {
+      if (src == kBnScaled) v = bn_row_stats<T, VEC, FULL, kBnScaled>(p, slot, kBnX, w, param, root2);
+      else if (src == kBnAlone) v = bn_row_stats<T, VEC, FULL, kBnAlone>(p, slot, kBnX, w, param, root2);
+      else if (src == kBnPlain) v = bn_row_stats<T, VEC, FULL, kBnPlain>(p, slot, kBnX, w, param, root2);
+      else if (FULL && src == kBnToken) v = bn_row_stats<T, VEC, FULL, FULL ? kBnToken : kBnAlone>(p, slot, kBnX, w, param, root2);
+      else v = bn_row_stats<T, VEC, FULL, kBnAny>(p, slot, kBnX, w, param, root2);
     }
     if (lane == 0) {
-      sh.stats[w.slot].mean = mean;
-      sh.stats[w.slot].root = rsqrtf(square + p.eps);
+      sh.stats[w.slot].mean = v.x;
+      sh.stats[w.slot].root = rsqrtf(v.y + p.eps);
       sh.stats[w.slot].root2 = root2;
       mbar_arrive(smem_u32(&sh.ready[w.slot]));
     }
@@ -564,6 +605,13 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kern
         bn_vector<T>(p.gate ? p.gate + sample * p.gate_sb : nullptr, p.mod_f32, col, p.width, 1.f, g[k]);
         bn_vector<T>(p.scale ? p.scale + sample * p.scale_sb : nullptr, p.mod_f32, col, p.width, 0.f, a[k]);
         bn_vector<T>(p.shift ? p.shift + sample * p.shift_sb : nullptr, p.mod_f32, col, p.width, 0.f, c[k]);
+        if constexpr (FULL) {  // r = x + g m, with the branch's weight in g
+          if (p.branch_w != nullptr) {
+            bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, wt);
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[k][i] = fmul2(g[k][i], wt[i]);
+          }
+        }
         bn_vector<T>(p.norm_w, p.w_f32, col, p.width, 1.f, wt);
         bn_vector<T>(p.norm_b, p.w_f32, col, p.width, 0.f, bias);
 #pragma unroll
@@ -590,13 +638,14 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kern
         uint64_t m[N];
         bn_get<T, VEC>(p, slot, kBnBranch, w, q, m);
         if constexpr (FULL) {
-          if (p.branch_norm) {
-            uint64_t w2[N];
-            bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, w2);
 #pragma unroll
-            for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], fmul2(bn_both(st.root2), w2[i]));
+          for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], bn_both(st.root2));
+          if (p.in[kBnGate] != nullptr) {
+            uint64_t of[N];
+            bn_get_mod<T, VEC>(p, slot, kBnGate, w, q, of);
+#pragma unroll
+            for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], of[i]);
           }
-          if (p.in[kBnGate] != nullptr) bn_get_mod<T, VEC>(p, slot, kBnGate, w, q, g[k]);
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = ffma2(g[k][i], m[i], r[i]);
@@ -674,122 +723,143 @@ __device__ __forceinline__ void bn_stream_grad(const BlockNormParams& p, const u
   }
 }
 
+// The factor a of dn = e a: ones, the statistics' copy, or (kBnAny) from memory.
+template <typename T, int SRC, int N>
+__device__ __forceinline__ void bn_factor(const BlockNormParams& p, const float* param, const BnWalk& w, int q, uint64_t (&a)[N]) {
+  if constexpr (SRC == kBnScaled) {
+    bn_param_get(param, q, a);
+  } else if constexpr (SRC == kBnPlain) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = bn_both(1.f);
+  } else {
+    uint64_t wt[N];
+    bn_vector<T>(p.scale ? p.scale + w.b * p.scale_sb : nullptr, p.mod_f32, q * 2 * N, p.width, 0.f, a);
+    bn_vector<T>(p.norm_w, p.w_f32, q * 2 * N, p.width, 1.f, wt);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = fmul2(fadd2(a[i], bn_both(1.f)), wt[i]);
+  }
+}
+
+// Sums of dn and dn n over a row.
+template <typename T, bool VEC, bool FULL, int SRC>
+__device__ __forceinline__ float2 bn_row_dn(const BlockNormParams& p, const uint8_t* slot, const BnWalk& w, const BnStats& st,
+                                            const float* param) {
+  constexpr int CH = kBnChunk<T>, N = CH / 2;
+  uint64_t s1[N] = {}, s2[N] = {};
+#pragma unroll 2
+  for (int q = threadIdx.x & 31; q * CH < p.width; q += 32) {
+    uint64_t e[N], n[N], a[N];
+    bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
+    bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
+    bn_factor<T, SRC>(p, param, w, q, a);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint64_t dn = fmul2(e[i], a[i]);
+      s1[i] = fadd2(s1[i], dn);
+      s2[i] = ffma2(dn, n[i], s2[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    s1[0] = fadd2(s1[0], s1[i]);
+    s2[0] = fadd2(s2[0], s2[i]);
+  }
+  float sums[2] = {bn_total(s1[0]), bn_total(s2[0])};
+  bn_warp_sum(sums);
+  return make_float2(sums[0], sums[1]);
+}
+
+// The sum of dn2 n2 over a row.  The second vector of the statistics' copy is
+// what R is multiplied by to dn2, without a gate of each token.
+template <typename T, bool VEC, int SRC>
+__device__ __forceinline__ float bn_row_dn2(const BlockNormParams& p, const uint8_t* slot, const BnWalk& w, const BnStats& st,
+                                            const float* param) {
+  constexpr int CH = kBnChunk<T>, N = CH / 2;
+  uint64_t part[N] = {};
+  for (int q = threadIdx.x & 31; q * CH < p.width; q += 32) {
+    uint64_t e[N], n[N], a[N], big[N];
+    if (p.mode != DGXM_BLOCK_NORM_NONE) {
+      bn_normed<T, VEC, true>(p, slot, w, st, q, e, n);
+      bn_modulate<T, VEC, true>(p, slot, w, q, e);
+      if (SRC == kBnScaled && p.factor == 0) bn_factor<T, kBnPlain>(p, param, w, q, a);
+      else bn_factor<T, SRC>(p, param, w, q, a);
+    }
+    bn_stream_grad<T, VEC>(p, slot, w, st, q, e, n, a, big);
+    bn_get<T, VEC>(p, slot, kBnBranchB, w, q, n);
+    if (p.in[kBnGateB] != nullptr) {
+      bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, a);
+#pragma unroll
+      for (int i = 0; i < N; ++i) big[i] = fmul2(big[i], a[i]);
+    }
+    if constexpr (SRC == kBnScaled) {
+      bn_param_get(param + p.param_bytes / 8, q, a);
+    } else {
+      bn_vector<T>(p.gate ? p.gate + w.b * p.gate_sb : nullptr, p.mod_f32, q * CH, p.width, 1.f, a);
+      bn_vector<T>(p.branch_w, p.w_f32, q * CH, p.width, 1.f, e);
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] = fmul2(a[i], e[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i] = ffma2(fmul2(big[i], a[i]), n[i], part[i]);
+  }
+#pragma unroll
+  for (int i = 1; i < N; ++i) part[0] = fadd2(part[0], part[i]);
+  float sum[1] = {bn_total(part[0])};
+  bn_warp_sum(sum);
+  return sum[0] * st.root2;
+}
+
 template <typename T, bool VEC, bool FULL, int STAT>
 __device__ __forceinline__ void bn_backward_stats(const BlockNormParams& p, float* param, const uint8_t* ring, BnShared& sh,
                                                   int t) {
-  constexpr int CH = kBnChunk<T>, N = CH / 2;
   const int lane = t & 31;
-  // Rows in turn, by no more warps than there are slots: none waits for a phase
-  // of a slot whose last one is still open.
+  // Rows in turn, by no more warps than there are slots, whose number is a
+  // multiple: all rows of a slot are one warp's, so that none waits for a phase
+  // of a slot whose last one may still be open (rows land in any order).
   const int warps = min(STAT, p.slots);
   int turn = t >> 5 < warps ? t >> 5 : 0x7fffffff;  // rows until this warp's next
   const bool norm = p.mode != DGXM_BLOCK_NORM_NONE, layer = p.mode == DGXM_BLOCK_NORM_LAYER;
+  const bool post = FULL && p.branch_norm;
   int sample = -1;
   bool dead = false;
   for (BnWalk w(p); w.more(); w.next()) {
-    const char* const scale = p.scale ? p.scale + w.b * p.scale_sb : nullptr;
     if (w.b != sample) {
       sample = w.b;
-      bn_param<STAT>(p, param, t, [&](int c) {
-        const float up = scale ? 1.f + bn_value<T>(scale, p.mod_f32, c) : 1.f;
-        return p.norm_w ? up * bn_value<T>(p.norm_w, p.w_f32, c) : up;
+      const char* const scale = p.scale ? p.scale + sample * p.scale_sb : nullptr;
+      const int each = post ? p.param_bytes / 8 : p.param_bytes / 4;  // values of a vector
+      bn_param<STAT>(p, param, t, each, [&](int c, int which) {
+        if (which == 0) {
+          const float up = scale ? 1.f + bn_value<T>(scale, p.mod_f32, c) : 1.f;
+          return p.norm_w ? up * bn_value<T>(p.norm_w, p.w_f32, c) : up;
+        }
+        const float g = p.gate ? bn_value<T>(p.gate + sample * p.gate_sb, p.mod_f32, c) : 1.f;
+        return p.branch_w ? g * bn_value<T>(p.branch_w, p.w_f32, c) : g;
       });
     }
     if (turn-- > 0) continue;
     turn = warps - 1;
     bn_wait(&sh.full[w.slot], w.parity, dead);
     const uint8_t* slot = ring + w.slot * p.slot_bytes;
-    auto factor = [&](int q, uint64_t (&a)[N]) {  // dn = e a
-      if (p.param_bytes > 0) {
-        bn_param_get(param, q, a);
-        return;
-      }
-      uint64_t wt[N];
-      bn_vector<T>(scale, p.mod_f32, q * CH, p.width, 0.f, a);
-      bn_vector<T>(p.norm_w, p.w_f32, q * CH, p.width, 1.f, wt);
-#pragma unroll
-      for (int i = 0; i < N; ++i) a[i] = fmul2(fadd2(a[i], bn_both(1.f)), wt[i]);
-    };
     BnStats st;
     st.mean = st.root = st.m1 = st.m2 = st.m3 = 0.f;
     st.root2 = 1.f;
     if (norm) {
-      BnMoments moments;
-      uint64_t ss = 0;
-#pragma unroll 2
-    for (int q = lane; q * CH < p.width; q += 32) {
-        uint64_t r[N];
-        bn_get<T, VEC>(p, slot, kBnR, w, q, r);
-        if (layer) {
-          bn_add_chunk(moments, r, VEC ? CH : min(CH, p.width - q * CH));
-        } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) ss = ffma2(r[i], r[i], ss);
-        }
-      }
-      if (layer) {
-        const float2 v = bn_warp_moments(moments);
-        st.mean = v.x;
-        st.root = rsqrtf(v.y + p.eps);
-      } else {
-        float sum[1] = {bn_total(ss)};
-        bn_warp_sum(sum);
-        st.root = rsqrtf(fmaf(sum[0], p.inv_width, p.eps));
-      }
+      float2 v = bn_row_stats<T, VEC, FULL, kBnAlone>(p, slot, kBnR, w, param, 1.f);
+      st.mean = v.x;
+      st.root = rsqrtf(v.y + p.eps);
+      if (p.factor == 0) v = bn_row_dn<T, VEC, FULL, kBnPlain>(p, slot, w, st, param);
+      else if (p.param_bytes > 0) v = bn_row_dn<T, VEC, FULL, kBnScaled>(p, slot, w, st, param);
+      else v = bn_row_dn<T, VEC, FULL, kBnAny>(p, slot, w, st, param);
+      st.m1 = layer ? v.x * p.inv_width : 0.f;
+      st.m2 = v.y * p.inv_width;
     }
-    float sums[3];
-    uint64_t s1 = 0, s2 = 0, s3 = 0;
-#pragma unroll 2
-    for (int q = lane; q * CH < p.width; q += 32) {
-      if (norm) {
-        uint64_t e[N], n[N], a[N];
-        bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
-        bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
-        factor(q, a);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint64_t dn = fmul2(e[i], a[i]);
-          s1 = fadd2(s1, dn);
-          s2 = ffma2(dn, n[i], s2);
-        }
+    if constexpr (FULL) {
+      if (post) {
+        st.root2 = rsqrtf(bn_row_sums<T, VEC, FULL, false, kBnAlone>(p, slot, kBnBranchB, w, param, 1.f).y + p.eps);
+        const float sum = p.param_bytes > 0 ? bn_row_dn2<T, VEC, kBnScaled>(p, slot, w, st, param)
+                                            : bn_row_dn2<T, VEC, kBnAny>(p, slot, w, st, param);
+        st.m3 = sum * p.inv_width;
       }
-      if (FULL && p.branch_norm) {
-        uint64_t m[N];
-        bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
-#pragma unroll
-        for (int i = 0; i < N; ++i) s3 = ffma2(m[i], m[i], s3);
-      }
-    }
-    sums[0] = bn_total(s1);
-    sums[1] = bn_total(s2);
-    sums[2] = bn_total(s3);
-    bn_warp_sum(sums);
-    st.m1 = layer ? sums[0] * p.inv_width : 0.f;
-    st.m2 = sums[1] * p.inv_width;
-    if (FULL && p.branch_norm) {
-      st.root2 = rsqrtf(fmaf(sums[2], p.inv_width, p.eps));
-      uint64_t part = 0;
-#pragma unroll 2
-    for (int q = lane; q * CH < p.width; q += 32) {
-        uint64_t e[N], n[N], a[N], big[N], m[N], v[N];
-        if (norm) {
-          bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
-          bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
-          factor(q, a);
-        }
-        bn_stream_grad<T, VEC>(p, slot, w, st, q, e, n, a, big);
-        bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
-        if (p.in[kBnGateB] != nullptr) bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, v);
-        else bn_vector<T>(p.gate ? p.gate + w.b * p.gate_sb : nullptr, p.mod_f32, q * CH, p.width, 1.f, v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) big[i] = fmul2(fmul2(big[i], v[i]), m[i]);
-        bn_vector<T>(p.branch_w, p.w_f32, q * CH, p.width, 1.f, v);
-#pragma unroll
-        for (int i = 0; i < N; ++i) part = ffma2(fmul2(big[i], v[i]), bn_both(st.root2), part);
-      }
-      float inner[1] = {bn_total(part)};
-      bn_warp_sum(inner);
-      st.m3 = inner[0] * p.inv_width;
     }
     if (lane == 0) {
       sh.stats[w.slot] = st;
@@ -845,6 +915,13 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
         uint64_t wt[N];
         bn_vector<T>(p.gate ? p.gate + sample * p.gate_sb : nullptr, p.mod_f32, col, p.width, 1.f, g[k]);
         bn_vector<T>(p.scale ? p.scale + sample * p.scale_sb : nullptr, p.mod_f32, col, p.width, 0.f, a[k]);
+        if constexpr (FULL) {  // dn2 = R g, with the branch's weight in g
+          if (p.branch_w != nullptr) {
+            bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, wt);
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[k][i] = fmul2(g[k][i], wt[i]);
+          }
+        }
         bn_vector<T>(p.norm_w, p.w_f32, col, p.width, 1.f, wt);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -889,35 +966,30 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
       if (!branch) continue;
       uint64_t m[N];
       bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
-      bool own = false;  // f = dm
       if constexpr (FULL) {
 #pragma unroll
         for (int i = 0; i < N; ++i) m[i] = fmul2(m[i], bn_both(st.root2));
         if (p.in[kBnGateB] != nullptr) {
-          own = true;
-          bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, g[k]);
+          uint64_t of[N];
           if (p.g_gate != nullptr) {
-            uint64_t dg[N];
-            bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, dg);
 #pragma unroll
-            for (int i = 0; i < N; ++i) dg[i] = fmul2(fmul2(big[i], m[i]), dg[i]);
-            bn_store_mod<T, VEC>(p.g_gate, w.row, p.mod_f32, col, p.width, dg);
+            for (int i = 0; i < N; ++i) of[i] = fmul2(fmul2(big[i], m[i]), g[k][i]);
+            bn_store_mod<T, VEC>(p.g_gate, w.row, p.mod_f32, col, p.width, of);
           }
+          bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, of);
+#pragma unroll
+          for (int i = 0; i < N; ++i) big[i] = fmul2(big[i], of[i]);  // f = dm
         }
       }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const uint64_t dm = fmul2(big[i], g[k][i]);
-        acc[2][k][i] = ffma2(own ? dm : big[i], m[i], acc[2][k][i]);
-        big[i] = dm;
+        acc[2][k][i] = ffma2(big[i], m[i], acc[2][k][i]);
+        big[i] = fmul2(big[i], g[k][i]);
       }
       if (p.out == nullptr) continue;
       if (FULL && p.branch_norm) {
-        uint64_t w2[N];
-        bn_vector<T>(p.branch_w, p.w_f32, col, p.width, 1.f, w2);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          big[i] = fmul2(bn_both(st.root2), ffma2(m[i], bn_both(-st.m3), fmul2(big[i], w2[i])));
+        for (int i = 0; i < N; ++i) big[i] = fmul2(bn_both(st.root2), ffma2(m[i], bn_both(-st.m3), big[i]));
       }
       bn_store<T, VEC, true>(to_m, col, p.width, big);
     }
@@ -936,8 +1008,8 @@ struct BlockNormSumParams {
   void *g_gate, *g_scale, *g_shift, *g_norm_w, *g_norm_b, *g_branch_w;
   int gate_form, mod_form;  // of the modulations
   int want, dtype, mod_dtype, weight_dtype;
-  int batch, seq, width, blocks;
-  int64_t rows;
+  int batch, seq, width, rows_more;
+  int64_t rows, rows_each;
 };
 
 __device__ __forceinline__ float bn_any(const char* base, int dtype, int col, float fill) {
@@ -993,8 +1065,15 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
     // The blocks that hold rows of this sample.
     int64_t lo = 0, hi = 0;
     if (p.rows > 0) {
-      const int64_t each = p.rows / p.blocks, more = p.rows % p.blocks, longer = more * (each + 1);
-      auto block = [&](int64_t row) { return row < longer ? row / (each + 1) : more + (row - longer) / each; };
+      auto block = [&](int64_t row) -> int64_t {
+        if (p.rows <= 0x7fffffff) {
+          const uint32_t r = static_cast<uint32_t>(row), each = static_cast<uint32_t>(p.rows_each);
+          const uint32_t more = p.rows_more, longer = more * (each + 1);
+          return r < longer ? r / (each + 1) : more + (r - longer) / each;
+        }
+        const int64_t longer = p.rows_more * (p.rows_each + 1);
+        return row < longer ? row / (p.rows_each + 1) : p.rows_more + (row - longer) / p.rows_each;
+      };
       lo = block(static_cast<int64_t>(b) * p.seq);
       hi = block(static_cast<int64_t>(b) * p.seq + p.seq - 1) + 1;
     }
@@ -1135,8 +1214,8 @@ static void bn_stream(BlockNormParams* p, int s, const void* base, const int64_t
 
 // Place the streams of a row in a slot of the ring, and as many slots as the
 // block's share of the shared memory holds.  `slack`: 16 bytes each for rows
-// off 16 bytes.  `param`: the statistics want a copy of a column vector.
-static void bn_layout(const dgxm_block_norm_desc* d, const BnCut& cut, BlockNormParams* p, bool param, bool slack) {
+// off 16 bytes.  `stat`: warps that take statistics; `vectors`: column vectors that the statistics want a copy of.
+static void bn_layout(const dgxm_block_norm_desc* d, const BnCut& cut, BlockNormParams* p, int stat, int vectors, bool slack) {
   const int ch = d->dtype == DGXM_DTYPE_F32 ? 4 : 8;
   const int padded = (d->width + ch - 1) / ch * ch, room = (224 / cut.per_sm - 4) * 1024;  // beside the static part
   int at = 0;
@@ -1147,9 +1226,10 @@ static void bn_layout(const dgxm_block_norm_desc* d, const BnCut& cut, BlockNorm
     at += p->in_pitch[s];
   }
   p->slot_bytes = at;
-  // the copy only where it leaves three slots (its reader can do without)
-  p->param_bytes = param && 3 * at + padded * 4 <= room ? padded * 4 : 0;
+  // copies only where they leave three slots (their readers can do without)
+  p->param_bytes = 3 * at + vectors * padded * 4 <= room ? vectors * padded * 4 : 0;
   p->slots = std::max(1, std::min(kBnMaxSlots, (room - p->param_bytes) / at));
+  if (p->slots > stat) p->slots -= p->slots % stat;
 }
 
 // Every row of every stream and output on 16 bytes.
@@ -1180,7 +1260,9 @@ static int bn_launch_as(const dgxm_block_norm_desc* d, BlockNormParams& p, cudaS
   const BnCut cut = bn_cut<BACK>(d);
   p.rows_each = p.rows / cut.blocks;
   p.rows_more = static_cast<int>(p.rows % cut.blocks);
-  bn_layout(d, cut, &p, BACK ? p.scale != nullptr || p.norm_w != nullptr : p.gate != nullptr, !VEC);
+  const bool forward_copy = p.gate != nullptr || p.branch_w != nullptr;
+  p.factor = BACK && (p.scale != nullptr || p.norm_w != nullptr);
+  bn_layout(d, cut, &p, K::kStat, BACK ? (p.branch_norm ? 2 : p.factor) : forward_copy, !VEC);
   DGXM_CUDA_TRY(set_smem_limit_once(kernel, 220 * 1024, done));
   DGXM_CUDA_TRY(launch_overlapped(kernel, cut.blocks, cut.threads + 32 * K::kStat + 32,
                                   p.param_bytes + p.slots * p.slot_bytes, st, p));
@@ -1383,8 +1465,11 @@ extern "C" int dgxm_block_norm_backward(const dgxm_block_norm_desc* d, const dgx
   sp.batch = d->batch;
   sp.seq = d->seq;
   sp.width = d->width;
-  sp.blocks = blocks;
   sp.rows = rows;
+  if (blocks > 0) {
+    sp.rows_each = rows / blocks;
+    sp.rows_more = static_cast<int>(rows % blocks);
+  }
   DGXM_CUDA_TRY(launch_overlapped(block_norm_sum_kernel, (d->width + 31) / 32, kBnSumWarps * 32, 0, st, sp));
   return DGXM_OK;
 }
