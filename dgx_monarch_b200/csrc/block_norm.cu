@@ -49,7 +49,7 @@ struct BlockNormParams {
   int in_elt[kBnMaxIn];      // bytes of a value: 4 for a modulation of fp32 beside 16-bit tensors
   int in_off[kBnMaxIn];      // bytes into the stage
   int in_pitch[kBnMaxIn];    // bytes of a row in the stage, a multiple of 16
-  int n_in, slot_bytes, slots, param_bytes;  // the ring, behind the statistics' copy of a column vector
+  int n_in, slot_bytes, slots, param_bytes, stage_bytes;  // the ring, behind the statistics' copies, before the warps' staging
   // Values of a column that serve every row of a sample (gate, scale, shift), or all rows; NULL: absent
   const char *gate, *scale, *shift, *norm_w, *norm_b, *branch_w;
   int64_t gate_sb, scale_sb, shift_sb;  // bytes between samples
@@ -184,59 +184,75 @@ __device__ __forceinline__ void bn_vector(const char* base, int f32, int col, in
   }
 }
 
-// Store N pairs of a row from column `col` on.  Off 16 bytes (!VEC) and with
-// neighbouring chunks in neighbouring lanes (NEXT), a lane stores the aligned
-// word that its chunk shares with the next lane's, and single values only
-// where there is none: at the ends of the warp's chunks and of the row.
-template <typename T, bool VEC, bool NEXT, int N>
-__device__ __forceinline__ void bn_store(char* row, int col, int width, const uint64_t (&v)[N]) {
+// Bytes of a warp's staging for rows off 16 bytes: its chunks, and 16 more.
+constexpr int kBnStage = 33 * 16;
+
+// Store N pairs of a row from column `col` on.  Off 16 bytes (!VEC) the warp's
+// chunks, neighbours in the row, pass through its staging: a lane stores an
+// aligned word out of two of them, and the few values before the first word
+// and behind the last go one by one.  (With the values of every chunk behind
+// conditions of their own a row took 8000 cycles instead of 2000.)
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void bn_store(char* row, int col, int width, const uint64_t (&v)[N], uint8_t* stage) {
   float f[2 * N];
 #pragma unroll
   for (int i = 0; i < N; ++i) upk2(v[i], f[2 * i], f[2 * i + 1]);
-  constexpr int CH = kBnChunk<T>;
-  if constexpr (!VEC && !(NEXT && 2 * N == CH)) {
+  constexpr int CH = 2 * N, kElt = static_cast<int>(sizeof(T)), kWords = CH * kElt / 16;
+  uint4 w[kWords];
 #pragma unroll
-    for (int i = 0; i < 2 * N; ++i)
-      if (col + i < width) reinterpret_cast<T*>(row)[col + i] = qk_narrow<T>(f[i]);
-  } else if constexpr (sizeof(T) == 4 && VEC) {
-#pragma unroll
-    for (int i = 0; i < 2 * N; i += 4)
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(row) + col + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-  } else {
-    uint4 w;
-    if constexpr (sizeof(T) == 4) {
-      w = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  for (int k = 0; k < kWords; ++k) {
+    const float* g = f + k * (16 / kElt);
+    if constexpr (kElt == 4) {
+      w[k] = make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3]));
     } else {
       constexpr bool kHalf = std::is_same<T, __half>::value;
-      static_assert(2 * N == CH, "one chunk");
-      w = make_uint4(pack16<kHalf>(f[0], f[1]), pack16<kHalf>(f[2], f[3]), pack16<kHalf>(f[4], f[5]), pack16<kHalf>(f[6], f[7]));
+      w[k] = make_uint4(pack16<kHalf>(g[0], g[1]), pack16<kHalf>(g[2], g[3]), pack16<kHalf>(g[4], g[5]), pack16<kHalf>(g[6], g[7]));
     }
-    T* to = reinterpret_cast<T*>(row) + col;
-    const uint32_t off = VEC ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) & 15u;
-    if (VEC || (off == 0 && col + CH <= width)) {
-      *reinterpret_cast<uint4*>(to) = w;
-      if (VEC) return;
-    }
-    // The lanes with a chunk of the row are the first ones of the warp.
-    const int lane = threadIdx.x & 31, lanes = min(32, (width - (col - lane * CH) + CH - 1) / CH);
-    const uint32_t mask = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u;
-    const uint4 n = make_uint4(__shfl_down_sync(mask, w.x, 1), __shfl_down_sync(mask, w.y, 1),
-                               __shfl_down_sync(mask, w.z, 1), __shfl_down_sync(mask, w.w, 1));
-    if (off == 0 && col + CH <= width) return;
-    const int head = off == 0 ? CH : static_cast<int>((16u - off) / sizeof(T));  // values before the aligned word
-    const bool before = off != 0 && lane > 0 && col + head <= width;  // they are the lane before's
-    const bool shared = off != 0 && lane < 31 && col + CH + head <= width;
-    if (shared) *reinterpret_cast<uint4*>(to + head) = fp4_bytes_from(w, n, 16u - off);
+  }
+  if constexpr (VEC) {
+    uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<T*>(row) + col);
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (col + i < width && (i < head ? !before : !shared)) to[i] = qk_narrow<T>(f[i]);
+    for (int k = 0; k < kWords; ++k) to[k] = w[k];
+  } else {
+    using Elt = typename std::conditional<kElt == 4, uint32_t, uint16_t>::type;
+    const int lane = threadIdx.x & 31, first = col - lane * CH;
+    // The lanes with a chunk of the row are the first ones of the warp.
+    const int lanes = min(32, (width - first + CH - 1) / CH);
+    const uint32_t mask = lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {  // (chunks of 32 bytes: first halves, then second ones)
+      char* const to = row + static_cast<int64_t>(first) * kElt;
+      if constexpr (kWords == 1) {
+        reinterpret_cast<uint4*>(stage)[lane] = w[0];
+        __syncwarp(mask);
+        const int bytes = min(lanes * CH, width - first) * kElt;
+        const int head = min(static_cast<int>(-reinterpret_cast<uintptr_t>(to) & 15u), bytes);
+        const int words = (bytes - head) / 16, end = head + 16 * words;
+        if (lane < words) {
+          const uint4 a = reinterpret_cast<const uint4*>(stage)[lane];
+          *reinterpret_cast<uint4*>(to + head + 16 * lane) =
+              head ? fp4_bytes_from(a, reinterpret_cast<const uint4*>(stage)[lane + 1], head) : a;
+        }
+        for (int at = lane * kElt; at < head; at += lanes * kElt)
+          *reinterpret_cast<Elt*>(to + at) = *reinterpret_cast<const Elt*>(stage + at);
+        for (int at = end + lane * kElt; at < bytes; at += lanes * kElt)
+          *reinterpret_cast<Elt*>(to + at) = *reinterpret_cast<const Elt*>(stage + at);
+        __syncwarp(mask);
+      } else {
+        const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + 4 * k + i < width) reinterpret_cast<uint32_t*>(row)[col + 4 * k + i] = u[i];
+      }
+    }
   }
 }
 
 template <typename T, bool VEC, int N>
-__device__ __forceinline__ void bn_store_mod(char* base, int64_t row, int f32, int col, int width, const uint64_t (&v)[N]) {
-  if (f32) bn_store<float, VEC, false>(base + row * width * 4, col, width, v);
-  else bn_store<T, VEC, true>(base + row * width * static_cast<int>(sizeof(T)), col, width, v);
+__device__ __forceinline__ void bn_store_mod(char* base, int64_t row, int f32, int col, int width, const uint64_t (&v)[N],
+                                             uint8_t* stage) {
+  if (f32) bn_store<float, VEC>(base + row * width * 4, col, width, v, stage);
+  else bn_store<T, VEC>(base + row * width * static_cast<int>(sizeof(T)), col, width, v, stage);
 }
 
 // A block's rows: contiguous, one after the other.
@@ -593,6 +609,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kern
   }
   const bool branch = p.in[kBnBranch] != nullptr, norm = p.mode != DGXM_BLOCK_NORM_NONE;
   uint64_t g[NV][N], a[NV][N], c[NV][N];
+  uint8_t* const stage = ring + p.slots * p.slot_bytes + (t >> 5) * kBnStage;  // (where !VEC)
   int sample = -1;
   bool dead = false;
   for (BnWalk w(p); w.more(); w.next()) {
@@ -649,7 +666,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kern
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) r[i] = ffma2(g[k][i], m[i], r[i]);
-        bn_store<T, VEC, true>(to_r, col, p.width, r);
+        bn_store<T, VEC>(to_r, col, p.width, r, stage);
       }
       if (!norm) continue;
 #pragma unroll
@@ -668,7 +685,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kern
           for (int i = 0; i < N; ++i) r[i] = fadd2(r[i], s[i]);
         }
       }
-      bn_store<T, VEC, true>(to_y, col, p.width, r);
+      bn_store<T, VEC>(to_y, col, p.width, r, stage);
     }
     __syncwarp();
     if ((t & 31) == 0) mbar_arrive(smem_u32(&sh.empty[w.slot]));
@@ -892,6 +909,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
   }
   const bool branch = p.in[kBnBranchB] != nullptr, norm = p.mode != DGXM_BLOCK_NORM_NONE;
   uint64_t g[NV][N], a[NV][N], acc[3][NV][N];
+  uint8_t* const stage = ring + p.slots * p.slot_bytes + (t >> 5) * kBnStage;  // (where !VEC)
   int sample = -1;
   bool dead = false;
   auto flush = [&]() {
@@ -902,7 +920,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
       char* to = reinterpret_cast<char*>(p.partial + ((blockIdx.x + static_cast<int64_t>(sample)) * 3 + j) * p.width);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (const int col = (t + k * threads) * CH; col < p.width) bn_store<float, VEC, false>(to, col, p.width, acc[j][k]);
+        if (const int col = (t + k * threads) * CH; col < p.width) bn_store<float, VEC>(to, col, p.width, acc[j][k], stage);
     }
   };
   for (BnWalk w(p); w.more(); w.next()) {
@@ -950,9 +968,9 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
             bn_vector<T>(p.norm_b, p.w_f32, col, p.width, 0.f, bias);
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = fmul2(e[i], ffma2(n[i], h[i], bias[i]));
-            bn_store_mod<T, VEC>(p.g_scale, w.row, p.mod_f32, col, p.width, h);
+            bn_store_mod<T, VEC>(p.g_scale, w.row, p.mod_f32, col, p.width, h, stage);
           }
-          if (p.g_shift != nullptr) bn_store_mod<T, VEC>(p.g_shift, w.row, p.mod_f32, col, p.width, e);
+          if (p.g_shift != nullptr) bn_store_mod<T, VEC>(p.g_shift, w.row, p.mod_f32, col, p.width, e, stage);
         }
         bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
 #pragma unroll
@@ -962,7 +980,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
         }
       }
       bn_stream_grad<T, VEC>(p, slot, w, st, q, e, n, a[k], big);
-      if (p.x_out != nullptr) bn_store<T, VEC, true>(to_x, col, p.width, big);
+      if (p.x_out != nullptr) bn_store<T, VEC>(to_x, col, p.width, big, stage);
       if (!branch) continue;
       uint64_t m[N];
       bn_get<T, VEC>(p, slot, kBnBranchB, w, q, m);
@@ -974,7 +992,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
           if (p.g_gate != nullptr) {
 #pragma unroll
             for (int i = 0; i < N; ++i) of[i] = fmul2(fmul2(big[i], m[i]), g[k][i]);
-            bn_store_mod<T, VEC>(p.g_gate, w.row, p.mod_f32, col, p.width, of);
+            bn_store_mod<T, VEC>(p.g_gate, w.row, p.mod_f32, col, p.width, of, stage);
           }
           bn_get_mod<T, VEC>(p, slot, kBnGateB, w, q, of);
 #pragma unroll
@@ -991,7 +1009,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
 #pragma unroll
         for (int i = 0; i < N; ++i) big[i] = fmul2(bn_both(st.root2), ffma2(m[i], bn_both(-st.m3), big[i]));
       }
-      bn_store<T, VEC, true>(to_m, col, p.width, big);
+      bn_store<T, VEC>(to_m, col, p.width, big, stage);
     }
     __syncwarp();
     if ((t & 31) == 0) mbar_arrive(smem_u32(&sh.empty[w.slot]));
@@ -1043,13 +1061,7 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
   const float w2 = in ? bn_any(p.branch_w, p.weight_dtype, col, 1.f) : 0.f;
   const bool many = p.batch >= kBnSumWarps;
   float all[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // shift, scale, gate, norm_b, norm_w, branch_w over samples
-  auto finish = [&](int b, const float (&s)[3]) {
-    const float up = p.mod_form == DGXM_MOD_TOKEN || p.scale == nullptr || !in
-                         ? 1.f
-                         : 1.f + bn_any(p.scale + b * p.scale_sb, p.mod_dtype, col, 0.f);
-    const float gate = p.gate_form == DGXM_MOD_TOKEN || p.gate == nullptr || !in
-                           ? 1.f
-                           : bn_any(p.gate + b * p.gate_sb, p.mod_dtype, col, 0.f);
+  auto finish = [&](int b, const float (&s)[3], float up, float gate) {
     const float v[6] = {s[0], fmaf(w, s[1], bias * s[0]), w2 * s[2], up * s[0], up * s[1], gate * s[2]};
     if (in && p.mod_form == DGXM_MOD_SAMPLE) {
       bn_put(p.g_shift, p.mod_dtype, static_cast<int64_t>(b) * p.width + col, v[0]);
@@ -1062,6 +1074,9 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
   };
   for (int b = many ? warp : 0; b < p.batch; b += many ? kBnSumWarps : 1) {
     float s[3] = {0.f, 0.f, 0.f};
+    const bool mine = in && (many || warp == 0);
+    const float up = !mine || p.scale == nullptr ? 1.f : 1.f + bn_any(p.scale + b * p.scale_sb, p.mod_dtype, col, 0.f);
+    const float gate = !mine || p.gate == nullptr ? 1.f : bn_any(p.gate + b * p.gate_sb, p.mod_dtype, col, 0.f);
     // The blocks that hold rows of this sample.
     int64_t lo = 0, hi = 0;
     if (p.rows > 0) {
@@ -1080,16 +1095,22 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
     const int64_t i0 = many ? lo : lo + (hi - lo) * warp / kBnSumWarps;
     const int64_t i1 = many ? hi : lo + (hi - lo) * (warp + 1) / kBnSumWarps;
     if (in) {
+      for (int64_t i = i0; i < i1; i += 4) {  // up to twelve loads under way
+        float v[4][3];
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        if (!(p.want >> j & 1)) continue;
-        const float* from = p.partial + ((i0 + b) * 3 + j) * p.width + col;
-#pragma unroll 4
-        for (int64_t i = i0; i < i1; ++i, from += 3 * static_cast<int64_t>(p.width)) s[j] += *from;
+        for (int u = 0; u < 4; ++u) {
+          const float* from = p.partial + (min(i + u, i1 - 1) + b) * 3 * p.width + col;
+#pragma unroll
+          for (int j = 0; j < 3; ++j) v[u][j] = (p.want >> j & 1) && i + u < i1 ? from[j * p.width] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int j = 0; j < 3; ++j) s[j] += v[u][j];
       }
     }
     if (many) {
-      finish(b, s);
+      finish(b, s, up, gate);
     } else {
 #pragma unroll
       for (int j = 0; j < 3; ++j) part[warp][j][lane] = s[j];
@@ -1099,7 +1120,7 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
         for (int k = 0; k < kBnSumWarps; ++k)
 #pragma unroll
           for (int j = 0; j < 3; ++j) t[j] += part[k][j][lane];
-        finish(b, t);
+        finish(b, t, up, gate);
       }
       __syncthreads();
     }
@@ -1217,7 +1238,10 @@ static void bn_stream(BlockNormParams* p, int s, const void* base, const int64_t
 // off 16 bytes.  `stat`: warps that take statistics; `vectors`: column vectors that the statistics want a copy of.
 static void bn_layout(const dgxm_block_norm_desc* d, const BnCut& cut, BlockNormParams* p, int stat, int vectors, bool slack) {
   const int ch = d->dtype == DGXM_DTYPE_F32 ? 4 : 8;
-  const int padded = (d->width + ch - 1) / ch * ch, room = (224 / cut.per_sm - 4) * 1024;  // beside the static part
+  const int padded = (d->width + ch - 1) / ch * ch;
+  int room = (224 / cut.per_sm - 4) * 1024;  // beside the static part
+  p->stage_bytes = slack ? cut.threads / 32 * kBnStage : 0;
+  room -= p->stage_bytes;
   int at = 0;
   for (int s = 0; s < p->n_in; ++s) {
     p->in_off[s] = at;
@@ -1265,7 +1289,7 @@ static int bn_launch_as(const dgxm_block_norm_desc* d, BlockNormParams& p, cudaS
   bn_layout(d, cut, &p, K::kStat, BACK ? (p.branch_norm ? 2 : p.factor) : forward_copy, !VEC);
   DGXM_CUDA_TRY(set_smem_limit_once(kernel, 220 * 1024, done));
   DGXM_CUDA_TRY(launch_overlapped(kernel, cut.blocks, cut.threads + 32 * K::kStat + 32,
-                                  p.param_bytes + p.slots * p.slot_bytes, st, p));
+                                  p.param_bytes + p.slots * p.slot_bytes + p.stage_bytes, st, p));
   return DGXM_OK;
 }
 
