@@ -17,7 +17,8 @@ namespace dgxm {
 
 // About one second at the B200 boost clock.  A correct kernel waits a few
 // microseconds on a barrier phase, or as long as one tile's products take: at
-// the most 33 ms, behind the 4-bit product's longest K (2^24 columns).
+// the most some 130 ms, behind the 16-bit product's longest K (2^24: 262,144
+// stages of 64, each below 0.5 us; the 4-bit product's takes 33 ms).
 constexpr long long kWaitBudgetCycles = 2000000000LL;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -128,6 +129,14 @@ __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bu
 // 16 bytes global -> this CTA's shared memory, asynchronously (L2 only).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// Wait until at most PENDING of this thread's newest committed groups are under way.
+template <int PENDING>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
 // Wait for every cp_async16 this thread issued.

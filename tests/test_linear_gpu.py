@@ -233,6 +233,27 @@ def test_activations_at_the_ends_of_the_range(name):
     assert ((got.double() - want).abs() <= 2.0 ** -20 * z.double().abs()).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("name", ["silu", "gelu", "gelu_tanh"])
+def test_slopes_at_the_ends_of_the_range(name, dtype):
+    """dz of one value a row, x's gradient behind a w of one column of ones: the slope rounded once, 0 or 1 far out."""
+    from dgx_monarch_b200.linear import linear_backward
+
+    top = torch.finfo(dtype).max
+    z = torch.tensor([[-float("inf"), -top, -1e4, -100.0, -20.0, -8.0, -0.75, -0.0, 0.0, 0.75, 8.0, 20.0, 100.0, 1e4, top,
+                       float("inf"), float("nan")]], device="cuda").to(dtype).t().contiguous()
+    w = torch.zeros(1, 8, device="cuda", dtype=dtype)
+    w[0, 0] = 1
+    grads = linear_backward(torch.ones_like(z), torch.zeros(z.shape[0], 8, device="cuda", dtype=dtype), w, activation=name,
+                            pre=z, w_grad=False)
+    leaf = z.double().clamp(-1e4, 1e4).requires_grad_(True)
+    act(leaf, name).sum().backward()
+    got, want = grads.x[:, 0].double(), leaf.grad[:, 0]
+    assert torch.isnan(got[-1])
+    # A rounding; fp32's slope loses 2^-19 of its value where e^-z does (z up to 20), a fp16 of 2^-24 is zero or itself.
+    assert ((got - want).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -18) * want.abs() + 2.0 ** -25)[:-1].all(), (got, want)
+
+
 def test_gradients_against_differences_of_the_kernel():
     """fp32 outputs, sixteen-bit steps: the Linear is linear in x, w and bias up to the activation; with steps of 2^-4 of
     the 16-bit arguments the third derivative leaves h^2, the sums 2^-20."""

@@ -219,3 +219,41 @@ def test_output_checks(monkeypatch, lib):
     assert all(g is None for g in ln.linear_backward(_t(2, 4, 8), x, w, x_grad=False, w_grad=False))
     with pytest.raises(RuntimeError, match="no_grad"):
         ln.linear(x, w.float().requires_grad_(True).bfloat16())
+
+
+def test_long_contractions_of_a_gradient(lib):
+    """w's gradient is a product along m: as long as k may be, no longer; the other gradients take any m."""
+    from dgx_monarch_b200 import _lib
+
+    d = _desc(m=2 ** 24 + 64, n=8, out_stride=8, k=8, x_stride=8, w_stride=8)
+    assert _backward(lib, d, {"w": FAKE}) == 2 and "2^24" in lib.dgxm_last_error_message().decode()
+    need = lambda **g: lib.dgxm_linear_backward_workspace(d, _lib.LinearGradPointers(**g), FAKE, FAKE, FAKE)
+    assert need(w=FAKE) == -1 and need(x=FAKE) >= 0 and need(bias=FAKE) > 0
+    d.m = 2 ** 24
+    assert need(w=FAKE) >= 0
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc is absent")
+def test_struct_layouts(tmp_path):
+    """Sizes and offsets of the new descriptors, as gcc lays out the header's."""
+    import ctypes
+    import subprocess
+    from pathlib import Path
+
+    from dgx_monarch_b200 import _lib
+
+    header = Path(__file__).resolve().parents[1] / "include" / "dgxm_sp.h"
+    structs = {"dgxm_block_norm_desc": _lib.BlockNormDesc, "dgxm_block_norm_grads": _lib.BlockNormGradPointers,
+               "dgxm_linear_desc": _lib.LinearDesc, "dgxm_linear_grads": _lib.LinearGradPointers}
+    lines, want = [], []
+    for name, cls in structs.items():
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        want.append(ctypes.sizeof(cls))
+        for field, _ in cls._fields_:
+            lines.append(f'printf("%zu\\n", offsetof({name}, {field}));')
+            want.append(getattr(cls, field).offset)
+    source = tmp_path / "layout.c"
+    source.write_text(f'#include <stdio.h>\n#include <stddef.h>\n#include "{header}"\nint main(void) {{ {" ".join(lines)} return 0; }}\n')
+    subprocess.run(["gcc", "-std=c11", "-o", str(tmp_path / "layout"), str(source)], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
+    assert [int(v) for v in out.split()] == want
