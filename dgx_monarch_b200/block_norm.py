@@ -161,8 +161,10 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor | None = None, *, gate: tor
     and branch_w: (C,) of x's dtype or fp32.  gate, scale and shift, of x's
     dtype or fp32: (C,), (B, C), (B, 1, C), or (B, L, C) with values for each
     token; scale and shift of one form.  Sums are fp32, each output is rounded
-    once, and the norm is of the sum before its rounding.  A row with a NaN or
-    an infinity gives NaN; one whose squares leave fp32's range, zero.
+    once, and the norm is of the sum before its rounding.  A NaN makes its row's
+    norm NaN; an infinity makes NORM_LAYER's row NaN, in NORM_RMS itself NaN and
+    the row's other values zero.  Where a row's squares leave fp32's range
+    (values above 1e18) its norm is zero, or NaN where its sum does too.
 
     x_out and out may each be x or branch themselves (same strides); they must
     not overlap the inputs, or each other, in any other way.  No autograd graph

@@ -1046,9 +1046,9 @@ __device__ __forceinline__ void bn_put(void* base, int dtype, int64_t at, float 
 
 constexpr int kBnSumWarps = 32;
 
-// A block takes 32 columns.  Its warps take the samples in turn where there
-// are many, or else share out the blocks of each; warp 0 adds their sums in
-// order.
+// A block takes 32 columns.  Its warps form groups of equal size, up to one a
+// sample; a group shares out the blocks with rows of a sample, and then takes
+// another.  Sums of warps are added in order.
 __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const __grid_constant__ BlockNormSumParams p) {
   __shared__ float part[kBnSumWarps][6][32];
   pdl_launch_dependents();
@@ -1059,7 +1059,9 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
   const float w = in ? bn_any(p.norm_w, p.weight_dtype, col, 1.f) : 0.f;
   const float bias = in ? bn_any(p.norm_b, p.weight_dtype, col, 0.f) : 0.f;
   const float w2 = in ? bn_any(p.branch_w, p.weight_dtype, col, 1.f) : 0.f;
-  const bool many = p.batch >= kBnSumWarps;
+  int groups = 1;
+  while (groups < kBnSumWarps && groups < p.batch) groups *= 2;
+  const int each = kBnSumWarps / groups, group = warp / each, turn = warp % each;
   float all[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // shift, scale, gate, norm_b, norm_w, branch_w over samples
   auto finish = [&](int b, const float (&s)[3], float up, float gate) {
     const float v[6] = {s[0], fmaf(w, s[1], bias * s[0]), w2 * s[2], up * s[0], up * s[1], gate * s[2]};
@@ -1072,14 +1074,16 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
 #pragma unroll
     for (int j = 0; j < 6; ++j) all[j] += v[j];
   };
-  for (int b = many ? warp : 0; b < p.batch; b += many ? kBnSumWarps : 1) {
+  for (int64_t b0 = 0; b0 < p.batch; b0 += groups) {
+    const bool there = b0 + group < p.batch;
+    const int b = there ? static_cast<int>(b0) + group : 0;
     float s[3] = {0.f, 0.f, 0.f};
-    const bool mine = in && (many || warp == 0);
+    const bool mine = in && there && turn == 0;
     const float up = !mine || p.scale == nullptr ? 1.f : 1.f + bn_any(p.scale + b * p.scale_sb, p.mod_dtype, col, 0.f);
     const float gate = !mine || p.gate == nullptr ? 1.f : bn_any(p.gate + b * p.gate_sb, p.mod_dtype, col, 0.f);
     // The blocks that hold rows of this sample.
     int64_t lo = 0, hi = 0;
-    if (p.rows > 0) {
+    if (p.rows > 0 && there) {
       auto block = [&](int64_t row) -> int64_t {
         if (p.rows <= 0x7fffffff) {
           const uint32_t r = static_cast<uint32_t>(row), each = static_cast<uint32_t>(p.rows_each);
@@ -1092,8 +1096,7 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
       lo = block(static_cast<int64_t>(b) * p.seq);
       hi = block(static_cast<int64_t>(b) * p.seq + p.seq - 1) + 1;
     }
-    const int64_t i0 = many ? lo : lo + (hi - lo) * warp / kBnSumWarps;
-    const int64_t i1 = many ? hi : lo + (hi - lo) * (warp + 1) / kBnSumWarps;
+    const int64_t i0 = lo + (hi - lo) * turn / each, i1 = lo + (hi - lo) * (turn + 1) / each;
     if (in) {
       for (int64_t i = i0; i < i1; i += 4) {  // up to twelve loads under way
         float v[4][3];
@@ -1109,23 +1112,22 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
           for (int j = 0; j < 3; ++j) s[j] += v[u][j];
       }
     }
-    if (many) {
-      finish(b, s, up, gate);
-    } else {
+    if (each > 1) {
 #pragma unroll
       for (int j = 0; j < 3; ++j) part[warp][j][lane] = s[j];
       __syncthreads();
-      if (warp == 0) {
-        float t[3] = {0.f, 0.f, 0.f};
-        for (int k = 0; k < kBnSumWarps; ++k)
+      if (turn == 0) {
 #pragma unroll
-          for (int j = 0; j < 3; ++j) t[j] += part[k][j][lane];
-        finish(b, t, up, gate);
+        for (int j = 0; j < 3; ++j) s[j] = 0.f;
+        for (int k = 0; k < each; ++k)
+#pragma unroll
+          for (int j = 0; j < 3; ++j) s[j] += part[warp + k][j][lane];
       }
       __syncthreads();
     }
+    if (there && turn == 0) finish(b, s, up, gate);
   }
-  if (many) {
+  if (groups > 1) {
 #pragma unroll
     for (int j = 0; j < 6; ++j) part[warp][j][lane] = all[j];
     __syncthreads();
@@ -1133,7 +1135,7 @@ __global__ void __launch_bounds__(kBnSumWarps * 32) block_norm_sum_kernel(const 
 #pragma unroll
       for (int j = 0; j < 6; ++j) {
         all[j] = 0.f;
-        for (int k = 0; k < kBnSumWarps; ++k) all[j] += part[k][j][lane];
+        for (int k = 0; k < groups; ++k) all[j] += part[k * each][j][lane];
       }
   }
   if (warp != 0 || !in) return;
@@ -1165,6 +1167,21 @@ static int bn_check(const dgxm_block_norm_desc* d) {
   if (d->norm_mode == DGXM_BLOCK_NORM_NONE && d->mod_form != DGXM_MOD_NONE)
     return fail(DGXM_ERR_INVALID, "a scale or shift without a norm");
   return DGXM_OK;
+}
+
+// Samples of one row each are the rows of one sample: what serves a sample
+// serves a token then, and comes with the rows instead of between them.
+static const dgxm_block_norm_desc* bn_fold(const dgxm_block_norm_desc* d, dgxm_block_norm_desc* as) {
+  if (d->seq != 1 || d->batch <= 1) return d;
+  *as = *d;
+  as->batch = 1;
+  as->seq = d->batch;
+  for (int64_t* stride : {as->x_stride, as->branch_stride, as->gate_stride, as->scale_stride, as->shift_stride, as->x_out_stride,
+                          as->out_stride, as->dy_stride, as->dx_out_stride})
+    stride[1] = stride[0];
+  for (int* form : {&as->gate_form, &as->mod_form})
+    if (*form == DGXM_MOD_SAMPLE) *form = DGXM_MOD_TOKEN;
+  return as;
 }
 
 static int64_t bn_rows(const dgxm_block_norm_desc* d) { return static_cast<int64_t>(d->batch) * d->seq; }
@@ -1323,6 +1340,8 @@ extern "C" int dgxm_block_norm(const dgxm_block_norm_desc* d, const void* x, con
                                const void* branch_w, void* x_out, void* out, void* stream) {
   using namespace dgxm;
   if (int rc = bn_check(d)) return rc;
+  dgxm_block_norm_desc folded;
+  d = bn_fold(d, &folded);
   if (bn_rows(d) == 0) return DGXM_OK;  // empty tensors may be NULL
   const bool norm = d->norm_mode != DGXM_BLOCK_NORM_NONE;
   if ((branch == nullptr) != (x_out == nullptr)) return fail(DGXM_ERR_INVALID, "a branch and x_out come together");
@@ -1378,6 +1397,8 @@ extern "C" int dgxm_block_norm(const dgxm_block_norm_desc* d, const void* x, con
 extern "C" int64_t dgxm_block_norm_backward_workspace(const dgxm_block_norm_desc* d) {
   using namespace dgxm;
   if (bn_check(d)) return -1;
+  dgxm_block_norm_desc folded;
+  d = bn_fold(d, &folded);
   return bn_rows(d) == 0 ? 0 : bn_partial_bytes(d);
 }
 
@@ -1388,6 +1409,8 @@ extern "C" int dgxm_block_norm_backward(const dgxm_block_norm_desc* d, const dgx
   using namespace dgxm;
   if (int rc = bn_check(d)) return rc;
   if (g == nullptr) return fail(DGXM_ERR_INVALID, "NULL gradients");
+  dgxm_block_norm_desc folded;
+  d = bn_fold(d, &folded);
   const bool norm = d->norm_mode != DGXM_BLOCK_NORM_NONE;
   const int64_t rows = bn_rows(d);
   if (rows > 0) {  // empty tensors may be NULL

@@ -413,6 +413,35 @@ __device__ __forceinline__ void lin_epilogue_full(const LinearParams& p, uint8_t
   }
 }
 
+// The epilogue of a transposed tile out of the partial sums of the CTAs that
+// share its K, this one having rows `rank` (128 / split) .. of it: four columns
+// of a row a thread and turn of the loop (a thread's 32 values unrolled miss the
+// instruction cache, one at a time has nothing to overlap: 8192 x 64 x 256 in
+// tiles of 64 columns takes 25 us, 15.5, and 12.5 with four).
+template <int TN>
+__device__ __forceinline__ void lin_finish_share(const LinearParams& p, const float4* part, int rank, int pt, int qt) {
+  const int most = (128 + p.split - 1) / p.split, rows = min(most, p.step - rank * most), pitch = most | 1;
+  for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
+    // neighbouring lanes take neighbouring output columns
+    const int r = i % rows, c = 4 * (i / rows);
+    const int n = pt * p.step + rank * most + r, m = qt * TN + c;
+    if (n >= p.p_rows || m >= p.q_rows) continue;
+    float4 sum = part[c / 4 * pitch + r];
+    for (int k = 1; k < p.split; ++k) {
+      const float4 more = part[(k * (TN / 4) + c / 4) * pitch + r];
+      sum.x += more.x;
+      sum.y += more.y;
+      sum.z += more.z;
+      sum.w += more.w;
+    }
+    const float bias = p.bias != nullptr ? lin_value(p.bias, p.bias_dtype, n) : 0.f;
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (m + e < p.q_rows) lin_finish(p, m + e, n, v[e], bias);
+  }
+}
+
 // What follows a product by rows: ELT bytes of an output, the activation, or
 // (kActFull) any of them with a gate, a residual or pre.  Kernels of their own:
 // together in one they spill, and miss the instruction cache.
@@ -593,7 +622,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
       if (!got) {
         report_device_error(kErrEpilogueTimeout);
         *abort_flag = 1;
-        break;
+        if (by_rows || p.split > 1) break;  // (the others meet at every tile, and no wait takes long from here on)
       }
       tc_fence_after();
       if constexpr (TN > 64) {
@@ -608,28 +637,27 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
         }
       }
       if constexpr (TN <= 64) {  // transposed, maybe a share of K
-        const int q0 = qt * TN + half * kCols;
-        const uint32_t from = tmem + lane_off + a * TN + half * kCols;
-        uint32_t r[kCols / 8][8];
+        if (got) {
+          const uint32_t from = tmem + lane_off + a * TN + half * kCols;
+          uint32_t r[kCols / 8][8];
 #pragma unroll
-        for (int c = 0; c < kCols / 8; ++c) tmem_ld8(from + 8 * c, r[c]);
-        tmem_wait_ld();
+          for (int c = 0; c < kCols / 8; ++c) tmem_ld8(from + 8 * c, r[c]);
+          tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < kCols / 8; ++c) reg_fence8(r[c]);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + a * 8);
-        if (p.split > 1) {
+          for (int c = 0; c < kCols / 8; ++c) reg_fence8(r[c]);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + a * 8);
           const int rows = (128 + p.split - 1) / p.split, pitch = rows | 1;
           const uint32_t to = mapa_shared(smem_u32(staging), row / rows) +
                               ((rank * (TN / 4) + half * (kCols / 4)) * pitch + row % rows) * 16;
 #pragma unroll
           for (int c = 0; c < kCols / 4; ++c) st_shared_cluster(to + c * pitch * 16, r[c / 2] + 4 * (c % 2));
-        } else if (const int n = pr0 + lane; n < p.p_rows && row < p.step) {  // the rows are output columns
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-            if (q0 + c < p.q_rows)
-              lin_finish(p, q0 + c, n, __uint_as_float(r[c / 8][c % 8]), p.bias != nullptr ? lin_value(p.bias, p.bias_dtype, n) : 0.f);
+        }
+        if (p.split == 1) {
+          named_barrier_sync(1, 256);  // the tile is in place
+          if (got) lin_finish_share<TN>(p, reinterpret_cast<const float4*>(staging), 0, pt, qt);
+          named_barrier_sync(1, 256);  // and read
         }
       }
     }
@@ -641,32 +669,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
   else __syncthreads();
   if constexpr (C::kSplits) {
     if (p.split > 1 && warp >= 2 && *abort_flag == 0) {
-      // A split tile: this CTA's share of its rows, four columns of a row a thread.
-      const float4* part = reinterpret_cast<const float4*>(staging);
       int pt, qt;
       fp4_tile_coords(p, first_tile, pt, qt);
-      const int most = (128 + p.split - 1) / p.split, rows = min(most, p.step - rank * most), pitch = most | 1;
-      for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
-        // neighbouring lanes take neighbouring output columns
-        const int r = p.q_is_tokens ? i % rows : i / (TN / 4), c = 4 * (p.q_is_tokens ? i / rows : i % (TN / 4));
-        const int pr = pt * p.step + rank * most + r, q = qt * TN + c;
-        if (pr >= p.p_rows || q >= p.q_rows) continue;
-        float4 sum = part[c / 4 * pitch + r];
-        for (int k = 1; k < p.split; ++k) {
-          const float4 more = part[(k * (TN / 4) + c / 4) * pitch + r];
-          sum.x += more.x;
-          sum.y += more.y;
-          sum.z += more.z;
-          sum.w += more.w;
-        }
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (q + e >= p.q_rows) continue;
-          const int m = p.q_is_tokens ? q + e : pr, n = p.q_is_tokens ? pr : q + e;
-          lin_finish(p, m, n, v[e], p.bias != nullptr ? lin_value(p.bias, p.bias_dtype, n) : 0.f);
-        }
-      }
+      lin_finish_share<TN>(p, reinterpret_cast<const float4*>(staging), rank, pt, qt);
     }
   }
   if (warp == 1) {
@@ -764,17 +769,19 @@ struct LinCut {
   int step;          // rows of a tile
 };
 
-// Tiles of up to 64 columns are transposed: the few rows (m) are B's, which is
-// K-major then.  (b_mn: B is MN-major, and comes in blocks of 64 rows.)
+// Tiles of up to 64 columns are transposed: the rows (m) are B's.  They serve
+// few rows, and (64) products of few tiles, whose K is long enough to share.
+// (MN-major operands come in blocks of 64 rows.)
 static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn, bool b_mn) {
   struct Kind {
     int tn;
     bool pair;
     double stage, tile, least;
   };
-  // Microseconds a stage of K, a tile, and at the least, as measured with all SMs at work (1024 and 2048 x 5120 x 5120 by rows,
-  // 1 .. 64 x 5120 x 5120 transposed); the sums order the cuts and are not the times of calls.
-  static const Kind kinds[] = {{16, false, 0.18, 0.4, 0.4},  {32, false, 0.19, 0.5, 0.5},  {64, false, 0.20, 0.8, 1.0},
+  // Microseconds a stage of K, a tile (transposed ones share its epilogue with the CTAs of a split K), and at the least, as
+  // measured with all SMs at work (1024 and 2048 x 5120 x 5120 by rows, 1 .. 64 x 5120 x 5120, 256 x 804 x 8064 and
+  // 8192 x 64 x 256 transposed); the sums order the cuts and are not the times of calls.
+  static const Kind kinds[] = {{16, false, 0.18, 2.2, 0.4},  {32, false, 0.19, 4.0, 0.5},  {64, false, 0.26, 8.0, 1.0},
                                {128, false, 0.24, 1.3, 1.6}, {128, true, 0.245, 1.5, 2.0}, {192, true, 0.285, 1.7, 2.2},
                                {256, true, 0.315, 2.0, 2.5}};
   static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};  // that the SMs hold at one time
@@ -782,15 +789,15 @@ static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn, bool b_mn) {
   double least = 1e30;
   for (const Kind& kind : kinds) {
     const bool swapped = kind.tn <= 64;
-    if ((swapped && (a_mn || m > kind.tn)) || (b_mn && kind.pair && kind.tn % 128 != 0)) continue;
+    if ((swapped && kind.tn < 64 && (a_mn || m > kind.tn)) || (b_mn && kind.pair && kind.tn % 128 != 0)) continue;
     const int64_t p_rows = swapped ? n : m, q_rows = swapped ? m : n;
     const int rows = kind.pair ? 256 : 128, at_once = kind.pair ? 74 : 148;
     const int64_t tiles = (p_rows + rows - 1) / rows * ((q_rows + kind.tn - 1) / kind.tn);
     for (int split = 1; split <= (swapped ? 8 : 1) && split <= k_tiles; ++split) {
       if (split > 1 && tiles > clusters[split]) continue;
       const int64_t waves = (tiles * split + at_once - 1) / at_once;
-      const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile, kind.least) +
-                        (split > 1 ? 0.8 + 0.026 * kind.tn : 0.0);
+      const double us = waves * std::max((k_tiles + split - 1) / split * kind.stage + kind.tile / split, kind.least) +
+                        (split > 1 ? 1.6 + 0.02 * kind.tn : 0.0);
       if (us < least) {
         least = us;
         best = {kind.tn, kind.pair, split, swapped, rows};
@@ -800,7 +807,7 @@ static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn, bool b_mn) {
   // A transposed product reads the weight once and DRAM bounds it: tiles of
   // fewer rows, so that every SM has as many as the others (2 x 30720 x 5120:
   // 240 tiles of 128 rows or 296 of 104 on 148 SMs).
-  if (best.q_is_tokens && best.split == 1) {
+  if (best.q_is_tokens && best.split == 1 && m <= best.tn) {
     const int64_t waves = ((n + 127) / 128 + 147) / 148;
     best.step = static_cast<int>(std::min<int64_t>(128, ((n + 148 * waves - 1) / (148 * waves) + 7) / 8 * 8));
   }
@@ -825,7 +832,9 @@ static int lin_product(LinearParams& p, const LinOperand& a, const LinOperand& b
   switch (cut.tn) {
     case 16: return amn ? lin_launch<16, false, true, false>(p, po, qo, st) : lin_launch<16, false, false, false>(p, po, qo, st);
     case 32: return amn ? lin_launch<32, false, true, false>(p, po, qo, st) : lin_launch<32, false, false, false>(p, po, qo, st);
-    case 64: return amn ? lin_launch<64, false, true, false>(p, po, qo, st) : lin_launch<64, false, false, false>(p, po, qo, st);
+    case 64:
+      if (bmn) return lin_launch<64, false, true, true>(p, po, qo, st);  // (w's gradient: both are)
+      return amn ? lin_launch<64, false, true, false>(p, po, qo, st) : lin_launch<64, false, false, false>(p, po, qo, st);
     default: break;
   }
   if (amn || bmn) {  // the gradients' products: 16-bit outputs and nothing more
@@ -1093,48 +1102,51 @@ struct LinSumParams {
   int n, pitch, sample_runs, bias_dtype, gate_dtype, gate_form;
 };
 
-// A block takes 32 columns.  Its warps take the samples in turn where there
-// are many, or else share out the runs of each; warp 0 adds their sums in order.
+// A block takes 32 columns.  Its warps form groups of equal size, up to one a
+// sample; a group shares out the runs of a sample, and then takes another.
 __global__ void __launch_bounds__(1024) linear_sum_kernel(const __grid_constant__ LinSumParams p) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float part[32][2][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
-  const bool in = col < p.n, gates = p.g_gate != nullptr, many = p.samples >= 32;
-  float bias = 0.f, shared = 0.f;
-  auto own = [&](int64_t s, float g) {
-    if (in && gates && p.gate_form == DGXM_MOD_SAMPLE) lin_put(p.g_gate, p.gate_dtype, s * p.n + col, g);
-  };
-  auto join = [&](float& b, float& g) {  // for warp 0
+  const bool in = col < p.n, gates = p.g_gate != nullptr;
+  int groups = 1;
+  while (groups < 32 && groups < p.samples) groups *= 2;
+  const int each = 32 / groups, group = warp / each, turn = warp % each;
+  // The sums of `count` warps from `first` on, `step` apart, in order.
+  auto join = [&](float& b, float& g, bool mine, int first, int step, int count) {
     part[warp][0][lane] = b;
     part[warp][1][lane] = g;
     __syncthreads();
-    if (warp == 0) {
+    if (mine) {
       b = g = 0.f;
-      for (int k = 0; k < 32; ++k) {
-        b += part[k][0][lane];
-        g += part[k][1][lane];
+      for (int k = 0; k < count; ++k) {
+        b += part[first + k * step][0][lane];
+        g += part[first + k * step][1][lane];
       }
     }
     __syncthreads();
   };
-  for (int64_t s = many ? warp : 0; s < p.samples; s += many ? 32 : 1) {
+  float bias = 0.f, shared = 0.f;
+  for (int64_t s0 = 0; s0 < p.samples; s0 += groups) {
+    const int64_t s = s0 + group;
     float b = 0.f, g = 0.f;
-    const int64_t r0 = s * p.sample_runs + (many ? 0 : static_cast<int64_t>(p.sample_runs) * warp / 32);
-    const int64_t r1 = s * p.sample_runs + (many ? p.sample_runs : static_cast<int64_t>(p.sample_runs) * (warp + 1) / 32);
-    if (in) {
+    const int64_t r0 = s * p.sample_runs + static_cast<int64_t>(p.sample_runs) * turn / each;
+    const int64_t r1 = s * p.sample_runs + static_cast<int64_t>(p.sample_runs) * (turn + 1) / each;
+    if (in && s < p.samples) {
 #pragma unroll 4
       for (int64_t r = r0; r < r1; ++r) {
         if (p.g_bias != nullptr) b += p.partial[r * 2 * p.pitch + col];
         if (gates) g += p.partial[(r * 2 + 1) * p.pitch + col];
       }
     }
-    if (!many) join(b, g);
-    if (many || warp == 0) own(s, g);
+    if (each > 1) join(b, g, turn == 0, warp, 1, each);
+    if (turn != 0) continue;
+    if (in && s < p.samples && gates && p.gate_form == DGXM_MOD_SAMPLE) lin_put(p.g_gate, p.gate_dtype, s * p.n + col, g);
     bias += b;
     shared += g;
   }
-  if (many) join(bias, shared);
+  if (groups > 1) join(bias, shared, warp == 0, 0, each, groups);
   if (warp != 0 || !in) return;
   if (gates && p.gate_form == DGXM_MOD_SHARED) lin_put(p.g_gate, p.gate_dtype, col, shared);
   if (p.g_bias != nullptr) lin_put(p.g_bias, p.bias_dtype, col, bias);

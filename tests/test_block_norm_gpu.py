@@ -116,6 +116,22 @@ def test_row_counts(b, l, width):
     run_backward(a, up, "layer")
 
 
+@pytest.mark.parametrize("gate,mod", [("sample", "sample"), ("sample3", "token"), ("shared", "sample3"), ("token", "shared"), (None, "sample")])
+@pytest.mark.parametrize("b,width", [(2, 192), (3, 1283), (700, 520)])
+def test_samples_of_one_row(b, width, gate, mod):
+    """Values of a sample that has one row; also slices of a wider projection, samples far apart."""
+    a, up = make(b, b, 1, width, torch.bfloat16, gate=gate, mod=mod, post=b == 3)
+    run_forward(a, "layer")
+    run_backward(a, up, "layer")
+    for name in ("x", "branch", "gate", "scale", "shift"):
+        t = a[name]
+        if t is not None and t.ndim > 1:
+            wide = torch.zeros(*t.shape[:-1], 2 * width + 8, device="cuda", dtype=t.dtype)
+            a[name] = wide[..., 8:8 + width].copy_(t)
+    run_forward(a, "rms" if a["norm_b"] is None else "layer")
+    run_backward(a, up, "layer")
+
+
 @pytest.mark.parametrize("b,l", [(0, 4), (2, 0)])
 def test_no_rows(b, l):
     from dgx_monarch_b200.block_norm import block_norm, block_norm_backward

@@ -156,6 +156,27 @@ def test_long_k():
     run_backward(a, dout)
 
 
+@pytest.mark.parametrize("m,n,k", [(200, 136, 4096), (257, 72, 2051), (70, 400, 1600), (1000, 8, 1024), (65, 129, 515)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_few_tiles(m, n, k, dtype):
+    """Products whose K is shared among CTAs, in each direction, with several tiles of rows and everything in the epilogue."""
+    a, res, dout = make(m, (m,), n, k, dtype, gate="token", residual=True)
+    _, pre = run_forward(a, res, "silu")
+    run_backward(a, dout, "silu", pre)
+    a, res, dout = make(m, (m,), n, k, dtype, gate="shared")
+    run_forward(a, res, out_dtype=torch.float32)
+    a, res, dout = make(m, (k,), n, m, dtype)  # w's gradient along k rows
+    run_backward(a, dout)
+
+
+@pytest.mark.parametrize("samples", [1, 2, 3, 31, 33, 70])
+def test_sums_over_samples(samples):
+    a, res, dout = make(samples, (samples, 9), 40, 64, torch.bfloat16, gate="sample")
+    run_backward(a, dout, "gelu")
+    a["gate"] = a["gate"][0].clone()
+    run_backward(a, dout, "gelu")
+
+
 @pytest.mark.parametrize("offset", [0, 1, 8])
 def test_strides(offset):
     """Slices (on and off 16 bytes), batch and rows exchanged, a transposed weight, expanded tensors, outputs beside others."""
