@@ -179,7 +179,7 @@ def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *, bia
     read).  dz = dout * gate * act'(pre) is rounded to x's dtype for the
     products and not in the sums over rows, which are fp32 in a fixed order:
     the same call gives the same bits.  Inputs without contiguous columns and
-    evenly spaced rows are copied first."""
+    evenly spaced rows are copied first.  w's gradient takes up to 2^24 rows."""
     x_grad, w_grad = bool(x_grad), bool(w_grad)
     key = ("lb", _meta(dout), _meta(x), _meta(w), _meta(bias), activation, _meta(gate), _meta(pre), x_grad, w_grad)
 

@@ -877,7 +877,8 @@ int dgxm_linear(const dgxm_linear_desc* desc, const void* x, const void* w, cons
  *   x: dz w,   w: dz^T x,   bias: sum dz,   gate: sum dout * act(pre)
  * The residual's gradient is dout.  pre is the forward's, or NULL without an
  * activation and a gradient of the gate.  dz is rounded to dtype before the
- * products, not in the sums, which are fp32 in a fixed order.
+ * products, not in the sums, which are fp32 in a fixed order.  w's gradient is
+ * refused above an m of 2^24.
  */
 typedef struct dgxm_linear_grads {
   void *x, *w, *bias, *gate;
