@@ -156,17 +156,6 @@ __device__ __forceinline__ void lin_put(void* base, int dtype, int64_t at, float
   else static_cast<float*>(base)[at] = v;
 }
 
-// The epilogue of one value, of token m and output n.
-__device__ __forceinline__ void lin_finish(const LinearParams& p, int m, int n, float v, float bias) {
-  v += bias;
-  if (p.pre != nullptr) lin_put(p.pre, p.pre_dtype, m * p.ld_pre + n, v);
-  v = lin_act(v, p.act);
-  if (p.gate != nullptr)
-    v *= lin_value(p.gate, p.gate_dtype, m / p.sample_rows * p.gate_sample + m % p.sample_rows * p.gate_row + n);
-  if (p.residual != nullptr) v += lin_value(p.residual, p.out_dtype, m * p.ld_res + n);
-  lin_put(p.out, p.out_dtype, m * p.ld_out + n, v);
-}
-
 // One operand's rows of a stage.  K-major: `rows` rows of 64 k.  MN-major:
 // blocks of 64 rows, each 64 k of 128 bytes.
 template <bool PAIR, bool MN, int ROWS>
@@ -420,30 +409,79 @@ __device__ __forceinline__ void lin_epilogue_full(const LinearParams& p, uint8_t
 
 // The epilogue of a transposed tile out of the partial sums of the CTAs that
 // share its K, this one having rows `rank` (128 / split) .. of it: four columns
-// of a row a thread and turn of the loop (a thread's 32 values unrolled miss the
-// instruction cache, one at a time has nothing to overlap: 8192 x 64 x 256 in
-// tiles of 64 columns takes 25 us, 15.5, and 12.5 with four).
+// of a row a thread and turn of the loop, each way of the epilogue taken for the
+// four together (8192 x 64 x 256 in tiles of 64 columns: 25 us with a thread's 32
+// values unrolled, which miss the instruction cache, 15.5 one at a time, 12.5 one
+// after another of four, 8.9; 64 x 5120 x 5120: 15.2 -> 12.4).
 template <int TN>
 __device__ __forceinline__ void lin_finish_share(const LinearParams& p, const float4* part, int rank, int pt, int qt) {
   const int most = (128 + p.split - 1) / p.split, rows = min(most, p.step - rank * most), pitch = most | 1;
-  for (int i = threadIdx.x - 64; i < rows * (TN / 4); i += 256) {
-    // neighbouring lanes take neighbouring output columns
-    const int r = i % rows, c = 4 * (i / rows);
-    const int n = pt * p.step + rank * most + r, m = qt * TN + c;
-    if (n >= p.p_rows || m >= p.q_rows) continue;
-    float4 sum = part[c / 4 * pitch + r];
-    for (int k = 1; k < p.split; ++k) {
-      const float4 more = part[(k * (TN / 4) + c / 4) * pitch + r];
-      sum.x += more.x;
-      sum.y += more.y;
-      sum.z += more.z;
-      sum.w += more.w;
-    }
-    const float bias = p.bias != nullptr ? lin_value(p.bias, p.bias_dtype, n) : 0.f;
-    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  if (rows <= 0) return;
+  const int down = 256 / rows, along = 256 - down * rows;  // from a thread's values to its next ones
+  int c4 = (threadIdx.x - 64) / rows, r = threadIdx.x - 64 - c4 * rows;
+  for (; c4 < TN / 4; c4 += down) {  // neighbouring lanes take neighbouring output columns
+    const int n = pt * p.step + rank * most + r, m = qt * TN + 4 * c4;
+    if (n < p.p_rows && m < p.q_rows) {
+      const float4 own = part[c4 * pitch + r];
+      float v[4] = {own.x, own.y, own.z, own.w};
+      for (int k = 1; k < p.split; ++k) {
+        const float4 more = part[(k * (TN / 4) + c4) * pitch + r];
+        v[0] += more.x;
+        v[1] += more.y;
+        v[2] += more.z;
+        v[3] += more.w;
+      }
+      const int count = min(4, p.q_rows - m);
+      if (p.bias != nullptr) {
+        const float bias = lin_value(p.bias, p.bias_dtype, n);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (m + e < p.q_rows) lin_finish(p, m + e, n, v[e], bias);
+        for (int e = 0; e < 4; ++e) v[e] += bias;
+      }
+      if (p.pre != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < count) lin_put(p.pre, p.pre_dtype, (m + e) * p.ld_pre + n, v[e]);
+      }
+      if (p.act == DGXM_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lin_act(v[e], DGXM_ACT_SILU);
+      } else if (p.act == DGXM_ACT_GELU) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lin_act(v[e], DGXM_ACT_GELU);
+      } else if (p.act == DGXM_ACT_GELU_TANH) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lin_act(v[e], DGXM_ACT_GELU_TANH);
+      }
+      float by[4], more[4];
+      if (p.gate != nullptr) {
+        const int last = p.q_rows - 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = min(m + e, last), sample = at / p.sample_rows;
+          by[e] = lin_value(p.gate, p.gate_dtype, sample * p.gate_sample + (at - sample * p.sample_rows) * p.gate_row + n);
+        }
+      }
+      if (p.residual != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) more[e] = e < count ? lin_value(p.residual, p.out_dtype, (m + e) * p.ld_res + n) : 0.f;
+      }
+      if (p.gate != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= by[e];
+      }
+      if (p.residual != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += more[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < count) lin_put(p.out, p.out_dtype, (m + e) * p.ld_out + n, v[e]);
+    }
+    r += along;
+    if (r >= rows) {
+      r -= rows;
+      ++c4;
+    }
   }
 }
 
@@ -786,7 +824,7 @@ static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn, bool b_mn) {
   // Microseconds a stage of K, a tile (transposed ones share its epilogue with the CTAs of a split K), and at the least, as
   // measured with all SMs at work (1024 and 2048 x 5120 x 5120 by rows, 1 .. 64 x 5120 x 5120, 256 x 804 x 8064 and
   // 8192 x 64 x 256 transposed); the sums order the cuts and are not the times of calls.
-  static const Kind kinds[] = {{16, false, 0.18, 2.2, 0.4},  {32, false, 0.19, 4.0, 0.5},  {64, false, 0.26, 8.0, 1.0},
+  static const Kind kinds[] = {{16, false, 0.18, 1.3, 0.4},  {32, false, 0.19, 2.3, 0.5},  {64, false, 0.22, 4.5, 1.0},
                                {128, false, 0.24, 1.3, 1.6}, {128, true, 0.245, 1.5, 2.0}, {192, true, 0.285, 1.7, 2.2},
                                {256, true, 0.315, 2.0, 2.5}};
   static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};  // that the SMs hold at one time
