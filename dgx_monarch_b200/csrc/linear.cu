@@ -19,7 +19,7 @@
 // Large products are bound by power (9450 x 13824 x 5120 with GELU: 853 us cold,
 // 1033 in a long run, 1.57 and 1.30 PFLOP/s), few rows by DRAM (2 x 30720 x 5120:
 // 51 us, 6.2 TB/s), and what lies between by the latency of stages of K, about
-// 0.25 us each (512 x 5120 x 4096: 25 us).
+// 0.25 us each (512 x 5120 x 4096: 22 us).
 #include <type_traits>
 
 #include "common.h"

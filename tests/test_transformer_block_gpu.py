@@ -60,7 +60,7 @@ def _forward64(p, heads):
     return x, x + g2[:, None] * (h @ t["down"].T)
 
 
-@pytest.mark.parametrize("b,l,heads,d", [(1, 1, 2, 128), (2, 77, 4, 64), (2, 300, 8, 128)])
+@pytest.mark.parametrize("b,l,heads,d", [(1, 1, 2, 128), (2, 77, 4, 64), (2, 300, 6, 128)])
 def test_block(b, l, heads, d):
     from dgx_monarch_b200.block_norm import block_norm
     from dgx_monarch_b200.linear import linear
@@ -84,7 +84,7 @@ def test_block(b, l, heads, d):
     assert rel(out, want) <= 10 * HALF  # and y, h, out
 
 
-@pytest.mark.parametrize("b,l,heads,d", [(1, 1, 2, 128), (2, 77, 4, 64), (2, 300, 8, 128)])
+@pytest.mark.parametrize("b,l,heads,d", [(1, 1, 2, 128), (2, 77, 4, 64), (2, 300, 6, 128)])
 def test_training_step_of_its_second_half(b, l, heads, d):
     from dgx_monarch_b200.block_norm import block_norm, block_norm_backward
     from dgx_monarch_b200.linear import linear, linear_backward
@@ -118,7 +118,7 @@ def test_block_in_a_graph():
     from dgx_monarch_b200.block_norm import block_norm
     from dgx_monarch_b200.linear import linear
 
-    p = _case(3, 2, 130, 4, 128)
+    p = _case(3, 2, 130, 5, 128)
     _, _, g1, s2, t2, g2 = p["mod"].chunk(6, dim=-1)
     branch = p["dout"].clone()
 
