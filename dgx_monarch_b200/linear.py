@@ -113,7 +113,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, *, bias: torch.Tensor | None = None
     "gelu_tanh"; gate (n,), (batch, n), (batch, 1, n) or one value for each
     output ((batch, rows, n), or (rows, n) beside a 2-D x); residual of out's
     shape and dtype; out_dtype x's dtype (the default) or fp32.  fp32
-    accumulation and epilogue, one rounding of out and of pre; any sizes.
+    accumulation and epilogue, one rounding of out and of pre; any sizes, n and
+    k up to 2^24.
 
     out may be residual itself, and must not overlap the inputs in any other
     way.  x, w or residual without contiguous columns and evenly spaced rows is
