@@ -203,7 +203,9 @@ def linear_backward(dout: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *, bia
     no_graph(_GRADS, dout, x, w, bias, gate, pre)
     if not even:
         dout, x, w, pre = _even(dout), _even(x), _even(w), _even(pre)
-    like = lambda t, wanted=True: torch.empty_like(t, memory_format=torch.contiguous_format) if wanted and t is not None else None
+    # without rows the sums are of nothing, and the C entry cannot tell of how many samples
+    fresh = torch.empty_like if desc.m else torch.zeros_like
+    like = lambda t, wanted=True: fresh(t, memory_format=torch.contiguous_format) if wanted and t is not None else None
     grads = LinearGrads(like(x, x_grad), like(w, w_grad), like(bias), like(gate))
     if all(t is None for t in grads):
         return grads

@@ -878,7 +878,8 @@ int dgxm_linear(const dgxm_linear_desc* desc, const void* x, const void* w, cons
  * The residual's gradient is dout.  pre is the forward's, or NULL without an
  * activation and a gradient of the gate.  dz is rounded to dtype before the
  * products, not in the sums, which are fp32 in a fixed order.  w's gradient is
- * refused above an m of 2^24.
+ * refused above an m of 2^24.  With an m of 0 the sums are zeros, but for a
+ * SAMPLE gate's, of whose samples the descriptor does not tell the number.
  */
 typedef struct dgxm_linear_grads {
   void *x, *w, *bias, *gate;

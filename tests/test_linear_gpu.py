@@ -343,3 +343,20 @@ def test_wanted_gradients_alone():
         for one, all_ in zip(got, whole):
             assert one is None or torch.equal(one, all_)
     assert math.isfinite(whole.x.float().sum().item())
+
+
+@pytest.mark.parametrize("lead,gate", [((2, 0), "shared"), ((2, 0), "sample"), ((2, 0), "sample3"), ((1, 0), "sample"), ((0, 3), "sample"),
+                                       ((2, 0), "token"), ((0,), None), ((0,), "one")])
+def test_gradients_of_no_rows(lead, gate):
+    """Zeros in memory that held something else."""
+    from dgx_monarch_b200.linear import linear_backward
+
+    a, _, dout = make(0, lead, 16, 32, torch.bfloat16, gate=None if gate == "one" else gate)
+    if gate == "one":
+        a["gate"] = torch.ones(1, 16, device="cuda").bfloat16()
+    dirty = [torch.full((n,), float("nan"), device="cuda").bfloat16() for n in (16, 32, 16 * 32) for _ in range(4)]
+    torch.cuda.synchronize()
+    del dirty
+    grads = linear_backward(dout, a["x"], a["w"], bias=a["bias"], gate=a["gate"], pre=dout)
+    for got, like in ((grads.x, a["x"]), (grads.w, a["w"]), (grads.bias, a["bias"]), (grads.gate, a["gate"])):
+        assert (got is None and like is None) or torch.equal(got, torch.zeros_like(like))

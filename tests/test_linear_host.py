@@ -257,3 +257,20 @@ def test_struct_layouts(tmp_path):
     subprocess.run(["gcc", "-std=c11", "-o", str(tmp_path / "layout"), str(source)], check=True)
     out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
     assert [int(v) for v in out.split()] == want
+
+
+@pytest.mark.parametrize("x_shape,gate_shape", [((2, 0, 64), (8,)), ((2, 0, 64), (2, 8)), ((2, 0, 64), (2, 1, 8)),
+                                                ((1, 0, 64), (1, 8)), ((0, 64), (1, 8)), ((0, 64), (8,)), ((2, 0, 64), (2, 0, 8)),
+                                                ((0, 4, 64), (0, 8))])
+def test_gradients_of_no_rows_are_zeros(monkeypatch, lib, x_shape, gate_shape):
+    """A sum over no rows is zero, whatever the memory held and however many samples have no rows."""
+    from dgx_monarch_b200 import linear as ln
+
+    monkeypatch.setattr(ln, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(ln, "launch", lambda *a: None)
+    monkeypatch.setattr(torch, "empty_like", lambda t, **kw: torch.full_like(t, float("nan")))
+    x, w, bias, gate = _t(*x_shape), _t(8, 64), _t(8), _t(*gate_shape)
+    dout = _t(*x_shape[:-1], 8)
+    grads = ln.linear_backward(dout, x, w, bias=bias, gate=gate, pre=dout)
+    for got, like in zip(grads, (x, w, bias, gate)):
+        assert torch.equal(got, torch.zeros_like(like))
