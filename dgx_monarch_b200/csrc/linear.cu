@@ -399,10 +399,14 @@ __device__ __forceinline__ void lin_epilogue_full(const LinearParams& p, uint8_t
     }
     fp4_flush_rows<CC, ELT>(p, stage, pr0, q0, lane);
     const int next = K::column(half, ch + 1);
-    if (p.res_bulk && ch + 1 < K::kOwn && next < p.tn && q_tile + next < p.q_rows && lane == 0) {
-      tma_store_wait_read();
-      mbar_expect_tx(res_bar, kGemmStageRows);
-      tma_load_4d(smem_u32(stage), &p.tmap_res, res_bar, q_tile + next, 0, pr0, 0);
+    if (p.res_bulk && ch + 1 < K::kOwn && next < p.tn && q_tile + next < p.q_rows) {
+      tma_store_fence();  // rows that went by the lanes' stores have been written and read before the load writes them
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_wait_read();
+        mbar_expect_tx(res_bar, kGemmStageRows);
+        tma_load_4d(smem_u32(stage), &p.tmap_res, res_bar, q_tile + next, 0, pr0, 0);
+      }
     }
   }
 }
@@ -639,6 +643,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
       const int pr0 = pt * p.step + cta * 128 + quarter * 32;  // this warp's first row
       if (ACT == kActFull && by_rows && p.residual != nullptr) {  // the residual's first chunk comes while the MMAs run
         if (lane == 0) tma_store_wait_read();
+        tma_store_fence();  // as between chunks
         __syncwarp();
         if (const int c0 = LinChunks<TN, ELT>::column(half, 0), q0 = qt * p.tn + c0; c0 < p.tn && q0 < p.q_rows) {
           if (!p.res_bulk) {
