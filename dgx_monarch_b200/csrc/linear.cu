@@ -641,6 +641,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
       int pt, qt;
       fp4_tile_coords(p, tile, pt, qt);
       const int pr0 = pt * p.step + cta * 128 + quarter * 32;  // this warp's first row
+      bool fetched = false;
       if (ACT == kActFull && by_rows && p.residual != nullptr) {  // the residual's first chunk comes while the MMAs run
         if (lane == 0) tma_store_wait_read();
         tma_store_fence();  // as between chunks
@@ -648,9 +649,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
         if (const int c0 = LinChunks<TN, ELT>::column(half, 0), q0 = qt * p.tn + c0; c0 < p.tn && q0 < p.q_rows) {
           if (!p.res_bulk) {
             lin_stage_residual<ELT>(p, stage, pr0, q0, lane);
-          } else if (lane == 0) {
-            mbar_expect_tx(res_bar, kGemmStageRows);
-            tma_load_4d(smem_u32(stage), &p.tmap_res, res_bar, q0, 0, pr0, 0);
+          } else {
+            fetched = true;
+            if (lane == 0) {
+              mbar_expect_tx(res_bar, kGemmStageRows);
+              tma_load_4d(smem_u32(stage), &p.tmap_res, res_bar, q0, 0, pr0, 0);
+            }
           }
         }
         __syncwarp();
@@ -670,6 +674,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) linear_kernel(const __grid_co
       if (!got) {
         report_device_error(kErrEpilogueTimeout);
         *abort_flag = 1;
+        if (fetched) mbar_wait(res_bar, res_phase, nullptr);  // the load lands before the CTA can exit
         if (by_rows || p.split > 1) break;  // (the others meet at every tile, and no wait takes long from here on)
       }
       tc_fence_after();
