@@ -356,6 +356,8 @@ __device__ __forceinline__ void bn_fetch(const BlockNormParams& p, uint8_t* ring
         const uint32_t dst = __shfl_sync(0xffffffffu, smem_u32(to) + off, s);
         if (at[i] != ~0u) asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + at[i]), "h"(end[i]) : "memory");
       }
+      // Rows of a slot lie at different offsets: this row's words cover bytes that an earlier row's ends were stored to.
+      tma_store_fence();
       to += off + head;
       from += head;
       bytes -= head + tail;
