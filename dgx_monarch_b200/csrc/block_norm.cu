@@ -322,8 +322,10 @@ __device__ __forceinline__ void bn_fetch(const BlockNormParams& p, uint8_t* ring
   const int lane = threadIdx.x & 31;
   const bool mine = lane < p.n_in && p.in[lane < kBnMaxIn ? lane : 0] != nullptr;
   bool dead = false;
-  for (BnWalk w(p); w.more(); w.next()) {
+  BnWalk w(p);
+  for (; w.more(); w.next()) {
     bn_wait(&sh.empty[w.slot], w.parity ^ 1, dead);
+    if ((dead = __any_sync(0xffffffffu, dead))) break;  // nothing more is loaded over what may still be read
     const uint32_t full = smem_u32(&sh.full[w.slot]);
     uint8_t* to = ring + w.slot * p.slot_bytes;
     const char* from = nullptr;
@@ -372,6 +374,9 @@ __device__ __forceinline__ void bn_fetch(const BlockNormParams& p, uint8_t* ring
     if (bytes > 0) bn_bulk_load(smem_u32(to), from, bytes, full);
   }
   if (dead) report_device_error(kErrProducerTimeout);
+  // Every load lands before the block can exit, also where its readers have given up waiting.  (Slots before the walk's are
+  // a round ahead of the others; of one never used the round before its first counts as over.)
+  for (int s = 0; s < p.slots; ++s) mbar_wait(smem_u32(&sh.full[s]), s < w.slot ? w.parity : w.parity ^ 1, nullptr);
 }
 
 // Bytes that a row of stream s lies behind a 16-byte border.
