@@ -9,6 +9,7 @@ handle of the current stream.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -44,8 +45,14 @@ def launch(name: str, index: int, *args) -> None:
 
 
 def no_graph(where: str, *tensors: torch.Tensor | None) -> None:
-    """Refuse tensors whose gradient the caller expects autograd to follow."""
+    """Refuse tensors whose gradient the caller expects autograd to follow, in
+    reverse or (under a dual level only, and whether or not reverse mode is on)
+    forward mode."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError("the B200 kernels record no autograd graph: call them under torch.no_grad()" + where)
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the B200 kernels carry no forward-mode tangent: pass the primal of a dual tensor")
