@@ -968,16 +968,16 @@ struct LinPacker {
 };
 
 // ------------------------------------------------------------ dz and the sums over rows
-// A thread takes eight columns of a run of rows of one sample; its sums go to (run, 2, n) partial sums of dz and dout
-// act(pre), which a second kernel adds in the order of the runs.  DRAM bounds it: dout and pre read, dz written.  Rows
-// come by asynchronous copies into a ring, three ahead (in registers the loop waits for a row when it moves it up), and
-// values are taken in pairs.  9450 x 13824 gelu_tanh with a bias: 235 -> 133 us (784 MB, 5.9 TB/s).
+// A thread takes eight columns of a run of rows of one sample; its sums of dz and dout act(pre), whichever are wanted, go
+// to (run, one or two, n) partial sums, which a second kernel adds in the order of the runs.  DRAM bounds it: dout and pre
+// read, dz written.  Rows come by asynchronous copies into a ring, three ahead (in registers the loop waits for a row when
+// it moves it up), and values are taken in pairs.  9450 x 13824 gelu_tanh with a bias: 235 -> 133 us (784 MB, 5.9 TB/s).
 constexpr int kDzSlots = 4, kDzLeast = 4;  // of rows under way; rows of the shortest run
 
 struct LinDzParams {
   const void *dout, *pre, *gate;
   void *dz, *g_gate;  // g_gate: a token's own, contiguous
-  float* partial;     // (runs, 2, pitch), or NULL
+  float* partial;     // (runs, sum_bias + sum_gate, pitch), or NULL
   int64_t pitch;
   int64_t ld_dout, ld_pre, ld_dz, gate_sample, gate_row;
   int64_t runs;
@@ -1134,8 +1134,9 @@ __global__ void __launch_bounds__(128) linear_dz_kernel(const __grid_constant__ 
         to[0] = make_ulonglong2(v[0], v[1]);
         to[1] = make_ulonglong2(v[2], v[3]);
       };
-      if (p.sum_bias) put(run * 2, sum);
-      if (GATES && p.sum_gate) put(run * 2 + 1, sum_gate);
+      const int64_t row = run * (p.sum_bias + p.sum_gate);
+      if (p.sum_bias) put(row, sum);
+      if (GATES && p.sum_gate) put(row + p.sum_bias, sum_gate);
     }
   }
 }
@@ -1162,7 +1163,8 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const __grid_constant_
   pdl_wait();
   __shared__ float part[32][2][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
-  const bool in = col < p.n, gates = p.g_gate != nullptr;
+  const bool in = col < p.n, biases = p.g_bias != nullptr, gates = p.g_gate != nullptr;
+  const int sums = biases + gates;
   int groups = 1;
   while (groups < 32 && groups < p.samples) groups *= 2;
   const int each = 32 / groups, group = warp / each, turn = warp % each;
@@ -1189,8 +1191,8 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const __grid_constant_
     if (in && s < p.samples) {
 #pragma unroll 4
       for (int64_t r = r0; r < r1; ++r) {
-        if (p.g_bias != nullptr) b += p.partial[r * 2 * p.pitch + col];
-        if (gates) g += p.partial[(r * 2 + 1) * p.pitch + col];
+        if (biases) b += p.partial[r * sums * p.pitch + col];
+        if (gates) g += p.partial[(r * sums + biases) * p.pitch + col];
       }
     }
     if (each > 1) join(b, g, turn == 0, warp, 1, each);
@@ -1202,7 +1204,7 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const __grid_constant_
   if (groups > 1) join(bias, shared, warp == 0, 0, each, groups);
   if (warp != 0 || !in) return;
   if (gates && p.gate_form == DGXM_MOD_SHARED) lin_put(p.g_gate, p.gate_dtype, col, shared);
-  if (p.g_bias != nullptr) lin_put(p.g_bias, p.bias_dtype, col, bias);
+  if (biases) lin_put(p.g_bias, p.bias_dtype, col, bias);
 }
 
 // ------------------------------------------------------------ the C entries
@@ -1309,7 +1311,8 @@ namespace dgxm {
 // Where the gradient's intermediates lie in the workspace.
 struct LinBackPlan {
   bool dz;      // dz is not dout itself
-  bool sums;
+  int sums;     // over rows that are wanted, bias' and a gate's
+  int64_t gate_sample, gate_row;
   int64_t runs, sample_runs, sample_rows, run_rows, dz_bytes, part_bytes, x_bytes, w_bytes, dout_bytes;
   int64_t total() const { return dz_bytes + part_bytes + x_bytes + w_bytes + dout_bytes; }
 };
@@ -1328,8 +1331,22 @@ static LinBackPlan lin_back_plan(const dgxm_linear_desc* d, const dgxm_linear_gr
   memset(&b, 0, sizeof(b));
   const bool products = g->x != nullptr || g->w != nullptr;
   b.dz = products && (d->activation != DGXM_ACT_NONE || d->gate_form != DGXM_MOD_NONE || d->out_dtype != d->dtype);
-  b.sums = g->bias != nullptr || (g->gate != nullptr && d->gate_form != DGXM_MOD_TOKEN);
-  b.sample_rows = d->gate_form != DGXM_MOD_NONE ? d->sample_rows : d->m;
+  b.sums = (g->bias != nullptr) + (g->gate != nullptr && d->gate_form != DGXM_MOD_TOKEN);
+  // Runs end where a sample does only for the sake of its gate's sum, or of samples whose tokens' gates are not a step
+  // apart: with a row a sample every run would be one row (9450 x 1 x 13824, a token's gate and a bias: 1.05 GB of partial
+  // sums, 8 MB here).
+  b.gate_sample = b.gate_row = 0;
+  b.sample_rows = d->m;
+  if (d->gate_form == DGXM_MOD_SAMPLE) {
+    b.gate_sample = d->gate_stride[0];
+    b.sample_rows = d->sample_rows;
+  } else if (d->gate_form == DGXM_MOD_TOKEN) {
+    b.gate_row = d->sample_rows == 1 ? d->gate_stride[0] : d->gate_stride[1];
+    if (d->m > d->sample_rows && d->gate_stride[0] != d->sample_rows * b.gate_row) {
+      b.gate_sample = d->gate_stride[0];
+      b.sample_rows = d->sample_rows;
+    }
+  }
   // Runs of 64 rows, or shorter ones where those would leave the SMs without work (512 x 5120: 51 us in runs of 64, 10 in
   // runs of 4; 9450 x 13824 133 in runs of 64, 141 in runs of 4 and four times as long for their sums).
   const int64_t across = (lin_pitch(d->n) / 8 + 127) / 128;
@@ -1338,7 +1355,7 @@ static LinBackPlan lin_back_plan(const dgxm_linear_desc* d, const dgxm_linear_gr
   b.runs = b.sample_rows > 0 ? d->m / b.sample_rows * b.sample_runs : 0;
   if (b.dz) b.dz_bytes = (d->m * lin_pitch(d->n) * 2 + 255) / 256 * 256;
   else if (products) b.dout_bytes = lin_packed_bytes(dout, d->out_stride, d->m, d->n);
-  if (b.sums) b.part_bytes = (b.runs * 2 * lin_pitch(d->n) * 4 + 255) / 256 * 256;
+  if (b.sums > 0) b.part_bytes = (b.runs * b.sums * lin_pitch(d->n) * 4 + 255) / 256 * 256;
   if (g->w != nullptr) b.x_bytes = lin_packed_bytes(x, d->x_stride, d->m, d->k);
   if (g->x != nullptr) b.w_bytes = lin_packed_bytes(w, d->w_stride, d->n, d->k);
   return b;
@@ -1388,7 +1405,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
   const void* dz = dout;
   int64_t ld_dz = d->out_stride;
   const bool tok = d->gate_form == DGXM_MOD_TOKEN;
-  if (plan.dz || plan.sums || (g->gate != nullptr && tok)) {
+  if (plan.dz || plan.sums > 0 || (g->gate != nullptr && tok)) {
     LinDzParams q;
     memset(&q, 0, sizeof(q));
     q.dout = dout;
@@ -1399,7 +1416,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
       q.ld_dz = lin_pitch(d->n);
       work += plan.dz_bytes;
     }
-    if (plan.sums) {
+    if (plan.sums > 0) {
       q.partial = reinterpret_cast<float*>(work);
       work += plan.part_bytes;
     }
@@ -1407,7 +1424,8 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
     q.g_gate = tok ? g->gate : nullptr;
     q.ld_dout = d->out_stride;
     q.ld_pre = d->pre_stride;
-    lin_gate_strides(d, &q.gate_sample, &q.gate_row);
+    q.gate_sample = plan.gate_sample;
+    q.gate_row = plan.gate_row;
     q.runs = plan.runs;
     q.n = static_cast<int>(d->n);
     q.sample_rows = static_cast<int>(plan.sample_rows);
@@ -1433,7 +1451,7 @@ extern "C" int dgxm_linear_backward(const dgxm_linear_desc* d, const dgxm_linear
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     DGXM_CUDA_TRY(cudaLaunchKernelEx(&cfg, g->gate != nullptr ? lin_dz_pick<true>(d->activation) : lin_dz_pick<false>(d->activation), q));
-    if (plan.sums) {
+    if (plan.sums > 0) {
       LinSumParams s;
       s.partial = q.partial;
       s.g_bias = g->bias;

@@ -360,3 +360,20 @@ def test_gradients_of_no_rows(lead, gate):
     grads = linear_backward(dout, a["x"], a["w"], bias=a["bias"], gate=a["gate"], pre=dout)
     for got, like in ((grads.x, a["x"]), (grads.w, a["w"]), (grads.bias, a["bias"]), (grads.gate, a["gate"])):
         assert (got is None and like is None) or torch.equal(got, torch.zeros_like(like))
+
+
+@pytest.mark.parametrize("gate", ["shared", "token", "apart", "expanded", "same"])
+@pytest.mark.parametrize("b,l", [(1, 1), (700, 1), (1, 700), (233, 3), (5, 131)])
+def test_sums_across_samples(b, l, gate):
+    """A bias' and a shared gate's sums over many short samples, and tokens' gates: rows a step apart, samples further apart
+    than their rows, and one row or one value for all tokens seen as tokens'."""
+    a, _, dout = make(b + l, (b, l), 136, 64, torch.bfloat16, gate="shared" if gate == "shared" else "token")
+    if gate == "apart":
+        wide = torch.zeros(b, l + 2, 136, device="cuda", dtype=torch.bfloat16)
+        a["gate"] = wide[:, 1:l + 1].copy_(a["gate"])
+    elif gate == "expanded":
+        a["gate"] = a["gate"][:, :1].expand(b, l, 136)
+    elif gate == "same":
+        a["gate"] = a["gate"][:1, :1].expand(b, l, 136)
+    for name in ("silu", "none"):
+        run_backward(a, dout, name)

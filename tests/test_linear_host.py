@@ -1,6 +1,7 @@
 """Refusals of the Linear calls, all before any device work."""
 from __future__ import annotations
 
+import ctypes
 import shutil
 
 import pytest
@@ -274,3 +275,21 @@ def test_gradients_of_no_rows_are_zeros(monkeypatch, lib, x_shape, gate_shape):
     grads = ln.linear_backward(dout, x, w, bias=bias, gate=gate, pre=dout)
     for got, like in zip(grads, (x, w, bias, gate)):
         assert torch.equal(got, torch.zeros_like(like))
+
+
+@pytest.mark.parametrize("form", ["shared", "token", "token apart"])
+def test_partial_sums_of_many_short_samples(lib, form):
+    """The workspace of a bias' gradient goes by the rows, not by the samples, where no sum is a sample's; one wanted sum
+    takes half of two."""
+    from dgx_monarch_b200 import _lib
+
+    m, n = 9450, 13824
+    need = lambda rows, **g: lib.dgxm_linear_backward_workspace(
+        _desc(m=m, n=n, out_stride=n, pre_stride=n, gate_form=_lib.MOD_SHARED if form == "shared" else _lib.MOD_TOKEN, sample_rows=rows,
+              gate_stride=(ctypes.c_int64 * 2)(*((0, 0) if form == "shared" else (2 * rows * n if form == "token apart" else rows * n, n)))),
+        _lib.LinearGradPointers(**g), FAKE, FAKE, FAKE)
+    whole = need(m, bias=FAKE)
+    assert whole == -(-m // 64) * n * 4
+    assert need(1, bias=FAKE) == whole  # (rows of samples of one are always a step apart)
+    assert need(3, bias=FAKE) == (m // 3 * n * 4 if form == "token apart" else whole)
+    assert need(1, bias=FAKE, gate=FAKE) == whole * (2 if form == "shared" else 1)
