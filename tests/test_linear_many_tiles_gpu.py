@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests.block_reference import U, check
-from tests.test_linear_gpu import act, gate_of, make
+from tests.test_linear_gpu import act, gate_of, make, run_backward, run_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,46 @@ def test_residual_on_words_beside_outputs_off_them(m, n, k, out_dtype):
     from dgx_monarch_b200.linear import linear
 
     assert torch.equal(linear(**a, residual=shared, out=shared), apart)
+
+
+# By rows: one tile a CTA or pair at the most, and several.
+BY_ROWS = [(300, 1000, 72), (511, 2048, 128), (1100, 1024, 192), SINGLE, PAIR_192, PAIR_256, (19000, 304, 64), (20000, 512, 64),
+           (20000, 384, 64)]
+
+
+@pytest.mark.parametrize("m,n,k", BY_ROWS)
+@pytest.mark.parametrize("name", ["none", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("out_dtype", [None, torch.float32], ids=["16", "fp32"])
+def test_bias_and_activation_alone(m, n, k, name, out_dtype):
+    """The kernels that have nothing else in their epilogue: each activation and output size, on one CTA and on a pair."""
+    a, _, _ = make(m + n, (m,), n, k, torch.float16 if n % 3 == 0 else torch.bfloat16)
+    run(a, None, name, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("m,n,k", BY_ROWS)
+@pytest.mark.parametrize("gate,residual,pre", [("sample", False, False), (None, True, False), ("token", True, True),
+                                               ("sample", False, True), ("shared", True, True)])
+def test_gate_residual_and_pre(m, n, k, gate, residual, pre):
+    """What the rolled epilogue does, over several tiles, with pre by bulk stores, by the lanes and beside a residual."""
+    lead = (2, m // 2) if gate == "sample" else (m,)
+    a, res, _ = make(m + n, lead, n, k, torch.bfloat16, gate=gate, residual=residual)
+    if not pre:
+        run(a, res, "silu")
+        run(a, None if res is None else res.float(), "gelu", out_dtype=torch.float32)
+    else:
+        run_forward(a, res, "gelu_tanh")
+        run_forward(a, None if res is None else res.float(), "gelu", out_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("m,n,k", [(19000, 64, 304), (40000, 64, 260), (38000, 64, 128), (20000, 128, 512)])
+def test_gradients_of_many_tiles(m, n, k):
+    """Products with w's rows contiguous along k, and along the rows, of more tiles than fit at one time."""
+    a, _, dout = make(m + k, (m,), n, k, torch.bfloat16)
+    run_backward(a, dout, "silu")
+
+
+@pytest.mark.parametrize("m,n,k", [(70, 4000, 1100), (40, 3001, 2000), (192, 5120, 5128)])
+def test_wide_gradients_of_many_tiles(m, n, k):
+    """w's gradient of more tiles than CTAs, and than pairs."""
+    a, _, dout = make(3, (m,), n, k, torch.bfloat16)
+    run_backward(a, dout)
