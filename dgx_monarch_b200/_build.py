@@ -15,10 +15,14 @@ CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libdgxm_sp.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
+# ptxas takes the kernels in parallel (4.6 minutes instead of 6, the same
+# registers).  nvcc's own --split-compile (2 to 3 minutes) cuts the optimiser's
+# work differently from run to run: two libraries of one source, one with
+# 140-byte spills where the other has none, 61 us where the other takes 44.
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "--split-compile=0", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
+    "-Xptxas", "-split-compile=0", "-shared", "-Xcompiler", "-fPIC", "-cudart", "static",
 ]
 
 

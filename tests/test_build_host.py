@@ -14,3 +14,12 @@ def test_tuning_defines_accept_only_the_kernel_macros(monkeypatch):
         _build.tuning_defines()
     monkeypatch.delenv("DGXM_NVCC_DEFINES")
     assert _build.tuning_defines() == []
+
+
+def test_one_source_gives_one_library():
+    """nvcc's own split compilation cuts the optimiser's work by what the threads happen to do: registers and spills of most
+    kernels, and times by up to 40 %, went one way or the other from build to build."""
+    from dgx_monarch_b200 import _build
+
+    assert not any(f.startswith(("--split-compile", "-split-compile=")) and _build.NVCC_FLAGS[i - 1] != "-Xptxas"
+                   for i, f in enumerate(_build.NVCC_FLAGS))
