@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_kern
 }
 
 // The gradient's row of one chunk: e = dy, under a scale of each token dh, and n.
-template <typename T, bool VEC, bool FULL, int N>
+template <typename T, bool VEC, int N>
 __device__ __forceinline__ void bn_normed(const BlockNormParams& p, const uint8_t* slot, const BnWalk& w, const BnStats& st,
                                           int q, uint64_t (&e)[N], uint64_t (&n)[N]) {
   bn_get<T, VEC>(p, slot, kBnDy, w, q, e);
@@ -778,7 +778,7 @@ __device__ __forceinline__ float2 bn_row_dn(const BlockNormParams& p, const uint
 #pragma unroll 2
   for (int q = threadIdx.x & 31; q * CH < p.width; q += 32) {
     uint64_t e[N], n[N], a[N];
-    bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
+    bn_normed<T, VEC>(p, slot, w, st, q, e, n);
     bn_modulate<T, VEC, FULL>(p, slot, w, q, e);
     bn_factor<T, SRC>(p, param, w, q, a);
 #pragma unroll
@@ -808,7 +808,7 @@ __device__ __forceinline__ float bn_row_dn2(const BlockNormParams& p, const uint
   for (int q = threadIdx.x & 31; q * CH < p.width; q += 32) {
     uint64_t e[N], n[N], a[N], big[N];
     if (p.mode != DGXM_BLOCK_NORM_NONE) {
-      bn_normed<T, VEC, true>(p, slot, w, st, q, e, n);
+      bn_normed<T, VEC>(p, slot, w, st, q, e, n);
       bn_modulate<T, VEC, true>(p, slot, w, q, e);
       if (SRC == kBnScaled && p.factor == 0) bn_factor<T, kBnPlain>(p, param, w, q, a);
       else bn_factor<T, SRC>(p, param, w, q, a);
@@ -972,7 +972,7 @@ __global__ void __launch_bounds__(MAXT + 32 * STAT + 32, PER_SM) block_norm_back
       if (col >= p.width) continue;
       uint64_t e[N], n[N], big[N];
       if (norm) {
-        bn_normed<T, VEC, FULL>(p, slot, w, st, q, e, n);
+        bn_normed<T, VEC>(p, slot, w, st, q, e, n);
         if constexpr (FULL) {
           if (p.g_scale != nullptr) {  // a token's own: dy h
             uint64_t h[N], bias[N];
@@ -1037,7 +1037,7 @@ struct BlockNormSumParams {
   int64_t gate_sb, scale_sb;
   void *g_gate, *g_scale, *g_shift, *g_norm_w, *g_norm_b, *g_branch_w;
   int gate_form, mod_form;  // of the modulations
-  int want, dtype, mod_dtype, weight_dtype;
+  int want, mod_dtype, weight_dtype;
   int batch, seq, width, rows_more;
   int64_t rows, rows_each;
 };
@@ -1520,7 +1520,6 @@ extern "C" int dgxm_block_norm_backward(const dgxm_block_norm_desc* d, const dgx
   sp.gate_form = d->gate_form;
   sp.mod_form = d->mod_form;
   sp.want = p.want;
-  sp.dtype = d->dtype;
   sp.mod_dtype = d->mod_dtype;
   sp.weight_dtype = d->weight_dtype;
   sp.batch = d->batch;

@@ -177,7 +177,7 @@ __device__ __forceinline__ uint64_t lin_desc(uint32_t addr) {
 template <bool MN>
 constexpr uint32_t kLinStep = MN ? 2048 / 16 : 32 / 16;
 
-// What fp4_store_rows is told of `pre`.
+// What fp4_piece and fp4_flush_rows are told of `pre`.
 struct LinPreOut {
   const CUtensorMap& tmap_out;
   void* out;
@@ -833,10 +833,10 @@ static LinCut lin_cut(int64_t m, int64_t n, int k_tiles, bool a_mn, bool b_mn) {
   };
   // Microseconds a stage of K, a tile (transposed ones share its epilogue with the CTAs of a split K), and at the least, as
   // measured with all SMs at work (1024 and 2048 x 5120 x 5120 by rows, 1 .. 64 x 5120 x 5120, 256 x 804 x 8064 and
-  // 8192 x 64 x 256 transposed); the sums order the cuts and are not the times of calls.
+  // 8192 x 64 x 256 transposed); the sums order the cuts and are not the times of calls.  (A pair with 128 columns, 0.245,
+  // 1.5 and 2.0, has no fewer passes than single CTAs ever, and a dearer one.)
   static const Kind kinds[] = {{16, false, 0.18, 1.3, 0.4},  {32, false, 0.19, 2.3, 0.5},  {64, false, 0.22, 4.5, 1.0},
-                               {128, false, 0.24, 1.3, 1.6}, {128, true, 0.245, 1.5, 2.0}, {192, true, 0.285, 1.7, 2.2},
-                               {256, true, 0.315, 2.0, 2.5}};
+                               {128, false, 0.24, 1.3, 1.6}, {192, true, 0.285, 1.7, 2.2}, {256, true, 0.315, 2.0, 2.5}};
   static const int clusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};  // that the SMs hold at one time
   LinCut best{128, false, 1, false, 128};
   double least = 1e30;
