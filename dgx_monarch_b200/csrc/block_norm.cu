@@ -27,10 +27,10 @@
 // Means and variances are fp32, gathered a chunk at a time from deviations
 // (never as a difference of squares); every output is rounded once.
 //
-// Calls on B200: 9450 x 5120 bf16 with branch, gate and modulation 72 to 76 us
-// (5.1 to 5.4 TB/s), its gradient 118 to 145; 2 x 2640 x 2048 with fp32 values
-// for each token 43 to 61; one row 10 us, which is the call.  With sums that all warps of a
-// block wait for, the first two took 82 and 173 us.
+// Calls on B200: 9450 x 5120 bf16 with branch, gate and modulation 76 us (5.1
+// TB/s), its gradient 118; 2 x 2640 x 2048 with fp32 values for each token 44;
+// one row 10 us, which is the call.  With sums that all warps of a block wait
+// for, the first two took 82 and 173 us.
 #include <algorithm>
 #include <type_traits>
 

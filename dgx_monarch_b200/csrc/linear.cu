@@ -16,10 +16,10 @@
 // M256 MMAs that read both CTAs' operands), others on single CTAs, and with
 // few rows, or few tiles and a long K, the weight gives the rows of a tile.
 //
-// Large products are bound by power (9450 x 13824 x 5120 with GELU: 853 us cold,
-// 1033 in a long run, 1.57 and 1.30 PFLOP/s), few rows by DRAM (2 x 30720 x 5120:
-// 51 us, 6.2 TB/s), and what lies between by the latency of stages of K, about
-// 0.25 us each (512 x 5120 x 4096: 22 us).
+// Large products are bound by power (9450 x 13824 x 5120 with GELU: 988 to 1021
+// us in a row, 1.31 to 1.35 PFLOP/s), few rows by DRAM (2 x 30720 x 5120: 51 us,
+// 6.1 TB/s), and what lies between by its few tiles, of 0.25 us a stage of K each
+// (512 x 5120 x 4096: 21 to 24 us).
 #include <type_traits>
 
 #include "common.h"
