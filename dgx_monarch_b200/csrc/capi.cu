@@ -40,6 +40,22 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+int encode_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const cuuint64_t (&dims)[3],
+                  const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(DGXM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], 1}, st[3] = {strides[0], strides[1], strides[1] * dims[2]};
+  const cuuint32_t bx[4] = {box[0], box[1], box[2], 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, dt, 4, const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DGXM_ERR_INVALID, "cuTensorMapEncodeTiled returned %d", (int)r);
+  return DGXM_OK;
+}
+
+static const ErrorWord* g_error_words = nullptr;  // set before any unit's constructors run
+
+ErrorWord::ErrorWord(const void* word) : symbol(word), next(g_error_words) { g_error_words = this; }
+
 int encode_map_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elt_bytes,
                   int64_t cols, int64_t heads, int64_t rows, int64_t batch, int64_t s_head,
                   int64_t s_row, int64_t s_batch, int box_cols, int box_rows) {
@@ -80,12 +96,16 @@ extern "C" int dgxm_device_error(int clear) {
   int value = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return -dgxm::cuda_fail(e, "cudaDeviceSynchronize");
-  e = cudaMemcpyFromSymbol(&value, dgxm::g_device_error, sizeof(int));
-  if (e != cudaSuccess) return -dgxm::cuda_fail(e, "cudaMemcpyFromSymbol");
-  if (clear) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbol(dgxm::g_device_error, &zero, sizeof(int));
-    if (e != cudaSuccess) return -dgxm::cuda_fail(e, "cudaMemcpyToSymbol");
+  for (const dgxm::ErrorWord* word = dgxm::g_error_words; word != nullptr; word = word->next) {
+    int bits = 0;
+    e = cudaMemcpyFromSymbol(&bits, word->symbol, sizeof(int));
+    if (e != cudaSuccess) return -dgxm::cuda_fail(e, "cudaMemcpyFromSymbol");
+    value |= bits;
+    if (clear && bits != 0) {
+      const int zero = 0;
+      e = cudaMemcpyToSymbol(word->symbol, &zero, sizeof(int));
+      if (e != cudaSuccess) return -dgxm::cuda_fail(e, "cudaMemcpyToSymbol");
+    }
   }
   return value;
 }

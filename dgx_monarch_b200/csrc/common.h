@@ -1,5 +1,6 @@
 // Host-side helpers shared by the C-ABI translation units: status plumbing,
-// a per-thread error message, CUDA error capture and TMA descriptor encoding.
+// a per-thread error message, CUDA error capture, the list of device error
+// words and TMA descriptor encoding.
 #pragma once
 
 #include <cuda.h>
@@ -69,6 +70,18 @@ cudaError_t launch_overlapped(void (*kernel)(Params), unsigned grid, unsigned bl
 int encode_map_4d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elt_bytes,
                   int64_t cols, int64_t heads, int64_t rows, int64_t batch, int64_t s_head,
                   int64_t s_row, int64_t s_batch, int box_cols, int box_rows);
+
+// A 3-D tensor map (strides in bytes), zero out of bounds.
+int encode_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const cuuint64_t (&dims)[3],
+                  const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle);
+
+// A translation unit's device error word, in the list of all units' that
+// dgxm_device_error() reads and clears.
+struct ErrorWord {
+  const void* symbol;
+  const ErrorWord* next;
+  explicit ErrorWord(const void* symbol);
+};
 
 // Stores into a per-device error word written by kernels whose bounded waits
 // expired (bit flags, see kErr* below).

@@ -1,13 +1,15 @@
-// The per-device error word.  Kernels OR a kErr* bit into it when a bounded
-// wait expires; the host reads it with dgxm_device_error().  The library is
-// built as one translation unit, so this single definition is shared by every
-// kernel without relocatable device code.
+// The error word, one a device and translation unit.  Kernels OR a kErr* bit
+// into it when a bounded wait expires; the host reads all units' words with
+// dgxm_device_error().  (A single one would need relocatable device code.)
 #pragma once
+
+#include "common.h"
 
 namespace dgxm {
 
-__device__ int g_device_error = 0;
+static __device__ int g_device_error = 0;
+static const ErrorWord g_device_error_word(&g_device_error);
 
-__device__ __forceinline__ void report_device_error(int bits) { atomicOr(&g_device_error, bits); }
+static __device__ __forceinline__ void report_device_error(int bits) { atomicOr(&g_device_error, bits); }
 
 }  // namespace dgxm

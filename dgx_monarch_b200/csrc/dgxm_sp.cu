@@ -1,6 +1,5 @@
-// Single translation unit of libdgxm_sp.so.  The kernels share one device
-// error word (device_error.cuh), so the library is built as one unit rather
-// than with relocatable device code.
+// The first translation unit of libdgxm_sp.so.  linear.cu and block_norm*.cu,
+// which take as long to compile, are units of their own.
 #include <math.h>
 #include <string.h>
 
@@ -19,5 +18,3 @@
 #include "qk_norm.cu"
 #include "fp4_quant.cu"
 #include "fp4_gemm.cu"
-#include "block_norm.cu"
-#include "linear.cu"

@@ -16,13 +16,18 @@
 // M256 MMAs that read both CTAs' operands), others on single CTAs, and with
 // few rows, or few tiles and a long K, the weight gives the rows of a tile.
 //
-// Large products are bound by power (9450 x 13824 x 5120 with GELU: 988 to 1021
-// us in a row, 1.31 to 1.35 PFLOP/s), few rows by DRAM (2 x 30720 x 5120: 51 us,
+// Large products are bound by power (9450 x 13824 x 5120 with GELU: 988 to 1034
+// us in a row, 1.29 to 1.35 PFLOP/s), few rows by DRAM (2 x 30720 x 5120: 51 us,
 // 6.1 TB/s), and what lies between by its few tiles, of 0.25 us a stage of K each
 // (512 x 5120 x 4096: 21 to 24 us).
+#include <string.h>
+
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
+#include "device_error.cuh"
+#include "gemm_tile.cuh"
 #include "ptx.cuh"
 
 namespace dgxm {
@@ -744,15 +749,15 @@ struct LinOperand {
 static int lin_map(CUtensorMap* map, const LinOperand& o, int64_t k, int box_rows) {
   const cuuint64_t row = static_cast<cuuint64_t>(o.ld) * 2;
   if (o.mn)
-    return fp4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.ptr, {(cuuint64_t)o.rows, 1, (cuuint64_t)k}, {row, row},
+    return encode_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.ptr, {(cuuint64_t)o.rows, 1, (cuuint64_t)k}, {row, row},
                    {64, 1, kLinK}, CU_TENSOR_MAP_SWIZZLE_128B);
-  return fp4_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.ptr, {(cuuint64_t)k, 1, (cuuint64_t)o.rows}, {row, row},
+  return encode_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, o.ptr, {(cuuint64_t)k, 1, (cuuint64_t)o.rows}, {row, row},
                  {kLinK, 1, (cuuint32_t)box_rows}, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 static int lin_out_map(CUtensorMap* map, const void* base, int64_t ld, int elt, const LinearParams& p) {
   const cuuint64_t row = static_cast<cuuint64_t>(ld) * elt;
-  return fp4_map(map, elt == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, base,
+  return encode_map_3d(map, elt == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, base,
                  {(cuuint64_t)p.q_rows, 1, (cuuint64_t)p.p_rows}, {row, row}, {(cuuint32_t)(128 / elt), 1, 32},
                  CU_TENSOR_MAP_SWIZZLE_128B);
 }

@@ -23,3 +23,17 @@ def test_one_source_gives_one_library():
 
     assert not any(f.startswith(("--split-compile", "-split-compile=")) and _build.NVCC_FLAGS[i - 1] != "-Xptxas"
                    for i, f in enumerate(_build.NVCC_FLAGS))
+
+
+def test_every_source_is_part_of_one_unit():
+    """A unit, or included by exactly one; kernels that report to the error word have their unit's."""
+    import re
+
+    from dgx_monarch_b200 import _build
+
+    included = {u: re.findall(r'^#include "(\w+\.cu)"', (_build.CSRC / u).read_text(), re.M) for u in _build.UNITS}
+    parts = sorted(_build.UNITS + [p for part in included.values() for p in part])
+    assert parts == sorted(p.name for p in _build.CSRC.glob("*.cu"))
+    for path in list(_build.CSRC.glob("*.cu")) + list(_build.CSRC.glob("*.cuh")):
+        if path.name != "device_error.cuh":
+            assert "__device__ int g_device_error" not in path.read_text()
